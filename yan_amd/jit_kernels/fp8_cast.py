@@ -1,4 +1,5 @@
-"""Quantisers in front of the block-scaled FP8 GEMM: per-token 1x128 for activations, per-block 128x128 for weights.
+"""Quantisers in front of the block-scaled FP8 GEMM: per-token 1x128 for activations, per-block 128x128 for weights; and
+per-channel 128x1, turned round, for the operands of weight gradients.
 
 The reference names the GEMM's operands (`lhs, lhs_scales, rhs, rhs_scales`, `yan/jit_kernels/gemm.py:23-30`) and has
 no code that produces them; callers of this convention build them with a chain of torch ops
@@ -9,13 +10,13 @@ amax and moves a code where `x * factor` lands on a rounding boundary. With true
 chain and these kernels agree bit for bit.
 """
 import functools
-from typing import Tuple
+from typing import Optional, Tuple
 
 import torch
 
-from .host_calls import PER_BLOCK, PER_TOKEN, remember_call, repeat_call
+from .host_calls import PER_BLOCK, PER_CHANNEL, PER_TOKEN, remember_call, repeat_call
 from .tuner import FrozenKeys, jit_tuner
-from .utils import ceil_div, current_raw_stream
+from .utils import assert_on_current_device, ceil_div, current_raw_stream
 
 includes = ('"gemm/fp8_cast.hpp"', )
 
@@ -29,6 +30,14 @@ per_block_template = """
 using namespace yan;
 // Templated args from Python JIT call: source element type {SRC}
 __return_code = static_cast<int>(launch_per_block_cast(x, q, scales, n, k, stream));
+"""
+
+per_channel_includes = ('"gemm/fp8_cast_transposed.hpp"', )
+
+per_channel_template = """
+using namespace yan;
+// Templated args from Python JIT call: source element type {SRC}
+__return_code = static_cast<int>(launch_per_channel_cast(x, gathered ? source : nullptr, q, scales, m, n, k_blocks, scales_stride, stream));
 """
 
 
@@ -47,12 +56,19 @@ def per_block_arg_defs(dtype: torch.dtype):
             ('stream', torch.cuda.Stream))
 
 
+def per_channel_arg_defs(dtype: torch.dtype):
+    return (('x', dtype), ('source', torch.int), ('q', torch.float8_e4m3fn), ('scales', torch.uint8), ('gathered', int), ('m', int), ('n', int),
+            ('k_blocks', int), ('scales_stride', int), ('stream', torch.cuda.Stream))
+
+
 @functools.lru_cache(maxsize=None)
 def cast_kernel_plan(kind: str, dtype: torch.dtype):
     """(name, keys, arg_defs, template) of the JIT kernel behind a quantiser; needs no GPU."""
     keys = FrozenKeys({'SRC': _src_name(dtype)})
     if kind == 'per_token':
         return 'per_token_cast_to_fp8', keys, per_token_arg_defs(dtype), per_token_template
+    if kind == 'per_channel':
+        return 'per_channel_cast_to_fp8', keys, per_channel_arg_defs(dtype), per_channel_template
     assert kind == 'per_block'
     return 'per_block_cast_to_fp8', keys, per_block_arg_defs(dtype), per_block_template
 
@@ -100,4 +116,42 @@ def per_block_cast_to_fp8(w: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     rc = runtime(*args)
     assert rc == 0, f'{name} failed with HIP error {rc}'
     remember_call((PER_BLOCK, w, q, scales), name, runtime, args)
+    return q, scales
+
+
+def per_channel_cast_to_fp8(x: torch.Tensor, source: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """
+    The columns of x as rows of an operand of `gemm_fp8_fp8_fp32_nt`: tokens become contiguous, a power-of-two scale for every 128 of them.
+
+    x: bf16 or fp32 `[m, n]`, contiguous, n % 8 == 0; gradients or activations, a token a row
+    source: int32 `[k]`, k % 128 == 0: token r of the result is `x[source[r]]`, or zeros where source[r] is none of x's rows (as
+            `moe_dispatch_to_fp8_contiguous` returns it). None: x's own rows, and zeros up to a multiple of 128.
+    Returns e4m3fn `[n, k]` (k = m rounded up to 128 without `source`) and uint8 `[n, k/128]`: exponents + 127 (E8M0), rows a multiple of 4 bytes
+    apart. A scale is the smallest power of two with `max|x| <= 448 * scale` (2^-108 for zeros); `x / scale` is rounded to the nearest code. NaN and
+    infinity become NaN and do not count for the scale.
+    """
+    assert x.dim() == 2 and x.size(1) % 8 == 0 and x.is_contiguous()
+    m, n = x.shape
+    if source is not None:
+        assert source.dim() == 1 and source.dtype == torch.int32 and source.is_contiguous() and source.numel() % 128 == 0
+    assert x.data_ptr() % 16 == 0 and (source is None or source.data_ptr() % 4 == 0), 'rows start at multiples of 16 bytes'
+    blocks = ceil_div(m, 128) if source is None else source.numel() // 128
+    assert m < 1 << 31 and n * ceil_div(blocks, 4) * 4 < 1 << 40
+    name, keys, arg_defs, template = cast_kernel_plan('per_channel', x.dtype)
+    assert_on_current_device(x, source)
+    q = torch.empty((n, blocks * 128), dtype=torch.float8_e4m3fn, device=x.device)
+    stride = ceil_div(blocks, 4) * 4
+    scales = torch.empty((n, stride), dtype=torch.uint8, device=x.device)[:, :blocks]
+    if n == 0 or blocks == 0:
+        return q, scales
+    gathered = int(source is not None)
+    held = source if gathered else torch.empty(1, dtype=torch.int32, device=x.device)       # stands for what is not there
+    call = (PER_CHANNEL, x, held, q, scales, gathered)
+    if repeat_call(*call):
+        return q, scales
+    args = (x, held, q, scales, gathered, m, n, blocks, stride, current_raw_stream())
+    runtime = jit_tuner.compile_and_tune(name=name, keys=keys, space=(), includes=per_channel_includes, arg_defs=arg_defs, template=template, args=args)
+    rc = runtime(*args)
+    assert rc == 0, f'{name} failed with HIP error {rc}'
+    remember_call((PER_CHANNEL, x, held, q, scales, gathered), name, runtime, args)
     return q, scales

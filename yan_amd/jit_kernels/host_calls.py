@@ -29,6 +29,7 @@ if getattr(_host_calls, 'built_for', None) != f'torch {torch.__version__} {torch
 
 # which entry a remembered call belongs to
 FP8, CAST_FP8, BF16, FP16, FLOAT, CONTIGUOUS, MASKED, PER_TOKEN, PER_BLOCK = range(1, 10)
+ROUTE, ROUTE_BACKWARD, DISPATCH, COMBINE, COMBINE_BACKWARD, PER_CHANNEL, WGRAD = range(10, 17)
 _TENSOR, _CONSTANT, _STREAM, _WORKSPACE = range(4)
 _THE_STREAM, _THE_WORKSPACE = (_STREAM, 0), (_WORKSPACE, 0)
 

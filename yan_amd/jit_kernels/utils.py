@@ -66,6 +66,13 @@ def get_num_sms_cap() -> int:
     return 0 if cap >= _device_cu_count() else cap
 
 
+def assert_on_current_device(*tensors) -> None:
+    """Refuses tensors (None: not given) that are not on the current device, whose stream the launch goes to."""
+    current = torch.cuda.current_device()
+    for x in tensors:
+        assert x is None or x.get_device() == current, 'tensors have to be on the current device'
+
+
 def ceil_div(x: int, y: int) -> int:
     return (x + y - 1) // y
 
