@@ -714,7 +714,39 @@ def jit_kernels_in_use(num_cus: int = 256):
     groups, m_max, n, k, _, expected_m = GROUPED_MASKED_TEST_CASES[6]
     name, keys, arg_defs, _ = m_grouped_gemm.grouped_kernel_plan('GroupedMasked', groups, min(expected_m, m_max), n, k, NUM_SMS_CAP)
     add(name, arg_defs, m_grouped_gemm.includes, m_grouped_gemm.template, keys)
+    # around the grouped GEMMs: router, dispatch, combine, the transposing quantiser, weight gradients; then the grouped GEMMs of the layers they are run in
+    from yan_amd.jit_kernels import moe, wgrad
+    for dtype in (torch.bfloat16, torch.float32):
+        for scoring in ('softmax', 'sigmoid'):
+            for experts in (64, 128, 256, 512, 1024):
+                for backward in (False, True):
+                    name, keys, arg_defs, code_template = moe.route_kernel_plan(dtype, scoring, experts, backward)
+                    add(name, arg_defs, moe._route_includes, code_template, keys)
+        name, keys, arg_defs, code_template = moe.dispatch_kernel_plan(dtype)
+        add(name, arg_defs, moe._dispatch_includes, code_template, keys)
+        name, keys, arg_defs, code_template = fp8_cast.cast_kernel_plan('per_channel', dtype)
+        add(name, arg_defs, fp8_cast.per_channel_includes, code_template, keys)
+    for top_k in (1, 2, 3, 4, 5, 6, 7, 8, 16):
+        for backward in (False, True):
+            name, keys, arg_defs, code_template = moe.combine_kernel_plan(top_k, backward)
+            add(name, arg_defs, moe._combine_includes, code_template, keys)
+    for kernel, parts in WGRAD_KERNELS:
+        name, keys, arg_defs, code_template = wgrad.wgrad_kernel_plan(kernel, parts)
+        add(name, arg_defs, wgrad.includes, code_template, keys)
+    tokens, hidden, inner, experts, top_k = MOE_TRAINING_LAYER
+    name, keys, arg_defs, _ = m_grouped_gemm.grouped_kernel_plan('GroupedContiguous', experts, moe.get_contiguous_layout_rows(tokens, top_k, experts), inner, hidden, num_cus)
+    add(name, arg_defs, m_grouped_gemm.includes, m_grouped_gemm.rows_on_device_template if 'ROWS' in keys else m_grouped_gemm.template, keys)
+    tokens, hidden, inner, experts, top_k, m_max, expected_m = MOE_DECODE_LAYER
+    name, keys, arg_defs, _ = m_grouped_gemm.grouped_kernel_plan('GroupedMasked', experts, expected_m, inner, hidden, num_cus)
+    add(name, arg_defs, m_grouped_gemm.includes, m_grouped_gemm.template, keys)
     return list(kernels.values())
+
+
+# (kernel, parts) of the weight-gradient kernels, the rule's choice first
+WGRAD_KERNELS = [('kWgradAny', 1), ('kWgradTall', 1), ('kWgrad128', 1), ('kWgrad64', 1), ('kWgradSplit', 2), ('kWgradSplit', 8)]
+# tokens, hidden, inner, experts, top_k; in decode also m_max and expected_m
+MOE_TRAINING_LAYER = (700, 512, 384, 6, 3)
+MOE_DECODE_LAYER = (37, 512, 256, 8, 2, 32, 8)
 
 
 def prebuild_jit_kernels(num_cus: int = 256, verbose: bool = False, jobs: int = 0) -> int:

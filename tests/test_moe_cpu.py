@@ -1,0 +1,153 @@
+"""The mixture-of-experts entries and the weight-gradient products without a GPU: what they refuse, and the rules that size their kernels."""
+import random
+
+import pytest
+import torch
+
+import yan_amd as yan
+from yan_amd.jit import cpp_format, generate
+from yan_amd.jit_kernels import fp8_cast, moe, wgrad
+
+F8 = torch.float8_e4m3fn
+
+
+def test_plans_generate_and_are_shared_between_sizes():
+    for dtype in (torch.bfloat16, torch.float32):
+        for scoring in ('softmax', 'sigmoid'):
+            for backward in (False, True):
+                plans = {moe.route_kernel_plan(dtype, scoring, experts, backward)[1]['LANES'] * 100 + moe.route_kernel_plan(dtype, scoring, experts, backward)[1]['VALUES']
+                         for experts in range(1, 1025)}
+                assert len(plans) == 5
+        for plan in (moe.dispatch_kernel_plan(dtype), fp8_cast.cast_kernel_plan('per_channel', dtype), moe.route_kernel_plan(dtype, 'softmax', 8)):
+            name, keys, arg_defs, template = plan
+            code = generate(('"moe/route.hpp"', ), arg_defs, cpp_format(template, dict(keys)))
+            assert 'launch_' in code and not any('{' + k + '}' in code for k in keys)
+    assert len(wgrad.arg_defs) <= 20 and len(moe.dispatch_kernel_plan(torch.bfloat16)[2]) <= 20      # what a native repeat call passes
+
+
+def test_lanes_hold_every_number_of_experts():
+    for experts in range(1, moe.MAX_EXPERTS + 1):
+        lanes, values = moe.route_lanes(experts)
+        assert lanes * values >= experts and lanes in (16, 32, 64) and lanes >= moe.MAX_TOP_K
+        for tokens in (0, 1, 15, 16, 17, 100, 4096, 1 << 20):
+            assert 1 <= moe.route_blocks(tokens, experts) <= 256
+
+
+def test_contiguous_rows_are_enough_and_no_more_than_that():
+    rng = random.Random(5)
+    for _ in range(300):
+        tokens, top_k, experts = rng.randint(1, 200), rng.randint(1, 8), rng.randint(1, 40)
+        most = yan.get_contiguous_layout_rows(tokens, top_k, experts)
+        assert most % 128 == 0
+        for _ in range(10):
+            counts = [0] * experts
+            for _ in range(tokens * top_k):
+                counts[rng.randrange(experts) if rng.random() < 0.8 else 0] += 1
+            assert sum((c + 127) // 128 * 128 for c in counts) <= most
+    # every expert but one has one pair, the last one the rest: the bound is reached
+    assert yan.get_contiguous_layout_rows(128, 1, 4) == 3 * 128 + 128 and yan.get_contiguous_layout_rows(0, 8, 4) == 0
+    assert yan.get_contiguous_layout_rows(1, 1, 256) == 128
+
+
+def _refused(fn, *args, **kwargs):
+    with pytest.raises(AssertionError):
+        fn(*args, **kwargs)
+
+
+def test_route_refuses():
+    x = torch.zeros(4, 8)
+    _refused(yan.moe_route, x, 9)
+    _refused(yan.moe_route, x, 0)
+    _refused(yan.moe_route, torch.zeros(4, 64), 17)
+    _refused(yan.moe_route, torch.zeros(4, 1025), 2)
+    _refused(yan.moe_route, x.half(), 2)
+    _refused(yan.moe_route, x, 2, 'tanh')
+    _refused(yan.moe_route, torch.zeros(8, 4).t(), 2)
+    _refused(yan.moe_route, x[None], 2)
+    _refused(yan.moe_route, x, 2, mask=torch.ones(3, dtype=torch.bool))
+    _refused(yan.moe_route, x, 2, mask=torch.ones(4, dtype=torch.uint8))
+    i, c, w, l = torch.zeros(4, 2, dtype=torch.int32), torch.zeros(8, dtype=torch.int32), torch.zeros(4, 2), torch.zeros(())
+    _refused(yan.moe_route_backward, x, i.long(), c, w, l)
+    _refused(yan.moe_route_backward, x, i[:3], c, w[:3], l)
+    _refused(yan.moe_route_backward, x, i, c[:7], w, l)
+    _refused(yan.moe_route_backward, x, i, c, w[:, :1], l)
+    _refused(yan.moe_route_backward, x, i, c, w, torch.zeros(2))
+    _refused(yan.moe_route_backward, x, i, c, w.double(), l)
+    _refused(yan.moe_route_backward, x, i, c, w, l, 'tanh')
+    _refused(yan.moe_route_backward, x, i[:, 0], c, w, l)
+
+
+def test_dispatch_refuses():
+    x, i = torch.zeros(4, 256), torch.zeros(4, 2, dtype=torch.int32)
+    codes, scales = torch.zeros(512, 256, dtype=torch.uint8).view(F8), torch.zeros(512, 2)
+    _refused(yan.moe_dispatch_to_fp8_contiguous, x, i, 1025, (codes, scales))
+    _refused(yan.moe_dispatch_to_fp8_contiguous, x, i, 0, (codes, scales))
+    _refused(yan.moe_dispatch_to_fp8_contiguous, x, i[:3], 4, (codes, scales))
+    _refused(yan.moe_dispatch_to_fp8_contiguous, x, i.long(), 4, (codes, scales))
+    _refused(yan.moe_dispatch_to_fp8_contiguous, x.half(), i, 4, (codes, scales))
+    _refused(yan.moe_dispatch_to_fp8_contiguous, x[:, :200].contiguous(), i, 4, (codes, scales))
+    _refused(yan.moe_dispatch_to_fp8_contiguous, x, i, 4, (codes[:500], scales[:500]))
+    _refused(yan.moe_dispatch_to_fp8_contiguous, x, i, 4, (codes, scales[:, :1]))
+    _refused(yan.moe_dispatch_to_fp8_contiguous, x, i, 4, (codes, scales.double()))
+    _refused(yan.moe_dispatch_to_fp8_contiguous, x, torch.zeros(4, 17, dtype=torch.int32), 4, (codes, scales))
+    _refused(yan.moe_dispatch_to_fp8_contiguous, x, i, 4, (codes.view(4, 128, 256), scales.view(4, 128, 2)))
+    _refused(yan.moe_dispatch_to_fp8_masked, x, i, (codes, scales))
+    _refused(yan.moe_dispatch_to_fp8_masked, x, i, (codes.view(4, 128, 256)[:, :100], scales.view(4, 128, 2)[:, :100]))
+    _refused(yan.moe_dispatch_to_fp8_masked, x, i, (codes.view(4, 128, 256), scales.view(4, 2, 128)))
+
+
+def test_combine_refuses():
+    y, rows, w, out = torch.zeros(128, 64, dtype=torch.bfloat16), torch.zeros(4, 2, dtype=torch.int32), torch.zeros(4, 2), torch.zeros(4, 64, dtype=torch.bfloat16)
+    source = torch.zeros(128, dtype=torch.int32)
+    _refused(yan.moe_combine, y.float(), rows, w, out)
+    _refused(yan.moe_combine, y[:, :60].contiguous(), rows, w, out[:, :60].contiguous())
+    _refused(yan.moe_combine, y.t(), rows, w, out)
+    _refused(yan.moe_combine, y, rows.long(), w, out)
+    _refused(yan.moe_combine, y, torch.zeros(4, 17, dtype=torch.int32), None, out)
+    _refused(yan.moe_combine, y, rows, w[:3], out)
+    _refused(yan.moe_combine, y, rows, w.bfloat16(), out)
+    _refused(yan.moe_combine, y, rows, w, out[:3])
+    _refused(yan.moe_combine, y, rows, w, out.float())
+    _refused(yan.moe_combine, y.view(2, 64, 64), rows, w, out)
+    _refused(yan.moe_combine_backward, out, y, rows, w, source[:64])
+    _refused(yan.moe_combine_backward, out, y, rows, w, source.long())
+    _refused(yan.moe_combine_backward, out[:3], y, rows, w, source)
+
+
+def test_per_channel_cast_refuses():
+    x = torch.zeros(8, 16)
+    _refused(yan.per_channel_cast_to_fp8, x[:, :12].contiguous())
+    _refused(yan.per_channel_cast_to_fp8, x.t())
+    _refused(yan.per_channel_cast_to_fp8, x[None])
+    _refused(yan.per_channel_cast_to_fp8, x.half())
+    _refused(yan.per_channel_cast_to_fp8, x, torch.zeros(100, dtype=torch.int32))
+    _refused(yan.per_channel_cast_to_fp8, x, torch.zeros(128, dtype=torch.int64))
+    _refused(yan.per_channel_cast_to_fp8, x, torch.zeros(2, 64, dtype=torch.int32))
+    _refused(yan.per_channel_cast_to_fp8, x, torch.zeros(129, dtype=torch.int32)[1:])          # not at a multiple of 16 bytes
+
+
+def _operand(rows, k):
+    codes, scales = torch.zeros(rows, k, dtype=torch.uint8).view(F8), torch.zeros(rows, (k // 128 + 3) // 4 * 4, dtype=torch.uint8)[:, :k // 128]
+    return codes, scales
+
+
+def test_weight_gradients_refuse():
+    a, b, out = _operand(16, 640), _operand(8, 640), torch.zeros(16, 8)
+    gemm, grouped = yan.gemm_fp8_fp8_fp32_nt, yan.k_grouped_gemm_fp8_fp8_fp32_nt_contiguous
+    _refused(gemm, a, b, out.bfloat16())
+    _refused(gemm, a, b, out[:15])
+    _refused(gemm, a, b, out[None])
+    _refused(gemm, a, _operand(8, 512), out)
+    _refused(gemm, a, _operand(6, 640), torch.zeros(16, 6))
+    _refused(gemm, (a[0], a[1].float()), b, out)
+    _refused(gemm, (a[0], a[1].contiguous()), b, out)                      # rows five bytes apart
+    _refused(gemm, (a[0], a[1][:, :4]), b, out)
+    _refused(gemm, (a[0][:, :600], a[1]), b, out)
+    _refused(gemm, (a[0].view(torch.uint8), a[1]), b, out)
+    _refused(gemm, (a[0], torch.zeros(5, 16, dtype=torch.uint8).t()), b, out)
+    _refused(gemm, a, b, torch.zeros(8, 16).t())
+    offsets = torch.zeros(3, dtype=torch.int32)
+    _refused(grouped, a, b, out, offsets)
+    _refused(grouped, a, b, torch.zeros(2, 16, 8), offsets[:2])
+    _refused(grouped, a, b, torch.zeros(2, 16, 8), offsets.long())
+    _refused(grouped, a, b, torch.zeros(0, 16, 8), offsets[:1])

@@ -10,6 +10,7 @@
 // Nothing is kept by address or identity: addresses are read from the tensors of each call, the workspace from split_k.py's own record.
 #include <Python.h>
 
+#include <ATen/ops/empty.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <array>
@@ -26,7 +27,13 @@ namespace {
 constexpr int kMaxKey = 96, kMaxArgs = 20, kMaxFloats = 2;
 constexpr size_t kMaxCalls = 4096;          // then the table starts anew: a program of ever new sizes does not grow it
 
-enum Kind : int { kTensor = 0, kConstant = 1, kStream = 2, kWorkspace = 3 };
+enum Kind : int { kTensor = 0, kConstant = 1, kStream = 2, kWorkspace = 3, kOutput = 4 };
+
+// A tensor that a call makes: allocated as `shape`, then given `sizes` and `strides` where they differ (rows further apart than they are long).
+struct Output {
+    at::ScalarType type;
+    std::vector<int64_t> shape, sizes, strides;
+};
 
 struct Launch {
     std::vector<int64_t> key;
@@ -36,6 +43,8 @@ struct Launch {
     bool workspace;
     std::array<int, kMaxArgs> kind;
     std::array<int64_t, kMaxArgs> value;        // a constant, or which tensor
+    std::vector<Output> outputs;
+    size_t returned = 0;                        // the first so many of them go to the caller, the others are scratch
 };
 
 std::unordered_multimap<uint64_t, std::shared_ptr<Launch>> g_launches;
@@ -107,6 +116,8 @@ bool describe(Call& c, PyObject* const* objs, Py_ssize_t n) {
             for (size_t d = 0; d < sizes.size(); ++d)
                 if (!c.put(sizes[d]) || !c.put(strides[d])) return false;
             c.address[c.tensors++] = address;
+        } else if (o == Py_None) {
+            if (!c.put(-11)) return false;
         } else if (PyFloat_CheckExact(o)) {
             if (c.num_floats == kMaxFloats || !c.put(-7)) return false;
             c.floats[c.num_floats++] = float(PyFloat_AS_DOUBLE(o));
@@ -201,6 +212,13 @@ PyObject* launch_failed(const std::string& name, PyObject* token, int rc) {
     return PyErr_Format(PyExc_AssertionError, "%s failed with HIP error %d", name.c_str(), rc);
 }
 
+bool current_stream(int64_t device, int64_t* stream) {
+    PyObject* index = PyLong_FromLongLong(device);
+    const bool ok = index && call_int(g_stream, index, stream);
+    Py_XDECREF(index);
+    return ok;
+}
+
 // call(entry, *arguments): True if the launch was made, AssertionError if it failed.
 PyObject* call(PyObject*, PyObject* const* objs, Py_ssize_t n) {
     if (!g_utils || g_launches.empty()) Py_RETURN_FALSE;
@@ -209,12 +227,9 @@ PyObject* call(PyObject*, PyObject* const* objs, Py_ssize_t n) {
         if (!usual_switches() || !describe(c, objs, n)) Py_RETURN_FALSE;
         // held, not looked at in the table: what is called below can run other Python code, and other threads, that clear it
         const std::shared_ptr<const Launch> l = find(c);
-        if (!l) Py_RETURN_FALSE;
-        PyObject* device = PyLong_FromLongLong(c.device);
+        if (!l || !l->outputs.empty()) Py_RETURN_FALSE;
         int64_t stream;
-        const bool have_stream = call_int(g_stream, device, &stream);
-        Py_DECREF(device);
-        if (!have_stream) Py_RETURN_FALSE;
+        if (!current_stream(c.device, &stream)) Py_RETURN_FALSE;
         PyObject *workspace = nullptr, *token = nullptr;
         uint64_t workspace_address = 0;
         if (l->workspace) {
@@ -252,12 +267,69 @@ PyObject* call(PyObject*, PyObject* const* objs, Py_ssize_t n) {
     }
 }
 
-// remember((entry, *arguments), name, address, ((kind, value), ...)): the launch that served these arguments.
+// call_new(entry, *arguments): the tensors that the call makes, if the launch was made, None if this is no call for this file, AssertionError
+// if the launch failed. They come from torch's allocator, in the state of a tensor that nobody has used, as torch.empty gives them.
+PyObject* call_new(PyObject*, PyObject* const* objs, Py_ssize_t n) {
+    if (!g_utils || g_launches.empty()) Py_RETURN_NONE;
+    try {
+        Call c;
+        if (!usual_switches() || !describe(c, objs, n)) Py_RETURN_NONE;
+        const std::shared_ptr<const Launch> l = find(c);
+        int64_t stream;
+        if (!l || l->outputs.empty() || l->workspace || !current_stream(c.device, &stream)) Py_RETURN_NONE;
+        std::vector<at::Tensor> made;
+        made.reserve(l->outputs.size());
+        for (const Output& o : l->outputs) {
+            at::Tensor t = at::empty(o.shape, at::TensorOptions().dtype(o.type).device(at::kCUDA, static_cast<c10::DeviceIndex>(c.device)));
+            if (!o.sizes.empty()) t.unsafeGetTensorImpl()->set_sizes_and_strides(o.sizes, o.strides);
+            made.push_back(std::move(t));
+        }
+        uint64_t args[kMaxArgs];
+        for (int i = 0; i < l->count; ++i) {
+            switch (l->kind[i]) {
+                case kTensor: args[i] = c.address[l->value[i]]; break;
+                case kOutput: args[i] = reinterpret_cast<uint64_t>(made[size_t(l->value[i])].data_ptr()); break;
+                case kStream: args[i] = uint64_t(stream); break;
+                default: args[i] = uint64_t(l->value[i]);
+            }
+        }
+        int rc;
+        Py_BEGIN_ALLOW_THREADS
+        rc = launch_of<kMaxArgs>(l->count, l->function, args, c.floats);
+        Py_END_ALLOW_THREADS
+        if (rc != 0) return launch_failed(l->name, nullptr, rc);
+        PyObject* result = PyTuple_New(Py_ssize_t(l->returned));
+        for (size_t i = 0; result && i < l->returned; ++i) {
+            PyObject* t = THPVariable_Wrap(made[i]);
+            if (!t) Py_CLEAR(result);
+            else PyTuple_SET_ITEM(result, Py_ssize_t(i), t);
+        }
+        return result;
+    } catch (...) {         // no memory, say: the calls in Python will say so
+        PyErr_Clear();
+        Py_RETURN_NONE;
+    }
+}
+
+bool int_list(PyObject* tuple, std::vector<int64_t>* v) {
+    if (!PyTuple_CheckExact(tuple)) return false;
+    for (Py_ssize_t i = 0; i < PyTuple_GET_SIZE(tuple); ++i) {
+        int64_t x;
+        if (!plain_int(PyTuple_GET_ITEM(tuple, i), &x)) return false;
+        v->push_back(x);
+    }
+    return true;
+}
+
+// remember((entry, *arguments), name, address, ((kind, value), ...)[, outputs, returned]): the launch that served these arguments. outputs: (a tensor of the
+// type, shape, sizes, strides) each, sizes and strides empty where the shape says all.
 PyObject* remember(PyObject*, PyObject* args) {
     PyObject *objs, *spec;
+    PyObject* outputs = nullptr;
     const char* name;
     unsigned long long address;
-    if (!PyArg_ParseTuple(args, "O!sKO!", &PyTuple_Type, &objs, &name, &address, &PyTuple_Type, &spec)) return nullptr;
+    long long returned = 0;
+    if (!PyArg_ParseTuple(args, "O!sKO!|O!L", &PyTuple_Type, &objs, &name, &address, &PyTuple_Type, &spec, &PyTuple_Type, &outputs, &returned)) return nullptr;
     try {
         Call c;
         std::vector<PyObject*> items;
@@ -273,11 +345,22 @@ PyObject* remember(PyObject*, PyObject* args) {
         for (Py_ssize_t i = 0; i < count; ++i) {
             long long kind, value;
             if (!PyArg_ParseTuple(PyTuple_GET_ITEM(spec, i), "LL", &kind, &value)) return nullptr;
-            if (kind < kTensor || kind > kWorkspace || (kind == kTensor && (value < 0 || value >= c.tensors))) Py_RETURN_FALSE;
+            if (kind < kTensor || kind > kOutput || (kind == kTensor && (value < 0 || value >= c.tensors))) Py_RETURN_FALSE;
+            if (kind == kOutput && (!outputs || value < 0 || value >= PyTuple_GET_SIZE(outputs))) Py_RETURN_FALSE;
             l->kind[size_t(i)] = int(kind);
             l->value[size_t(i)] = value;
             l->workspace |= kind == kWorkspace;
         }
+        for (Py_ssize_t i = 0; outputs && i < PyTuple_GET_SIZE(outputs); ++i) {
+            PyObject *like, *shape, *sizes, *strides;
+            if (!PyArg_ParseTuple(PyTuple_GET_ITEM(outputs, i), "OOOO", &like, &shape, &sizes, &strides)) return nullptr;
+            Output o;
+            if (!THPVariable_CheckExact(like) || !int_list(shape, &o.shape) || !int_list(sizes, &o.sizes) || !int_list(strides, &o.strides)) Py_RETURN_FALSE;
+            o.type = THPVariable_Unpack(like).scalar_type();
+            l->outputs.push_back(std::move(o));
+        }
+        if (returned < 0 || size_t(returned) > l->outputs.size()) Py_RETURN_FALSE;
+        l->returned = size_t(returned);
         if (g_launches.size() >= kMaxCalls) g_launches.clear();
         const auto range = g_launches.equal_range(c.hash());
         auto at = range.first;
@@ -309,6 +392,7 @@ PyObject* setup(PyObject*, PyObject* args) {
 
 PyMethodDef methods[] = {
     {"call", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(call)), METH_FASTCALL, nullptr},
+    {"call_new", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(call_new)), METH_FASTCALL, nullptr},
     {"remember", remember, METH_VARARGS, nullptr},
     {"forget", forget, METH_NOARGS, nullptr},
     {"setup", setup, METH_VARARGS, nullptr},

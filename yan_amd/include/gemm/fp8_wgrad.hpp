@@ -17,6 +17,9 @@
 #include <hip/hip_runtime.h>
 #include <hip/hip_fp8.h>
 
+#include <algorithm>
+#include <type_traits>
+
 #include "utils.hpp"
 #include "mfma_utils.hpp"
 #include "scheduler.hpp"
@@ -30,6 +33,12 @@ struct WgradProblem {
     const int* offsets;                     // [groups + 1], or null: one group, all of K
     int m, n, k, ld_sa, ld_sb, groups;
     bool accumulate;
+};
+
+// Sums of K parts and the counters of their arrival, a counter a wave of every tile.
+struct WgradWorkspace {
+    float* sums;
+    unsigned* counters;
 };
 
 // K range of a group in k-tiles. Offsets are the caller's, on the device: whatever they hold, the range lies inside K.
@@ -52,10 +61,49 @@ __device__ __forceinline__ bf16x8 wgrad_decode(int lo, int hi, float scale) {
 // The scale of a k-tile out of the dword that holds those of four: `shift` is 8 times its place.
 __device__ __forceinline__ float wgrad_scale(int quad, int shift) { return __builtin_bit_cast(float, ((uint32_t(quad) >> shift) & 0xff) << 23); }
 
-template <int BLOCK_M, int BLOCK_N, int STAGES>
-__global__ void __launch_bounds__(256)
-fp8_wgrad_kernel(WgradProblem p) {
-    constexpr int NW = 4, WTM = BLOCK_M / 2, WTN = BLOCK_N / 2, TM = WTM / 32, TN = WTN / 32;
+// Four sums to memory. All of the offset is in the lane's register: of a store of 16 bytes whose offset is partly in a scalar register the compiler
+// thinks that its data may be overwritten by the next instruction. It may not: the second register of some lanes then held what came next.
+__device__ __forceinline__ void wgrad_store(f32x4 v, __amdgpu_buffer_rsrc_t rsrc, uint32_t offset, bool streaming) {
+    buffer_store_16(__builtin_bit_cast(i32x4, v), rsrc, offset, streaming);
+}
+
+// Where the `parts` parts of a tile's K range meet, wave by wave, as in the other GEMMs (meet_partials in tile_io.hpp) with their number known at run
+// time: a wave leaves its sums, and the one that comes last adds up all parts in the order of their ranges. True for that one. Written and read
+// at device scope: the parts run on different XCDs. The counters are zero before and after.
+template <int NW, int TN, int TM>
+__device__ __forceinline__ bool wgrad_meet(f32x4 (&acc)[TN][TM], const WgradWorkspace& w, int tile, int part, int parts, int wave, int lane) {
+    constexpr int kDeviceScope = 16, VECS = TN * TM;
+    constexpr uint32_t VEC_BYTES = kWaveSize * 16, WAVE_BYTES = VECS * VEC_BYTES, PART_BYTES = NW * WAVE_BYTES;
+    const __amdgpu_buffer_rsrc_t sums = make_rsrc(w.sums + size_t(tile) * parts * (PART_BYTES / 4), uint32_t(parts) * PART_BYTES);
+    const uint32_t at = uint32_t(wave) * WAVE_BYTES + lane * 16;
+#pragma unroll
+    for (int v = 0; v < VECS; ++v)
+        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(i32x4, acc[v / TM][v % TM]), sums, at + part * PART_BYTES + v * VEC_BYTES, 0, kDeviceScope);
+    __builtin_amdgcn_s_waitcnt(waitcnt_imm(0, kNoWaitLgkm));            // the sums have reached memory before the count is taken
+    asm volatile("" ::: "memory");
+    unsigned before = 0;
+    unsigned* const counter = w.counters + tile * NW + wave;
+    if (lane == 0) before = __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    before = __builtin_amdgcn_readfirstlane(before);
+    asm volatile("" ::: "memory");
+    if (before != unsigned(parts) - 1) return false;
+#pragma unroll
+    for (int v = 0; v < VECS; ++v) acc[v / TM][v % TM] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+    for (int s = 0; s < parts; ++s)
+#pragma unroll
+        for (int v = 0; v < VECS; ++v)
+            acc[v / TM][v % TM] += __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(sums, at + s * PART_BYTES + v * VEC_BYTES, 0, kDeviceScope));
+    if (lane == 0) __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    return true;
+}
+
+// The smaller tiles: 4 waves, two workgroups a compute unit, which hide each other's waits; one tile a workgroup, or a walk under a cap. SPLIT: a slot
+// is one of `parts` parts of a tile's K range.
+template <int BLOCK_M, int BLOCK_N, int STAGES, bool SPLIT>
+__global__ void __launch_bounds__(256, 2)
+fp8_wgrad_kernel(WgradProblem p, WgradWorkspace w, int parts) {
+    constexpr int NW = 4, WTM = BLOCK_M / 2, WTN = BLOCK_N / 2, TM = WTM / 16, TN = WTN / 16;
     using StA = TileStager<BLOCK_M, NW>;
     using StB = TileStager<BLOCK_N, NW>;
     constexpr int NUM_COPIES = StA::PASSES + StB::PASSES, A_BYTES = BLOCK_M * kRowBytes, STAGE_BYTES = (BLOCK_M + BLOCK_N) * kRowBytes;
@@ -63,127 +111,520 @@ fp8_wgrad_kernel(WgradProblem p) {
     __shared__ __attribute__((aligned(1024))) uint8_t ring[STAGES * STAGE_BYTES];
 
     const XcdTileScheduler<> sched(p.m, p.n, BLOCK_M, BLOCK_N);
-    const int slots = sched.grid_size(), group = blockIdx.x / slots;
-    const TileCoord tile = sched.tile_of(blockIdx.x % slots);
-    if (!tile.valid) return;
-    const int m0 = tile.m_idx * BLOCK_M, n0 = tile.n_idx * BLOCK_N;
-    int lo, hi;
-    wgrad_range(p, group, lo, hi);
-    if (p.accumulate && lo == hi) return;
-
+    const int per_group = sched.grid_size(), slots = per_group * p.groups * (SPLIT ? parts : 1);
     const int lane = get_lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWaveSize);
-    const int wn = wave % 2, wm = wave / 2, g = lane / 32, row = lane % 32;
-    // descriptors start at the tile and at the group's first column, so that 32-bit offsets reach whatever the operands' sizes
-    const int rows_a = min(BLOCK_M, p.m - m0), rows_b = min(BLOCK_N, p.n - n0);
-    const __amdgpu_buffer_rsrc_t rsrc_a = make_rsrc(p.a + size_t(m0) * p.k + size_t(lo) * 128, uint32_t(rows_a) * p.k - uint32_t(lo) * 128);
-    const __amdgpu_buffer_rsrc_t rsrc_b = make_rsrc(p.b + size_t(n0) * p.k + size_t(lo) * 128, uint32_t(rows_b) * p.k - uint32_t(lo) * 128);
-    const __amdgpu_buffer_rsrc_t rsrc_none = make_rsrc(p.a, 0);
-    const __amdgpu_buffer_rsrc_t rsrc_sa = make_rsrc(p.sa + size_t(m0) * p.ld_sa, uint32_t(rows_a) * p.ld_sa);
-    const __amdgpu_buffer_rsrc_t rsrc_sb = make_rsrc(p.sb + size_t(n0) * p.ld_sb, uint32_t(rows_b) * p.ld_sb);
+    const int wn = wave % 2, wm = wave / 2, g = lane / 16, col = lane % 16;
+    for (int slot = blockIdx.x; slot < slots; slot += gridDim.x) {
+        // the parts of a tile are neighbouring slots
+        const int part = SPLIT ? slot % parts : 0, tile_slot = SPLIT ? slot / parts : slot, group = tile_slot / per_group;
+        const TileCoord tile = sched.tile_of(tile_slot - group * per_group);
+        if (!tile.valid) continue;
+        const int m0 = tile.m_idx * BLOCK_M, n0 = tile.n_idx * BLOCK_N;
+        int lo, hi;
+        wgrad_range(p, group, lo, hi);
+        if (p.accumulate && lo == hi) continue;
+        if constexpr (SPLIT) {
+            const int share = ceil_div(hi - lo, parts), end = hi;
+            lo = min(lo + part * share, end);
+            hi = min(lo + share, end);
+        }
+        // the ring is used again: everybody is out of it
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+
+        // descriptors start at the tile and at the range's first column, so that 32-bit offsets reach whatever the operands' sizes
+        const int rows_a = min(BLOCK_M, p.m - m0), rows_b = min(BLOCK_N, p.n - n0);
+        const __amdgpu_buffer_rsrc_t rsrc_a = make_rsrc(p.a + size_t(m0) * p.k + size_t(lo) * 128, uint32_t(rows_a) * p.k - uint32_t(lo) * 128);
+        const __amdgpu_buffer_rsrc_t rsrc_b = make_rsrc(p.b + size_t(n0) * p.k + size_t(lo) * 128, uint32_t(rows_b) * p.k - uint32_t(lo) * 128);
+        const __amdgpu_buffer_rsrc_t rsrc_sa = make_rsrc(p.sa + size_t(m0) * p.ld_sa, uint32_t(rows_a) * p.ld_sa);
+        const __amdgpu_buffer_rsrc_t rsrc_sb = make_rsrc(p.sb + size_t(n0) * p.ld_sb, uint32_t(rows_b) * p.ld_sb);
+        StA stage_a;
+        StB stage_b;
+        stage_a.init(0, p.k, wave, lane);
+        stage_b.init(0, p.k, wave, lane);
+        const int count = hi - lo;
+        // (a copy of nothing, out of range, may still write its zeros when it has been counted as done: none is issued, the ring is used again below)
+        auto copy = [&](int kt, uint8_t* stage) {
+            if (kt >= count) return;
+            stage_a.issue(rsrc_a, stage, kt * kRowBytes, wave);
+            stage_b.issue(rsrc_b, stage + A_BYTES, kt * kRowBytes, wave);
+        };
+        // a lane reads chunks 2 g and 2 g + 1 of its row, sixteen codes each for two 16x16x32 MFMAs
+        const int off[2] = {frag_offset<16>(lane, 2 * g), frag_offset<16>(lane, 2 * g + 1)};
+
+        f32x4 acc[TN][TM];
+#pragma unroll
+        for (int i = 0; i < TN; ++i)
+#pragma unroll
+            for (int j = 0; j < TM; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+        for (int t = 0; t < STAGES - 1; ++t) copy(t, ring + t * STAGE_BYTES);
+        int st = 0, quad_a[TM], quad_b[TN];
+        for (int kt = 0; kt < count; ++kt) {
+            const int at = lo + kt;
+            if (kt == 0 || at % 4 == 0) {
+#pragma unroll
+                for (int j = 0; j < TM; ++j) quad_a[j] = __builtin_amdgcn_raw_buffer_load_b32(rsrc_sa, uint32_t(wm * WTM + j * 16 + col) * p.ld_sa, at & ~3, 0);
+#pragma unroll
+                for (int i = 0; i < TN; ++i) quad_b[i] = __builtin_amdgcn_raw_buffer_load_b32(rsrc_sb, uint32_t(wn * WTN + i * 16 + col) * p.ld_sb, at & ~3, 0);
+            }
+            // the copies behind this k-tile's are those of STAGES - 2 k-tiles, until the range ends
+            if (STAGES > 2 && kt + STAGES - 2 < count) __builtin_amdgcn_s_waitcnt(waitcnt_imm((STAGES - 2) * NUM_COPIES, 0));
+            else __builtin_amdgcn_s_waitcnt(waitcnt_imm(0, 0));
+            asm volatile("" ::: "memory");
+            __builtin_amdgcn_s_barrier();
+            asm volatile("" ::: "memory");
+            copy(kt + STAGES - 1, ring + (st == 0 ? STAGES - 1 : st - 1) * STAGE_BYTES);
+            const uint8_t* pa = ring + st * STAGE_BYTES + wm * WTM * kRowBytes;
+            const uint8_t* pb = ring + st * STAGE_BYTES + A_BYTES + wn * WTN * kRowBytes;
+            const int shift = at % 4 * 8;
+            float scale_a[TM], scale_b[TN];
+#pragma unroll
+            for (int j = 0; j < TM; ++j) scale_a[j] = wgrad_scale(quad_a[j], shift);
+#pragma unroll
+            for (int i = 0; i < TN; ++i) scale_b[i] = wgrad_scale(quad_b[i], shift);
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                i32x4 raw_a[TM], raw_b[TN];
+#pragma unroll
+                for (int j = 0; j < TM; ++j) raw_a[j] = *reinterpret_cast<const i32x4*>(pa + j * 16 * kRowBytes + off[c]);
+#pragma unroll
+                for (int i = 0; i < TN; ++i) raw_b[i] = *reinterpret_cast<const i32x4*>(pb + i * 16 * kRowBytes + off[c]);
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    bf16x8 fa[TM], fb[TN];
+#pragma unroll
+                    for (int j = 0; j < TM; ++j) fa[j] = wgrad_decode(raw_a[j][2 * h], raw_a[j][2 * h + 1], scale_a[j]);
+#pragma unroll
+                    for (int i = 0; i < TN; ++i) fb[i] = wgrad_decode(raw_b[i][2 * h], raw_b[i][2 * h + 1], scale_b[i]);
+#pragma unroll
+                    for (int i = 0; i < TN; ++i)
+#pragma unroll
+                        for (int j = 0; j < TM; ++j) acc[i][j] = MfmaBF16_16x16x32::mma(fb[i], fa[j], acc[i][j]);
+                }
+            }
+            st = st + 1 == STAGES ? 0 : st + 1;
+        }
+
+        // The 4 registers of atom (i, j) are columns 16 i + 4 g + {0..3} of row 16 j + col of the slab. Stored from there an instruction covers 16 rows by 64
+        // bytes, half lines, which the memory takes at 3.2 to 4.8 TB/s; a wave turns its slab round through LDS and stores whole lines. Chunk c (16
+        // bytes) of a row sits in slot c ^ row, so that neither side meets a bank twice.
+        __builtin_amdgcn_s_waitcnt(waitcnt_imm(kNoWaitVm, 0));          // every wave has read the last k-tile
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        if (SPLIT && !wgrad_meet<NW>(acc, w, tile_slot, part, parts, wave, lane)) continue;
+        constexpr int LANES_PER_ROW = WTN / 4, ROWS_PER_STORE = kWaveSize / LANES_PER_ROW, STORES = WTM / ROWS_PER_STORE;
+        static_assert(NW * WTM * WTN * 4 <= STAGES * STAGE_BYTES && kWaveSize % LANES_PER_ROW == 0);
+        uint8_t* const region = ring + wave * (WTM * WTN * 4);
+        const auto place = [](int row, int chunk) { return row * (WTN * 4) + ((chunk ^ (row & (LANES_PER_ROW - 1))) * 16); };
+        const int row_in = lane / LANES_PER_ROW, chunk = lane % LANES_PER_ROW;
+        const bool stream_out = size_t(p.groups) * p.m * p.n * 4 > (size_t(32) << 20);
+        const uint32_t row_bytes = uint32_t(p.n) * 4;
+        const __amdgpu_buffer_rsrc_t rsrc_out = make_rsrc(p.out + (size_t(group) * p.m + m0) * p.n + n0, uint32_t(rows_a) * row_bytes - uint32_t(n0) * 4);
+        const int c0 = wn * WTN + 4 * chunk;
+        const uint32_t to = n0 + c0 < p.n ? uint32_t(wm * WTM + row_in) * row_bytes + uint32_t(c0) * 4 : kOutOfRange;
+        i32x4 held[STORES];
+        if (p.accumulate) {
+#pragma unroll
+            for (int u = 0; u < STORES; ++u) held[u] = __builtin_amdgcn_raw_buffer_load_b128(rsrc_out, to, u * ROWS_PER_STORE * row_bytes, 0);
+        }
+#pragma unroll
+        for (int j = 0; j < TM; ++j)
+#pragma unroll
+            for (int i = 0; i < TN; ++i) *reinterpret_cast<f32x4*>(region + place(16 * j + col, 4 * i + g)) = acc[i][j];
+#pragma unroll
+        for (int u = 0; u < STORES; ++u) {
+            f32x4 v = *reinterpret_cast<const f32x4*>(region + place(u * ROWS_PER_STORE + row_in, chunk));
+            if (p.accumulate) v += __builtin_bit_cast(f32x4, held[u]);
+            wgrad_store(v, rsrc_out, to + u * ROWS_PER_STORE * row_bytes, stream_out);
+        }
+    }
+}
+
+// The large tile: 256 x BLOCK_N on 4 waves, one per SIMD, each with a 128 x BLOCK_N / 2 slab of 16x16x32 MFMAs, its sums in the accumulation registers.
+// A k-tile of 128 is four steps of 32; a step is TN rows of 8 MFMAs. A lone wave has nobody to hide behind, so everything else it issues stands in
+// the shadow of an MFMA:
+//   * a lane reads 16 codes of a row at a time, which are two steps: activation fragments are decoded one step ahead of their MFMAs (`mf`, two
+//     buffers), weight fragments one row ahead (`nf`), one or two conversions behind every MFMA. The registers of the codes are read again as soon
+//     as their second half is decoded, 7 rows or more before the next use;
+//   * LDS holds two k-tiles. In the middle of k-tile t every wave has read all of t, and t + 1 has to have landed: one barrier a k-tile, in whose wake
+//     the copies of t + 2 go out into the half that t leaves, one a row, with two steps to land after the last of them;
+//   * scale bytes come as dwords of four k-tiles, loaded while the last k-tile that needs the old ones is under way, and become floats in the last
+//     step of a k-tile, each where the next one's first fragment needs it;
+//   * the walk is persistent (one workgroup per compute unit), and the stream of k-tiles does not stop at the end of a tile: the copies, scales and
+//     first fragments of the next tile are under way when the sums of this one are stored.
+// 64-bit bases per tile, 32-bit offsets inside.
+struct WgradTile {
+    int slot, group, m0, n0, lo, count;
+};
+
+template <int BLOCK_N>
+__global__ void __launch_bounds__(256, 1)
+fp8_wgrad_tall_kernel(WgradProblem p) {
+    constexpr int BLOCK_M = 256, NW = 4, TM = 8, TN = BLOCK_N / 32, WTM = 128, WTN = BLOCK_N / 2;
+    static_assert(BLOCK_N % 128 == 0 && TN >= 4 && TN <= 8);
+    using StA = TileStager<BLOCK_M, NW>;
+    using StB = TileStager<BLOCK_N, NW>;
+    static_assert(StA::PADDED_ROWS == BLOCK_M && StB::PADDED_ROWS == BLOCK_N);
+    constexpr int A_BYTES = BLOCK_M * kRowBytes, STAGE_BYTES = (BLOCK_M + BLOCK_N) * kRowBytes, PASSES = StA::PASSES + StB::PASSES;
+    static_assert(PASSES <= 2 * TN);            // one copy a row of the two steps behind the barrier
+    // the sums leave through pieces of 16 rows by PIECE columns, two a wave
+    constexpr int PIECE = 64, PIECE_BYTES = 16 * PIECE * 4, PIECES_PER_ROW = WTN / PIECE, PIECES = TM * PIECES_PER_ROW;
+    constexpr int LANES_PER_ROW = PIECE / 4, ROWS_PER_STORE = kWaveSize / LANES_PER_ROW, PIECE_STORES = 16 / ROWS_PER_STORE;
+    static_assert(WTN % PIECE == 0 && 2 * STAGE_BYTES + NW * 2 * PIECE_BYTES <= 160 * 1024);
+    __shared__ __attribute__((aligned(1024))) uint8_t stages[2 * STAGE_BYTES + NW * 2 * PIECE_BYTES];
+    uint8_t* const turn = stages + 2 * STAGE_BYTES;
+
+    const XcdTileScheduler<> sched(p.m, p.n, BLOCK_M, BLOCK_N);
+    const int per_group = sched.grid_size(), slots = per_group * p.groups;
+    const int lane = get_lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWaveSize);
+    const int wn = wave % 2, wm = wave / 2, g = lane / 16, col = lane % 16;
+
+    auto tile_at = [&](int slot) {
+        WgradTile t{slot, 0, 0, 0, 0, 0};
+        t.group = slot / per_group;
+        const TileCoord c = sched.tile_of(slot - t.group * per_group);
+        if (!c.valid) { t.count = -1; return t; }
+        t.m0 = c.m_idx * BLOCK_M, t.n0 = c.n_idx * BLOCK_N;
+        int hi;
+        wgrad_range(p, t.group, t.lo, hi);
+        t.count = hi - t.lo;
+        return t;
+    };
+    // the next slot of this workgroup's walk, from `slot` on, whose tile has something to add up; count 0: the walk ends
+    auto seek = [&](int slot) {
+        for (; slot < slots; slot += gridDim.x) {
+            const WgradTile t = tile_at(slot);
+            if (t.count > 0) return t;
+        }
+        return WgradTile{slots, 0, 0, 0, 0, 0};
+    };
+    // the tiles of groups without columns
+    if (p.offsets && !p.accumulate)
+        for (int slot = blockIdx.x; slot < slots; slot += gridDim.x) {
+            const WgradTile t = tile_at(slot);
+            if (t.count != 0) continue;
+            for (int r = wave; r < min(BLOCK_M, p.m - t.m0); r += NW) {
+                float* const line = p.out + (size_t(t.group) * p.m + t.m0 + r) * p.n + t.n0;
+                for (int c = 4 * lane; c < min(BLOCK_N, p.n - t.n0); c += 4 * kWaveSize) *reinterpret_cast<f32x4*>(line + c) = f32x4{0.f, 0.f, 0.f, 0.f};
+            }
+        }
+
     StA stage_a;
     StB stage_b;
     stage_a.init(0, p.k, wave, lane);
     stage_b.init(0, p.k, wave, lane);
-    const int count = hi - lo;
-    auto copy = [&](int kt, uint8_t* stage) {
-        const bool live = kt < count;
-        stage_a.issue(live ? rsrc_a : rsrc_none, stage, kt * kRowBytes, wave);
-        stage_b.issue(live ? rsrc_b : rsrc_none, stage + A_BYTES, kt * kRowBytes, wave);
+    const int koff[2] = {frag_offset<16>(lane, 2 * g), frag_offset<16>(lane, 2 * g + 1)};
+    const int a_lane = wm * WTM * kRowBytes, b_lane = A_BYTES + wn * WTN * kRowBytes;
+
+    // What the copies read: k-tile `copy_kt` of `copy_tile`
+    WgradTile copy_tile = seek(blockIdx.x);
+    if (copy_tile.count == 0) return;
+    WgradTile cur = copy_tile;
+    int copy_kt = 0;
+    __amdgpu_buffer_rsrc_t rsrc_a, rsrc_b;
+    auto aim_copies = [&] {
+        const WgradTile& t = copy_tile;
+        const int rows_a = t.count ? min(BLOCK_M, p.m - t.m0) : 0, rows_b = t.count ? min(BLOCK_N, p.n - t.n0) : 0;
+        rsrc_a = make_rsrc(p.a + size_t(t.m0) * p.k + size_t(t.lo) * 128, rows_a ? uint32_t(rows_a) * p.k - uint32_t(t.lo) * 128 : 0);
+        rsrc_b = make_rsrc(p.b + size_t(t.n0) * p.k + size_t(t.lo) * 128, rows_b ? uint32_t(rows_b) * p.k - uint32_t(t.lo) * 128 : 0);
     };
-    // a lane reads chunks 2 c + g of its row, c = 0 .. 3: eight codes each for two 32x32x16 MFMAs
-    int off[4];
+    auto advance_copies = [&] {
+        if (++copy_kt < copy_tile.count) return;
+        copy_kt = 0;
+        if (copy_tile.count) copy_tile = seek(copy_tile.slot + gridDim.x);
+        aim_copies();           // behind the last tile: descriptors of nothing
+    };
+    auto copy = [&](int d, int stage) __attribute__((always_inline)) {
+        if (d < StA::PASSES) stage_a.issue_pass(rsrc_a, stages + stage, copy_kt * kRowBytes, wave, d);
+        else stage_b.issue_pass(rsrc_b, stages + stage + A_BYTES, copy_kt * kRowBytes, wave, d - StA::PASSES);
+    };
+    // the dwords with the scales of k-tile `at` (counted from the start of K) of tile `t`
+    int quad_a[TM], quad_b[TN];
+    float sa[TM], sb[TN];
+    auto load_scales = [&](const WgradTile& t, int at) __attribute__((always_inline)) {
+        const int rows_a = t.count ? min(BLOCK_M, p.m - t.m0) : 0, rows_b = t.count ? min(BLOCK_N, p.n - t.n0) : 0;
+        const __amdgpu_buffer_rsrc_t rsrc_sa = make_rsrc(p.sa + size_t(t.m0) * p.ld_sa, uint32_t(rows_a) * p.ld_sa);
+        const __amdgpu_buffer_rsrc_t rsrc_sb = make_rsrc(p.sb + size_t(t.n0) * p.ld_sb, uint32_t(rows_b) * p.ld_sb);
 #pragma unroll
-    for (int c = 0; c < 4; ++c) off[c] = frag_offset<32>(lane, 2 * c + g);
+        for (int j = 0; j < TM; ++j) quad_a[j] = __builtin_amdgcn_raw_buffer_load_b32(rsrc_sa, uint32_t(wm * WTM + col) * p.ld_sa, (at & ~3) + j * 16 * p.ld_sa, 0);
+#pragma unroll
+        for (int i = 0; i < TN; ++i) quad_b[i] = __builtin_amdgcn_raw_buffer_load_b32(rsrc_sb, uint32_t(wn * WTN + col) * p.ld_sb, (at & ~3) + i * 16 * p.ld_sb, 0);
+    };
 
-    f32x16 acc[TN][TM];
-#pragma unroll
-    for (int i = 0; i < TN; ++i)
-#pragma unroll
-        for (int j = 0; j < TM; ++j)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
+    f32x4 acc[TN][TM];
+    i32x4 raw_m[TM], raw_n[TN], mf[2][TM], nf[2];
+    typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+    // two codes; the empty asm keeps the conversion where it stands (the compiler would move it down to its use, in front of the MFMA)
+    auto decode = [](int codes, float scale, bool upper) __attribute__((always_inline)) {
+        int two = __builtin_bit_cast(int, upper ? __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(uint32_t(codes), scale, true)
+                                                : __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(uint32_t(codes), scale, false));
+        asm volatile("" : "+v"(two));
+        return two;
+    };
+    auto mma = [&](auto first_c, int q, int i, int j) __attribute__((always_inline)) {
+        f32x4& sum = acc[i][j];
+        const i32x4 &n = nf[i & 1], &m = mf[q & 1][j];
+        if constexpr (decltype(first_c)::value) asm volatile("v_mfma_f32_16x16x32_bf16 %0, %1, %2, 0" : "=a"(sum) : "v"(n), "v"(m));
+        else asm volatile("v_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+a"(sum) : "v"(n), "v"(m));
+    };
+    auto read_m = [&](int j, int stage, int set) __attribute__((always_inline)) {
+        raw_m[j] = *reinterpret_cast<const i32x4*>(stages + stage + a_lane + j * 16 * kRowBytes + koff[set]);
+    };
+    auto read_n = [&](int i, int stage, int set) __attribute__((always_inline)) {
+        raw_n[i] = *reinterpret_cast<const i32x4*>(stages + stage + b_lane + i * 16 * kRowBytes + koff[set]);
+    };
+    auto float_scale = [](int quad, int shift) __attribute__((always_inline)) {
+        float scale = wgrad_scale(quad, shift);
+        asm volatile("" : "+v"(scale));
+        return scale;
+    };
 
-    for (int t = 0; t < STAGES - 1; ++t) copy(t, ring + t * STAGE_BYTES);
-    int st = 0, quad_a[TM], quad_b[TN];
-    for (int kt = 0; kt < count; ++kt) {
-        const int at = lo + kt;
-        if (kt == 0 || at % 4 == 0) {
+    // Step Q of the k-tile staged at `here`; the next one is staged at `there`, its scales are in the dwords at bit `shift`. FIRST: the sums start here.
+    auto step = [&](auto first_c, auto q_c, int here, int there, int shift) __attribute__((always_inline)) {
+        constexpr int Q = decltype(q_c)::value;
+        constexpr bool EVEN = Q % 2 == 0;
+        // the codes read in steps 0 and 1 are the second set of this k-tile, in steps 2 and 3 the first set of the next
+        const int from = Q < 2 ? here : there;
+        constexpr int SET = Q < 2 ? 1 : 0;
+        // the next step's fragments lie in the half of their 16 codes that its number says
+        constexpr int M_HALF = (Q + 1) % 2;
 #pragma unroll
-            for (int j = 0; j < TM; ++j) quad_a[j] = __builtin_amdgcn_raw_buffer_load_b32(rsrc_sa, uint32_t(wm * WTM + j * 32 + row) * p.ld_sa, at & ~3, 0);
+        for (int i = 0; i < TN; ++i) {
+            const int next = i + 1 < TN ? i + 1 : 0, n_half = i + 1 < TN ? Q % 2 : M_HALF;      // weight row decoded behind this one's MFMAs
+            const bool more = i + TN < TM;                                                      // fewer rows than activation fragments: two in one row
 #pragma unroll
-            for (int i = 0; i < TN; ++i) quad_b[i] = __builtin_amdgcn_raw_buffer_load_b32(rsrc_sb, uint32_t(wn * WTN + i * 32 + row) * p.ld_sb, at & ~3, 0);
-        }
-        // every wave has as many copies under way: at most those of the STAGES - 2 k-tiles behind this one are left out here
-        __builtin_amdgcn_s_waitcnt(waitcnt_imm((STAGES - 2) * NUM_COPIES, 0));
-        asm volatile("" ::: "memory");
-        __builtin_amdgcn_s_barrier();
-        asm volatile("" ::: "memory");
-        copy(kt + STAGES - 1, ring + (st == 0 ? STAGES - 1 : st - 1) * STAGE_BYTES);
-        const uint8_t* pa = ring + st * STAGE_BYTES + wm * WTM * kRowBytes;
-        const uint8_t* pb = ring + st * STAGE_BYTES + A_BYTES + wn * WTN * kRowBytes;
-        const int shift = at % 4 * 8;
-        float scale_a[TM], scale_b[TN];
-#pragma unroll
-        for (int j = 0; j < TM; ++j) scale_a[j] = wgrad_scale(quad_a[j], shift);
-#pragma unroll
-        for (int i = 0; i < TN; ++i) scale_b[i] = wgrad_scale(quad_b[i], shift);
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-            i32x4 raw_a[TM], raw_b[TN];
-#pragma unroll
-            for (int j = 0; j < TM; ++j) raw_a[j] = *reinterpret_cast<const i32x4*>(pa + j * 32 * kRowBytes + off[c]);
-#pragma unroll
-            for (int i = 0; i < TN; ++i) raw_b[i] = *reinterpret_cast<const i32x4*>(pb + i * 32 * kRowBytes + off[c]);
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                bf16x8 fa[TM], fb[TN];
-#pragma unroll
-                for (int j = 0; j < TM; ++j) fa[j] = wgrad_decode(raw_a[j][2 * h], raw_a[j][2 * h + 1], scale_a[j]);
-#pragma unroll
-                for (int i = 0; i < TN; ++i) fb[i] = wgrad_decode(raw_b[i][2 * h], raw_b[i][2 * h + 1], scale_b[i]);
-#pragma unroll
-                for (int i = 0; i < TN; ++i)
-#pragma unroll
-                    for (int j = 0; j < TM; ++j) acc[i][j] = MfmaBF16_32x32x16::mma(fb[i], fa[j], acc[i][j]);
+            for (int j = 0; j < TM; ++j) {
+                mma(first_c, Q, i, j);
+                if (j < 4) {
+                    nf[next & 1][j] = decode(raw_n[next][2 * n_half + j / 2], sb[next], j % 2);
+                    if (more) mf[M_HALF][(i + TN) % TM][j] = decode(raw_m[(i + TN) % TM][2 * M_HALF + j / 2], sa[(i + TN) % TM], j % 2);
+                } else {
+                    mf[M_HALF][i][j - 4] = decode(raw_m[i][2 * M_HALF + (j - 4) / 2], sa[i], j % 2);
+                }
+                if (EVEN && j == 1 && i > 0) {          // both halves of these are decoded
+                    read_m(i - 1, from, SET);
+                    if (i - 1 + TN < TM) read_m((i - 1 + TN) % TM, from, SET);
+                }
+                if (!EVEN && j == 2 && i == 0) read_m(TN - 1, from, SET);
+                if (!EVEN && j == 1) read_n(i, from, SET);
+                if (Q >= 2 && j == 5 && (Q - 2) * TN + i < PASSES) copy((Q - 2) * TN + i, here);
+                if (Q == 2 && j == 3 && 2 * TN + i < PASSES) copy(2 * TN + i, here);
+                if (Q == 2 && j == 6 && more) sa[(i + TN) % TM] = float_scale(quad_a[(i + TN) % TM], shift);
+                if (Q == 3 && j == 3) sa[i] = float_scale(quad_a[i], shift);
+                if (Q == 3 && j == 6) sb[i] = float_scale(quad_b[i], shift);
+                __builtin_amdgcn_sched_barrier(0);
             }
         }
-        st = st + 1 == STAGES ? 0 : st + 1;
+    };
+    using Q0 = std::integral_constant<int, 0>;
+    using Q1 = std::integral_constant<int, 1>;
+    using Q2 = std::integral_constant<int, 2>;
+    using Q3 = std::integral_constant<int, 3>;
+    constexpr int STORES = PIECES * PIECE_STORES;       // of a tile, by every wave, whatever of it exists
+
+    // the first two k-tiles of the walk, the scales and first fragments of the first
+    aim_copies();
+    for (int s = 0; s < 2; ++s) {
+        for (int d = 0; d < StA::PASSES; ++d) copy(d, s * STAGE_BYTES);
+        for (int d = 0; d < StB::PASSES; ++d) copy(StA::PASSES + d, s * STAGE_BYTES);
+        advance_copies();
     }
+    load_scales(cur, cur.lo);
+    {
+        const int shift = cur.lo % 4 * 8;
+#pragma unroll
+        for (int j = 0; j < TM; ++j) sa[j] = float_scale(quad_a[j], shift);
+#pragma unroll
+        for (int i = 0; i < TN; ++i) sb[i] = float_scale(quad_b[i], shift);
+    }
+    __builtin_amdgcn_s_waitcnt(waitcnt_imm(0, 0));
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+#pragma unroll
+    for (int j = 0; j < TM; ++j) read_m(j, 0, 0);
+#pragma unroll
+    for (int i = 0; i < TN; ++i) read_n(i, 0, 0);
+#pragma unroll
+    for (int j = 0; j < TM; ++j)
+#pragma unroll
+        for (int w = 0; w < 4; ++w) mf[0][j][w] = decode(raw_m[j][w / 2], sa[j], w % 2);
+#pragma unroll
+    for (int w = 0; w < 4; ++w) nf[0][w] = decode(raw_n[0][w / 2], sb[0], w % 2);
+    __builtin_amdgcn_sched_barrier(0);
 
-    // registers 4 q .. 4 q + 3 of atom (i, j): columns 8 q + 4 g + {0..3} of row `row`
+    const bool stream_out = size_t(p.groups) * p.m * p.n * 4 > (size_t(32) << 20);
+    const uint32_t row_bytes = uint32_t(p.n) * 4;
+    int here = 0;
+    while (true) {
+        const WgradTile nxt = seek(cur.slot + gridDim.x);
+        auto k_tile = [&](auto first_c, int kt) __attribute__((always_inline)) {
+            const bool last = kt + 1 == cur.count;
+            const int next_at = last ? nxt.lo : cur.lo + kt + 1, shift = next_at % 4 * 8, there = STAGE_BYTES - here;
+            if (last) load_scales(nxt, next_at);
+            else if (next_at % 4 == 0) load_scales(cur, next_at);
+            step(first_c, Q0{}, here, there, shift);
+            step(std::false_type{}, Q1{}, here, there, shift);
+            // k-tile t + 1 has landed, and every wave has read k-tile t. Behind the copies of t + 1 a wave has issued nothing, or, in a tile's
+            // first k-tile, the stores of the tile before, which need not be done.
+            __builtin_amdgcn_s_waitcnt(waitcnt_imm(decltype(first_c)::value ? (STORES < 63 ? STORES : 63) : 0, 0));
+            asm volatile("" ::: "memory");
+            __builtin_amdgcn_s_barrier();
+            asm volatile("" ::: "memory");
+            step(std::false_type{}, Q2{}, here, there, shift);
+            step(std::false_type{}, Q3{}, here, there, shift);
+            advance_copies();
+            here = there;
+        };
+        k_tile(std::true_type{}, 0);
+        for (int kt = 1; kt < cur.count; ++kt) k_tile(std::false_type{}, kt);
+        asm volatile("s_nop 15\n\ts_nop 15" ::: "memory");      // the last MFMAs retire before the sums are read
+
+        // The 4 registers of atom (i, j) are columns 16 i + 4 g + {0..3} of row 16 j + col of the slab. A wave turns it round through LDS of its own, 16
+        // rows by PIECE columns at a time and two such pieces in turn: the sums of piece u go in, piece u - 1 comes out as runs of whole lines,
+        // piece u - 2 is stored. Chunk c (16 bytes) of a row sits in slot c ^ row. Every wave issues all STORES stores, those outside of the output out
+        // of range.
+        auto epilogue = [&](auto policy_c, auto accumulate_c) __attribute__((always_inline)) {
+            constexpr bool ACCUMULATE = decltype(accumulate_c)::value;
+            constexpr int AHEAD = 2;            // pieces of what is added to that are under way
+            uint8_t* const buffers = turn + wave * (2 * PIECE_BYTES);
+            const __amdgpu_buffer_rsrc_t rsrc_out = make_rsrc(p.out + (size_t(cur.group) * p.m + cur.m0) * p.n + cur.n0,
+                                                              uint32_t(min(BLOCK_M, p.m - cur.m0)) * row_bytes - uint32_t(cur.n0) * 4);
+            const int row_in = lane / LANES_PER_ROW, chunk = lane % LANES_PER_ROW;
+            uint32_t off[PIECES_PER_ROW];
 #pragma unroll
-    for (int j = 0; j < TM; ++j) {
-        const int mm = m0 + wm * WTM + j * 32 + row;
-        if (mm >= p.m) continue;
-        float* const line = p.out + (size_t(group) * p.m + mm) * p.n;
-#pragma unroll
-        for (int i = 0; i < TN; ++i)
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                const int nn = n0 + wn * WTN + i * 32 + 8 * q + 4 * g;
-                if (nn >= p.n) continue;
-                f32x4 v = {acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
-                f32x4* const to = reinterpret_cast<f32x4*>(line + nn);
-                if (p.accumulate) v += *to;
-                *to = v;
+            for (int h = 0; h < PIECES_PER_ROW; ++h) {
+                const int c = wn * WTN + PIECE * h + 4 * chunk;
+                off[h] = cur.n0 + c < p.n ? uint32_t(wm * WTM + row_in) * row_bytes + uint32_t(c) * 4 : kOutOfRange;
             }
+            i32x4 back[2][PIECE_STORES], held[ACCUMULATE ? AHEAD + 1 : 1][PIECE_STORES];
+            auto load = [&](int u) __attribute__((always_inline)) {
+#pragma unroll
+                for (int s = 0; s < PIECE_STORES; ++s)
+                    held[u % (AHEAD + 1)][s] = __builtin_amdgcn_raw_buffer_load_b128(rsrc_out, off[u % PIECES_PER_ROW], (u / PIECES_PER_ROW * 16 + ROWS_PER_STORE * s) * row_bytes, 0);
+            };
+            if constexpr (ACCUMULATE) {
+#pragma unroll
+                for (int u = 0; u < AHEAD; ++u) load(u);
+            }
+#pragma unroll
+            for (int u = 0; u < PIECES + 2; ++u) {
+                if (u < PIECES) {
+                    const int j = u / PIECES_PER_ROW, h = u % PIECES_PER_ROW;
+#pragma unroll
+                    for (int a = 0; a < PIECE / 16; ++a) {
+                        const f32x4& sum = acc[h * (PIECE / 16) + a][j];
+                        f32x4 v;
+                        asm volatile("v_accvgpr_read_b32 %0, %1" : "=v"(v[0]) : "a"(sum[0]));
+                        asm volatile("v_accvgpr_read_b32 %0, %1" : "=v"(v[1]) : "a"(sum[1]));
+                        asm volatile("v_accvgpr_read_b32 %0, %1" : "=v"(v[2]) : "a"(sum[2]));
+                        asm volatile("v_accvgpr_read_b32 %0, %1" : "=v"(v[3]) : "a"(sum[3]));
+                        *reinterpret_cast<f32x4*>(buffers + (u & 1) * PIECE_BYTES + col * (PIECE * 4) + (((4 * a + g) ^ (col & (LANES_PER_ROW - 1))) * 16)) = v;
+                    }
+                }
+                __builtin_amdgcn_sched_barrier(0);
+                if (u >= 1 && u - 1 < PIECES) {
+#pragma unroll
+                    for (int s = 0; s < PIECE_STORES; ++s) {
+                        const int row = ROWS_PER_STORE * s + row_in;
+                        back[(u - 1) & 1][s] = *reinterpret_cast<const i32x4*>(buffers + ((u - 1) & 1) * PIECE_BYTES + row * (PIECE * 4) + ((chunk ^ (row & (LANES_PER_ROW - 1))) * 16));
+                    }
+                }
+                if (u >= 2) {
+                    const int w = u - 2;
+                    if constexpr (ACCUMULATE) {
+                        if (w + AHEAD < PIECES) load(w + AHEAD);
+                    }
+#pragma unroll
+                    for (int s = 0; s < PIECE_STORES; ++s) {
+                        f32x4 v = __builtin_bit_cast(f32x4, back[w & 1][s]);
+                        if constexpr (ACCUMULATE) v += __builtin_bit_cast(f32x4, held[w % (AHEAD + 1)][s]);
+                        wgrad_store(v, rsrc_out, off[w % PIECES_PER_ROW] + (w / PIECES_PER_ROW * 16 + ROWS_PER_STORE * s) * row_bytes, decltype(policy_c)::value);
+                    }
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        };
+        using Kept = std::false_type;
+        using Streamed = std::true_type;
+        if (p.accumulate) {
+            if (stream_out) epilogue(Streamed{}, std::true_type{});
+            else epilogue(Kept{}, std::true_type{});
+        } else {
+            if (stream_out) epilogue(Streamed{}, std::false_type{});
+            else epilogue(Kept{}, std::false_type{});
+        }
+        if (nxt.count == 0) break;
+        cur = nxt;
     }
 }
 
+// Which kernel a problem runs on, and in how many parts its K ranges. Measured over 220 shapes (us):
+//   * up to two 64 x 64 tiles a compute unit run those (44 k-tiles, 348 of them: 41.5, 128 x 128 55.4; 539 of them, 67 k-tiles: 112, 128 x 128 85), and
+//     in 2, 4 or 8 parts as long as that leaves two parts a compute unit or less and a part 8 k-tiles (8 tiles of 199 k-tiles: 121.7 whole, 65.6, 41.3 and
+//     31.7 in 2, 4 and 8, 31.8 in 16; 56 tiles of 39: 26.7 whole, 15.7 in 4, 21.1 in 8);
+//   * between the other two goes an estimate in us of rounds over the chip times a k-tile of the tile, 2.6 for 256 x 256, 1.7 for two of 128 x 128 on a
+//     compute unit, and what storing it takes. 448 large tiles of 128 k-tiles 692 against 868; 420 of 33 188 / 215; 192 of 60 155 / 173; 104 of 38
+//     94.6 / 75.8; 7168 of 2.5 398 / 459, accumulated 835 / 776. The smaller tile is kept where the two are within 5 %, which is where the output's
+//     traffic decides (1725 of 1 192 / 150).
+enum WgradKernel { kWgradAny, kWgradTall, kWgrad128, kWgrad64, kWgradSplit };
+struct WgradPlan {
+    WgradKernel kernel;
+    int parts;
+};
+constexpr long long kWgradMostParts = (kSplitKWorkspaceBytes - kSplitKCounterBytes) / (64 * 64 * 4);        // what a workspace holds, sums and counters
+static_assert(kWgradMostParts * 4 * 4 <= (long long)kSplitKCounterBytes);
+inline WgradPlan wgrad_plan(int m, int n, int k, int groups, bool accumulate, int num_cus, bool may_split) {
+    const auto tiles = [&](int block) { return (long long)ceil_div(m, block) * ceil_div(n, block) * groups; };
+    const double k_tiles = double(k / 128) / groups;
+    if (tiles(64) <= 2ll * num_cus) {
+        const long long slots = (long long)XcdTileScheduler<>(m, n, 64, 64).grid_size() * groups;
+        for (int parts = 8; may_split && parts > 1; parts /= 2)
+            if (tiles(64) * parts <= 2ll * num_cus && k_tiles >= 8 * parts && slots * parts <= kWgradMostParts) return {kWgradSplit, parts};
+        return {kWgrad64, 1};
+    }
+    const double tall = ceil_div(tiles(256), (long long)num_cus) * (2.6 * k_tiles + (accumulate ? 18 : 10));
+    const double middle = ceil_div(tiles(128), 2ll * num_cus) * (1.7 * k_tiles + (accumulate ? 7 : 5));
+    return {tall < 0.95 * middle ? kWgradTall : kWgrad128, 1};
+}
+
 // m, n, k: codes a [m, k], b [n, k], n % 4 == 0, k % 128 == 0; scale rows ld_sa, ld_sb bytes apart (multiples of 4, k / 128 rounded up to 4 or more),
-// 4-byte aligned; out [groups, m, n], 16-byte aligned. offsets null: groups is 1.
-template <int = 0>
+// 4-byte aligned; out [groups, m, n], 16-byte aligned. offsets null: groups is 1. `workspace`: a split-K workspace (kSplitKWorkspaceBytes, its
+// counters zero), or null: K is not split. num_sms: compute units to use, 0 for all.
+template <WgradKernel KERNEL = kWgradAny, int PARTS = 1>
 inline hipError_t launch_fp8_wgrad(const void* a, const uint8_t* sa, int ld_sa, const void* b, const uint8_t* sb, int ld_sb, float* out, const int* offsets,
-                                   int groups, int m, int n, int k, bool accumulate, hipStream_t stream) {
+                                   int groups, int m, int n, int k, bool accumulate, void* workspace, int num_sms, hipStream_t stream) {
     if (m < 0 || n < 0 || n % 4 != 0 || k < 0 || k % 128 != 0 || groups < 0 || (!offsets && groups != 1)) return hipErrorInvalidValue;
-    if (k >= 1 << 23 || ld_sa % 4 != 0 || ld_sb % 4 != 0 || ld_sa < ceil_div(k / 128, 4) * 4 || ld_sb < ceil_div(k / 128, 4) * 4 || ld_sa >= 1 << 23 || ld_sb >= 1 << 23) return hipErrorInvalidValue;
+    if (k >= 1 << 23 || n >= 1 << 21 || ld_sa % 4 != 0 || ld_sb % 4 != 0 || ld_sa >= 1 << 23 || ld_sb >= 1 << 23) return hipErrorInvalidValue;
+    if (ld_sa < ceil_div(k / 128, 4) * 4 || ld_sb < ceil_div(k / 128, 4) * 4) return hipErrorInvalidValue;
     if (m == 0 || n == 0 || groups == 0) return hipSuccess;
     if (!out || (k && (!a || !b || !sa || !sb))) return hipErrorInvalidValue;
     const WgradProblem p{static_cast<const uint8_t*>(a), static_cast<const uint8_t*>(b), sa, sb, out, offsets, m, n, k, ld_sa, ld_sb, groups, accumulate};
-    const long long slots = XcdTileScheduler<>(m, n, 128, 128).grid_size();
-    if (slots * groups >= 1ll << 31) return hipErrorInvalidValue;
-    hipLaunchKernelGGL((fp8_wgrad_kernel<128, 128, 4>), dim3(uint32_t(slots * groups)), dim3(256), 0, stream, p);
-    return hipGetLastError();
+    const bool capped = num_sms > 0 && num_sms < device_cu_count();
+    const int cus = capped ? num_sms : device_cu_count();
+    const WgradPlan plan = KERNEL == kWgradAny ? wgrad_plan(m, n, k, groups, accumulate, cus, workspace != nullptr) : WgradPlan{KERNEL, PARTS};
+    const int block = plan.kernel == kWgradTall ? 256 : plan.kernel == kWgrad128 ? 128 : 64;
+    const long long slots = (long long)XcdTileScheduler<>(m, n, block, block).grid_size() * groups * plan.parts;
+    if (slots >= 1ll << 30) return hipErrorInvalidValue;
+    WgradWorkspace w{nullptr, nullptr};
+    if (plan.kernel == kWgradSplit) {
+        if (!workspace || slots > kWgradMostParts) return hipErrorInvalidValue;
+        w = {reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + kSplitKCounterBytes), static_cast<unsigned*>(workspace)};
+    }
+    const auto launch = [&](auto kernel, long long grid, auto... more) {
+        hipLaunchKernelGGL(kernel, dim3(uint32_t(grid)), dim3(256), 0, stream, p, more...);
+        return hipGetLastError();
+    };
+    const long long most = capped ? std::min<long long>(cus, slots) : slots;
+    switch (plan.kernel) {
+        case kWgradTall: return launch(fp8_wgrad_tall_kernel<256>, std::min<long long>(cus, slots));
+        case kWgrad128: return launch(fp8_wgrad_kernel<128, 128, 2, false>, most, w, 1);
+        case kWgrad64: return launch(fp8_wgrad_kernel<64, 64, 4, false>, most, w, 1);
+        default: return launch(fp8_wgrad_kernel<64, 64, 4, true>, most, w, plan.parts);
+    }
 }
 
 } // namespace yan

@@ -30,24 +30,30 @@ __device__ __forceinline__ i32x4 float_to_bf16x8(const float (&f)[8]) {
     return __builtin_bit_cast(i32x4, v);
 }
 
-// A thread has eight columns of a token. rows_of / weights: [tokens, TOP_K]; weights may be null (all 1).
+// A wave has 512 columns of a token, a lane eight of them, so that rows and weights are the wave's own and come by scalar loads. rows_of / weights:
+// [tokens, TOP_K]; weights may be null (all 1).
 template <int TOP_K>
 __global__ void __launch_bounds__(256)
 moe_combine_kernel(const __bf16* __restrict__ y, const int* __restrict__ rows_of, const float* __restrict__ weights, __bf16* __restrict__ out,
-                   int tokens, int pieces, int rows) {
-    const long long unit = (long long)blockIdx.x * 256 + threadIdx.x;
-    if (unit >= (long long)tokens * pieces) return;
-    const int t = int(unit / pieces), c = int(unit - (long long)t * pieces);
+                   int tokens, int pieces, int rows, int waves_per_token) {
+    const long long unit = (long long)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x / kWaveSize);
+    const int t = int(unit / waves_per_token), c = int(unit - (long long)t * waves_per_token) * kWaveSize + int(threadIdx.x % kWaveSize);
+    if (t >= tokens) return;
+    if (c >= pieces) return;
     i32x4 raw[TOP_K];
     float w[TOP_K];
+    bool live[TOP_K];
 #pragma unroll
-    for (int i = 0; i < TOP_K; ++i) {
+    for (int i = 0; i < TOP_K; ++i) {           // without branches between the loads: a pair without a row reads row 0 and forgets it
         const int row = rows_of[size_t(t) * TOP_K + i];
-        const bool live = uint32_t(row) < uint32_t(rows);
-        w[i] = !live ? 0.f : weights ? weights[size_t(t) * TOP_K + i] : 1.f;
+        live[i] = uint32_t(row) < uint32_t(rows);
+        w[i] = weights ? weights[size_t(t) * TOP_K + i] : 1.f;
         raw[i] = i32x4{0, 0, 0, 0};
-        if (live) raw[i] = reinterpret_cast<const i32x4*>(y)[size_t(row) * pieces + c];
+        if (rows) raw[i] = reinterpret_cast<const i32x4*>(y)[size_t(live[i] ? row : 0) * pieces + c];
     }
+#pragma unroll
+    for (int i = 0; i < TOP_K; ++i)
+        if (!live[i]) w[i] = 0.f, raw[i] = i32x4{0, 0, 0, 0};
     float sum[8] = {};
 #pragma unroll
     for (int i = 0; i < TOP_K; ++i) {
@@ -56,12 +62,16 @@ moe_combine_kernel(const __bf16* __restrict__ y, const int* __restrict__ rows_of
 #pragma unroll
         for (int j = 0; j < 8; ++j) sum[j] = fmaf(w[i], f[j], sum[j]);
     }
-    reinterpret_cast<i32x4*>(out)[unit] = float_to_bf16x8(sum);
+    reinterpret_cast<i32x4*>(out)[size_t(t) * pieces + c] = float_to_bf16x8(sum);
 }
 
-// THREADS a token (64 or 256), 256 / THREADS tokens a workgroup; the workgroups from `token_blocks` on clear the rows that no pair has.
+// THREADS a token, 256 / THREADS tokens a workgroup; the workgroups from `token_blocks` on clear the rows that no pair has. A wave a token only where it
+// holds all of the columns (1024 columns, 4000 x 8 pairs, forward and backward: 55.0 us with a wave a token, 35.1 with a workgroup). STREAM: y is read for the
+// last time and dy outgrows the L2s by so much that both go past them; forward and backward of tokens x 8 x 4096, plain / so: 4097 (300 MB of dy)
+// 231.7 / 208.9 us, 2048 117.0 / 110.7, 1024 65.0 / 61.8, 512 34.7 / 37.1.
+constexpr long long kCombineStreamBytes = 64ll << 20;
 constexpr int kRowsPerClearBlock = 32;
-template <int TOP_K, int THREADS>
+template <int TOP_K, int THREADS, bool STREAM>
 __global__ void __launch_bounds__(256)
 moe_combine_backward_kernel(const __bf16* __restrict__ grad_out, const __bf16* __restrict__ y, const int* __restrict__ rows_of,
                             const float* __restrict__ weights, const int* __restrict__ source, __bf16* __restrict__ grad_y, float* __restrict__ grad_weights,
@@ -95,7 +105,8 @@ moe_combine_backward_kernel(const __bf16* __restrict__ grad_out, const __bf16* _
 #pragma unroll
                 for (int i = 0; i < TOP_K; ++i) {
                     raw[i] = i32x4{0, 0, 0, 0};
-                    if (row[i] >= 0) raw[i] = reinterpret_cast<const i32x4*>(y)[size_t(row[i]) * pieces + c];
+                    const i32x4* const from = reinterpret_cast<const i32x4*>(y) + size_t(row[i]) * pieces + c;
+                    if (row[i] >= 0) raw[i] = STREAM ? __builtin_nontemporal_load(from) : *from;
                 }
             }
 #pragma unroll
@@ -104,7 +115,9 @@ moe_combine_backward_kernel(const __bf16* __restrict__ grad_out, const __bf16* _
                 float f[8];
 #pragma unroll
                 for (int j = 0; j < 8; ++j) f[j] = w[i] * d[j];
-                reinterpret_cast<i32x4*>(grad_y)[size_t(row[i]) * pieces + c] = float_to_bf16x8(f);
+                i32x4* const to = reinterpret_cast<i32x4*>(grad_y) + size_t(row[i]) * pieces + c;
+                if (STREAM) __builtin_nontemporal_store(float_to_bf16x8(f), to);
+                else *to = float_to_bf16x8(f);
                 if (grad_weights) {
                     bf16x8_to_float(f, raw[i]);
 #pragma unroll
@@ -137,9 +150,10 @@ inline hipError_t launch_moe_combine(const __bf16* y, const int* rows_of, const 
     if (tokens == 0 || columns == 0) return hipSuccess;
     if (!rows_of || !out || (rows && !y)) return hipErrorInvalidValue;
     const int pieces = columns / 8;
-    const long long blocks = ceil_div((long long)tokens * pieces, 256ll);
+    const int waves_per_token = ceil_div(pieces, kWaveSize);
+    const long long blocks = ceil_div((long long)tokens * waves_per_token, 4ll);
     if (blocks >= 1ll << 31) return hipErrorInvalidValue;
-    hipLaunchKernelGGL(moe_combine_kernel<TOP_K>, dim3(uint32_t(blocks)), dim3(256), 0, stream, y, rows_of, weights, out, tokens, pieces, rows);
+    hipLaunchKernelGGL(moe_combine_kernel<TOP_K>, dim3(uint32_t(blocks)), dim3(256), 0, stream, y, rows_of, weights, out, tokens, pieces, rows, waves_per_token);
     return hipGetLastError();
 }
 
@@ -150,7 +164,7 @@ inline hipError_t launch_moe_combine_backward(const __bf16* grad_out, const __bf
     if (tokens && (!grad_out || !rows_of)) return hipErrorInvalidValue;
     if (rows && (!source || !grad_y || !y)) return hipErrorInvalidValue;
     const int pieces = columns / 8;
-    const bool wide = pieces > 128;
+    const bool wide = pieces > kWaveSize;
     const int token_blocks = wide ? tokens : ceil_div(tokens, 4), clear_blocks = ceil_div(rows, kRowsPerClearBlock);
     if ((long long)token_blocks + clear_blocks >= 1ll << 31) return hipErrorInvalidValue;
     if (token_blocks + clear_blocks == 0) return hipSuccess;
@@ -159,7 +173,9 @@ inline hipError_t launch_moe_combine_backward(const __bf16* grad_out, const __bf
                            pieces, rows, token_blocks);
         return hipGetLastError();
     };
-    return wide ? launch(moe_combine_backward_kernel<TOP_K, 256>) : launch(moe_combine_backward_kernel<TOP_K, 64>);
+    if (!wide) return launch(moe_combine_backward_kernel<TOP_K, 64, false>);
+    return (long long)rows * columns * 2 > kCombineStreamBytes ? launch(moe_combine_backward_kernel<TOP_K, 256, true>)
+                                                               : launch(moe_combine_backward_kernel<TOP_K, 256, false>);
 }
 
 } // namespace yan

@@ -8,7 +8,7 @@
 // one whose expert is none (below 0 or from E on). Rows that no pair has are left as they were.
 //
 // Bound by HBM: a token is read once, quantised once and stored top_k times. Few pairs are numbered by every workgroup for itself, one launch;
-// many by a histogram of the pairs of each workgroup's tokens, a scan along the workgroups, and the workgroup's own pairs behind that.
+// many by a histogram of the pairs of each chunk of tokens, a scan along the chunks, and the chunk's own pairs behind that.
 #pragma once
 
 #include "../gemm/fp8_cast.hpp"
@@ -19,7 +19,8 @@ namespace yan {
 
 constexpr int kExpertAlignment = 128;
 constexpr int kFewPairs = 4096;             // up to here every workgroup counts all pairs itself
-constexpr int kTokensPerBlock = 16;         // above: tokens of a workgroup
+constexpr int kTokensPerBlock = 16;         // above: tokens of a chunk
+constexpr long long kDispatchCacheBytes = 256ll << 20;
 
 struct DispatchShape {
     int tokens, k_blocks, top_k, experts, m_max;        // m_max 0: contiguous
@@ -66,22 +67,35 @@ __device__ __forceinline__ void describe_rows(const int* counts, const int* star
     }
 }
 
-// Quantises K blocks kb0, kb0 + 16 * step, ... of token `t` (16 lanes a block) and stores them to the token's rows.
-template <typename T, bool STREAM>
-__device__ __forceinline__ void scatter_token(const T* __restrict__ x, uint8_t* __restrict__ codes, float* __restrict__ scales, const DispatchShape& s,
-                                              int t, int kb0, int step, const int* row_of, const int* expert_of) {
+// Quantises the blocks of 128 of tokens t0, t0 + 1, ... numbered first .. last - 1 (k_blocks a token) and stores them to their tokens' rows: 16 lanes a
+// block, 16 blocks a step, UNROLL steps' loads under way at once. row_of, expert_of: [tokens][top_k], of token t0 on.
+template <int UNROLL, CastStream STREAM, typename T>
+__device__ __forceinline__ void scatter_blocks(const T* __restrict__ x, uint8_t* __restrict__ codes, float* __restrict__ scales, const DispatchShape& s, int t0,
+                                               int first, int last, const int* row_of, const int* expert_of) {
     const int part = threadIdx.x & 15;
-    for (int kb = kb0; kb < s.k_blocks; kb += step) {
-        const F32x8 f = to_f32(load8<STREAM>(x + (size_t(t) * s.k_blocks + kb) * 128, part));
-        const float amax = fmaxf(max_over_16_lanes(abs_max8(f)), 1e-4f);
-        const uint2 q = quantise8(f, kFp8Max / amax);
-        for (int i = 0; i < s.top_k; ++i) {
-            const int row = row_of[i];
-            if (row < 0) continue;
-            store_codes8<T, false>(codes + (size_t(row) * s.k_blocks + kb) * 128, part, q);
-            if (part == 0) {
-                const int g = s.m_max ? expert_of[i] : 0, m = s.m_max ? row - g * s.m_max : row;
-                scales[g * s.stride_g + m * s.stride_m + kb * s.stride_k] = amax / kFp8Max;
+    const T* const from = x + size_t(t0) * s.k_blocks * 128;
+    for (int at = first + int(threadIdx.x >> 4); at < last; at += 16 * UNROLL) {
+        Raw8<T> raw[UNROLL];
+#pragma unroll
+        for (int u = 0; u < UNROLL; ++u) {
+            raw[u] = Raw8<T>{};
+            if (at + 16 * u < last) raw[u] = load8<STREAM != kPlain>(from + size_t(at + 16 * u) * 128, part);
+        }
+#pragma unroll
+        for (int u = 0; u < UNROLL; ++u) {
+            const int block = at + 16 * u, token = block / s.k_blocks, kb = block - token * s.k_blocks;
+            const F32x8 f = to_f32(raw[u]);
+            const float amax = fmaxf(max_over_16_lanes(abs_max8(f)), 1e-4f);
+            const uint2 q = quantise8(f, kFp8Max / amax);
+            if (block >= last) continue;
+            for (int i = 0; i < s.top_k; ++i) {
+                const int row = row_of[token * s.top_k + i];
+                if (row < 0) continue;
+                store_codes8<T, STREAM == kStreamBoth>(codes + (size_t(row) * s.k_blocks + kb) * 128, part, q);
+                if (part == 0) {
+                    const int g = s.m_max ? expert_of[token * s.top_k + i] : 0, m = s.m_max ? row - g * s.m_max : row;
+                    scales[g * s.stride_g + m * s.stride_m + kb * s.stride_k] = amax / kFp8Max;
+                }
             }
         }
     }
@@ -93,9 +107,8 @@ __device__ __forceinline__ int row_of_pair(const DispatchShape& s, const int* st
     return row < s.rows ? row : -1;
 }
 
-// What the counts say of the layout as a whole: the first workgroup's.
+// What the counts say of the layout as a whole: one workgroup's.
 __device__ __forceinline__ void describe_experts(const int* counts, const int* starts, const DispatchShape& s, int* offsets, int* masked_m) {
-    if (blockIdx.x != 0) return;
     if (s.m_max) {
         for (int x = threadIdx.x; x < s.experts; x += 256) masked_m[x] = counts[x] < s.m_max ? counts[x] : s.m_max;
     } else {
@@ -140,11 +153,12 @@ moe_dispatch_few_kernel(const T* __restrict__ x, const int* __restrict__ indices
         const int share = ceil_div(s.rows, int(gridDim.x)), first = min(s.rows, int(blockIdx.x) * share);
         describe_rows(counts, starts, s, first, min(s.rows, first + share), m_indices, source);
     }
-    describe_experts(counts, starts, s, offsets, m_indices);
-    if (t < s.tokens) scatter_token<T, false>(x, codes, scales, s, t, piece * 16 + int(threadIdx.x >> 4), parts * 16, row_of, expert_of);
+    if (blockIdx.x == 0) describe_experts(counts, starts, s, offsets, m_indices);
+    const int share = ceil_div(s.k_blocks, parts);
+    if (t < s.tokens) scatter_blocks<2, kPlain>(x, codes, scales, s, t, piece * share, min(s.k_blocks, (piece + 1) * share), row_of, expert_of);
 }
 
-// Many pairs, first: the histogram of every workgroup's tokens, [blocks][E].
+// Many pairs, first: the histogram of every chunk of tokens, [chunks][E].
 template <int = 0>
 __global__ void __launch_bounds__(256)
 moe_dispatch_count_kernel(const int* __restrict__ indices, int* __restrict__ table, int pairs, int pairs_per_block, int e) {
@@ -184,17 +198,23 @@ moe_dispatch_scan_kernel(int* __restrict__ table, int blocks, int e) {
     if (part == 63) table[size_t(blocks) * e + x] = before;
 }
 
-// Third: the rows of the workgroup's pairs and the tokens themselves.
-template <typename T, bool STREAM>
+// Third: the rows of the chunk's pairs and the tokens themselves, by `parts` workgroups a chunk.
+template <typename T, CastStream STREAM>
 __global__ void __launch_bounds__(256)
 moe_dispatch_kernel(const T* __restrict__ x, const int* __restrict__ indices, const int* __restrict__ table, uint8_t* __restrict__ codes,
                     float* __restrict__ scales, int* __restrict__ rows, int* __restrict__ m_indices, int* __restrict__ source, int* __restrict__ offsets,
-                    DispatchShape s) {
+                    DispatchShape s, int parts) {
     constexpr int PAIRS = kTokensPerBlock * kMaxTopK;
     static_assert(PAIRS == 256, "a thread a pair");
     __shared__ int counts[kMaxExperts], starts[kMaxExperts + 1], row_of[PAIRS], expert_of[PAIRS];
-    const int t0 = blockIdx.x * kTokensPerBlock, here = min(kTokensPerBlock, s.tokens - t0), pairs = here * s.top_k, p = threadIdx.x;
-    for (int e = threadIdx.x; e < s.experts; e += 256) counts[e] = table[size_t(gridDim.x) * s.experts + e];
+    // Neighbouring chunks run on one XCD, at about the same time: an expert's scales of one K block are 4 bytes from each of its tokens, and come together to
+    // lines in the L2 that way.
+    const int chunks = ceil_div(s.tokens, kTokensPerBlock), per_xcd = ceil_div(chunks * parts, kNumXCD);
+    const int work = int(blockIdx.x % kNumXCD) * per_xcd + int(blockIdx.x / kNumXCD);
+    if (work >= chunks * parts) return;
+    const int chunk = work / parts, piece = work - chunk * parts;
+    const int t0 = chunk * kTokensPerBlock, here = min(kTokensPerBlock, s.tokens - t0), pairs = here * s.top_k, p = threadIdx.x;
+    for (int e = threadIdx.x; e < s.experts; e += 256) counts[e] = table[size_t(chunks) * s.experts + e];
     const int e = p < pairs ? indices[size_t(t0) * s.top_k + p] : -1;
     expert_of[p] = e;
     __syncthreads();
@@ -202,22 +222,24 @@ moe_dispatch_kernel(const T* __restrict__ x, const int* __restrict__ indices, co
     if (p < pairs) {
         int row = -1;
         if (uint32_t(e) < uint32_t(s.experts)) {
-            int rank = table[size_t(blockIdx.x) * s.experts + e];
+            int rank = table[size_t(chunk) * s.experts + e];
             for (int i = 0; i < p; ++i) rank += expert_of[i] == e;
             row = row_of_pair(s, starts, e, rank);
         }
         row_of[p] = row;
-        rows[size_t(t0) * s.top_k + p] = row;
-        if (!s.m_max && row >= 0) source[row] = t0 + p / s.top_k;
+        if (piece == 0) {
+            rows[size_t(t0) * s.top_k + p] = row;
+            if (!s.m_max && row >= 0) source[row] = t0 + p / s.top_k;
+        }
     }
     __syncthreads();
     if (!s.m_max) {
-        const int share = ceil_div(s.rows, int(gridDim.x)), first = min(s.rows, int(blockIdx.x) * share);
+        const int share = ceil_div(s.rows, chunks * parts), first = min(s.rows, work * share);
         describe_rows(counts, starts, s, first, min(s.rows, first + share), m_indices, source);
     }
-    describe_experts(counts, starts, s, offsets, m_indices);
-    for (int t = 0; t < here; ++t)
-        scatter_token<T, STREAM>(x, codes, scales, s, t0 + t, threadIdx.x >> 4, 16, row_of + t * s.top_k, expert_of + t * s.top_k);
+    if (work == 0) describe_experts(counts, starts, s, offsets, m_indices);
+    const int blocks = here * s.k_blocks, share = ceil_div(blocks, parts);
+    scatter_blocks<4, STREAM>(x, codes, scales, s, t0, piece * share, min(blocks, (piece + 1) * share), row_of, expert_of);
 }
 
 // Bytes of workspace a launch wants: the table of many pairs.
@@ -255,11 +277,19 @@ inline hipError_t launch_moe_dispatch(const T* x, const int* indices, void* code
     if (const hipError_t rc = hipGetLastError(); rc != hipSuccess) return rc;
     hipLaunchKernelGGL(moe_dispatch_scan_kernel<0>, dim3(ceil_div(experts, 16)), dim3(1024), 0, stream, table, blocks, experts);
     if (const hipError_t rc = hipGetLastError(); rc != hipSuccess) return rc;
+    // Workgroups a chunk: each has 64 blocks of 128, one step of four loads, or fewer where the chunks are too few for the chip (us with 1, 2, 4, 8, 16:
+    // 8192 tokens of 7168 182.5, 175.6, 171.0, 172.5, 166.5; 2048 of 7168 104.7, 66.7, 51.5, 51.6, 47.5; 8192 of 1024 36.7, 31.3, 37.1, 39.4, 46.9; 1024 of 2048
+    // 34.1, 23.5, 18.4, 16.6, 16.2)
+    const int in_chunk = kTokensPerBlock * s.k_blocks, parts = std::max(ceil_div(in_chunk, 64), std::min(ceil_div(in_chunk, 16), 4 * device_cu_count() / blocks));
+    if ((long long)blocks * parts >= 1ll << 30) return hipErrorInvalidValue;
+    const int grid = ceil_div(blocks * parts, kNumXCD) * kNumXCD;
     const auto launch = [&](auto kernel) {
-        hipLaunchKernelGGL(kernel, dim3(blocks), dim3(256), 0, stream, x, indices, table, to, scales, rows_of, m_indices, source, offsets, s);
+        hipLaunchKernelGGL(kernel, dim3(grid), dim3(256), 0, stream, x, indices, table, to, scales, rows_of, m_indices, source, offsets, s, parts);
         return hipGetLastError();
     };
-    return cast_stream((long long)tokens * k, sizeof(T), true) == kPlain ? launch(moe_dispatch_kernel<T, false>) : launch(moe_dispatch_kernel<T, true>);
+    if (cast_stream((long long)tokens * k, sizeof(T), true) == kPlain) return launch(moe_dispatch_kernel<T, kPlain>);
+    // codes that outgrow the memory-side cache are not found there by the GEMM behind (8192 x 8 pairs of 7168, 470 MB: 174.9 us plain, 161.6 past the caches)
+    return (long long)pairs * k > kDispatchCacheBytes ? launch(moe_dispatch_kernel<T, kStreamBoth>) : launch(moe_dispatch_kernel<T, kStreamSource>);
 }
 
 } // namespace yan

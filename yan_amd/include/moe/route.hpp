@@ -7,16 +7,17 @@
 //   picks), zero elsewhere:   softmax: dl = s (h + g - sum_e s_e (h_e + g_e));   sigmoid: dl = s (1 - s) (h + (g - sum_e p_e g_e) / sum_e s_e)
 //
 // A group of LANES lanes holds a row, VALUES neighbouring logits a lane, so that lower lanes have lower experts. Picks are made on the logits
-// (both scores grow with them) as unsigned keys of the same order: a round is the maximum over the lane's keys and over the group, and the
-// lowest lane that has it takes out its lowest such key and counts it. What is summed over tokens, p and the counts, stays in the registers of the lane
-// that owns the expert; a workgroup leaves one row of both, and a second, small kernel adds the rows up in their order: no float atomics, the
-// same bits every time.
+// (both scores grow with them) as unsigned keys of the same order: every lane sorts its own, then a round is the maximum over the lanes' first keys, and the
+// lowest lane that has it gives up its first. What is summed over tokens, p, stays in the registers of the lane that owns the expert, picks are
+// counted in LDS; a workgroup leaves one row of both, and a second, small kernel adds the rows up in their order: no float atomics, the same bits
+// every time.
 #pragma once
 
 #include <hip/hip_runtime.h>
 #include <hip/hip_bf16.h>
 
 #include <limits>
+#include <type_traits>
 
 #include "lanes.hpp"
 
@@ -24,6 +25,7 @@ namespace yan {
 
 constexpr int kMaxTopK = 16;            // lane i of a group holds pick i
 constexpr int kMaxExperts = 1024;
+constexpr int kRouteThreads = 1024;     // of a workgroup of the forward: what is left of it is added up by few
 
 // The order of floats as the order of unsigned numbers; above 0, which is left for what has been taken out. -0 and 0 are one value. A NaN
 // is picked after everything else, as -infinity is (its row's weights are NaN all the same).
@@ -65,22 +67,47 @@ __host__ __device__ inline bool rows_in_pieces(const void* base, int e) {
     return e % PIECE == 0 && reinterpret_cast<uintptr_t>(base) % (PIECE * sizeof(T)) == 0;
 }
 
-// A row's scores: v are the logits (-infinity past the row's end), `top` the largest; returns their sum. A logit of +infinity counts as the
-// largest finite number; a row of -infinity alone has scores of zero.
+// exp(x) for x <= 88, within 2 units in the last place; 0 below -87 (the smallest normal numbers), NaN for NaN. The product with log2(e) is carried to twice
+// the bits, its lower part applied to the result. The library's function, with its care for every x, and the division it goes with were 200 of
+// the 450 vector instructions of a row.
+__device__ __forceinline__ float exp_of(float x) {
+    constexpr float LOG2_E = 1.44269504f, LOG2_E_LOW = 1.92596299e-8f, LN_2 = 0.693147181f;
+    const float high = x * LOG2_E, low = fmaf(x, LOG2_E, -high) + x * LOG2_E_LOW;
+    const float y = __builtin_amdgcn_exp2f(high);
+    return x < -87.f ? 0.f : fmaf(y, low * LN_2, y);
+}
+// 1 / x for normal numbers, one step of Newton behind the hardware's estimate; 0 for 0
+__device__ __forceinline__ float inverse_of(float x) {
+    const float r = __builtin_amdgcn_rcpf(x);
+    return x == 0.f ? 0.f : fmaf(fmaf(-x, r, 1.f), r, r);
+}
+constexpr float kMostLogit = std::numeric_limits<float>::max();
+__device__ __forceinline__ float finite_top(float top) { return top < -kMostLogit ? 0.f : (top > kMostLogit ? kMostLogit : top); }
+// sigmoid(l), or exp(l - top); a logit of +infinity counts as the largest finite number
+template <bool SIGMOID>
+__device__ __forceinline__ float score_of(float l, float top) {
+    if constexpr (SIGMOID) {
+        // of the magnitude, so that no exponential overflows: 1 / (1 + e^-|l|), or that times e^-|l|
+        const float t = exp_of(-fabsf(l)), r = inverse_of(1.f + t);
+        return l < 0.f ? t * r : r;
+    } else {
+        return exp_of((l > kMostLogit ? kMostLogit : l) - top);
+    }
+}
+
+// A row's scores: v are the logits (-infinity past the row's end), `top` the largest as finite_top gives it; returns their sum (softmax: before they
+// were divided by it). A row of -infinity alone has scores of zero.
 template <bool SIGMOID, int LANES, int VALUES>
 __device__ __forceinline__ float row_scores(float (&s)[VALUES], const float (&v)[VALUES], float top) {
-    constexpr float MOST = std::numeric_limits<float>::max();
-    top = top < -MOST ? 0.f : (top > MOST ? MOST : top);
     float sum = 0.f;
 #pragma unroll
     for (int j = 0; j < VALUES; ++j) {
-        const float l = v[j] > MOST ? MOST : v[j];
-        s[j] = SIGMOID ? 1.f / (1.f + expf(-l)) : expf(l - top);
+        s[j] = score_of<SIGMOID>(v[j], top);
         sum += s[j];
     }
     sum = sum_lanes<LANES>(sum);
     if constexpr (!SIGMOID) {
-        const float inverse = sum == 0.f ? 0.f : 1.f / sum;
+        const float inverse = inverse_of(sum);
 #pragma unroll
         for (int j = 0; j < VALUES; ++j) s[j] *= inverse;
     }
@@ -111,89 +138,99 @@ __device__ __forceinline__ float balance_loss(float pull, int picks, int top_k, 
 }
 
 template <typename T, bool SIGMOID, int LANES, int VALUES>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(kRouteThreads)
 moe_route_kernel(const T* __restrict__ logits, const uint8_t* __restrict__ mask, float* __restrict__ weights, int* __restrict__ indices,
                  int* __restrict__ counts, float* __restrict__ loss, void* workspace, int tokens, int e, int top_k, bool renormalize, bool whole) {
-    constexpr int GROUPS = 256 / LANES;
-    __shared__ float lds_share[4][LANES * VALUES];
-    __shared__ int lds_counts[4][LANES * VALUES];
-    __shared__ float lds_pull[4];
-    __shared__ int lds_picks[4];
+    constexpr int GROUPS = kRouteThreads / LANES, WAVES = kRouteThreads / kWaveSize;
+    __shared__ float lds_share[WAVES][LANES * VALUES];
+    __shared__ int lds_counts[LANES * VALUES], lds_pick[GROUPS][kMaxTopK];
+    __shared__ float lds_pull[WAVES];
+    __shared__ int lds_picks[WAVES];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, in_group = lane % LANES, first = in_group * VALUES, group_base = lane - in_group;
     float share[VALUES];
-    int count[VALUES];
 #pragma unroll
-    for (int j = 0; j < VALUES; ++j) share[j] = 0.f, count[j] = 0;
+    for (int j = 0; j < VALUES; ++j) share[j] = 0.f;
+    for (int x = threadIdx.x; x < LANES * VALUES; x += kRouteThreads) lds_counts[x] = 0;
+    __syncthreads();
 
+    // the logits of a round are loaded in the round before
+    float ahead[VALUES];
+    const auto load = [&](int t) { load_row(ahead, logits + size_t(t < tokens ? t : 0) * e, first, t < tokens ? e : 0, whole, -std::numeric_limits<float>::infinity()); };
+    load(blockIdx.x * GROUPS + int(threadIdx.x) / LANES);
     for (int t0 = blockIdx.x * GROUPS; t0 < tokens; t0 += gridDim.x * GROUPS) {
         const int t = t0 + int(threadIdx.x) / LANES;
         const bool live = t < tokens && (!mask || mask[t]);
         float v[VALUES], s[VALUES];
-        load_row(v, logits + size_t(t < tokens ? t : 0) * e, first, e, whole, -std::numeric_limits<float>::infinity());
-        uint32_t key[VALUES];
 #pragma unroll
-        for (int j = 0; j < VALUES; ++j) key[j] = first + j < e ? order_key(v[j]) : 0u;
-        uint32_t my_key = 0;
-        int my_pick = 0;
+        for (int j = 0; j < VALUES; ++j) v[j] = ahead[j];
+        load(t + gridDim.x * GROUPS);
+        // this lane's logits in descending order, equal ones in their own; `places`: which they were, four bits each, the first in the lowest
+        uint32_t key[VALUES];
+        int place[VALUES];
+#pragma unroll
+        for (int j = 0; j < VALUES; ++j) key[j] = first + j < e ? order_key(v[j]) : 0u, place[j] = j;
+#pragma unroll
+        for (int round = 0; round < VALUES; ++round)
+#pragma unroll
+            for (int j = round & 1; j + 1 < VALUES; j += 2) {          // neighbours change places only if the later one is larger: equal ones never do
+                const bool swap = key[j + 1] > key[j];
+                const uint32_t high = swap ? key[j + 1] : key[j], low = swap ? key[j] : key[j + 1];
+                const int p = swap ? place[j + 1] : place[j], q = swap ? place[j] : place[j + 1];
+                key[j] = high, key[j + 1] = low, place[j] = p, place[j + 1] = q;
+            }
+        using Places = std::conditional_t<(VALUES > 8), unsigned long long, uint32_t>;
+        Places places = 0;
+#pragma unroll
+        for (int j = 0; j < VALUES; ++j) places |= Places(place[j]) << (4 * j);
+        uint32_t my_key = 0, best = 0;
+        int* const picks = lds_pick[threadIdx.x / LANES];
         float top = 0.f;
         for (int i = 0; i < top_k; ++i) {
-            uint32_t mine = key[0];
+            best = max_lanes<LANES>(key[0]);
+            const unsigned long long have = __ballot(key[0] == best) >> group_base;
+            const bool mine = in_group == __ffsll((long long)have) - 1;
+            if (mine) picks[i] = first + int(places & 15);
+            places = mine ? places >> 4 : places;
 #pragma unroll
-            for (int j = 1; j < VALUES; ++j) mine = mine > key[j] ? mine : key[j];
-            const uint32_t best = max_lanes<LANES>(mine);
-            const unsigned long long have = __ballot(mine == best) >> group_base;
-            const int winner = __ffsll((long long)have) - 1;
-            int place = 0;
-            bool open = in_group == winner;
-#pragma unroll
-            for (int j = 0; j < VALUES; ++j) {
-                const bool hit = open && key[j] == best;
-                place = hit ? j : place;
-                key[j] = hit ? 0u : key[j];
-                count[j] += hit && live;
-                open = open && !hit;
-            }
-            const int pick = __shfl(first + place, group_base + winner, 64);
+            for (int j = 0; j + 1 < VALUES; ++j) key[j] = mine ? key[j + 1] : key[j];
+            key[VALUES - 1] = mine ? 0u : key[VALUES - 1];
             if (i == 0) top = value_of_key(best);
-            if (in_group == i) my_key = best, my_pick = pick;
+            if (in_group == i) my_key = best;
         }
-        const float sum = row_scores<SIGMOID, LANES>(s, v, top);
+        asm volatile("" ::: "memory");          // a wave's LDS operations are done in order
+        const int my_pick = in_group < top_k ? picks[in_group] : 0;
+        if (live && in_group < top_k) atomicAdd(&lds_counts[my_pick], 1);
+        asm volatile("" ::: "memory");
+        top = finite_top(top);
+        const float sum = row_scores<SIGMOID, LANES>(s, v, top), inverse = inverse_of(sum);
         // lane i has pick i: its score again, from the logit that its key stands for
-        float mine = 0.f;
-        {
-            constexpr float MOST = std::numeric_limits<float>::max();
-            const float t_ = top < -MOST ? 0.f : (top > MOST ? MOST : top), l = fminf(value_of_key(my_key), MOST);
-            if (in_group < top_k) mine = SIGMOID ? 1.f / (1.f + expf(-l)) : expf(l - t_) * (sum == 0.f ? 0.f : 1.f / sum);
-            if (sum != sum) mine = sum;
-        }
-        if (renormalize) {
-            const float chosen = sum_lanes<LANES>(in_group < top_k ? mine : 0.f);
-            mine = chosen == 0.f ? 0.f : mine / chosen;
-        }
+        float mine = in_group < top_k ? score_of<SIGMOID>(value_of_key(my_key), top) * (SIGMOID ? 1.f : inverse) : 0.f;
+        if (renormalize) mine *= inverse_of(sum_lanes<LANES>(mine));
+        if (sum != sum) mine = sum;
         if (t < tokens && in_group < top_k) {
             weights[size_t(t) * top_k + in_group] = live ? mine : 0.f;
             indices[size_t(t) * top_k + in_group] = live ? my_pick : -1;
         }
-        const float part = !live ? 0.f : SIGMOID ? (sum == 0.f ? 0.f : 1.f / sum) : 1.f;
 #pragma unroll
-        for (int j = 0; j < VALUES; ++j) share[j] += live ? s[j] * part : 0.f;
+        for (int j = 0; j < VALUES; ++j) share[j] += live ? s[j] * (SIGMOID ? inverse : 1.f) : 0.f;
     }
 
     // the workgroup's row
 #pragma unroll
     for (int j = 0; j < VALUES; ++j) {
         share[j] = sum_groups<LANES>(share[j]);
-        count[j] = sum_groups<LANES>(count[j]);
-        if (lane < LANES) lds_share[wave][first + j] = share[j], lds_counts[wave][first + j] = count[j];
+        if (lane < LANES) lds_share[wave][first + j] = share[j];
     }
     __syncthreads();
     const RouteWorkspace to(workspace, gridDim.x, e);
     const bool alone = gridDim.x == 1;
     float pull = 0.f;
     int picks = 0;
-    for (int x = threadIdx.x; x < e; x += 256) {
-        const float sum = (lds_share[0][x] + lds_share[1][x]) + (lds_share[2][x] + lds_share[3][x]);
-        const int number = lds_counts[0][x] + lds_counts[1][x] + lds_counts[2][x] + lds_counts[3][x];
+    for (int x = threadIdx.x; x < e; x += kRouteThreads) {
+        float sum = 0.f;
+#pragma unroll
+        for (int w = 0; w < WAVES; ++w) sum += lds_share[w][x];
+        const int number = lds_counts[x];
         if (alone) {
             counts[x] = number;
             pull += float(number) * sum;
@@ -210,8 +247,10 @@ moe_route_kernel(const T* __restrict__ logits, const uint8_t* __restrict__ mask,
     pull = sum_lanes<64>(pull), picks = sum_lanes<64>(picks);
     if (lane == 0) lds_pull[wave] = pull, lds_picks[wave] = picks;
     __syncthreads();
-    if (threadIdx.x == 0)
-        *loss = balance_loss((lds_pull[0] + lds_pull[1]) + (lds_pull[2] + lds_pull[3]), lds_picks[0] + lds_picks[1] + lds_picks[2] + lds_picks[3], top_k, e);
+    if (wave == 0) {
+        pull = sum_lanes<16>(lane < WAVES ? lds_pull[lane] : 0.f), picks = sum_lanes<16>(lane < WAVES ? lds_picks[lane] : 0);
+        if (lane == 0) *loss = balance_loss(pull, picks, top_k, e);
+    }
 }
 
 // Adds up the workgroups' rows, 16 experts a workgroup; the last workgroup to arrive adds up what the loss takes of each, in their order.
@@ -301,15 +340,12 @@ moe_route_backward_kernel(const T* __restrict__ logits, const int* __restrict__ 
         float top = v[0];
 #pragma unroll
         for (int j = 1; j < VALUES; ++j) top = fmaxf(top, v[j]);
-        top = max_lanes<LANES>(top);
-        const float sum = row_scores<SIGMOID, LANES>(s, v, top);
+        top = finite_top(max_lanes<LANES>(top));
+        const float sum = row_scores<SIGMOID, LANES>(s, v, top), inverse = inverse_of(sum);
         if (renormalize) {
-            constexpr float MOST = std::numeric_limits<float>::max();
-            const float t_ = top < -MOST ? 0.f : (top > MOST ? MOST : top), l = fminf(logit, MOST);
-            float mine = SIGMOID ? 1.f / (1.f + expf(-l)) : expf(l - t_) * (sum == 0.f ? 0.f : 1.f / sum);
-            if (pick < 0) mine = 0.f;
-            const float chosen = sum_lanes<LANES>(mine), inverse = chosen == 0.f ? 0.f : 1.f / chosen;
-            dw = (dw - sum_lanes<LANES>(mine * inverse * dw)) * inverse;
+            const float mine = pick < 0 ? 0.f : score_of<SIGMOID>(logit, top) * (SIGMOID ? 1.f : inverse);
+            const float part = inverse_of(sum_lanes<LANES>(mine));
+            dw = (dw - sum_lanes<LANES>(mine * part * dw)) * part;
         }
         asm volatile("" ::: "memory");              // a wave's LDS operations are done in order: the zeros, the picks, then the reads
         if (pick >= 0) h_row[pick] = dw;
@@ -322,7 +358,6 @@ moe_route_backward_kernel(const T* __restrict__ logits, const int* __restrict__ 
         }
         asm volatile("" ::: "memory");
         dot = sum_lanes<LANES>(dot);
-        const float inverse = sum == 0.f ? 0.f : 1.f / sum;
 #pragma unroll
         for (int j = 0; j < VALUES; ++j) {
             if constexpr (SIGMOID) d[j] = s[j] * (1.f - s[j]) * (d[j] + (g[j] - dot * inverse) * inverse);
@@ -354,8 +389,8 @@ template <typename T, bool SIGMOID, int LANES, int VALUES>
 inline hipError_t launch_moe_route(const T* logits, const uint8_t* mask, float* weights, int* indices, int* counts, float* loss, void* workspace,
                                    int blocks, int tokens, int e, int top_k, bool renormalize, hipStream_t stream) {
     if (tokens < 0 || e < 1 || e > LANES * VALUES || top_k < 1 || top_k > e || top_k > kMaxTopK || top_k > LANES || blocks < 1) return hipErrorInvalidValue;
-    if (!logits || !weights || !indices || !counts || !loss || (blocks > 1 && !workspace)) return hipErrorInvalidValue;
-    hipLaunchKernelGGL((moe_route_kernel<T, SIGMOID, LANES, VALUES>), dim3(blocks), dim3(256), 0, stream, logits, mask, weights, indices, counts, loss,
+    if (!counts || !loss || (tokens && (!logits || !weights || !indices)) || (blocks > 1 && !workspace)) return hipErrorInvalidValue;
+    hipLaunchKernelGGL((moe_route_kernel<T, SIGMOID, LANES, VALUES>), dim3(blocks), dim3(kRouteThreads), 0, stream, logits, mask, weights, indices, counts, loss,
                        workspace, tokens, e, top_k, renormalize, rows_in_pieces<VALUES, T>(logits, e));
     if (const hipError_t rc = hipGetLastError(); rc != hipSuccess || blocks == 1) return rc;
     hipLaunchKernelGGL(moe_route_finish_kernel<0>, dim3(ceil_div(e, 16)), dim3(1024), 0, stream, counts, loss, workspace, blocks, e, top_k);

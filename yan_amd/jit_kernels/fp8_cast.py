@@ -14,7 +14,7 @@ from typing import Optional, Tuple
 
 import torch
 
-from .host_calls import PER_BLOCK, PER_CHANNEL, PER_TOKEN, remember_call, repeat_call
+from .host_calls import PER_BLOCK, PER_CHANNEL, PER_TOKEN, remember_call, remember_new, repeat_call, repeat_new
 from .tuner import FrozenKeys, jit_tuner
 from .utils import assert_on_current_device, ceil_div, current_raw_stream
 
@@ -130,28 +130,30 @@ def per_channel_cast_to_fp8(x: torch.Tensor, source: Optional[torch.Tensor] = No
     apart. A scale is the smallest power of two with `max|x| <= 448 * scale` (2^-108 for zeros); `x / scale` is rounded to the nearest code. NaN and
     infinity become NaN and do not count for the scale.
     """
+    call = (PER_CHANNEL, x, source)
+    made = repeat_new(*call)
+    if made is not None:
+        return made
     assert x.dim() == 2 and x.size(1) % 8 == 0 and x.is_contiguous()
     m, n = x.shape
     if source is not None:
         assert source.dim() == 1 and source.dtype == torch.int32 and source.is_contiguous() and source.numel() % 128 == 0
-    assert x.data_ptr() % 16 == 0 and (source is None or source.data_ptr() % 4 == 0), 'rows start at multiples of 16 bytes'
+    assert x.data_ptr() % 16 == 0 and (source is None or source.data_ptr() % 16 == 0), 'tensors start at multiples of 16 bytes'
     blocks = ceil_div(m, 128) if source is None else source.numel() // 128
-    assert m < 1 << 31 and n * ceil_div(blocks, 4) * 4 < 1 << 40
+    assert m < 1 << 31 and blocks < 1 << 24
     name, keys, arg_defs, template = cast_kernel_plan('per_channel', x.dtype)
     assert_on_current_device(x, source)
     q = torch.empty((n, blocks * 128), dtype=torch.float8_e4m3fn, device=x.device)
     stride = ceil_div(blocks, 4) * 4
-    scales = torch.empty((n, stride), dtype=torch.uint8, device=x.device)[:, :blocks]
+    scales = torch.empty((n, stride), dtype=torch.uint8, device=x.device)
+    if stride != blocks:
+        scales = scales[:, :blocks]
     if n == 0 or blocks == 0:
         return q, scales
-    gathered = int(source is not None)
-    held = source if gathered else torch.empty(1, dtype=torch.int32, device=x.device)       # stands for what is not there
-    call = (PER_CHANNEL, x, held, q, scales, gathered)
-    if repeat_call(*call):
-        return q, scales
-    args = (x, held, q, scales, gathered, m, n, blocks, stride, current_raw_stream())
+    nothing = torch.empty(1, dtype=torch.int32, device=x.device)            # stands for what is not there
+    args = (x, nothing if source is None else source, q, scales, int(source is not None), m, n, blocks, stride, current_raw_stream())
     runtime = jit_tuner.compile_and_tune(name=name, keys=keys, space=(), includes=per_channel_includes, arg_defs=arg_defs, template=template, args=args)
     rc = runtime(*args)
     assert rc == 0, f'{name} failed with HIP error {rc}'
-    remember_call((PER_CHANNEL, x, held, q, scales, gathered), name, runtime, args)
+    remember_new(call, name, runtime, args, (q, scales))
     return q, scales

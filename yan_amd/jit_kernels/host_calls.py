@@ -30,12 +30,16 @@ if getattr(_host_calls, 'built_for', None) != f'torch {torch.__version__} {torch
 # which entry a remembered call belongs to
 FP8, CAST_FP8, BF16, FP16, FLOAT, CONTIGUOUS, MASKED, PER_TOKEN, PER_BLOCK = range(1, 10)
 ROUTE, ROUTE_BACKWARD, DISPATCH, COMBINE, COMBINE_BACKWARD, PER_CHANNEL, WGRAD = range(10, 17)
-_TENSOR, _CONSTANT, _STREAM, _WORKSPACE = range(4)
+_TENSOR, _CONSTANT, _STREAM, _WORKSPACE, _OUTPUT = range(5)
 _THE_STREAM, _THE_WORKSPACE = (_STREAM, 0), (_WORKSPACE, 0)
 
 
 def _never(*_) -> bool:
     return False
+
+
+def _nothing(*_) -> None:
+    return None
 
 
 def setup_native() -> None:
@@ -45,10 +49,11 @@ def setup_native() -> None:
 
 
 repeat_call = _never
+repeat_new = _nothing
 if _host_calls is not None and utils._environ is not None:
     try:
         setup_native()
-        repeat_call = _host_calls.call
+        repeat_call, repeat_new = _host_calls.call, _host_calls.call_new
     except (AttributeError, TypeError):          # a torch without the raw accessors
         pass
 
@@ -82,3 +87,36 @@ def remember_call(call: tuple, name: str, runtime: Runtime, args: tuple, workspa
             spec.append(_THE_WORKSPACE)
     if tensors == sum([isinstance(a, torch.Tensor) for a in call]):
         _host_calls.remember(call, name, address, tuple(spec))
+
+
+def remember_new(call: tuple, name: str, runtime: Runtime, args: tuple, outputs: tuple = (), scratch: tuple = (), views: dict = {}, workspace=None) -> None:
+    """As `remember_call`, for a call that makes the tensors `outputs`, which it returns, and `scratch`: `repeat_new` makes them anew (`repeat_call` where there
+    are none). `call` has what the caller gave, in any order, None among it. A tensor of `args` that is none of all these stands for one that is not there, and its
+    address is of no account; `views` says which of the caller's tensors (by id of what is in `args`) another one is a view of."""
+    if repeat_new is _nothing or type(runtime) is not Runtime or runtime._launch is None or not split_k.split_k_enabled() or tuning_enabled():
+        return
+    utils.get_num_sms()         # part of what a call is looked up by; not every entry has asked for it
+    if runtime.native is None:
+        runtime.native = _native_parts(runtime)
+    address, kinds = runtime.native
+    given, made = [a for a in call if isinstance(a, torch.Tensor)], (*outputs, *scratch)
+    spec = []
+    for arg, kind in zip(args, kinds):
+        if kind is _CONSTANT:
+            spec.append((_CONSTANT, arg))
+        elif kind is _STREAM:
+            spec.append(_THE_STREAM)
+        elif workspace is not None and arg is workspace:
+            spec.append(_THE_WORKSPACE)
+        else:
+            arg = views.get(id(arg), arg)
+            new = [i for i, t in enumerate(made) if t is arg]
+            old = [i for i, t in enumerate(given) if t is arg]
+            spec.append((_OUTPUT, new[0]) if new else (_TENSOR, old[0]) if old else (_CONSTANT, 0))
+    shapes = []
+    for t in made:
+        # a tensor whose rows are further apart than they are long is the front of one without gaps
+        whole = t if t._base is None else t._base
+        assert whole.is_contiguous() and t.storage_offset() == 0
+        shapes.append((t, tuple(whole.shape), *(((), ()) if whole is t else (tuple(t.shape), tuple(t.stride())))))
+    _host_calls.remember(call, name, address, tuple(spec), tuple(shapes), len(outputs))

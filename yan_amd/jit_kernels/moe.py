@@ -17,7 +17,7 @@ from typing import Optional, Tuple
 
 import torch
 
-from .host_calls import COMBINE, COMBINE_BACKWARD, DISPATCH, ROUTE, ROUTE_BACKWARD, remember_call, repeat_call
+from .host_calls import COMBINE, COMBINE_BACKWARD, DISPATCH, ROUTE, ROUTE_BACKWARD, remember_new, repeat_call, repeat_new
 from .tuner import FrozenKeys, jit_tuner
 from .utils import assert_on_current_device, ceil_div, current_raw_stream, get_m_alignment_for_contiguous_layout
 
@@ -28,13 +28,15 @@ FEW_PAIRS = 4096
 TOKENS_PER_BLOCK = 16
 
 _ELEMENTS = {torch.bfloat16: '__bf16', torch.float32: 'float'}
+_SCORINGS = {'softmax': 0, 'sigmoid': 1}
 
 
-def _run(name, keys, includes, arg_defs, template, args, call):
+def _run(plan, includes, args):
+    name, keys, arg_defs, template = plan
     runtime = jit_tuner.compile_and_tune(name=name, keys=keys, space=(), includes=includes, arg_defs=arg_defs, template=template, args=args)
     rc = runtime(*args)
     assert rc == 0, f'{name} failed with HIP error {rc}'
-    remember_call(call, name, runtime, args)
+    return name, runtime, args
 
 
 # Router
@@ -81,8 +83,8 @@ def route_lanes(experts: int) -> Tuple[int, int]:
 
 def route_blocks(tokens: int, experts: int) -> int:
     """Workgroups of the router's kernel; one alone needs no second kernel to add up counts and shares."""
-    at_once = 256 // route_lanes(experts)[0]
-    return 1 if tokens <= 16 * at_once else min(ceil_div(tokens, at_once), 512)
+    at_once = 1024 // route_lanes(experts)[0]
+    return min(max(1, ceil_div(tokens, at_once)), 256)
 
 
 @functools.lru_cache(maxsize=None)
@@ -116,6 +118,10 @@ def moe_route(logits: torch.Tensor, top_k: int, scoring: str = 'softmax', renorm
     Logits of -infinity are picked after all others, with weight 0, and +infinity counts as the largest finite number. A NaN makes its token's
     weights and the loss NaN.
     """
+    call = (ROUTE, logits, mask, top_k, _SCORINGS.get(scoring, -1), 1 if renormalize else 0)
+    made = repeat_new(*call)
+    if made is not None:
+        return made
     _check_route(logits, top_k, scoring)
     tokens, experts = logits.shape
     if mask is not None:
@@ -130,13 +136,12 @@ def moe_route(logits: torch.Tensor, top_k: int, scoring: str = 'softmax', renorm
     # RouteWorkspace::bytes of moe/route.hpp
     workspace = torch.empty(4 * (2 * blocks * experts + 2 * ceil_div(experts, 16) + 1) if blocks > 1 else 4, dtype=torch.uint8, device=device)
     mask_bytes = workspace if mask is None else mask.view(torch.uint8)
-    flags = (int(mask is not None), blocks, tokens, experts, top_k, int(renormalize))
-    call = (ROUTE, logits, mask_bytes, weights, indices, counts, loss, workspace, *flags, int(scoring == 'sigmoid'))
-    if not repeat_call(*call):
-        name, keys, arg_defs, template = route_kernel_plan(logits.dtype, scoring, experts)
-        _run(name, keys, _route_includes, arg_defs, template,
-             (logits, mask_bytes, weights, indices, counts, loss, workspace, *flags, current_raw_stream()), call)
-    return weights, indices, counts, loss
+    done = _run(route_kernel_plan(logits.dtype, scoring, experts), _route_includes,
+                (logits, mask_bytes, weights, indices, counts, loss, workspace, int(mask is not None), blocks, tokens, experts, top_k, int(bool(renormalize)),
+                 current_raw_stream()))
+    made = (weights, indices, counts, loss)
+    remember_new(call, *done, made, (workspace, ), {} if mask is None else {id(mask_bytes): mask})
+    return made
 
 
 def moe_route_backward(logits: torch.Tensor, indices: torch.Tensor, counts: torch.Tensor, grad_weights: Optional[torch.Tensor],
@@ -147,7 +152,12 @@ def moe_route_backward(logits: torch.Tensor, indices: torch.Tensor, counts: torc
     grad_weights: fp32 `[tokens, top_k]`, or None for zero; grad_loss: fp32 with one element, on the device, or None for zero
     The picks and `counts` are constants of the loss. Masked tokens (indices -1) get zeros.
     """
-    top_k = indices.size(-1)
+    call = (ROUTE_BACKWARD, logits, indices, counts, grad_weights, grad_loss, _SCORINGS.get(scoring, -1), 1 if renormalize else 0)
+    made = repeat_new(*call)
+    if made is not None:
+        return made[0]
+    assert indices.dim() == 2
+    top_k = indices.size(1)
     _check_route(logits, top_k, scoring)
     tokens, experts = logits.shape
     assert indices.shape == (tokens, top_k) and indices.dtype == torch.int32 and indices.is_contiguous()
@@ -160,15 +170,11 @@ def moe_route_backward(logits: torch.Tensor, indices: torch.Tensor, counts: torc
     grad_logits = torch.empty_like(logits)
     if tokens == 0:
         return grad_logits
-    flags = (int(grad_weights is not None), int(grad_loss is not None), tokens, experts, top_k, int(renormalize))
-    if grad_weights is None or grad_loss is None:
-        given = grad_loss if grad_weights is None else grad_weights
-        given = torch.empty(1, dtype=torch.float32, device=logits.device) if given is None else given       # its address stands for what is not there
-        grad_weights, grad_loss = given if grad_weights is None else grad_weights, given if grad_loss is None else grad_loss
-    call = (ROUTE_BACKWARD, logits, indices, counts, grad_weights, grad_loss, grad_logits, *flags, int(scoring == 'sigmoid'))
-    if not repeat_call(*call):
-        name, keys, arg_defs, template = route_kernel_plan(logits.dtype, scoring, experts, True)
-        _run(name, keys, _route_includes, arg_defs, template, (logits, indices, counts, grad_weights, grad_loss, grad_logits, *flags, current_raw_stream()), call)
+    nothing = torch.empty(1, dtype=torch.float32, device=logits.device)         # stands for what is not there
+    done = _run(route_kernel_plan(logits.dtype, scoring, experts, True), _route_includes,
+                (logits, indices, counts, nothing if grad_weights is None else grad_weights, nothing if grad_loss is None else grad_loss, grad_logits,
+                 int(grad_weights is not None), int(grad_loss is not None), tokens, experts, top_k, int(bool(renormalize)), current_raw_stream()))
+    remember_new(call, *done, (grad_logits, ))
     return grad_logits
 
 
@@ -213,7 +219,8 @@ def _check_dispatch(x, indices, codes, scales, num_experts):
     assert x.data_ptr() % 16 == 0 and codes.data_ptr() % 16 == 0, 'activations and codes start at multiples of 16 bytes'
 
 
-def _dispatch(x, indices, codes, scales, num_experts, m_max, rows_of, m_indices, source, offsets):
+def _dispatch(call, x, indices, codes, scales, num_experts, m_max, made):
+    # `made`: rows and masked_m of the masked layout; rows, m_indices, source and offsets of the contiguous one
     tokens, k = x.shape
     top_k, rows = indices.size(1), codes.numel() // k
     few = tokens * top_k <= FEW_PAIRS
@@ -222,12 +229,12 @@ def _dispatch(x, indices, codes, scales, num_experts, m_max, rows_of, m_indices,
     assert workspace_bytes < 1 << 31
     workspace = torch.empty(max(workspace_bytes, 4), dtype=torch.uint8, device=x.device)
     strides = scales.stride() if m_max else (0, *scales.stride())
-    numbers = (workspace_bytes, *strides, tokens, k, top_k, num_experts, m_max, rows)
-    call = (DISPATCH, x, indices, codes, scales, rows_of, m_indices, source, offsets, workspace, num_experts, m_max)
-    if not repeat_call(*call):
-        name, keys, arg_defs, template = dispatch_kernel_plan(x.dtype)
-        _run(name, keys, _dispatch_includes, arg_defs, template,
-             (x, indices, codes, scales, rows_of, m_indices, source, offsets, workspace, *numbers, current_raw_stream()), call)
+    rows_of, m_indices, source, offsets = made if not m_max else (made[0], made[1], made[1], made[1])
+    done = _run(dispatch_kernel_plan(x.dtype), _dispatch_includes,
+                (x, indices, codes, scales, rows_of, m_indices, source, offsets, workspace, workspace_bytes, *strides, tokens, k, top_k, num_experts, m_max, rows,
+                 current_raw_stream()))
+    remember_new(call, *done, made, (workspace, ))
+    return made
 
 
 def moe_dispatch_to_fp8_contiguous(x: torch.Tensor, indices: torch.Tensor, num_experts: int,
@@ -245,6 +252,10 @@ def moe_dispatch_to_fp8_contiguous(x: torch.Tensor, indices: torch.Tensor, num_e
     (token, pick).
     """
     codes, scales = out
+    call = (DISPATCH, x, indices, codes, scales, num_experts)
+    made = repeat_new(*call)
+    if made is not None:
+        return made
     _check_dispatch(x, indices, codes, scales, num_experts)
     m_sum = codes.size(0)
     assert codes.dim() == 2 and m_sum % get_m_alignment_for_contiguous_layout() == 0
@@ -254,8 +265,7 @@ def moe_dispatch_to_fp8_contiguous(x: torch.Tensor, indices: torch.Tensor, num_e
     m_indices = torch.empty((m_sum, ), dtype=torch.int32, device=device)
     source = torch.empty((m_sum, ), dtype=torch.int32, device=device)
     offsets = torch.empty((num_experts + 1, ), dtype=torch.int32, device=device)
-    _dispatch(x, indices, codes, scales, num_experts, 0, rows, m_indices, source, offsets)
-    return rows, m_indices, source, offsets
+    return _dispatch(call, x, indices, codes, scales, num_experts, 0, (rows, m_indices, source, offsets))
 
 
 def moe_dispatch_to_fp8_masked(x: torch.Tensor, indices: torch.Tensor, out: Tuple[torch.Tensor, torch.Tensor]) -> Tuple[torch.Tensor, torch.Tensor]:
@@ -267,14 +277,17 @@ def moe_dispatch_to_fp8_masked(x: torch.Tensor, indices: torch.Tensor, out: Tupl
     and masked_m int32 `[num_experts]`, the rows that every expert has.
     """
     codes, scales = out
+    call = (DISPATCH, x, indices, codes, scales)
+    made = repeat_new(*call)
+    if made is not None:
+        return made
     assert codes.dim() == 3 and codes.size(1) > 0
     num_experts, m_max, _ = codes.shape
     _check_dispatch(x, indices, codes, scales, num_experts)
     assert_on_current_device(x, indices, codes, scales)
     rows = torch.empty_like(indices)
     masked_m = torch.empty((num_experts, ), dtype=torch.int32, device=x.device)
-    _dispatch(x, indices, codes, scales, num_experts, m_max, rows, masked_m, masked_m, masked_m)
-    return rows, masked_m
+    return _dispatch(call, x, indices, codes, scales, num_experts, m_max, (rows, masked_m))
 
 
 # And back
@@ -330,18 +343,18 @@ def moe_combine(y: torch.Tensor, rows: torch.Tensor, weights: Optional[torch.Ten
     weights: fp32 `[tokens, top_k]`, or None for 1 (the gradient of what was dispatched)
     out: bf16 `[tokens, n]`, written in place
     """
+    call = (COMBINE, y, rows, out, weights)
+    if repeat_call(*call):
+        return
     _check_combine(y, rows, weights, out)
     assert_on_current_device(y, rows, weights, out)
     tokens, columns = out.shape
     if tokens == 0 or columns == 0:
         return
-    weighted = int(weights is not None)
-    if weights is None:
-        weights = torch.empty(1, dtype=torch.float32, device=y.device)          # stands for what is not there
-    call = (COMBINE, y, rows, weights, out, weighted)
-    if not repeat_call(*call):
-        name, keys, arg_defs, template = combine_kernel_plan(rows.size(1))
-        _run(name, keys, _combine_includes, arg_defs, template, (y, rows, weights, out, weighted, tokens, columns, y.size(0), current_raw_stream()), call)
+    nothing = torch.empty(1, dtype=torch.float32, device=y.device)          # stands for what is not there
+    done = _run(combine_kernel_plan(rows.size(1)), _combine_includes,
+                (y, rows, nothing if weights is None else weights, out, int(weights is not None), tokens, columns, y.size(0), current_raw_stream()))
+    remember_new(call, *done)
 
 
 def moe_combine_backward(grad_out: torch.Tensor, y: torch.Tensor, rows: torch.Tensor, weights: Optional[torch.Tensor],
@@ -352,17 +365,19 @@ def moe_combine_backward(grad_out: torch.Tensor, y: torch.Tensor, rows: torch.Te
     grad_out: bf16 `[tokens, n]`; y, rows, weights: as given to `moe_combine`, no row twice; source: int32 `[m]`, negative for the rows that no
     pair has, as `moe_dispatch_to_fp8_contiguous` returns it
     """
+    call = (COMBINE_BACKWARD, grad_out, y, rows, weights, source)
+    made = repeat_new(*call)
+    if made is not None:
+        return made if weights is not None else (made[0], None)
     _check_combine(y, rows, weights, grad_out)
     assert source.shape == (y.size(0), ) and source.dtype == torch.int32 and source.is_contiguous()
     assert_on_current_device(grad_out, y, rows, weights, source)
     tokens, columns = grad_out.shape
     grad_y = torch.empty_like(y)
-    weighted = int(weights is not None)
-    grad_weights = torch.empty_like(weights) if weighted else torch.empty(1, dtype=torch.float32, device=y.device)
-    given = weights if weighted else grad_weights
-    call = (COMBINE_BACKWARD, grad_out, y, rows, given, source, grad_y, grad_weights, weighted)
-    if not repeat_call(*call):
-        name, keys, arg_defs, template = combine_kernel_plan(rows.size(1), True)
-        _run(name, keys, _combine_includes, arg_defs, template,
-             (grad_out, y, rows, given, source, grad_y, grad_weights, weighted, tokens, columns, y.size(0), current_raw_stream()), call)
-    return grad_y, grad_weights if weighted else None
+    grad_weights = None if weights is None else torch.empty_like(weights)
+    nothing = torch.empty(1, dtype=torch.float32, device=y.device)          # stands for what is not there
+    done = _run(combine_kernel_plan(rows.size(1), True), _combine_includes,
+                (grad_out, y, rows, nothing if weights is None else weights, source, grad_y, nothing if weights is None else grad_weights,
+                 int(weights is not None), tokens, columns, y.size(0), current_raw_stream()))
+    remember_new(call, *done, (grad_y, ) if weights is None else (grad_y, grad_weights))
+    return grad_y, grad_weights

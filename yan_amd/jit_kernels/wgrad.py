@@ -11,29 +11,31 @@ from typing import Optional, Tuple
 
 import torch
 
-from .host_calls import WGRAD, remember_call, repeat_call
+from .host_calls import WGRAD, remember_new, repeat_call
 from .tuner import FrozenKeys, jit_tuner
-from .utils import assert_on_current_device, ceil_div, current_raw_stream
+from .split_k import SPLIT_K_WORKSPACE_BYTES, split_k_launch_failed, split_k_workspace
+from .utils import assert_on_current_device, ceil_div, current_raw_stream, get_num_sms
 
 includes = ('"gemm/fp8_wgrad.hpp"', )
 
 template = """
 using namespace yan;
-__return_code = static_cast<int>(launch_fp8_wgrad(lhs, lhs_scales, ld_lhs_scales, rhs, rhs_scales, ld_rhs_scales, out, grouped ? offsets : nullptr, groups, m, n, k,
-                                                  accumulate != 0, stream));
+// Templated args from Python JIT call: {KERNEL} (kWgradAny: what wgrad_plan says) in {PARTS} parts
+__return_code = static_cast<int>(launch_fp8_wgrad<{KERNEL}, {PARTS}>(lhs, lhs_scales, ld_lhs_scales, rhs, rhs_scales, ld_rhs_scales, out, grouped ? offsets : nullptr,
+                                                                    groups, m, n, k, accumulate != 0, workspace_bytes ? workspace : nullptr, num_sms, stream));
 """
 
 arg_defs = (('lhs', torch.float8_e4m3fn), ('lhs_scales', torch.uint8), ('rhs', torch.float8_e4m3fn), ('rhs_scales', torch.uint8), ('out', torch.float),
-            ('offsets', torch.int), ('ld_lhs_scales', int), ('ld_rhs_scales', int), ('grouped', int), ('groups', int), ('m', int), ('n', int), ('k', int),
-            ('accumulate', int), ('stream', torch.cuda.Stream))
+            ('offsets', torch.int), ('workspace', torch.uint8), ('ld_lhs_scales', int), ('ld_rhs_scales', int), ('grouped', int), ('groups', int), ('m', int), ('n', int), ('k', int),
+            ('accumulate', int), ('workspace_bytes', int), ('num_sms', int), ('stream', torch.cuda.Stream))
 
-MAX_K = 1 << 23
+MAX_K, MAX_N = 1 << 23, 1 << 21
 
 
 @functools.lru_cache(maxsize=None)
-def wgrad_kernel_plan():
-    """(name, keys, arg_defs, template) of the weight-gradient kernels; needs no GPU."""
-    return 'fp8_wgrad', FrozenKeys({}), arg_defs, template
+def wgrad_kernel_plan(kernel: str = 'kWgradAny', parts: int = 1):
+    """(name, keys, arg_defs, template) of the weight-gradient kernels; needs no GPU. The entries let `wgrad_plan` of gemm/fp8_wgrad.hpp choose."""
+    return 'fp8_wgrad', FrozenKeys({'KERNEL': kernel, 'PARTS': parts}), arg_defs, template
 
 
 def _check_operand(codes, scales):
@@ -48,12 +50,15 @@ def _check_operand(codes, scales):
         assert codes.data_ptr() % 16 == 0
 
 
-def _wgrad(lhs, rhs, out, offsets: Optional[torch.Tensor], groups: int, accumulate: bool) -> None:
+def _wgrad(lhs, rhs, out, offsets: Optional[torch.Tensor], accumulate: bool, kernel: tuple = ()) -> None:
     (lhs, lhs_scales), (rhs, rhs_scales) = lhs, rhs
+    call = (WGRAD, lhs, lhs_scales, rhs, rhs_scales, out, offsets, 1 if accumulate else 0)
+    if kernel == () and repeat_call(*call):
+        return
     _check_operand(lhs, lhs_scales)
     _check_operand(rhs, rhs_scales)
     m, n, k = lhs.size(0), rhs.size(0), lhs.size(1)
-    assert rhs.size(1) == k and n % 4 == 0 and out.shape[-2:] == (m, n)
+    assert rhs.size(1) == k and n % 4 == 0 and n < MAX_N and out.shape[-2:] == (m, n)
     assert out.dtype == torch.float32 and out.is_contiguous() and out.data_ptr() % 16 == 0
     assert_on_current_device(lhs, lhs_scales, rhs, rhs_scales, out, offsets)
     if out.numel() == 0:
@@ -62,17 +67,20 @@ def _wgrad(lhs, rhs, out, offsets: Optional[torch.Tensor], groups: int, accumula
         if not accumulate:
             out.zero_()
         return
-    grouped = int(offsets is not None)
-    held = offsets if grouped else torch.empty(1, dtype=torch.int32, device=out.device)         # stands for what is not there
-    call = (WGRAD, lhs, lhs_scales, rhs, rhs_scales, out, held, grouped, int(accumulate))
-    if repeat_call(*call):
-        return
-    args = (lhs, lhs_scales, rhs, rhs_scales, out, held, lhs_scales.stride(0), rhs_scales.stride(0), grouped, groups, m, n, k, int(accumulate), current_raw_stream())
-    name, keys, defs, code_template = wgrad_kernel_plan()
+    stream = current_raw_stream()
+    workspace, token = split_k_workspace(out.device, stream)
+    nothing = torch.empty(1, dtype=torch.int32, device=out.device)          # stands for what is not there
+    args = (lhs, lhs_scales, rhs, rhs_scales, out, nothing if offsets is None else offsets, nothing.view(torch.uint8) if workspace is None else workspace,
+            lhs_scales.stride(0), rhs_scales.stride(0), int(offsets is not None), 1 if offsets is None else out.size(0), m, n, k, int(bool(accumulate)),
+            0 if workspace is None else SPLIT_K_WORKSPACE_BYTES, get_num_sms(), stream)
+    name, keys, defs, code_template = wgrad_kernel_plan(*kernel)
     runtime = jit_tuner.compile_and_tune(name=name, keys=keys, space=(), includes=includes, arg_defs=defs, template=code_template, args=args)
     rc = runtime(*args)
+    if rc != 0 and token is not None:
+        split_k_launch_failed(token)
     assert rc == 0, f'{name} failed with HIP error {rc}'
-    remember_call(call, name, runtime, args)
+    if kernel == ():
+        remember_new(call, name, runtime, args, workspace=workspace)
 
 
 def gemm_fp8_fp8_fp32_nt(lhs: Tuple[torch.Tensor, torch.Tensor], rhs: Tuple[torch.Tensor, torch.Tensor], out: torch.Tensor, accumulate: bool = False) -> None:
@@ -85,7 +93,7 @@ def gemm_fp8_fp8_fp32_nt(lhs: Tuple[torch.Tensor, torch.Tensor], rhs: Tuple[torc
     Requires k % 128 == 0 and n % 4 == 0; m is arbitrary.
     """
     assert out.dim() == 2
-    _wgrad(lhs, rhs, out, None, 1, accumulate)
+    _wgrad(lhs, rhs, out, None, accumulate)
 
 
 def k_grouped_gemm_fp8_fp8_fp32_nt_contiguous(lhs: Tuple[torch.Tensor, torch.Tensor], rhs: Tuple[torch.Tensor, torch.Tensor], out: torch.Tensor,
@@ -100,4 +108,4 @@ def k_grouped_gemm_fp8_fp8_fp32_nt_contiguous(lhs: Tuple[torch.Tensor, torch.Ten
     """
     assert out.dim() == 3 and out.size(0) > 0
     assert offsets.shape == (out.size(0) + 1, ) and offsets.dtype == torch.int32 and offsets.is_contiguous()
-    _wgrad(lhs, rhs, out, offsets, out.size(0), accumulate)
+    _wgrad(lhs, rhs, out, offsets, accumulate)
