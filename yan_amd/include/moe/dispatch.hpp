@@ -67,11 +67,21 @@ __device__ __forceinline__ void describe_rows(const int* counts, const int* star
     }
 }
 
+// Where a pair's codes and scales start, in bytes and elements; codes below 0: the pair has no row.
+struct PairPlace {
+    long long codes, scales;
+};
+__device__ __forceinline__ PairPlace place_of_row(const DispatchShape& s, int row, int expert) {
+    const int g = s.m_max ? expert : 0, m = s.m_max ? row - g * s.m_max : row;
+    return row < 0 ? PairPlace{-1, 0} : PairPlace{(long long)row * s.k_blocks * 128, g * s.stride_g + m * s.stride_m};
+}
+
 // Quantises the blocks of 128 of tokens t0, t0 + 1, ... numbered first .. last - 1 (k_blocks a token) and stores them to their tokens' rows: 16 lanes a
-// block, 16 blocks a step, UNROLL steps' loads under way at once. row_of, expert_of: [tokens][top_k], of token t0 on.
+// block, 16 blocks a step, UNROLL steps' loads under way at once. places: [tokens][top_k], of token t0 on. All lanes store a pair's codes, then lane i
+// the scale of pair i.
 template <int UNROLL, CastStream STREAM, typename T>
 __device__ __forceinline__ void scatter_blocks(const T* __restrict__ x, uint8_t* __restrict__ codes, float* __restrict__ scales, const DispatchShape& s, int t0,
-                                               int first, int last, const int* row_of, const int* expert_of) {
+                                               int first, int last, const PairPlace* places) {
     const int part = threadIdx.x & 15;
     const T* const from = x + size_t(t0) * s.k_blocks * 128;
     for (int at = first + int(threadIdx.x >> 4); at < last; at += 16 * UNROLL) {
@@ -88,15 +98,13 @@ __device__ __forceinline__ void scatter_blocks(const T* __restrict__ x, uint8_t*
             const float amax = fmaxf(max_over_16_lanes(abs_max8(f)), 1e-4f);
             const uint2 q = quantise8(f, kFp8Max / amax);
             if (block >= last) continue;
+            const PairPlace* const of = places + token * s.top_k;
+            uint8_t* const to = codes + kb * 128;
             for (int i = 0; i < s.top_k; ++i) {
-                const int row = row_of[token * s.top_k + i];
-                if (row < 0) continue;
-                store_codes8<T, STREAM == kStreamBoth>(codes + (size_t(row) * s.k_blocks + kb) * 128, part, q);
-                if (part == 0) {
-                    const int g = s.m_max ? expert_of[token * s.top_k + i] : 0, m = s.m_max ? row - g * s.m_max : row;
-                    scales[g * s.stride_g + m * s.stride_m + kb * s.stride_k] = amax / kFp8Max;
-                }
+                const long long at_row = of[i].codes;
+                if (at_row >= 0) store_codes8<T, STREAM == kStreamBoth>(to + at_row, part, q);
             }
+            if (part < s.top_k && of[part].codes >= 0) scales[of[part].scales + kb * s.stride_k] = amax / kFp8Max;
         }
     }
 }
@@ -121,7 +129,8 @@ template <typename T>
 __global__ void __launch_bounds__(256)
 moe_dispatch_few_kernel(const T* __restrict__ x, const int* __restrict__ indices, uint8_t* __restrict__ codes, float* __restrict__ scales,
                         int* __restrict__ rows, int* __restrict__ m_indices, int* __restrict__ source, int* __restrict__ offsets, DispatchShape s, int parts) {
-    __shared__ int counts[kMaxExperts], before[kMaxExperts], starts[kMaxExperts + 1], row_of[kMaxTopK], expert_of[kMaxTopK];
+    __shared__ int counts[kMaxExperts], before[kMaxExperts], starts[kMaxExperts + 1];
+    __shared__ PairPlace places[kMaxTopK];
     const int t = blockIdx.x / parts, piece = blockIdx.x % parts, pairs = s.tokens * s.top_k;
     for (int e = threadIdx.x; e < s.experts; e += 256) counts[e] = before[e] = 0;
     __syncthreads();
@@ -142,7 +151,7 @@ moe_dispatch_few_kernel(const T* __restrict__ x, const int* __restrict__ indices
             for (int i = 0; i < int(threadIdx.x); ++i) rank += mine[i] == e;
             row = row_of_pair(s, starts, e, rank);
         }
-        row_of[threadIdx.x] = row, expert_of[threadIdx.x] = e;
+        places[threadIdx.x] = place_of_row(s, row, e);
         if (piece == 0) {
             rows[t * s.top_k + threadIdx.x] = row;
             if (!s.m_max && row >= 0) source[row] = t;
@@ -155,7 +164,7 @@ moe_dispatch_few_kernel(const T* __restrict__ x, const int* __restrict__ indices
     }
     if (blockIdx.x == 0) describe_experts(counts, starts, s, offsets, m_indices);
     const int share = ceil_div(s.k_blocks, parts);
-    if (t < s.tokens) scatter_blocks<2, kPlain>(x, codes, scales, s, t, piece * share, min(s.k_blocks, (piece + 1) * share), row_of, expert_of);
+    if (t < s.tokens) scatter_blocks<2, kPlain>(x, codes, scales, s, t, piece * share, min(s.k_blocks, (piece + 1) * share), places);
 }
 
 // Many pairs, first: the histogram of every chunk of tokens, [chunks][E].
@@ -206,7 +215,8 @@ moe_dispatch_kernel(const T* __restrict__ x, const int* __restrict__ indices, co
                     DispatchShape s, int parts) {
     constexpr int PAIRS = kTokensPerBlock * kMaxTopK;
     static_assert(PAIRS == 256, "a thread a pair");
-    __shared__ int counts[kMaxExperts], starts[kMaxExperts + 1], row_of[PAIRS], expert_of[PAIRS];
+    __shared__ int counts[kMaxExperts], starts[kMaxExperts + 1], expert_of[PAIRS];
+    __shared__ PairPlace places[PAIRS];
     // Neighbouring chunks run on one XCD, at about the same time: an expert's scales of one K block are 4 bytes from each of its tokens, and come together to
     // lines in the L2 that way.
     const int chunks = ceil_div(s.tokens, kTokensPerBlock), per_xcd = ceil_div(chunks * parts, kNumXCD);
@@ -226,7 +236,7 @@ moe_dispatch_kernel(const T* __restrict__ x, const int* __restrict__ indices, co
             for (int i = 0; i < p; ++i) rank += expert_of[i] == e;
             row = row_of_pair(s, starts, e, rank);
         }
-        row_of[p] = row;
+        places[p] = place_of_row(s, row, e);
         if (piece == 0) {
             rows[size_t(t0) * s.top_k + p] = row;
             if (!s.m_max && row >= 0) source[row] = t0 + p / s.top_k;
@@ -239,7 +249,7 @@ moe_dispatch_kernel(const T* __restrict__ x, const int* __restrict__ indices, co
     }
     if (work == 0) describe_experts(counts, starts, s, offsets, m_indices);
     const int blocks = here * s.k_blocks, share = ceil_div(blocks, parts);
-    scatter_blocks<4, STREAM>(x, codes, scales, s, t0, piece * share, min(blocks, (piece + 1) * share), row_of, expert_of);
+    scatter_blocks<4, STREAM>(x, codes, scales, s, t0, piece * share, min(blocks, (piece + 1) * share), places);
 }
 
 // Bytes of workspace a launch wants: the table of many pairs.

@@ -143,7 +143,8 @@ moe_route_kernel(const T* __restrict__ logits, const uint8_t* __restrict__ mask,
                  int* __restrict__ counts, float* __restrict__ loss, void* workspace, int tokens, int e, int top_k, bool renormalize, bool whole) {
     constexpr int GROUPS = kRouteThreads / LANES, WAVES = kRouteThreads / kWaveSize;
     __shared__ float lds_share[WAVES][LANES * VALUES];
-    __shared__ int lds_counts[LANES * VALUES], lds_pick[GROUPS][kMaxTopK];
+    __shared__ int lds_counts[LANES * VALUES];
+    __shared__ uint2 lds_pick[GROUPS][kMaxTopK];
     __shared__ float lds_pull[WAVES];
     __shared__ int lds_picks[WAVES];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, in_group = lane % LANES, first = in_group * VALUES, group_base = lane - in_group;
@@ -182,23 +183,25 @@ moe_route_kernel(const T* __restrict__ logits, const uint8_t* __restrict__ mask,
         Places places = 0;
 #pragma unroll
         for (int j = 0; j < VALUES; ++j) places |= Places(place[j]) << (4 * j);
-        uint32_t my_key = 0, best = 0;
-        int* const picks = lds_pick[threadIdx.x / LANES];
+        uint2* const picks = lds_pick[threadIdx.x / LANES];
         float top = 0.f;
+#pragma unroll 2
         for (int i = 0; i < top_k; ++i) {
-            best = max_lanes<LANES>(key[0]);
+            const uint32_t best = max_lanes<LANES>(key[0]);
             const unsigned long long have = __ballot(key[0] == best) >> group_base;
-            const bool mine = in_group == __ffsll((long long)have) - 1;
-            if (mine) picks[i] = first + int(places & 15);
-            places = mine ? places >> 4 : places;
+            if (in_group == __ffsll((long long)have) - 1) {
+                picks[i] = make_uint2(uint32_t(first) + uint32_t(places & 15), best);
+                places >>= 4;
 #pragma unroll
-            for (int j = 0; j + 1 < VALUES; ++j) key[j] = mine ? key[j + 1] : key[j];
-            key[VALUES - 1] = mine ? 0u : key[VALUES - 1];
+                for (int j = 0; j + 1 < VALUES; ++j) key[j] = key[j + 1];
+                key[VALUES - 1] = 0u;
+            }
             if (i == 0) top = value_of_key(best);
-            if (in_group == i) my_key = best;
         }
         asm volatile("" ::: "memory");          // a wave's LDS operations are done in order
-        const int my_pick = in_group < top_k ? picks[in_group] : 0;
+        const uint2 mine_at = in_group < top_k ? picks[in_group] : make_uint2(0, 0);
+        const int my_pick = int(mine_at.x);
+        const uint32_t my_key = mine_at.y;
         if (live && in_group < top_k) atomicAdd(&lds_counts[my_pick], 1);
         asm volatile("" ::: "memory");
         top = finite_top(top);
