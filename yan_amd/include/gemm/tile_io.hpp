@@ -210,10 +210,12 @@ meet_partials(Sums&& sums, float* __restrict__ partials, unsigned* __restrict__ 
     constexpr int kDeviceScope = 16;        // cache-policy bit sc1 of gfx950 buffer instructions
     constexpr uint32_t VEC_BYTES = kWaveSize * 16, WAVE_BYTES = VECS * VEC_BYTES, PART_BYTES = NW * WAVE_BYTES;
     const __amdgpu_buffer_rsrc_t parts = make_rsrc(partials + size_t(tile_slot) * (SPLIT_K * PART_BYTES / 4), SPLIT_K * PART_BYTES);
-    const uint32_t lane_off = uint32_t(wave) * WAVE_BYTES + lane * 16;
+    const uint32_t lane_off = uint32_t(wave) * WAVE_BYTES + lane * 16, mine = lane_off + uint32_t(split) * PART_BYTES;
+    // All of a store's offset is in the lane's register: of one whose offset is partly in a scalar register the compiler thinks that its 16 bytes may be
+    // overwritten by the next instruction, and the last lanes then store what came next.
 #pragma unroll
     for (int v = 0; v < VECS; ++v)
-        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(i32x4, f32x4(sums(v))), parts, lane_off + v * VEC_BYTES, split * PART_BYTES, kDeviceScope);
+        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(i32x4, f32x4(sums(v))), parts, mine + v * VEC_BYTES, 0, kDeviceScope);
     // the sums have reached memory before the count is taken
     __builtin_amdgcn_s_waitcnt(waitcnt_imm(0, kNoWaitLgkm));
     asm volatile("" ::: "memory");
