@@ -719,8 +719,8 @@ def jit_kernels_in_use(num_cus: int = 256):
     for dtype in (torch.bfloat16, torch.float32):
         for scoring in ('softmax', 'sigmoid'):
             for experts in (64, 128, 256, 512, 1024):
-                for backward in (False, True):
-                    name, keys, arg_defs, code_template = moe.route_kernel_plan(dtype, scoring, experts, backward)
+                for backward, threads in ((False, 256), (False, 1024), (True, 0)):
+                    name, keys, arg_defs, code_template = moe.route_kernel_plan(dtype, scoring, experts, backward, threads)
                     add(name, arg_defs, moe._route_includes, code_template, keys)
         name, keys, arg_defs, code_template = moe.dispatch_kernel_plan(dtype)
         add(name, arg_defs, moe._dispatch_includes, code_template, keys)

@@ -685,6 +685,24 @@ def test_on_other_streams_and_at_the_same_time():
             assert all(torch.equal(p, q) for p, q in zip(a, b)), round_
 
 
+@pytest.mark.parametrize('tokens,experts,top_k', [(5, 256, 8), (256, 256, 8), (257, 256, 8), (1024, 64, 6), (1025, 64, 6), (100, 500, 4), (70, 1024, 2)])
+def test_route_joined_by_the_last_workgroup_and_by_a_second_kernel(tokens, experts, top_k, monkeypatch):
+    """Counts and loss of few tokens are joined in the split-K workspace, which products use too; without it, by a second kernel."""
+    logits = 2 * torch.randn(tokens, experts, generator=_gen(tokens), device='cuda')
+    a = torch.randint(0, 100, (16, 4096), generator=_gen(1), device='cuda').to(torch.uint8).view(F8), torch.full((16, 32), 120, dtype=torch.uint8, device='cuda')
+    products = torch.zeros(2, 16, 16, device='cuda')
+    joined = []
+    for n in range(2):          # the second natively
+        joined.append(yan.moe_route(logits, top_k))
+        yan.gemm_fp8_fp8_fp32_nt(a, a, products[n])
+    monkeypatch.setenv('YAN_SPLIT_K', '0')
+    apart = yan.moe_route(logits, top_k)
+    assert all(torch.equal(p, q) for p, q in zip(*joined)) and torch.equal(products[0], products[1])
+    assert all(torch.equal(p, q) for p, q in zip(joined[0][:3], apart[:3]))
+    # the sums of a share have at most 64 rows added in one order or in another, each addition off by u of what is not negative
+    _close(joined[0][3], apart[3].double(), 2 * 64 * U * apart[3].double().abs())
+
+
 def test_repeated_calls_take_what_each_is_given():
     """Calls of known sizes are made natively: other inputs, other settings, other layouts and other memory each time, and new outputs."""
     x, logits, grad = _inputs(31)

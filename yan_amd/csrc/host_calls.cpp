@@ -200,6 +200,31 @@ bool eager_workspace(int64_t device, int64_t stream, PyObject** token, PyObject*
     return found;
 }
 
+// The workspace of a launch for as long as the launch takes.
+struct Workspace {
+    PyObject *tensor = nullptr, *token = nullptr;
+    uint64_t address = 0;
+    Workspace() = default;
+    Workspace(const Workspace&) = delete;
+    Workspace& operator=(const Workspace&) = delete;
+    ~Workspace() {
+        Py_XDECREF(tensor);
+        Py_XDECREF(token);
+    }
+    // False in a capture, which has its own, and where Python has to make or clear one
+    bool take(int64_t device, int64_t stream) {
+        PyObject* capturing = PyObject_CallNoArgs(g_capturing);
+        const bool eager = capturing == Py_False;
+        Py_XDECREF(capturing);
+        if (!eager || !eager_workspace(device, stream, &token, &tensor)) {
+            PyErr_Clear();
+            return false;
+        }
+        address = reinterpret_cast<uint64_t>(THPVariable_Unpack(tensor).data_ptr());
+        return true;
+    }
+};
+
 // A launch that reported an error, as the Python way reports it. It is not made again: the code can be that of an older error of this
 // thread, asked for behind a launch that did run (c = alpha a b + beta c would be applied twice).
 PyObject* launch_failed(const std::string& name, PyObject* token, int rc) {
@@ -230,36 +255,22 @@ PyObject* call(PyObject*, PyObject* const* objs, Py_ssize_t n) {
         if (!l || !l->outputs.empty()) Py_RETURN_FALSE;
         int64_t stream;
         if (!current_stream(c.device, &stream)) Py_RETURN_FALSE;
-        PyObject *workspace = nullptr, *token = nullptr;
-        uint64_t workspace_address = 0;
-        if (l->workspace) {
-            // a capture has its own
-            PyObject* capturing = PyObject_CallNoArgs(g_capturing);
-            const bool eager = capturing == Py_False;
-            Py_XDECREF(capturing);
-            if (!eager || !eager_workspace(c.device, stream, &token, &workspace)) {
-                PyErr_Clear();
-                Py_RETURN_FALSE;
-            }
-            workspace_address = reinterpret_cast<uint64_t>(THPVariable_Unpack(workspace).data_ptr());
-        }
+        Workspace workspace;
+        if (l->workspace && !workspace.take(c.device, stream)) Py_RETURN_FALSE;
         uint64_t args[kMaxArgs];
         for (int i = 0; i < l->count; ++i) {
             switch (l->kind[i]) {
                 case kTensor: args[i] = c.address[l->value[i]]; break;
                 case kConstant: args[i] = uint64_t(l->value[i]); break;
                 case kStream: args[i] = uint64_t(stream); break;
-                default: args[i] = workspace_address;
+                default: args[i] = workspace.address;
             }
         }
         int rc;
         Py_BEGIN_ALLOW_THREADS
         rc = launch_of<kMaxArgs>(l->count, l->function, args, c.floats);
         Py_END_ALLOW_THREADS
-        Py_XDECREF(workspace);
-        PyObject* const failed = rc != 0 ? launch_failed(l->name, token, rc) : nullptr;
-        Py_XDECREF(token);
-        if (rc != 0) return failed;
+        if (rc != 0) return launch_failed(l->name, workspace.token, rc);
         Py_RETURN_TRUE;
     } catch (...) {         // a tensor without storage, say: the checks in Python will say so
         PyErr_Clear();
@@ -276,7 +287,9 @@ PyObject* call_new(PyObject*, PyObject* const* objs, Py_ssize_t n) {
         if (!usual_switches() || !describe(c, objs, n)) Py_RETURN_NONE;
         const std::shared_ptr<const Launch> l = find(c);
         int64_t stream;
-        if (!l || l->outputs.empty() || l->workspace || !current_stream(c.device, &stream)) Py_RETURN_NONE;
+        if (!l || l->outputs.empty() || !current_stream(c.device, &stream)) Py_RETURN_NONE;
+        Workspace workspace;
+        if (l->workspace && !workspace.take(c.device, stream)) Py_RETURN_NONE;
         std::vector<at::Tensor> made;
         made.reserve(l->outputs.size());
         for (const Output& o : l->outputs) {
@@ -290,6 +303,7 @@ PyObject* call_new(PyObject*, PyObject* const* objs, Py_ssize_t n) {
                 case kTensor: args[i] = c.address[l->value[i]]; break;
                 case kOutput: args[i] = reinterpret_cast<uint64_t>(made[size_t(l->value[i])].data_ptr()); break;
                 case kStream: args[i] = uint64_t(stream); break;
+                case kWorkspace: args[i] = workspace.address; break;
                 default: args[i] = uint64_t(l->value[i]);
             }
         }
@@ -297,7 +311,7 @@ PyObject* call_new(PyObject*, PyObject* const* objs, Py_ssize_t n) {
         Py_BEGIN_ALLOW_THREADS
         rc = launch_of<kMaxArgs>(l->count, l->function, args, c.floats);
         Py_END_ALLOW_THREADS
-        if (rc != 0) return launch_failed(l->name, nullptr, rc);
+        if (rc != 0) return launch_failed(l->name, workspace.token, rc);
         PyObject* result = PyTuple_New(Py_ssize_t(l->returned));
         for (size_t i = 0; result && i < l->returned; ++i) {
             PyObject* t = THPVariable_Wrap(made[i]);

@@ -9,8 +9,8 @@
 // A group of LANES lanes holds a row, VALUES neighbouring logits a lane, so that lower lanes have lower experts. Picks are made on the logits
 // (both scores grow with them) as unsigned keys of the same order: every lane sorts its own, then a round is the maximum over the lanes' first keys, and the
 // lowest lane that has it gives up its first. What is summed over tokens, p, stays in the registers of the lane that owns the expert, picks are
-// counted in LDS; a workgroup leaves one row of both, and a second, small kernel adds the rows up in their order: no float atomics, the same bits
-// every time.
+// counted in LDS; a workgroup leaves one row of both. Few rows are added up by the workgroup that arrives last, many by a second, small kernel, both in the
+// order of the workgroups: no float atomics, the same bits every time.
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -19,13 +19,13 @@
 #include <limits>
 #include <type_traits>
 
+#include "../gemm/scheduler.hpp"
 #include "lanes.hpp"
 
 namespace yan {
 
 constexpr int kMaxTopK = 16;            // lane i of a group holds pick i
 constexpr int kMaxExperts = 1024;
-constexpr int kRouteThreads = 1024;     // of a workgroup of the forward: what is left of it is added up by few
 
 // The order of floats as the order of unsigned numbers; above 0, which is left for what has been taken out. -0 and 0 are one value. A NaN
 // is picked after everything else, as -infinity is (its row's weights are NaN all the same).
@@ -137,11 +137,11 @@ __device__ __forceinline__ float balance_loss(float pull, int picks, int top_k, 
     return picks == 0 ? 0.f : pull * float(e) / (float(top_k) * n * n);
 }
 
-template <typename T, bool SIGMOID, int LANES, int VALUES>
-__global__ void __launch_bounds__(kRouteThreads)
+template <typename T, bool SIGMOID, int LANES, int VALUES, int THREADS>
+__global__ void __launch_bounds__(THREADS)
 moe_route_kernel(const T* __restrict__ logits, const uint8_t* __restrict__ mask, float* __restrict__ weights, int* __restrict__ indices,
-                 int* __restrict__ counts, float* __restrict__ loss, void* workspace, int tokens, int e, int top_k, bool renormalize, bool whole) {
-    constexpr int GROUPS = kRouteThreads / LANES, WAVES = kRouteThreads / kWaveSize;
+                 int* __restrict__ counts, float* __restrict__ loss, void* workspace, int tokens, int e, int top_k, bool renormalize, bool whole, bool join) {
+    constexpr int GROUPS = THREADS / LANES, WAVES = THREADS / kWaveSize;
     __shared__ float lds_share[WAVES][LANES * VALUES];
     __shared__ int lds_counts[LANES * VALUES];
     __shared__ uint2 lds_pick[GROUPS][kMaxTopK];
@@ -151,7 +151,7 @@ moe_route_kernel(const T* __restrict__ logits, const uint8_t* __restrict__ mask,
     float share[VALUES];
 #pragma unroll
     for (int j = 0; j < VALUES; ++j) share[j] = 0.f;
-    for (int x = threadIdx.x; x < LANES * VALUES; x += kRouteThreads) lds_counts[x] = 0;
+    for (int x = threadIdx.x; x < LANES * VALUES; x += THREADS) lds_counts[x] = 0;
     __syncthreads();
 
     // the logits of a round are loaded in the round before
@@ -227,9 +227,12 @@ moe_route_kernel(const T* __restrict__ logits, const uint8_t* __restrict__ mask,
     __syncthreads();
     const RouteWorkspace to(workspace, gridDim.x, e);
     const bool alone = gridDim.x == 1;
+    // Joined here: expert by expert a sum and a count, written and read at device scope, since the workgroups are on different XCDs, whose L2s do not
+    // see each other's lines.
+    unsigned long long* const meet = reinterpret_cast<unsigned long long*>(static_cast<uint8_t*>(workspace) + kSplitKCounterBytes);
     float pull = 0.f;
     int picks = 0;
-    for (int x = threadIdx.x; x < e; x += kRouteThreads) {
+    for (int x = threadIdx.x; x < e; x += THREADS) {
         float sum = 0.f;
 #pragma unroll
         for (int w = 0; w < WAVES; ++w) sum += lds_share[w][x];
@@ -238,14 +241,43 @@ moe_route_kernel(const T* __restrict__ logits, const uint8_t* __restrict__ mask,
             counts[x] = number;
             pull += float(number) * sum;
             picks += number;
+        } else if (join) {
+            __hip_atomic_store(meet + size_t(blockIdx.x) * e + x, uint64_t(uint32_t(number)) << 32 | __builtin_bit_cast(uint32_t, sum), __ATOMIC_RELAXED,
+                               __HIP_MEMORY_SCOPE_AGENT);
         } else {
             to.share[size_t(blockIdx.x) * e + x] = sum;
             to.counts[size_t(blockIdx.x) * e + x] = number;
         }
     }
-    if (!alone) {
+    if (!alone && !join) {
         if (blockIdx.x == 0 && threadIdx.x == 0) *to.arrived = 0;
         return;
+    }
+    if (!alone) {
+        // the workgroup that arrives last adds up, in the order of the workgroups whichever it is, and leaves the counter at zero
+        __shared__ unsigned lds_before;
+        unsigned* const counter = static_cast<unsigned*>(workspace);
+        __builtin_amdgcn_s_waitcnt(waitcnt_imm(0, 0));
+        __syncthreads();
+        if (threadIdx.x == 0) lds_before = __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        __syncthreads();
+        if (lds_before != gridDim.x - 1) return;
+        if (threadIdx.x == 0) __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        for (int x = threadIdx.x; x < e; x += THREADS) {
+            float sum = 0.f;
+            int number = 0;
+            for (int b0 = 0; b0 < int(gridDim.x); b0 += 16) {
+                unsigned long long part[16];
+#pragma unroll
+                for (int b = 0; b < 16; ++b)
+                    part[b] = b0 + b < int(gridDim.x) ? __hip_atomic_load(meet + size_t(b0 + b) * e + x, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : 0;
+#pragma unroll
+                for (int b = 0; b < 16; ++b) sum += __builtin_bit_cast(float, uint32_t(part[b])), number += int(part[b] >> 32);
+            }
+            counts[x] = number;
+            pull += float(number) * sum;
+            picks += number;
+        }
     }
     pull = sum_lanes<64>(pull), picks = sum_lanes<64>(picks);
     if (lane == 0) lds_pull[wave] = pull, lds_picks[wave] = picks;
@@ -387,15 +419,17 @@ moe_route_backward_kernel(const T* __restrict__ logits, const int* __restrict__ 
     }
 }
 
-// `blocks`: workgroups of the launch; with more than one, `workspace` has RouteWorkspace::bytes(blocks, e) bytes.
-template <typename T, bool SIGMOID, int LANES, int VALUES>
+// `blocks`: workgroups of the launch. With more than one, `workspace` has RouteWorkspace::bytes(blocks, e) bytes; or, with `join`, it is a split-K workspace
+// (kSplitKWorkspaceBytes, its counters at zero), and there is no second kernel.
+template <typename T, bool SIGMOID, int LANES, int VALUES, int THREADS>
 inline hipError_t launch_moe_route(const T* logits, const uint8_t* mask, float* weights, int* indices, int* counts, float* loss, void* workspace,
-                                   int blocks, int tokens, int e, int top_k, bool renormalize, hipStream_t stream) {
+                                   int blocks, bool join, int tokens, int e, int top_k, bool renormalize, hipStream_t stream) {
     if (tokens < 0 || e < 1 || e > LANES * VALUES || top_k < 1 || top_k > e || top_k > kMaxTopK || top_k > LANES || blocks < 1) return hipErrorInvalidValue;
     if (!counts || !loss || (tokens && (!logits || !weights || !indices)) || (blocks > 1 && !workspace)) return hipErrorInvalidValue;
-    hipLaunchKernelGGL((moe_route_kernel<T, SIGMOID, LANES, VALUES>), dim3(blocks), dim3(kRouteThreads), 0, stream, logits, mask, weights, indices, counts, loss,
-                       workspace, tokens, e, top_k, renormalize, rows_in_pieces<VALUES, T>(logits, e));
-    if (const hipError_t rc = hipGetLastError(); rc != hipSuccess || blocks == 1) return rc;
+    if (join && size_t(blocks) * e * 8 > kSplitKWorkspaceBytes - kSplitKCounterBytes) return hipErrorInvalidValue;
+    hipLaunchKernelGGL((moe_route_kernel<T, SIGMOID, LANES, VALUES, THREADS>), dim3(blocks), dim3(THREADS), 0, stream, logits, mask, weights, indices, counts,
+                       loss, workspace, tokens, e, top_k, renormalize, rows_in_pieces<VALUES, T>(logits, e), join);
+    if (const hipError_t rc = hipGetLastError(); rc != hipSuccess || blocks == 1 || join) return rc;
     hipLaunchKernelGGL(moe_route_finish_kernel<0>, dim3(ceil_div(e, 16)), dim3(1024), 0, stream, counts, loss, workspace, blocks, e, top_k);
     return hipGetLastError();
 }
