@@ -568,8 +568,8 @@ fp8_wgrad_tall_kernel(WgradProblem p) {
 //     31.7 in 2, 4 and 8, 31.8 in 16; 56 tiles of 39: 26.7 whole, 15.7 in 4, 21.1 in 8);
 //   * between the other two goes an estimate in us of rounds over the chip times a k-tile of the tile, 2.6 for 256 x 256, 1.7 for two of 128 x 128 on a
 //     compute unit, and what storing it takes. 448 large tiles of 128 k-tiles 692 against 868; 420 of 33 188 / 215; 192 of 60 155 / 173; 104 of 38
-//     94.6 / 75.8; 7168 of 2.5 398 / 459, accumulated 835 / 776. The smaller tile is kept where the two are within 5 %, which is where the output's
-//     traffic decides (1725 of 1 192 / 150).
+//     94.6 / 75.8; 7168 of 2 398 / 503, of 5 575 / 732, accumulated 803 / 771 and 1036 / 1044; 2048 of 4, accumulated, 267 / 312. The smaller tile is kept
+//     where the two are within 5 %, which is where the output's traffic decides (1725 of 1 192 / 150).
 enum WgradKernel { kWgradAny, kWgradTall, kWgrad128, kWgrad64, kWgradSplit };
 struct WgradPlan {
     WgradKernel kernel;
@@ -587,7 +587,7 @@ inline WgradPlan wgrad_plan(int m, int n, int k, int groups, bool accumulate, in
         return {kWgrad64, 1};
     }
     const double tall = ceil_div(tiles(256), (long long)num_cus) * (2.6 * k_tiles + (accumulate ? 18 : 10));
-    const double middle = ceil_div(tiles(128), 2ll * num_cus) * (1.7 * k_tiles + (accumulate ? 7 : 5));
+    const double middle = ceil_div(tiles(128), 2ll * num_cus) * (1.7 * k_tiles + (accumulate ? 8.5 : 5));
     return {tall < 0.95 * middle ? kWgradTall : kWgrad128, 1};
 }
 

@@ -248,13 +248,14 @@ def _dispatch(call, x, indices, codes, scales, num_experts, m_max, made):
     # moe_dispatch_workspace_bytes of moe/dispatch.hpp
     workspace_bytes = 0 if few else (ceil_div(tokens, TOKENS_PER_BLOCK) + 1) * num_experts * 4
     assert workspace_bytes < 1 << 31
-    workspace = torch.empty(max(workspace_bytes, 4), dtype=torch.uint8, device=x.device)
+    scratch = None if few else torch.empty(workspace_bytes, dtype=torch.uint8, device=x.device)
+    workspace = made[0].view(torch.uint8) if few else scratch           # no call with few pairs looks at it
     strides = scales.stride() if m_max else (0, *scales.stride())
     rows_of, m_indices, source, offsets = made if not m_max else (made[0], made[1], made[1], made[1])
     done = _run(dispatch_kernel_plan(x.dtype), _dispatch_includes,
                 (x, indices, codes, scales, rows_of, m_indices, source, offsets, workspace, workspace_bytes, *strides, tokens, k, top_k, num_experts, m_max, rows,
                  current_raw_stream()))
-    remember_new(call, *done, made, (workspace, ))
+    remember_new(call, *done, made, () if few else (scratch, ))
     return made
 
 
