@@ -151,3 +151,15 @@ def test_weight_gradients_refuse():
     _refused(grouped, a, b, torch.zeros(2, 16, 8), offsets[:2])
     _refused(grouped, a, b, torch.zeros(2, 16, 8), offsets.long())
     _refused(grouped, a, b, torch.zeros(0, 16, 8), offsets[:1])
+
+
+def test_more_tokens_than_a_launch_counts_are_refused():
+    most = moe.MAX_TOKENS
+    for tokens in (most, most + 1):
+        logits, out = torch.empty(tokens, 4, device='meta'), torch.empty(tokens, 8, dtype=torch.bfloat16, device='meta')
+        y, rows = torch.empty(4, 8, dtype=torch.bfloat16, device='meta'), torch.empty(tokens, 1, dtype=torch.int32, device='meta')
+        if tokens <= most:
+            moe._check_route(logits, 2, 'softmax')
+        else:
+            _refused(moe._check_route, logits, 2, 'softmax')
+            _refused(moe._check_combine, y, rows, None, out)

@@ -106,9 +106,14 @@ fp8_wgrad_kernel(WgradProblem p, WgradWorkspace w, int parts) {
     constexpr int NW = 4, WTM = BLOCK_M / 2, WTN = BLOCK_N / 2, TM = WTM / 16, TN = WTN / 16;
     using StA = TileStager<BLOCK_M, NW>;
     using StB = TileStager<BLOCK_N, NW>;
-    constexpr int NUM_COPIES = StA::PASSES + StB::PASSES, A_BYTES = BLOCK_M * kRowBytes, STAGE_BYTES = (BLOCK_M + BLOCK_N) * kRowBytes;
+    constexpr int NUM_COPIES = StA::PASSES + StB::PASSES + 1, A_BYTES = BLOCK_M * kRowBytes, STAGE_BYTES = (BLOCK_M + BLOCK_N) * kRowBytes;
     static_assert(StA::PADDED_ROWS == BLOCK_M && StB::PADDED_ROWS == BLOCK_N && (STAGES - 2) * NUM_COPIES <= 63);
+    // Scales are copied with their k-tile, a dword of four k-tiles' a row, a row a lane: loaded into registers every fourth k-tile they made the wave wait for all
+    // copies under way (SCALES_MEASURED).
+    constexpr int SCALE_ROWS = NW * kWaveSize;
+    static_assert(BLOCK_M % kWaveSize == 0 && BLOCK_M + BLOCK_N <= SCALE_ROWS);
     __shared__ __attribute__((aligned(1024))) uint8_t ring[STAGES * STAGE_BYTES];
+    __shared__ __attribute__((aligned(1024))) uint32_t ring_scales[STAGES * SCALE_ROWS];
 
     const XcdTileScheduler<> sched(p.m, p.n, BLOCK_M, BLOCK_N);
     const int per_group = sched.grid_size(), slots = per_group * p.groups * (SPLIT ? parts : 1);
@@ -137,18 +142,23 @@ fp8_wgrad_kernel(WgradProblem p, WgradWorkspace w, int parts) {
         const int rows_a = min(BLOCK_M, p.m - m0), rows_b = min(BLOCK_N, p.n - n0);
         const __amdgpu_buffer_rsrc_t rsrc_a = make_rsrc(p.a + size_t(m0) * p.k + size_t(lo) * 128, uint32_t(rows_a) * p.k - uint32_t(lo) * 128);
         const __amdgpu_buffer_rsrc_t rsrc_b = make_rsrc(p.b + size_t(n0) * p.k + size_t(lo) * 128, uint32_t(rows_b) * p.k - uint32_t(lo) * 128);
-        const __amdgpu_buffer_rsrc_t rsrc_sa = make_rsrc(p.sa + size_t(m0) * p.ld_sa, uint32_t(rows_a) * p.ld_sa);
-        const __amdgpu_buffer_rsrc_t rsrc_sb = make_rsrc(p.sb + size_t(n0) * p.ld_sb, uint32_t(rows_b) * p.ld_sb);
+        // this wave's rows of scales: of a, of b, or (64 x 64) once more b's, which nobody reads; the last row stands for those behind it
+        const bool of_a = wave < BLOCK_M / kWaveSize;
+        const int ld_s = of_a ? p.ld_sa : p.ld_sb, rows_s = of_a ? rows_a : rows_b;
+        const __amdgpu_buffer_rsrc_t rsrc_s = make_rsrc(of_a ? p.sa + size_t(m0) * ld_s : p.sb + size_t(n0) * ld_s, uint32_t(rows_s) * ld_s);
+        const uint32_t off_s = uint32_t(min(wave * kWaveSize + lane - (of_a ? 0 : BLOCK_M), rows_s - 1)) * ld_s;
         StA stage_a;
         StB stage_b;
         stage_a.init(0, p.k, wave, lane);
         stage_b.init(0, p.k, wave, lane);
         const int count = hi - lo;
         // (a copy of nothing, out of range, may still write its zeros when it has been counted as done: none is issued, the ring is used again below)
-        auto copy = [&](int kt, uint8_t* stage) {
+        auto copy = [&](int kt, int st) {
             if (kt >= count) return;
+            uint8_t* const stage = ring + st * STAGE_BYTES;
             stage_a.issue(rsrc_a, stage, kt * kRowBytes, wave);
             stage_b.issue(rsrc_b, stage + A_BYTES, kt * kRowBytes, wave);
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc_s, YAN_LDS_PTR(ring_scales + st * SCALE_ROWS + wave * kWaveSize), 4, off_s, (lo + kt) & ~3, 0, 0);
         };
         // a lane reads chunks 2 g and 2 g + 1 of its row, sixteen codes each for two 16x16x32 MFMAs
         const int off[2] = {frag_offset<16>(lane, 2 * g), frag_offset<16>(lane, 2 * g + 1)};
@@ -159,31 +169,25 @@ fp8_wgrad_kernel(WgradProblem p, WgradWorkspace w, int parts) {
 #pragma unroll
             for (int j = 0; j < TM; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
 
-        for (int t = 0; t < STAGES - 1; ++t) copy(t, ring + t * STAGE_BYTES);
-        int st = 0, quad_a[TM], quad_b[TN];
+        for (int t = 0; t < STAGES - 1; ++t) copy(t, t);
+        int st = 0;
         for (int kt = 0; kt < count; ++kt) {
-            const int at = lo + kt;
-            if (kt == 0 || at % 4 == 0) {
-#pragma unroll
-                for (int j = 0; j < TM; ++j) quad_a[j] = __builtin_amdgcn_raw_buffer_load_b32(rsrc_sa, uint32_t(wm * WTM + j * 16 + col) * p.ld_sa, at & ~3, 0);
-#pragma unroll
-                for (int i = 0; i < TN; ++i) quad_b[i] = __builtin_amdgcn_raw_buffer_load_b32(rsrc_sb, uint32_t(wn * WTN + i * 16 + col) * p.ld_sb, at & ~3, 0);
-            }
             // the copies behind this k-tile's are those of STAGES - 2 k-tiles, until the range ends
             if (STAGES > 2 && kt + STAGES - 2 < count) __builtin_amdgcn_s_waitcnt(waitcnt_imm((STAGES - 2) * NUM_COPIES, 0));
             else __builtin_amdgcn_s_waitcnt(waitcnt_imm(0, 0));
             asm volatile("" ::: "memory");
             __builtin_amdgcn_s_barrier();
             asm volatile("" ::: "memory");
-            copy(kt + STAGES - 1, ring + (st == 0 ? STAGES - 1 : st - 1) * STAGE_BYTES);
+            copy(kt + STAGES - 1, st == 0 ? STAGES - 1 : st - 1);
             const uint8_t* pa = ring + st * STAGE_BYTES + wm * WTM * kRowBytes;
             const uint8_t* pb = ring + st * STAGE_BYTES + A_BYTES + wn * WTN * kRowBytes;
-            const int shift = at % 4 * 8;
+            const uint32_t* const scales = ring_scales + st * SCALE_ROWS + col;
+            const int shift = (lo + kt) % 4 * 8;
             float scale_a[TM], scale_b[TN];
 #pragma unroll
-            for (int j = 0; j < TM; ++j) scale_a[j] = wgrad_scale(quad_a[j], shift);
+            for (int j = 0; j < TM; ++j) scale_a[j] = wgrad_scale(int(scales[wm * WTM + j * 16]), shift);
 #pragma unroll
-            for (int i = 0; i < TN; ++i) scale_b[i] = wgrad_scale(quad_b[i], shift);
+            for (int i = 0; i < TN; ++i) scale_b[i] = wgrad_scale(int(scales[BLOCK_M + wn * WTN + i * 16]), shift);
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
                 i32x4 raw_a[TM], raw_b[TN];

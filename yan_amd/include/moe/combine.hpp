@@ -146,7 +146,7 @@ moe_combine_backward_kernel(const __bf16* __restrict__ grad_out, const __bf16* _
 // y [rows, columns], columns % 8 == 0, both 16-byte aligned
 template <int TOP_K>
 inline hipError_t launch_moe_combine(const __bf16* y, const int* rows_of, const float* weights, __bf16* out, int tokens, int columns, int rows, hipStream_t stream) {
-    if (tokens < 0 || columns < 0 || columns % 8 != 0 || rows < 0) return hipErrorInvalidValue;
+    if (tokens < 0 || tokens > kMaxTokens || columns < 0 || columns % 8 != 0 || rows < 0) return hipErrorInvalidValue;
     if (tokens == 0 || columns == 0) return hipSuccess;
     if (!rows_of || !out || (rows && !y)) return hipErrorInvalidValue;
     const int pieces = columns / 8;
@@ -160,7 +160,7 @@ inline hipError_t launch_moe_combine(const __bf16* y, const int* rows_of, const 
 template <int TOP_K>
 inline hipError_t launch_moe_combine_backward(const __bf16* grad_out, const __bf16* y, const int* rows_of, const float* weights, const int* source,
                                               __bf16* grad_y, float* grad_weights, int tokens, int columns, int rows, hipStream_t stream) {
-    if (tokens < 0 || columns < 0 || columns % 8 != 0 || rows < 0) return hipErrorInvalidValue;
+    if (tokens < 0 || tokens > kMaxTokens || columns < 0 || columns % 8 != 0 || rows < 0) return hipErrorInvalidValue;
     if (tokens && (!grad_out || !rows_of)) return hipErrorInvalidValue;
     if (rows && (!source || !grad_y || !y)) return hipErrorInvalidValue;
     const int pieces = columns / 8;

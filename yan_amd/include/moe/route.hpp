@@ -26,6 +26,7 @@ namespace yan {
 
 constexpr int kMaxTopK = 16;            // lane i of a group holds pick i
 constexpr int kMaxExperts = 1024;
+constexpr int kMaxTokens = 1 << 30;     // so that a launch's last token, rounded up to whole workgroups, is a number of 32 bits
 
 // The order of floats as the order of unsigned numbers; above 0, which is left for what has been taken out. -0 and 0 are one value. A NaN
 // is picked after everything else, as -infinity is (its row's weights are NaN all the same).
@@ -424,7 +425,7 @@ moe_route_backward_kernel(const T* __restrict__ logits, const int* __restrict__ 
 template <typename T, bool SIGMOID, int LANES, int VALUES, int THREADS>
 inline hipError_t launch_moe_route(const T* logits, const uint8_t* mask, float* weights, int* indices, int* counts, float* loss, void* workspace,
                                    int blocks, bool join, int tokens, int e, int top_k, bool renormalize, hipStream_t stream) {
-    if (tokens < 0 || e < 1 || e > LANES * VALUES || top_k < 1 || top_k > e || top_k > kMaxTopK || top_k > LANES || blocks < 1) return hipErrorInvalidValue;
+    if (tokens < 0 || tokens > kMaxTokens || e < 1 || e > LANES * VALUES || top_k < 1 || top_k > e || top_k > kMaxTopK || top_k > LANES || blocks < 1) return hipErrorInvalidValue;
     if (!counts || !loss || (tokens && (!logits || !weights || !indices)) || (blocks > 1 && !workspace)) return hipErrorInvalidValue;
     if (join && size_t(blocks) * e * 8 > kSplitKWorkspaceBytes - kSplitKCounterBytes) return hipErrorInvalidValue;
     hipLaunchKernelGGL((moe_route_kernel<T, SIGMOID, LANES, VALUES, THREADS>), dim3(blocks), dim3(THREADS), 0, stream, logits, mask, weights, indices, counts,
@@ -437,7 +438,7 @@ inline hipError_t launch_moe_route(const T* logits, const uint8_t* mask, float* 
 template <typename T, bool SIGMOID, int LANES, int VALUES>
 inline hipError_t launch_moe_route_backward(const T* logits, const int* indices, const int* counts, const float* grad_weights, const float* grad_loss,
                                             T* grad_logits, int tokens, int e, int top_k, bool renormalize, hipStream_t stream) {
-    if (tokens < 0 || e < 1 || e > LANES * VALUES || top_k < 1 || top_k > kMaxTopK || top_k > LANES) return hipErrorInvalidValue;
+    if (tokens < 0 || tokens > kMaxTokens || e < 1 || e > LANES * VALUES || top_k < 1 || top_k > kMaxTopK || top_k > LANES) return hipErrorInvalidValue;
     if (tokens == 0) return hipSuccess;
     if (!logits || !indices || !counts || !grad_logits) return hipErrorInvalidValue;
     const int blocks = ceil_div(tokens, 256 / LANES);

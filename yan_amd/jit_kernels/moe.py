@@ -22,8 +22,9 @@ from .split_k import split_k_launch_failed, split_k_workspace
 from .tuner import FrozenKeys, jit_tuner
 from .utils import assert_on_current_device, ceil_div, current_raw_stream, get_m_alignment_for_contiguous_layout
 
-# kMaxTopK and kMaxExperts of moe/route.hpp, kFewPairs and kTokensPerBlock of moe/dispatch.hpp
+# kMaxTopK, kMaxTokens and kMaxExperts of moe/route.hpp, kFewPairs and kTokensPerBlock of moe/dispatch.hpp
 MAX_TOP_K = 16
+MAX_TOKENS = 1 << 30
 MAX_EXPERTS = 1024
 FEW_PAIRS = 4096
 TOKENS_PER_BLOCK = 16
@@ -115,7 +116,7 @@ def route_kernel_plan(dtype: torch.dtype, scoring: str, experts: int, backward: 
 
 
 def _check_route(logits, top_k, scoring):
-    assert logits.dim() == 2 and logits.dtype in _ELEMENTS and logits.is_contiguous()
+    assert logits.dim() == 2 and logits.dtype in _ELEMENTS and logits.is_contiguous() and logits.size(0) <= MAX_TOKENS
     assert 1 <= logits.size(1) <= MAX_EXPERTS and 1 <= top_k <= min(MAX_TOP_K, logits.size(1))
     assert scoring in ('softmax', 'sigmoid')
 
@@ -350,7 +351,7 @@ def _check_combine(y, rows, weights, out):
     assert y.dim() == 2 and y.dtype == torch.bfloat16 and y.is_contiguous() and y.size(1) % 8 == 0
     assert rows.dim() == 2 and rows.dtype == torch.int32 and rows.is_contiguous() and 1 <= rows.size(1) <= MAX_TOP_K
     assert out.shape == (rows.size(0), y.size(1)) and out.dtype == torch.bfloat16 and out.is_contiguous()
-    assert y.size(0) < 1 << 31 and rows.size(0) < 1 << 31
+    assert y.size(0) < 1 << 31 and rows.size(0) <= MAX_TOKENS
     if weights is not None:
         assert weights.shape == rows.shape and weights.dtype == torch.float32 and weights.is_contiguous()
     assert y.data_ptr() % 16 == 0 and out.data_ptr() % 16 == 0, 'rows start at multiples of 16 bytes'
