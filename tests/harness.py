@@ -743,7 +743,7 @@ def jit_kernels_in_use(num_cus: int = 256):
 
 
 # (kernel, parts) of the weight-gradient kernels, the rule's choice first
-WGRAD_KERNELS = [('kWgradAny', 1), ('kWgradTall', 1), ('kWgrad128', 1), ('kWgrad64', 1), ('kWgradSplit', 2), ('kWgradSplit', 8)]
+WGRAD_KERNELS = [('kWgradAny', 1), ('kWgradTall', 1), ('kWgrad128', 1), ('kWgrad64', 1), ('kWgradSplit', 2), ('kWgradSplit', 8), ('kWgradSplit', 16), ('kWgradMiddle', 1)]
 # tokens, hidden, inner, experts, top_k; in decode also m_max and expected_m
 MOE_TRAINING_LAYER = (700, 512, 384, 6, 3)
 MOE_DECODE_LAYER = (37, 512, 256, 8, 2, 32, 8)

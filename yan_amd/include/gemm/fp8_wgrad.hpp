@@ -89,16 +89,24 @@ __device__ __forceinline__ bool wgrad_meet(f32x4 (&acc)[TN][TM], const WgradWork
     if (before != unsigned(parts) - 1) return false;
 #pragma unroll
     for (int v = 0; v < VECS; ++v) acc[v / TM][v % TM] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
-    for (int s = 0; s < parts; ++s)
+    constexpr int TOGETHER = 8;             // parts whose loads are under way at once
+    for (int s0 = 0; s0 < parts; s0 += TOGETHER) {
+        i32x4 raw[TOGETHER][VECS];
 #pragma unroll
-        for (int v = 0; v < VECS; ++v)
-            acc[v / TM][v % TM] += __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(sums, at + s * PART_BYTES + v * VEC_BYTES, 0, kDeviceScope));
+        for (int s = 0; s < TOGETHER; ++s)
+#pragma unroll
+            for (int v = 0; v < VECS; ++v)          // (past the last part: out of range, zeros)
+                raw[s][v] = __builtin_amdgcn_raw_buffer_load_b128(sums, s0 + s < parts ? at + (s0 + s) * PART_BYTES + v * VEC_BYTES : kOutOfRange, 0, kDeviceScope);
+#pragma unroll
+        for (int s = 0; s < TOGETHER; ++s)
+#pragma unroll
+            for (int v = 0; v < VECS; ++v) acc[v / TM][v % TM] += __builtin_bit_cast(f32x4, raw[s][v]);
+    }
     if (lane == 0) __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     return true;
 }
 
-// The smaller tiles: 4 waves, two workgroups a compute unit, which hide each other's waits; one tile a workgroup, or a walk under a cap. SPLIT: a slot
+// The smaller tiles: 4 waves, up to two workgroups a compute unit, which hide each other's waits; one tile a workgroup, or a walk under a cap. SPLIT: a slot
 // is one of `parts` parts of a tile's K range.
 template <int BLOCK_M, int BLOCK_N, int STAGES, bool SPLIT>
 __global__ void __launch_bounds__(256, 2)
@@ -107,9 +115,9 @@ fp8_wgrad_kernel(WgradProblem p, WgradWorkspace w, int parts) {
     using StA = TileStager<BLOCK_M, NW>;
     using StB = TileStager<BLOCK_N, NW>;
     constexpr int NUM_COPIES = StA::PASSES + StB::PASSES + 1, A_BYTES = BLOCK_M * kRowBytes, STAGE_BYTES = (BLOCK_M + BLOCK_N) * kRowBytes;
-    static_assert(StA::PADDED_ROWS == BLOCK_M && StB::PADDED_ROWS == BLOCK_N && (STAGES - 2) * NUM_COPIES <= 63);
+    static_assert(StA::PADDED_ROWS == BLOCK_M && StB::PADDED_ROWS == BLOCK_N && (STAGES - 1) * NUM_COPIES <= 63);
     // Scales are copied with their k-tile, a dword of four k-tiles' a row, a row a lane: loaded into registers every fourth k-tile they made the wave wait for all
-    // copies under way (SCALES_MEASURED).
+    // copies under way (64 tiles of 64 x 64, 64 k-tiles: 54.7 us, 36.5 so; 512 of 128 x 128, 64 k-tiles: 87.5 / 82.2).
     constexpr int SCALE_ROWS = NW * kWaveSize;
     static_assert(BLOCK_M % kWaveSize == 0 && BLOCK_M + BLOCK_N <= SCALE_ROWS);
     __shared__ __attribute__((aligned(1024))) uint8_t ring[STAGES * STAGE_BYTES];
@@ -169,46 +177,92 @@ fp8_wgrad_kernel(WgradProblem p, WgradWorkspace w, int parts) {
 #pragma unroll
             for (int j = 0; j < TM; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
 
-        for (int t = 0; t < STAGES - 1; ++t) copy(t, t);
-        int st = 0;
-        for (int kt = 0; kt < count; ++kt) {
-            // the copies behind this k-tile's are those of STAGES - 2 k-tiles, until the range ends
-            if (STAGES > 2 && kt + STAGES - 2 < count) __builtin_amdgcn_s_waitcnt(waitcnt_imm((STAGES - 2) * NUM_COPIES, 0));
-            else __builtin_amdgcn_s_waitcnt(waitcnt_imm(0, 0));
-            asm volatile("" ::: "memory");
-            __builtin_amdgcn_s_barrier();
-            asm volatile("" ::: "memory");
-            copy(kt + STAGES - 1, st == 0 ? STAGES - 1 : st - 1);
-            const uint8_t* pa = ring + st * STAGE_BYTES + wm * WTM * kRowBytes;
-            const uint8_t* pb = ring + st * STAGE_BYTES + A_BYTES + wn * WTN * kRowBytes;
+        // What a wave reads of a k-tile: sixteen codes a row and chunk, and the dwords with the rows' scales.
+        struct Fragments {
+            i32x4 a[2][TM], b[2][TN];
+            uint32_t scales_a[TM], scales_b[TN];
+        };
+        auto read = [&](Fragments& f, int st) __attribute__((always_inline)) {
+            const uint8_t* const pa = ring + st * STAGE_BYTES + wm * WTM * kRowBytes;
+            const uint8_t* const pb = ring + st * STAGE_BYTES + A_BYTES + wn * WTN * kRowBytes;
             const uint32_t* const scales = ring_scales + st * SCALE_ROWS + col;
+#pragma unroll
+            for (int j = 0; j < TM; ++j) f.scales_a[j] = scales[wm * WTM + j * 16];
+#pragma unroll
+            for (int i = 0; i < TN; ++i) f.scales_b[i] = scales[BLOCK_M + wn * WTN + i * 16];
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+#pragma unroll
+                for (int j = 0; j < TM; ++j) f.a[c][j] = *reinterpret_cast<const i32x4*>(pa + j * 16 * kRowBytes + off[c]);
+#pragma unroll
+                for (int i = 0; i < TN; ++i) f.b[c][i] = *reinterpret_cast<const i32x4*>(pb + i * 16 * kRowBytes + off[c]);
+            }
+        };
+        auto multiply = [&](const Fragments& f, int kt) __attribute__((always_inline)) {
             const int shift = (lo + kt) % 4 * 8;
             float scale_a[TM], scale_b[TN];
 #pragma unroll
-            for (int j = 0; j < TM; ++j) scale_a[j] = wgrad_scale(int(scales[wm * WTM + j * 16]), shift);
+            for (int j = 0; j < TM; ++j) scale_a[j] = wgrad_scale(int(f.scales_a[j]), shift);
 #pragma unroll
-            for (int i = 0; i < TN; ++i) scale_b[i] = wgrad_scale(int(scales[BLOCK_M + wn * WTN + i * 16]), shift);
+            for (int i = 0; i < TN; ++i) scale_b[i] = wgrad_scale(int(f.scales_b[i]), shift);
 #pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                i32x4 raw_a[TM], raw_b[TN];
-#pragma unroll
-                for (int j = 0; j < TM; ++j) raw_a[j] = *reinterpret_cast<const i32x4*>(pa + j * 16 * kRowBytes + off[c]);
-#pragma unroll
-                for (int i = 0; i < TN; ++i) raw_b[i] = *reinterpret_cast<const i32x4*>(pb + i * 16 * kRowBytes + off[c]);
+            for (int c = 0; c < 2; ++c)
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
                     bf16x8 fa[TM], fb[TN];
 #pragma unroll
-                    for (int j = 0; j < TM; ++j) fa[j] = wgrad_decode(raw_a[j][2 * h], raw_a[j][2 * h + 1], scale_a[j]);
+                    for (int j = 0; j < TM; ++j) fa[j] = wgrad_decode(f.a[c][j][2 * h], f.a[c][j][2 * h + 1], scale_a[j]);
 #pragma unroll
-                    for (int i = 0; i < TN; ++i) fb[i] = wgrad_decode(raw_b[i][2 * h], raw_b[i][2 * h + 1], scale_b[i]);
+                    for (int i = 0; i < TN; ++i) fb[i] = wgrad_decode(f.b[c][i][2 * h], f.b[c][i][2 * h + 1], scale_b[i]);
 #pragma unroll
                     for (int i = 0; i < TN; ++i)
 #pragma unroll
                         for (int j = 0; j < TM; ++j) acc[i][j] = MfmaBF16_16x16x32::mma(fb[i], fa[j], acc[i][j]);
                 }
+        };
+        // `ahead` stages behind the wanted one have been asked for, if the range has them
+        auto landed = [&](auto ahead_c, bool all_there) __attribute__((always_inline)) {
+            constexpr int AHEAD = decltype(ahead_c)::value;
+            if (AHEAD > 0 && all_there) __builtin_amdgcn_s_waitcnt(waitcnt_imm(AHEAD * NUM_COPIES, 0));
+            else __builtin_amdgcn_s_waitcnt(waitcnt_imm(0, 0));
+            asm volatile("" ::: "memory");
+            __builtin_amdgcn_s_barrier();
+            asm volatile("" ::: "memory");
+        };
+        int st = 0;
+        const auto behind = [](int at) { return at + 1 == STAGES ? 0 : at + 1; };
+        if constexpr (BLOCK_M == 64) {
+            // Fragments of the next k-tile are read while this one's are multiplied, so that a stage is free again as soon as it is begun (27 tiles of 199
+            // k-tiles: 106 us, 95 so). Of the 0.48 us that a k-tile takes a workgroup alone on its compute unit 0.11 are MFMAs; 0.4 were left without conversions
+            // and copies, for a barrier, the LDS, and chains of four MFMAs. Eight stages instead of four: no difference. The larger tile has no registers for it.
+            Fragments f[2];
+            for (int t = 0; t < STAGES; ++t) copy(t, t);
+            if (count > 0) {
+                landed(std::integral_constant<int, STAGES - 1>{}, count >= STAGES);
+                read(f[0], 0);
             }
-            st = st + 1 == STAGES ? 0 : st + 1;
+            auto step = [&](int kt, const Fragments& now, Fragments& next) __attribute__((always_inline)) {
+                landed(std::integral_constant<int, STAGES - 2>{}, kt + STAGES <= count);
+                copy(kt + STAGES, st);
+                st = behind(st);
+                if (kt + 1 < count) read(next, st);
+                __builtin_amdgcn_sched_barrier(0);
+                multiply(now, kt);
+            };
+            for (int kt = 0; kt < count; kt += 2) {
+                step(kt, f[0], f[1]);
+                if (kt + 1 < count) step(kt + 1, f[1], f[0]);
+            }
+        } else {
+            for (int t = 0; t < STAGES - 1; ++t) copy(t, t);
+            for (int kt = 0; kt < count; ++kt) {
+                landed(std::integral_constant<int, STAGES - 2>{}, kt + STAGES - 2 < count);
+                copy(kt + STAGES - 1, st == 0 ? STAGES - 1 : st - 1);
+                Fragments f;
+                read(f, st);
+                multiply(f, kt);
+                st = behind(st);
+            }
         }
 
         // The 4 registers of atom (i, j) are columns 16 i + 4 g + {0..3} of row 16 j + col of the slab. Stored from there an instruction covers 16 rows by 64
@@ -247,7 +301,7 @@ fp8_wgrad_kernel(WgradProblem p, WgradWorkspace w, int parts) {
     }
 }
 
-// The large tile: 256 x BLOCK_N on 4 waves, one per SIMD, each with a 128 x BLOCK_N / 2 slab of 16x16x32 MFMAs, its sums in the accumulation registers.
+// The large tiles: 256 x BLOCK_N on 4 waves, one per SIMD, each with a 128 x BLOCK_N / 2 slab of 16x16x32 MFMAs, its sums in the accumulation registers.
 // A k-tile of 128 is four steps of 32; a step is TN rows of 8 MFMAs. A lone wave has nobody to hide behind, so everything else it issues stands in
 // the shadow of an MFMA:
 //   * a lane reads 16 codes of a row at a time, which are two steps: activation fragments are decoded one step ahead of their MFMAs (`mf`, two
@@ -273,7 +327,7 @@ fp8_wgrad_tall_kernel(WgradProblem p) {
     using StB = TileStager<BLOCK_N, NW>;
     static_assert(StA::PADDED_ROWS == BLOCK_M && StB::PADDED_ROWS == BLOCK_N);
     constexpr int A_BYTES = BLOCK_M * kRowBytes, STAGE_BYTES = (BLOCK_M + BLOCK_N) * kRowBytes, PASSES = StA::PASSES + StB::PASSES;
-    static_assert(PASSES <= 2 * TN);            // one copy a row of the two steps behind the barrier
+    static_assert(PASSES <= 3 * TN);            // a row of the step behind the barrier has two copies at most, of the one after it one
     // the sums leave through pieces of 16 rows by PIECE columns, two a wave
     constexpr int PIECE = 64, PIECE_BYTES = 16 * PIECE * 4, PIECES_PER_ROW = WTN / PIECE, PIECES = TM * PIECES_PER_ROW;
     constexpr int LANES_PER_ROW = PIECE / 4, ROWS_PER_STORE = kWaveSize / LANES_PER_ROW, PIECE_STORES = 16 / ROWS_PER_STORE;
@@ -412,7 +466,10 @@ fp8_wgrad_tall_kernel(WgradProblem p) {
                     read_m(i - 1, from, SET);
                     if (i - 1 + TN < TM) read_m((i - 1 + TN) % TM, from, SET);
                 }
-                if (!EVEN && j == 2 && i == 0) read_m(TN - 1, from, SET);
+                if (!EVEN && j == 2 && i == 0) {
+                    read_m(TN - 1, from, SET);
+                    if (2 * TN - 1 < TM) read_m((2 * TN - 1) % TM, from, SET);
+                }
                 if (!EVEN && j == 1) read_n(i, from, SET);
                 if (Q >= 2 && j == 5 && (Q - 2) * TN + i < PASSES) copy((Q - 2) * TN + i, here);
                 if (Q == 2 && j == 3 && 2 * TN + i < PASSES) copy(2 * TN + i, here);
@@ -566,15 +623,15 @@ fp8_wgrad_tall_kernel(WgradProblem p) {
     }
 }
 
-// Which kernel a problem runs on, and in how many parts its K ranges. Measured over 220 shapes (us):
-//   * up to two 64 x 64 tiles a compute unit run those (44 k-tiles, 348 of them: 41.5, 128 x 128 55.4; 539 of them, 67 k-tiles: 112, 128 x 128 85), and
-//     in 2, 4 or 8 parts as long as that leaves two parts a compute unit or less and a part 8 k-tiles (8 tiles of 199 k-tiles: 121.7 whole, 65.6, 41.3 and
-//     31.7 in 2, 4 and 8, 31.8 in 16; 56 tiles of 39: 26.7 whole, 15.7 in 4, 21.1 in 8);
-//   * between the other two goes an estimate in us of rounds over the chip times a k-tile of the tile, 2.6 for 256 x 256, 1.7 for two of 128 x 128 on a
-//     compute unit, and what storing it takes. 448 large tiles of 128 k-tiles 692 against 868; 420 of 33 188 / 215; 192 of 60 155 / 173; 104 of 38
-//     94.6 / 75.8; 7168 of 2 398 / 503, of 5 575 / 732, accumulated 803 / 771 and 1036 / 1044; 2048 of 4, accumulated, 267 / 312. The smaller tile is kept
-//     where the two are within 5 %, which is where the output's traffic decides (1725 of 1 192 / 150).
-enum WgradKernel { kWgradAny, kWgradTall, kWgrad128, kWgrad64, kWgradSplit };
+// Which kernel a problem runs on, and in how many parts its K ranges. Every kernel was timed on 246 shapes (32 to 8192 rows and columns, 1 to 199 k-tiles, 1
+// to 64 groups); the choice is 0.8 % slower than the fastest on average and 16 % at most, where half a us decides.
+//   * Up to two 64 x 64 tiles a compute unit run those, in 2 parts as long as that is two workgroups a compute unit (counted as launched, a multiple of 8 a
+//     group), in 4, 8 or 16 as long as it is one, and from 12, 12, 24 and 64 k-tiles on (us whole, in 2, 4, 8: 64 tiles of 64 k-tiles 33, 21, 14.6, 15.8; 27 of 199 95, 52, 29.5, 19.8).
+//   * Others by an estimate in us. 256 x 256: rounds over the chip times 2.6 a k-tile and 12 for the output, 20 accumulated, which a lone workgroup stores with
+//     little else to do, and 4 for the start. 256 x 128: 1.3, 8 and 12.5. 128 x 128 and 64 x 64, two workgroups on a compute unit: 1.65 and 0.66 a k-tile, 6 and
+//     2.5 for the output; alone on one, as in a last round of one workgroup a compute unit or less, 1.1 and 0.47. (99 k-tiles of 2048 x 4096: 228, 157 and 186;
+//     512 x 512, 5 k-tiles of 64 groups: 55, 38 and 35; 7168 tiles of 256 x 256 and 5 k-tiles 575 / 732 for 128 x 128, accumulated 1036 / 1044.)
+enum WgradKernel { kWgradAny, kWgradTall, kWgradMiddle, kWgrad128, kWgrad64, kWgradSplit };
 struct WgradPlan {
     WgradKernel kernel;
     int parts;
@@ -582,17 +639,27 @@ struct WgradPlan {
 constexpr long long kWgradMostParts = (kSplitKWorkspaceBytes - kSplitKCounterBytes) / (64 * 64 * 4);        // what a workspace holds, sums and counters
 static_assert(kWgradMostParts * 4 * 4 <= (long long)kSplitKCounterBytes);
 inline WgradPlan wgrad_plan(int m, int n, int k, int groups, bool accumulate, int num_cus, bool may_split) {
-    const auto tiles = [&](int block) { return (long long)ceil_div(m, block) * ceil_div(n, block) * groups; };
+    const auto tiles = [&](int block_m, int block_n) { return (long long)ceil_div(m, block_m) * ceil_div(n, block_n) * groups; };
     const double k_tiles = double(k / 128) / groups;
-    if (tiles(64) <= 2ll * num_cus) {
+    const long long small = tiles(64, 64);
+    if (small <= 2ll * num_cus) {
         const long long slots = (long long)XcdTileScheduler<>(m, n, 64, 64).grid_size() * groups;
-        for (int parts = 8; may_split && parts > 1; parts /= 2)
-            if (tiles(64) * parts <= 2ll * num_cus && k_tiles >= 8 * parts && slots * parts <= kWgradMostParts) return {kWgradSplit, parts};
+        const struct { int parts, per_cu; double k_tiles; } ways[] = {{16, 1, 64}, {8, 1, 24}, {4, 1, 12}, {2, 2, 12}};
+        for (const auto& way : ways)
+            if (may_split && slots * way.parts <= (long long)way.per_cu * num_cus && k_tiles >= way.k_tiles && slots * way.parts <= kWgradMostParts)
+                return {kWgradSplit, way.parts};
         return {kWgrad64, 1};
     }
-    const double tall = ceil_div(tiles(256), (long long)num_cus) * (2.6 * k_tiles + (accumulate ? 18 : 10));
-    const double middle = ceil_div(tiles(128), 2ll * num_cus) * (1.7 * k_tiles + (accumulate ? 8.5 : 5));
-    return {tall < 0.95 * middle ? kWgradTall : kWgrad128, 1};
+    const double rounds = double(ceil_div(tiles(256, 256), (long long)num_cus)), rounds_middle = double(ceil_div(tiles(256, 128), (long long)num_cus));
+    const double tall = 4 + rounds * (2.6 * k_tiles + (accumulate ? 20 : 12)), middle = rounds_middle * (1.3 * k_tiles + (accumulate ? 12.5 : 8));
+    const auto in_twos = [&](long long count, double two, double one) {
+        const long long rest = count % (2 * num_cus);
+        return double(count / (2 * num_cus)) * two + (rest == 0 ? 0. : rest <= num_cus ? one : two);
+    };
+    const double flat = in_twos(tiles(128, 128), 1.65 * k_tiles + (accumulate ? 9.5 : 6), 1.1 * k_tiles + (accumulate ? 4.5 : 3.5));
+    const double least = 2 + in_twos(small, 0.66 * k_tiles + (accumulate ? 3.5 : 2.5), 0.47 * k_tiles + (accumulate ? 2 : 1.5));
+    if (std::min(tall, middle) < 0.92 * std::min(flat, least)) return {tall < middle ? kWgradTall : kWgradMiddle, 1};
+    return {flat < least ? kWgrad128 : kWgrad64, 1};
 }
 
 // m, n, k: codes a [m, k], b [n, k], n % 4 == 0, k % 128 == 0; scale rows ld_sa, ld_sb bytes apart (multiples of 4, k / 128 rounded up to 4 or more),
@@ -610,8 +677,9 @@ inline hipError_t launch_fp8_wgrad(const void* a, const uint8_t* sa, int ld_sa, 
     const bool capped = num_sms > 0 && num_sms < device_cu_count();
     const int cus = capped ? num_sms : device_cu_count();
     const WgradPlan plan = KERNEL == kWgradAny ? wgrad_plan(m, n, k, groups, accumulate, cus, workspace != nullptr) : WgradPlan{KERNEL, PARTS};
-    const int block = plan.kernel == kWgradTall ? 256 : plan.kernel == kWgrad128 ? 128 : 64;
-    const long long slots = (long long)XcdTileScheduler<>(m, n, block, block).grid_size() * groups * plan.parts;
+    const int block_m = plan.kernel == kWgradTall || plan.kernel == kWgradMiddle ? 256 : plan.kernel == kWgrad128 ? 128 : 64;
+    const int block_n = plan.kernel == kWgradMiddle ? 128 : block_m;
+    const long long slots = (long long)XcdTileScheduler<>(m, n, block_m, block_n).grid_size() * groups * plan.parts;
     if (slots >= 1ll << 30) return hipErrorInvalidValue;
     WgradWorkspace w{nullptr, nullptr};
     if (plan.kernel == kWgradSplit) {
@@ -625,6 +693,7 @@ inline hipError_t launch_fp8_wgrad(const void* a, const uint8_t* sa, int ld_sa, 
     const long long most = capped ? std::min<long long>(cus, slots) : slots;
     switch (plan.kernel) {
         case kWgradTall: return launch(fp8_wgrad_tall_kernel<256>, std::min<long long>(cus, slots));
+        case kWgradMiddle: return launch(fp8_wgrad_tall_kernel<128>, std::min<long long>(cus, slots));
         case kWgrad128: return launch(fp8_wgrad_kernel<128, 128, 2, false>, most, w, 1);
         case kWgrad64: return launch(fp8_wgrad_kernel<64, 64, 4, false>, most, w, 1);
         default: return launch(fp8_wgrad_kernel<64, 64, 4, true>, most, w, plan.parts);
