@@ -375,6 +375,19 @@ def test_per_channel_cast(m, n, dtype):
         assert torch.equal(codes.float().cpu().nan_to_num(500.0), want.float().nan_to_num(500.0))
 
 
+@pytest.mark.parametrize('dtype,m,n', [(torch.bfloat16, 600, 7168), (torch.float32, 4000, 6000)])
+def test_per_channel_cast_of_many_gathered_rows(dtype, m, n):
+    """The same bits from one call as from one for every 1280 rows."""
+    g = _gen(n)
+    x = torch.randn(m, n, generator=g, device='cuda').to(dtype)
+    source = torch.randint(-1, m, (8 * 1280, ), generator=g, device='cuda').int()
+    codes, scales = yan.per_channel_cast_to_fp8(x, source)
+    for r in range(0, source.numel(), 1280):
+        part, part_scales = yan.per_channel_cast_to_fp8(x, source[r:r + 1280].contiguous())
+        assert torch.equal(codes[:, r:r + 1280].contiguous().view(torch.uint8), part.view(torch.uint8))
+        assert torch.equal(scales[:, r // 128:r // 128 + 10], part_scales)
+
+
 # Weight gradients
 
 def _operand(g, rows, k, wide=False):

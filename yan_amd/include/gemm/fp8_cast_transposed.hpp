@@ -21,6 +21,7 @@
 namespace yan {
 
 constexpr int kCastColumns = 64;
+constexpr long long kCastPastBytes = 64ll << 20;
 
 // Four rows of eight columns of a thread, and what is done with them; `columns` by their place among the thread's eight.
 //   sizes        the columns' largest magnitudes, as bits, without what is not finite
@@ -125,8 +126,10 @@ template <> struct CastTile<4> {
 
 // by_columns: all K blocks of a column tile run on one XCD, where enough of them are for all eight: its L2 then holds the tile's columns, and neighbouring
 // K blocks' lines are written at about the same time (fp32 4096 x 4096 gathered four times over 47.8 -> 39.5 us, bf16 4096 x 7168 19.2 -> 17.8 gathered once,
-// 21.9 -> 21.1 as it is).
-template <typename T, bool GATHER, bool STREAM>
+// 21.9 -> 21.1 as it is). PAST: codes of more than 64 MB of rows gathered twice or more are stored past the caches, which plain stores push the source out of
+// (bf16, gathered four times: 4096 x 7168 55.0 -> 31.1 us, 8192 x 4096 66.5 -> 37.5; fp32 4096 x 4096 gathered eight times 71 -> 44). The product behind reads
+// them from further away: both together 665 -> 651 and 344 -> 340 us; below 64 MB, or as they are, they would lose 1 to 5 % (2048 x 2048 x 8 88.7 -> 93.0).
+template <typename T, bool GATHER, bool STREAM, bool PAST>
 __global__ void __launch_bounds__(256)
 per_channel_cast_kernel(const T* __restrict__ x, const int* __restrict__ source, uint8_t* __restrict__ codes, uint8_t* __restrict__ scales,
                         int m, int n, int k_blocks, int scales_stride, int column_tiles, bool by_columns) {
@@ -203,7 +206,8 @@ per_channel_cast_kernel(const T* __restrict__ x, const int* __restrict__ source,
         const u32x2 lo = *reinterpret_cast<const u32x2*>(turned + column * PITCH + part * 16), hi = *reinterpret_cast<const u32x2*>(turned + column * PITCH + part * 16 + 8);
         const i32x4 v = i32x4{int(lo[0]), int(lo[1]), int(hi[0]), int(hi[1])};
         i32x4* const to = reinterpret_cast<i32x4*>(codes + (size_t(j0 + column) * k_blocks + kb) * 128 + part * 16);
-        *to = v;
+        if constexpr (PAST) __builtin_nontemporal_store(v, to);
+        else *to = v;
     }
 }
 
@@ -222,8 +226,12 @@ inline hipError_t launch_per_channel_cast(const T* x, const int* source, void* c
         hipLaunchKernelGGL(kernel, dim3(uint32_t(blocks)), dim3(256), 0, stream, x, source, static_cast<uint8_t*>(codes), scales, m, n, k_blocks, scales_stride, column_tiles, by_columns);
         return hipGetLastError();
     };
-    if (source) return launch(per_channel_cast_kernel<T, true, false>);
-    return (long long)m * n * (long long)sizeof(T) > kCastL2Bytes ? launch(per_channel_cast_kernel<T, false, true>) : launch(per_channel_cast_kernel<T, false, false>);
+    if (source) {
+        // a source whose rows are read over and over stays in the L2s if the codes go past them
+        const bool past = (long long)n * k_blocks * 128 > kCastPastBytes && 128ll * k_blocks >= 2ll * m;
+        return past ? launch(per_channel_cast_kernel<T, true, false, true>) : launch(per_channel_cast_kernel<T, true, false, false>);
+    }
+    return (long long)m * n * (long long)sizeof(T) > kCastL2Bytes ? launch(per_channel_cast_kernel<T, false, true, false>) : launch(per_channel_cast_kernel<T, false, false, false>);
 }
 
 } // namespace yan
