@@ -624,13 +624,15 @@ fp8_wgrad_tall_kernel(WgradProblem p) {
 }
 
 // Which kernel a problem runs on, and in how many parts its K ranges. Every kernel was timed on 246 shapes (32 to 8192 rows and columns, 1 to 199 k-tiles, 1
-// to 64 groups); the choice is 0.8 % slower than the fastest on average and 16 % at most, where half a us decides.
+// to 64 groups); the choice is 0.8 % slower than the fastest on average, 1.4 % over 163 others drawn afterwards.
 //   * Up to two 64 x 64 tiles a compute unit run those, in 2 parts as long as that is two workgroups a compute unit (counted as launched, a multiple of 8 a
-//     group), in 4, 8 or 16 as long as it is one, and from 12, 12, 24 and 64 k-tiles on (us whole, in 2, 4, 8: 64 tiles of 64 k-tiles 33, 21, 14.6, 15.8; 27 of 199 95, 52, 29.5, 19.8).
+//     group), in 4, 8 or 16 as long as it is one, and from 12, 12, 24 and 64 k-tiles on (us whole, in 2, 4, 8: 64 tiles of 64 k-tiles 33, 21, 14.6, 15.8; 27
+//     of 199 95, 52, 29.5, 19.8).
 //   * Others by an estimate in us. 256 x 256: rounds over the chip times 2.6 a k-tile and 12 for the output, 20 accumulated, which a lone workgroup stores with
 //     little else to do, and 4 for the start. 256 x 128: 1.3, 8 and 12.5. 128 x 128 and 64 x 64, two workgroups on a compute unit: 1.65 and 0.66 a k-tile, 6 and
 //     2.5 for the output; alone on one, as in a last round of one workgroup a compute unit or less, 1.1 and 0.47. (99 k-tiles of 2048 x 4096: 228, 157 and 186;
-//     512 x 512, 5 k-tiles of 64 groups: 55, 38 and 35; 7168 tiles of 256 x 256 and 5 k-tiles 575 / 732 for 128 x 128, accumulated 1036 / 1044.)
+//     512 x 512, 5 k-tiles of 64 groups: 55, 38 and 35; 7168 tiles of 256 x 256 and 5 k-tiles 575 / 732 for 128 x 128, accumulated 1036 / 1044.) The large tiles have
+//     to be 8 % ahead.
 enum WgradKernel { kWgradAny, kWgradTall, kWgradMiddle, kWgrad128, kWgrad64, kWgradSplit };
 struct WgradPlan {
     WgradKernel kernel;
