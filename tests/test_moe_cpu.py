@@ -1,5 +1,6 @@
 """The mixture-of-experts entries and the weight-gradient products without a GPU: what they refuse, and the rules that size their kernels."""
 import random
+import re
 
 import pytest
 import torch
@@ -163,3 +164,33 @@ def test_more_tokens_than_a_launch_counts_are_refused():
         else:
             _refused(moe._check_route, logits, 2, 'softmax')
             _refused(moe._check_combine, y, rows, None, out)
+
+
+def _stores_of_16_bytes(tmp_path, code):
+    import subprocess
+    from yan_amd.jit.compiler import get_hipcc_compiler, get_jit_include_dir, get_offload_arch
+    src, asm = tmp_path / 'kernel.cu', tmp_path / 'kernel.s'
+    src.write_text(code)
+    subprocess.check_call([get_hipcc_compiler()[0], '-x', 'hip', '--cuda-device-only', '-S', '-std=c++20', '-O3', f'--offload-arch={get_offload_arch()}',
+                           '-Xclang', '-target-feature', '-Xclang', '-packed-fp32-ops', f'-I{get_jit_include_dir()}', str(src), '-o', str(asm)])
+    lines = [line.split(';')[0].strip() for line in asm.read_text().split('\n')]
+    return [line for line in lines if line.startswith('buffer_store_dwordx4')]
+
+
+@pytest.mark.parametrize('which', ['weight gradients', 'bf16 split-K', 'FP8 split-K'])
+def test_no_store_of_16_bytes_has_a_scalar_offset(tmp_path, which):
+    """Such a store may read its data after the next vector instruction has overwritten it, and the compiler leaves it without a wait."""
+    from yan_amd.jit_kernels import bf16_gemm, gemm
+    if which == 'weight gradients':
+        _, keys, arg_defs, template = wgrad.wgrad_kernel_plan()
+        includes = wgrad.includes
+    elif which == 'bf16 split-K':
+        _, keys, arg_defs = bf16_gemm.dense_split_k_plan(256, 5120, 5120, torch.bfloat16, 256)
+        includes, template = bf16_gemm.includes, bf16_gemm.split_k_template
+    else:
+        _, keys, arg_defs, template = gemm.fp8_split_k_plan(64, 4096, 7168, 256)
+        includes = gemm.includes
+    stores = _stores_of_16_bytes(tmp_path, generate(includes, arg_defs, cpp_format(template, dict(keys))))
+    # vector data, vector offset, descriptor, scalar offset with the modifiers behind it
+    # (the smallest, 64 x 64 on 8 waves: two vectors of partial sums a lane, one of outputs in either of two policies)
+    assert len(stores) >= 4 and all(re.match(r'buffer_store_dwordx4 v\[\d+:\d+\], v\d+, s\[\d+:\d+\], 0 ', line) for line in stores), stores[:3]

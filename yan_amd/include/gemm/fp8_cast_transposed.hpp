@@ -221,7 +221,7 @@ inline hipError_t launch_per_channel_cast(const T* x, const int* source, void* c
     const int column_tiles = ceil_div(n, kCastColumns);
     const bool by_columns = column_tiles % kNumXCD == 0 || column_tiles >= 4 * kNumXCD;
     const long long blocks = (long long)(by_columns ? ceil_div(column_tiles, kNumXCD) * kNumXCD : column_tiles) * k_blocks;
-    if (blocks >= 1ll << 31) return hipErrorInvalidValue;
+    if (blocks >= 1ll << 24) return hipErrorInvalidValue;         // a launch has less than 2^32 threads
     const auto launch = [&](auto kernel) {
         hipLaunchKernelGGL(kernel, dim3(uint32_t(blocks)), dim3(256), 0, stream, x, source, static_cast<uint8_t*>(codes), scales, m, n, k_blocks, scales_stride, column_tiles, by_columns);
         return hipGetLastError();

@@ -682,7 +682,7 @@ inline hipError_t launch_fp8_wgrad(const void* a, const uint8_t* sa, int ld_sa, 
     const int block_m = plan.kernel == kWgradTall || plan.kernel == kWgradMiddle ? 256 : plan.kernel == kWgrad128 ? 128 : 64;
     const int block_n = plan.kernel == kWgradMiddle ? 128 : block_m;
     const long long slots = (long long)XcdTileScheduler<>(m, n, block_m, block_n).grid_size() * groups * plan.parts;
-    if (slots >= 1ll << 30) return hipErrorInvalidValue;
+    if (slots >= 1ll << 24) return hipErrorInvalidValue;          // a launch has less than 2^32 threads
     WgradWorkspace w{nullptr, nullptr};
     if (plan.kernel == kWgradSplit) {
         if (!workspace || slots > kWgradMostParts) return hipErrorInvalidValue;

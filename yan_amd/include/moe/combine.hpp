@@ -152,7 +152,7 @@ inline hipError_t launch_moe_combine(const __bf16* y, const int* rows_of, const 
     const int pieces = columns / 8;
     const int waves_per_token = ceil_div(pieces, kWaveSize);
     const long long blocks = ceil_div((long long)tokens * waves_per_token, 4ll);
-    if (blocks >= 1ll << 31) return hipErrorInvalidValue;
+    if (blocks > kMaxWorkgroups) return hipErrorInvalidValue;
     hipLaunchKernelGGL(moe_combine_kernel<TOP_K>, dim3(uint32_t(blocks)), dim3(256), 0, stream, y, rows_of, weights, out, tokens, pieces, rows, waves_per_token);
     return hipGetLastError();
 }
@@ -166,7 +166,7 @@ inline hipError_t launch_moe_combine_backward(const __bf16* grad_out, const __bf
     const int pieces = columns / 8;
     const bool wide = pieces > kWaveSize;
     const int token_blocks = wide ? tokens : ceil_div(tokens, 4), clear_blocks = ceil_div(rows, kRowsPerClearBlock);
-    if ((long long)token_blocks + clear_blocks >= 1ll << 31) return hipErrorInvalidValue;
+    if ((long long)token_blocks + clear_blocks > kMaxWorkgroups) return hipErrorInvalidValue;
     if (token_blocks + clear_blocks == 0) return hipSuccess;
     const auto launch = [&](auto kernel) {
         hipLaunchKernelGGL(kernel, dim3(token_blocks + clear_blocks), dim3(256), 0, stream, grad_out, y, rows_of, weights, source, grad_y, grad_weights, tokens,

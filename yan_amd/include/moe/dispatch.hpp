@@ -291,7 +291,7 @@ inline hipError_t launch_moe_dispatch(const T* x, const int* indices, void* code
     // 8192 tokens of 7168 182.5, 175.6, 171.0, 172.5, 166.5; 2048 of 7168 104.7, 66.7, 51.5, 51.6, 47.5; 8192 of 1024 36.7, 31.3, 37.1, 39.4, 46.9; 1024 of 2048
     // 34.1, 23.5, 18.4, 16.6, 16.2)
     const int in_chunk = kTokensPerBlock * s.k_blocks, parts = std::max(ceil_div(in_chunk, 64), std::min(ceil_div(in_chunk, 16), 4 * device_cu_count() / blocks));
-    if ((long long)blocks * parts >= 1ll << 30) return hipErrorInvalidValue;
+    if ((long long)blocks * parts > kMaxWorkgroups - kNumXCD) return hipErrorInvalidValue;
     const int grid = ceil_div(blocks * parts, kNumXCD) * kNumXCD;
     const auto launch = [&](auto kernel) {
         hipLaunchKernelGGL(kernel, dim3(grid), dim3(256), 0, stream, x, indices, table, to, scales, rows_of, m_indices, source, offsets, s, parts);

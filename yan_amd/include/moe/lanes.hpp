@@ -7,6 +7,8 @@
 
 namespace yan {
 
+constexpr long long kMaxWorkgroups = (1ll << 24) - 1;       // of 256 threads: a launch has less than 2^32 threads
+
 template <int ROTATE>
 __device__ __forceinline__ uint32_t rotate_row(uint32_t a) {
     constexpr int ROW_ROR = 0x120;
