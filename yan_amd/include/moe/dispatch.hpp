@@ -183,28 +183,48 @@ moe_dispatch_count_kernel(const int* __restrict__ indices, int* __restrict__ tab
     for (int x = threadIdx.x; x < e; x += 256) table[size_t(blockIdx.x) * e + x] = counts[x];
 }
 
-// Second: every entry of the table becomes the sum of those above it, row `blocks` the sum of all. 16 experts a workgroup, 64 threads an expert.
+// Second: every entry of the table becomes the sum of those above it, row `blocks` the sum of all. 16 experts a workgroup, 64 threads an expert, each
+// with a run of rows, eight of them under way at once; the runs' sums are scanned by a wave an expert.
 template <int = 0>
 __global__ void __launch_bounds__(1024)
 moe_dispatch_scan_kernel(int* __restrict__ table, int blocks, int e) {
-    __shared__ int sums[64][16];
-    const int column = threadIdx.x & 15, part = threadIdx.x >> 4, x = blockIdx.x * 16 + column;
-    const int share = ceil_div(blocks, 64), first = min(blocks, part * share), last = min(blocks, first + share);
-    int sum = 0;
-    if (x < e)
-        for (int b = first; b < last; ++b) sum += table[size_t(b) * e + x];
+    constexpr int TOGETHER = 8;
+    __shared__ int sums[64][17];
+    const int column = threadIdx.x & 15, part = threadIdx.x >> 4, x = blockIdx.x * 16 + column, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int share = ceil_div(blocks, 64), first = min(blocks, part * share), last = x < e ? min(blocks, first + share) : first;
+    const auto load = [&](int (&v)[TOGETHER], int b0) {
+#pragma unroll
+        for (int i = 0; i < TOGETHER; ++i) v[i] = b0 + i < last ? table[size_t(b0 + i) * e + x] : 0;
+    };
+    int v[TOGETHER], sum = 0;
+    for (int b0 = first; b0 < last; b0 += TOGETHER) {
+        load(v, b0);
+#pragma unroll
+        for (int i = 0; i < TOGETHER; ++i) sum += v[i];
+    }
     sums[part][column] = sum;
     __syncthreads();
-    int before = 0;
-    for (int p = 0; p < part; ++p) before += sums[p][column];
-    if (x >= e) return;
-    for (int b = first; b < last; ++b) {
-        int& at = table[size_t(b) * e + x];
-        const int here = at;
-        at = before;
-        before += here;
+    {
+        const int mine = sums[lane][wave];
+        int upto = mine;
+#pragma unroll
+        for (int d = 1; d < 64; d *= 2) {
+            const int below = __shfl_up(upto, d, 64);
+            if (lane >= d) upto += below;
+        }
+        sums[lane][wave] = upto - mine;
     }
-    if (part == 63) table[size_t(blocks) * e + x] = before;
+    __syncthreads();
+    int before = sums[part][column];
+    for (int b0 = first; b0 < last; b0 += TOGETHER) {
+        if (share > TOGETHER) load(v, b0);          // else they are still here
+#pragma unroll
+        for (int i = 0; i < TOGETHER; ++i) {
+            if (b0 + i < last) table[size_t(b0 + i) * e + x] = before;
+            before += v[i];
+        }
+    }
+    if (part == 63 && x < e) table[size_t(blocks) * e + x] = before;
 }
 
 // Third: the rows of the chunk's pairs and the tokens themselves, by `parts` workgroups a chunk.
