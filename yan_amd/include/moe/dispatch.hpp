@@ -20,7 +20,7 @@ namespace yan {
 constexpr int kExpertAlignment = 128;
 constexpr int kFewPairs = 4096;             // up to here every workgroup counts all pairs itself
 constexpr int kTokensPerBlock = 16;         // above: tokens of a chunk
-constexpr long long kDispatchCacheBytes = 256ll << 20;
+constexpr long long kDispatchCacheBytes = 192ll << 20;
 
 struct DispatchShape {
     int tokens, k_blocks, top_k, experts, m_max;        // m_max 0: contiguous
@@ -318,7 +318,8 @@ inline hipError_t launch_moe_dispatch(const T* x, const int* indices, void* code
         return hipGetLastError();
     };
     if (cast_stream((long long)tokens * k, sizeof(T), true) == kPlain) return launch(moe_dispatch_kernel<T, kPlain>);
-    // codes that outgrow the memory-side cache are not found there by the GEMM behind (8192 x 8 pairs of 7168, 470 MB: 174.9 us plain, 161.6 past the caches)
+    // codes that outgrow the memory-side cache are not found there by the GEMM behind, plain / past the caches (us): 8192 x 8 pairs of 7168, 470 MB, 174.9 / 161.6; 4096 x
+    // 8, 224 MB, 93.3 / 84.8, with the product (n 2048) 630 / 627; 8192 x 8 of 2048, 128 MB, 54.0 / 51.7, but with the product (n 1024) 263 / 269
     return (long long)pairs * k > kDispatchCacheBytes ? launch(moe_dispatch_kernel<T, kStreamBoth>) : launch(moe_dispatch_kernel<T, kStreamSource>);
 }
 
