@@ -100,8 +100,8 @@ def route_blocks(tokens: int, experts: int) -> int:
 
 def route_joins(blocks: int, experts: int) -> bool:
     """Whether the last of the workgroups adds up all their rows. 64 tokens of 256 experts, 16 workgroups: 6.5 us on the device instead of 7.7 with a second
-    kernel, 6.1 a call instead of 10.1; 1024 tokens, 256 workgroups: 19.8 instead of 9.4."""
-    return 1 < blocks <= 64 and blocks * experts <= 16384
+    kernel, 5.9 a call instead of 7.8; 256 tokens, 64 workgroups: 8.6 instead of 8.1; 1024 tokens, 256 workgroups: 19.8 instead of 9.4. In two levels of 16: 10.4."""
+    return 1 < blocks <= 64 and blocks * experts <= 8192
 
 
 @functools.lru_cache(maxsize=None)
