@@ -16,6 +16,7 @@
 #include <hip/hip_runtime.h>
 #include <hip/hip_bf16.h>
 
+#include <algorithm>
 #include <limits>
 #include <type_traits>
 
@@ -441,8 +442,11 @@ inline hipError_t launch_moe_route_backward(const T* logits, const int* indices,
     if (tokens < 0 || tokens > kMaxTokens || e < 1 || e > LANES * VALUES || top_k < 1 || top_k > kMaxTopK || top_k > LANES) return hipErrorInvalidValue;
     if (tokens == 0) return hipSuccess;
     if (!logits || !indices || !counts || !grad_logits) return hipErrorInvalidValue;
-    const int blocks = ceil_div(tokens, 256 / LANES);
-    hipLaunchKernelGGL((moe_route_backward_kernel<T, SIGMOID, LANES, VALUES>), dim3(blocks < 2048 ? blocks : 2048), dim3(256), 0, stream, logits, indices,
+    // as many workgroups as are resident, so that each reads the counts once (fp32, 16384 tokens, 1024 / 2048 / 4096 workgroups: 256 experts 12.1, 11.8, 12.4 us,
+    // 512 experts 18.6, 20.8, 25.9)
+    constexpr int MOST = VALUES > 4 ? 1024 : 2048;
+    const int blocks = std::min(ceil_div(tokens, 256 / LANES), MOST);
+    hipLaunchKernelGGL((moe_route_backward_kernel<T, SIGMOID, LANES, VALUES>), dim3(blocks), dim3(256), 0, stream, logits, indices,
                        counts, grad_weights, grad_loss, grad_logits, tokens, e, top_k, renormalize,
                        rows_in_pieces<VALUES, T>(logits, e) && rows_in_pieces<VALUES, T>(grad_logits, e));
     return hipGetLastError();
