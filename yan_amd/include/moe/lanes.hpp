@@ -40,6 +40,20 @@ template <int LANES> __device__ __forceinline__ int sum_lanes(int v) { return re
 template <int LANES> __device__ __forceinline__ float max_lanes(float v) { return reduce_lanes<LANES>(v, [](float a, float b) { return fmaxf(a, b); }); }
 template <int LANES> __device__ __forceinline__ uint32_t max_lanes(uint32_t v) { return reduce_lanes<LANES>(v, [](uint32_t a, uint32_t b) { return a > b ? a : b; }); }
 
+// The maximum over a whole wave as a scalar: rows of 16 as above, then every second row takes its neighbour's, the upper half the lower half's, and the last
+// lane has it all (zero, which is what lanes outside of the masks are given, is the least there is). Router, 16384 rows of 256: 16.3 -> 15.8 us.
+__device__ __forceinline__ uint32_t max_wave(uint32_t v) {
+    constexpr int ROW_BCAST_15 = 0x142, ROW_BCAST_31 = 0x143;
+    const auto larger = [](uint32_t a, uint32_t b) { return a > b ? a : b; };
+    v = larger(v, rotate_row<8>(v));
+    v = larger(v, rotate_row<4>(v));
+    v = larger(v, rotate_row<2>(v));
+    v = larger(v, rotate_row<1>(v));
+    v = larger(v, uint32_t(__builtin_amdgcn_update_dpp(0, int(v), ROW_BCAST_15, 0xa, 0xf, false)));
+    v = larger(v, uint32_t(__builtin_amdgcn_update_dpp(0, int(v), ROW_BCAST_31, 0xc, 0xf, false)));
+    return uint32_t(__builtin_amdgcn_readlane(int(v), 63));
+}
+
 // Across the groups of a wave: every group gets the sum over the lanes that have its place in their groups.
 template <int LANES, typename T>
 __device__ __forceinline__ T sum_groups(T v) {

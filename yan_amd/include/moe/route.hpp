@@ -189,7 +189,7 @@ moe_route_kernel(const T* __restrict__ logits, const uint8_t* __restrict__ mask,
         float top = 0.f;
 #pragma unroll 2
         for (int i = 0; i < top_k; ++i) {
-            const uint32_t best = max_lanes<LANES>(key[0]);
+            const uint32_t best = LANES == 64 ? max_wave(key[0]) : max_lanes<LANES>(key[0]);
             const unsigned long long have = __ballot(key[0] == best) >> group_base;
             if (in_group == __ffsll((long long)have) - 1) {
                 picks[i] = make_uint2(uint32_t(first) + uint32_t(places & 15), best);
