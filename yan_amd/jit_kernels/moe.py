@@ -10,7 +10,8 @@ fills the layouts or empties them; callers of `m_grouped_gemm_fp8_fp8_bf16_nt_*`
 
 and back: `moe_combine_backward`, `per_channel_cast_to_fp8` of both sides and `k_grouped_gemm_fp8_fp8_fp32_nt_contiguous` for the experts' weights,
 `moe_combine` without weights for the tokens' gradients, `moe_route_backward` for the logits. Work is enqueued on the current stream; what the
-entries return is allocated from torch's caching allocator, and so is the scratch of a call.
+entries return is allocated from torch's caching allocator, and so is the scratch of a call. The router's workgroups for few tokens meet in the
+stream's split-K workspace (`split_k.py`), unless `YAN_SPLIT_K=0`.
 """
 import functools
 from typing import Optional, Tuple
