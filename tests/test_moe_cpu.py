@@ -1,4 +1,5 @@
 """The mixture-of-experts entries and the weight-gradient products without a GPU: what they refuse, and the rules that size their kernels."""
+import ctypes
 import random
 import re
 
@@ -194,3 +195,80 @@ def test_no_store_of_16_bytes_has_a_scalar_offset(tmp_path, which):
     # vector data, vector offset, descriptor, scalar offset with the modifiers behind it
     # (the smallest, 64 x 64 on 8 waves: two vectors of partial sums a lane, one of outputs in either of two policies)
     assert len(stores) >= 4 and all(re.match(r'buffer_store_dwordx4 v\[\d+:\d+\], v\d+, s\[\d+:\d+\], 0 ', line) for line in stores), stores[:3]
+
+
+class _Notes:
+    """Stands in for the device and for the native module: launches report success, and what is noted of them is kept."""
+
+    def __init__(self, monkeypatch):
+        from yan_amd.jit.runtime import Runtime
+        from yan_amd.jit_kernels import host_calls, utils
+        self.noted = []
+        for name in ('YAN_SPLIT_K', 'YAN_TUNE_TILES'):
+            monkeypatch.delenv(name, raising=False)
+        monkeypatch.setattr(host_calls, '_host_calls', type('Module', (), {'remember': staticmethod(lambda *note: self.noted.append(note))}))
+        monkeypatch.setattr(host_calls, 'repeat_new', lambda *_: None)
+        monkeypatch.setattr(utils, '_num_sms', 256)
+        monkeypatch.setattr(Runtime, 'is_path_valid', staticmethod(lambda path: True))
+        monkeypatch.setattr(Runtime, '__call__', lambda self, *args: 0)
+
+        def compile_and_tune(name, arg_defs, **_):
+            runtime = Runtime(name)
+            runtime._launch, runtime.args = ctypes.CFUNCTYPE(None)(lambda: None), arg_defs
+            return runtime
+        monkeypatch.setattr(moe.jit_tuner, 'compile_and_tune', compile_and_tune)
+        for module in (moe, wgrad, fp8_cast):
+            monkeypatch.setattr(module, 'current_raw_stream', lambda: 0)
+            monkeypatch.setattr(module, 'assert_on_current_device', lambda *_: None)
+        monkeypatch.setattr(wgrad, 'get_num_sms', lambda: 256)
+        for module in (moe, wgrad):
+            monkeypatch.setattr(module, 'split_k_workspace', lambda device, stream: (torch.empty(8, dtype=torch.uint8, device='meta'), None))
+
+    def tensors(self, arg_defs, call):
+        """By name: which of the noted call's tensors each of the launch's is, None for one that the caller did not give."""
+        call()
+        (_, _, _, spec, *_), = self.noted
+        self.noted.clear()
+        assert len(spec) == len(arg_defs)
+        return {name: value if kind == 0 else None for (name, dtype), (kind, value) in zip(arg_defs, spec) if isinstance(dtype, torch.dtype)}
+
+
+def test_notes_of_a_call_say_which_argument_is_which_also_where_two_are_the_same(monkeypatch):
+    """A later call of the same sizes takes its addresses by place: it may have two tensors where the noted one had the same twice."""
+    notes = _Notes(monkeypatch)
+    meta = lambda *shape, dtype=torch.float32: torch.empty(shape, dtype=dtype, device='meta')
+    a, b = [(meta(64, 512, dtype=F8), meta(64, 4, dtype=torch.uint8)) for _ in range(2)]
+    out, offsets = meta(64, 64), meta(3, dtype=torch.int32)
+    want = {'lhs': 0, 'lhs_scales': 1, 'rhs': 2, 'rhs_scales': 3, 'out': 4, 'offsets': None, 'workspace': None}
+    for lhs, rhs in ((a, b), (a, a), (a, (b[0], a[1])), (a, (a[0], b[1]))):
+        assert notes.tensors(wgrad.arg_defs, lambda: yan.gemm_fp8_fp8_fp32_nt(lhs, rhs, out)) == want
+        assert notes.tensors(wgrad.arg_defs, lambda: yan.k_grouped_gemm_fp8_fp8_fp32_nt_contiguous(lhs, rhs, meta(2, 64, 64), offsets)) == {**want, 'offsets': 5}
+    y, d, rows, w, source = meta(4, 64, dtype=torch.bfloat16), meta(4, 64, dtype=torch.bfloat16), meta(4, 2, dtype=torch.int32), meta(4, 2), meta(4, dtype=torch.int32)
+    for grad_out in (d, y):
+        got = notes.tensors(moe.combine_backward_arg_defs, lambda: yan.moe_combine_backward(grad_out, y, rows, w, source))
+        assert got == {'grad_out': 0, 'y': 1, 'rows_of': 2, 'weights': 3, 'source': 4, 'grad_y': None, 'grad_weights': None}
+        got = notes.tensors(moe.combine_backward_arg_defs, lambda: yan.moe_combine_backward(grad_out, y, rows, None, source))
+        assert got == {'grad_out': 0, 'y': 1, 'rows_of': 2, 'weights': None, 'source': 3, 'grad_y': None, 'grad_weights': None}
+    for weights, after in ((w, 3), (None, 2)):
+        got = notes.tensors(moe.combine_arg_defs, lambda: yan.moe_combine(y, rows, weights, d))
+        assert got['y'] == 0 and got['rows_of'] == 1 and sorted(v for v in got.values() if v is not None) == list(range(after + 1))
+        assert (got['weights'] is None) == (weights is None) and got['weights'] != got['out']
+    logits, indices, counts, loss = meta(4, 2), meta(4, 2, dtype=torch.int32), meta(2, dtype=torch.int32), meta()
+    defs = moe.route_kernel_plan(torch.float32, 'softmax', 2, True)[2]
+    for grad_weights in (w, logits):
+        got = notes.tensors(defs, lambda: yan.moe_route_backward(logits, indices, counts, grad_weights, loss))
+        assert got == {'logits': 0, 'indices': 1, 'counts': 2, 'grad_weights': 3, 'grad_loss': 4, 'grad_logits': None}
+    got = notes.tensors(defs, lambda: yan.moe_route_backward(logits, indices, counts, None, loss))
+    assert got == {'logits': 0, 'indices': 1, 'counts': 2, 'grad_weights': None, 'grad_loss': 3, 'grad_logits': None}
+    defs = moe.route_kernel_plan(torch.float32, 'softmax', 2)[2]
+    for mask in (None, meta(4, dtype=torch.bool)):
+        got = notes.tensors(defs, lambda: yan.moe_route(logits, 1, mask=mask))
+        assert got['logits'] == 0 and got['mask'] == (None if mask is None else 1)
+    x, codes, scales = meta(4, 128, dtype=torch.bfloat16), meta(128, 128, dtype=F8), meta(128, 1)
+    got = notes.tensors(moe.dispatch_kernel_plan(x.dtype)[2], lambda: yan.moe_dispatch_to_fp8_contiguous(x, indices, 2, (codes, scales)))
+    assert [got[name] for name in ('x', 'indices', 'codes', 'scales', 'rows_of')] == [0, 1, 2, 3, None]
+    got = notes.tensors(moe.dispatch_kernel_plan(x.dtype)[2], lambda: yan.moe_dispatch_to_fp8_masked(x, indices, (codes.view(2, 64, 128), scales.view(2, 64, 1))))
+    assert [got[name] for name in ('x', 'indices', 'codes', 'scales', 'rows_of')] == [0, 1, 2, 3, None]
+    for picked in (None, meta(128, dtype=torch.int32)):
+        got = notes.tensors(fp8_cast.per_channel_arg_defs(x.dtype), lambda: yan.per_channel_cast_to_fp8(x, picked))
+        assert got == {'x': 0, 'source': None if picked is None else 1, 'q': None, 'scales': None}

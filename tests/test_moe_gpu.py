@@ -744,3 +744,33 @@ def test_repeated_calls_take_what_each_is_given():
     yan.gemm_fp8_fp8_fp32_nt((codes, scales), (codes, scales), size)
     # four times the same product, added three times: each addition off by half a step of a sum up to four of it
     _close(out, 4 * size.double(), 3 * 4 * U * size.abs().double())
+
+
+def test_a_call_with_one_tensor_twice_and_then_with_two():
+    """A call that gives the same tensor twice says nothing about the next call of its sizes."""
+    g = _gen(41)
+    a, b = _operand(g, 192, 1152), _operand(g, 192, 1152)
+    turns = [(a, a), (a, b), (b, a), (b, b), (a, (b[0], a[1])), (a, b), ((b[0], a[1]), a)]
+    for lhs, rhs in turns:
+        out, grouped = torch.zeros(192, 192, device='cuda'), torch.zeros(2, 192, 192, device='cuda')
+        yan.gemm_fp8_fp8_fp32_nt(lhs, rhs, out)
+        _check_product(out, _decode(lhs), _decode(rhs), None)
+        yan.k_grouped_gemm_fp8_fp8_fp32_nt_contiguous(lhs, rhs, grouped, torch.tensor([0, 256, 1152], dtype=torch.int32, device='cuda'))
+        for q, (lo, hi) in enumerate([(0, 256), (256, 1152)]):
+            _check_product(grouped[q], _decode(lhs)[:, lo:hi].contiguous(), _decode(rhs)[:, lo:hi].contiguous(), None)
+    y, d = [torch.randn(48, 136, generator=g, device='cuda').bfloat16() for _ in range(2)]
+    rows = torch.arange(48, dtype=torch.int32, device='cuda')[:, None].contiguous()
+    w = torch.randn(48, 1, generator=g, device='cuda')
+    for grad_out, of in ((y, y), (d, y), (y, d), (d, d)):
+        grad_y, grad_w = yan.moe_combine_backward(grad_out, of, rows, w, rows[:, 0].contiguous())
+        _close(grad_y, w.double() * grad_out.double(), (2.0 ** -8 + 2 * U) * (w.double() * grad_out.double()).abs(), 'grad_y')
+        size = (grad_out.double() * of.double()).abs().sum(1, keepdim=True)
+        _close(grad_w, (grad_out.double() * of.double()).sum(1, keepdim=True), (136 / 64 + 16) * U * size, 'grad_weights')
+    logits, dw = torch.randn(40, 6, generator=g, device='cuda'), torch.randn(40, 6, generator=g, device='cuda')
+    _, indices, counts, _ = yan.moe_route(logits, 6)
+    apart = yan.moe_route_backward(logits, indices, counts, logits.clone(), None)
+    assert torch.equal(yan.moe_route_backward(logits, indices, counts, logits, None), apart)
+    leaf = logits.double().requires_grad_()
+    (torch.softmax(leaf, 1).gather(1, indices.long()) * dw.double()).sum().backward()
+    # the terms are products of a score and a gradient of up to 5, each off by 60 u at most, of which there are 7 in a sum
+    _close(yan.moe_route_backward(logits, indices, counts, dw, None), leaf.grad, torch.full_like(leaf, 7 * 5 * 60 * U).detach(), 'grad_logits')

@@ -91,8 +91,9 @@ def remember_call(call: tuple, name: str, runtime: Runtime, args: tuple, workspa
 
 def remember_new(call: tuple, name: str, runtime: Runtime, args: tuple, outputs: tuple = (), scratch: tuple = (), views: dict = {}, workspace=None) -> None:
     """As `remember_call`, for a call that makes the tensors `outputs`, which it returns, and `scratch`: `repeat_new` makes them anew (`repeat_call` where there
-    are none). `call` has what the caller gave, in any order, None among it. A tensor of `args` that is none of all these stands for one that is not there, and its
-    address is of no account; `views` says which of the caller's tensors (by id of what is in `args`) another one is a view of."""
+    are none). `call` has what the caller gave, None among it, its tensors in the order of `args`: which of them an argument is goes by its place, since a caller
+    may give one tensor twice and two the next time. A tensor of `args` that is none of all these stands for one that is not there, and its address is of
+    no account; `views` says which of the caller's tensors (by id of what is in `args`) another one is a view of."""
     if repeat_new is _nothing or type(runtime) is not Runtime or runtime._launch is None or not split_k.split_k_enabled() or tuning_enabled():
         return
     utils.get_num_sms()         # part of what a call is looked up by; not every entry has asked for it
@@ -100,7 +101,7 @@ def remember_new(call: tuple, name: str, runtime: Runtime, args: tuple, outputs:
         runtime.native = _native_parts(runtime)
     address, kinds = runtime.native
     given, made = [a for a in call if isinstance(a, torch.Tensor)], (*outputs, *scratch)
-    spec = []
+    spec, tensors = [], 0
     for arg, kind in zip(args, kinds):
         if kind is _CONSTANT:
             spec.append((_CONSTANT, arg))
@@ -108,11 +109,14 @@ def remember_new(call: tuple, name: str, runtime: Runtime, args: tuple, outputs:
             spec.append(_THE_STREAM)
         elif workspace is not None and arg is workspace:
             spec.append(_THE_WORKSPACE)
+        elif tensors < len(given) and views.get(id(arg), arg) is given[tensors]:
+            spec.append((_TENSOR, tensors))
+            tensors += 1
         else:
-            arg = views.get(id(arg), arg)
             new = [i for i, t in enumerate(made) if t is arg]
-            old = [i for i, t in enumerate(given) if t is arg]
-            spec.append((_OUTPUT, new[0]) if new else (_TENSOR, old[0]) if old else (_CONSTANT, 0))
+            spec.append((_OUTPUT, new[0]) if new else (_CONSTANT, 0))
+    if tensors != len(given):
+        return
     shapes = []
     for t in made:
         # a tensor whose rows are further apart than they are long is the front of one without gaps

@@ -367,7 +367,7 @@ def moe_combine(y: torch.Tensor, rows: torch.Tensor, weights: Optional[torch.Ten
     weights: fp32 `[tokens, top_k]`, or None for 1 (the gradient of what was dispatched)
     out: bf16 `[tokens, n]`, written in place
     """
-    call = (COMBINE, y, rows, out, weights)
+    call = (COMBINE, y, rows, weights, out)
     if repeat_call(*call):
         return
     _check_combine(y, rows, weights, out)
