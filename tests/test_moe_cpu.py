@@ -272,3 +272,27 @@ def test_notes_of_a_call_say_which_argument_is_which_also_where_two_are_the_same
     for picked in (None, meta(128, dtype=torch.int32)):
         got = notes.tensors(fp8_cast.per_channel_arg_defs(x.dtype), lambda: yan.per_channel_cast_to_fp8(x, picked))
         assert got == {'x': 0, 'source': None if picked is None else 1, 'q': None, 'scales': None}
+
+
+def test_no_copy_of_a_weight_gradient_is_out_of_range_for_every_lane(tmp_path):
+    """The LDS that the copies go to is used again: each one has a row to wait for, whatever the operand's number of rows."""
+    import subprocess
+    from yan_amd.jit.compiler import get_hipcc_compiler, get_jit_include_dir
+    source, exe = tmp_path / 'rows.cpp', tmp_path / 'rows'
+    source.write_text("""
+#include "gemm/fp8_wgrad.hpp"
+template <int ROWS>
+int check() {
+    using Stager = yan::WgradStager<ROWS, 4>;
+    for (int rows = 1; rows <= ROWS; ++rows)
+        for (int group = 0; group < Stager::PASSES * 4; ++group) {
+            const int wave = group % 4, from = Stager::first_group(wave, rows) + 4 * Stager::source_pass(group / 4, Stager::passes_behind(wave, rows));
+            if (from < 0 || from * 8 >= rows || (group * 8 < rows && from != group)) return 1;
+        }
+    return Stager::PASSES * 32 != ROWS;
+}
+int main() { return check<64>() + check<128>() + check<256>(); }
+""")
+    subprocess.check_call([get_hipcc_compiler()[0], '-x', 'hip', '--cuda-host-only', '-std=c++20', '-O1', '-w', f'-I{get_jit_include_dir()}', str(source),
+                           '-o', str(exe)])
+    assert subprocess.run([str(exe)]).returncode == 0

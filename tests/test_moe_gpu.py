@@ -456,6 +456,27 @@ def test_grouped_weight_gradient_kernels(kernel, m, n, tiles):
                 _check_product(out[q], _decode(a)[:, lo:hi].contiguous(), _decode(b)[:, lo:hi].contiguous(), held[q].double() if accumulate else None)
 
 
+@pytest.mark.parametrize('m,n', [(1, 64), (3, 100), (8, 2000), (65, 132), (72, 64), (136, 4), (193, 260), (257, 68), (264, 520)])
+@pytest.mark.parametrize('kernel', KERNELS)
+def test_weight_gradients_of_one_k_tile_with_few_rows_in_the_last_tile(kernel, m, n):
+    """Right behind the copies of the only k-tile the sums are turned round, in the smaller kernels in the same LDS; rows behind the last one are none of theirs."""
+    g = _gen(m * n)
+    a, b = _operand(g, m, 128), _operand(g, n, 128)
+    out = torch.full((m + 1, n), 7.0, device='cuda')
+    wgrad._wgrad(a, b, out[:m], None, False, kernel)
+    _check_product(out[:m], _decode(a), _decode(b), None)
+    assert bool((out[m:] == 7.0).all())
+    groups = 2 if kernel[1] > 8 else 3
+    if kernel[1] * groups * ((-(-m // 64) * -(-n // 64) + 7) // 8 * 8) > 1024:              # more parts than a workspace holds
+        return
+    a, b = _operand(g, m, 128 * groups), _operand(g, n, 128 * groups)
+    held = torch.randn(groups, m, n, generator=g, device='cuda')
+    grouped = held.clone()
+    wgrad._wgrad(a, b, grouped, torch.arange(groups + 1, device='cuda').int() * 128, True, kernel)
+    for q in range(groups):
+        _check_product(grouped[q], _decode(a)[:, 128 * q:128 * q + 128].contiguous(), _decode(b)[:, 128 * q:128 * q + 128].contiguous(), held[q].double())
+
+
 def test_weight_gradient_edges():
     """K of zero, NaN codes, offsets that do not ascend or leave K (whatever they say, nothing outside is read), a cap on compute units."""
     g = _gen(1)

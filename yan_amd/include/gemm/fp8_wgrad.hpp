@@ -51,6 +51,42 @@ __device__ __forceinline__ void wgrad_range(const WgradProblem& p, int group, in
     }
 }
 
+// Copies of a tile's k-tiles into LDS, in TileStager's layout: an instruction has 8 rows, pass j of wave w the group j * NUM_WAVES + w. Of the rows behind the
+// operand's last one those in its group are out of range and become zeros; in the place of a group that is wholly behind it another one's rows are copied once more,
+// sums of which nobody stores. That way no copy is out of range for every lane. Such a copy waits for nothing in memory, and the kernels below use the LDS
+// again, for the next tile's rows and for their sums: they are not to rest on its zeros being there by the time that the wave's counter has it as done.
+template <int ROWS, int NUM_WAVES>
+struct WgradStager {
+    static_assert(ROWS % (8 * NUM_WAVES) == 0 && NUM_WAVES % 2 == 0);
+    static constexpr int PASSES = ROWS / 8 / NUM_WAVES;
+    uint32_t voff;                  // of this lane's chunk in a group
+    uint32_t first_at, pass_pitch;  // where the wave's first group starts, and from one pass's group to the next one's (uniform)
+    int last_pass;                  // that has rows
+
+    // Of an operand with `rows` >= 1 rows in the tile: the first group that `wave` copies, and how many passes more have rows.
+    __host__ __device__ __forceinline__ static int first_group(int wave, int rows) { return wave < (rows - 1) >> 3 ? wave : (rows - 1) >> 3; }
+    __host__ __device__ __forceinline__ static int passes_behind(int wave, int rows) { return (((rows - 1) >> 3) - first_group(wave, rows)) / NUM_WAVES; }
+    __host__ __device__ __forceinline__ static int source_pass(int pass, int last_pass) { return pass < last_pass ? pass : last_pass; }
+
+    __device__ __forceinline__ void init(uint32_t ld_bytes, int wave, int lane) {
+        const int sub = lane >> 3, slot = lane & 7;
+        voff = uint32_t(sub) * ld_bytes + (slot ^ sub ^ (wave & 1)) * kChunk;         // (slot ^ swizzle_of_row of the row that the place in LDS is for)
+        pass_pitch = uint32_t(NUM_WAVES * 8) * ld_bytes;
+    }
+    __device__ __forceinline__ void aim(int rows, uint32_t ld_bytes, int wave) {
+        first_at = uint32_t(first_group(wave, rows) * 8) * ld_bytes;
+        last_pass = passes_behind(wave, rows);
+    }
+    __device__ __forceinline__ void issue_pass(__amdgpu_buffer_rsrc_t rsrc, uint8_t* lds_tile, int k_byte0, int wave, int j) const {
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, YAN_LDS_PTR(lds_tile + (j * NUM_WAVES + wave) * 8 * kRowBytes), kChunk, voff,
+                                                 k_byte0 + first_at + uint32_t(source_pass(j, last_pass)) * pass_pitch, 0, 0);
+    }
+    __device__ __forceinline__ void issue(__amdgpu_buffer_rsrc_t rsrc, uint8_t* lds_tile, int k_byte0, int wave) const {
+#pragma unroll
+        for (int j = 0; j < PASSES; ++j) issue_pass(rsrc, lds_tile, k_byte0, wave, j);
+    }
+};
+
 // Eight codes times a power of two (a float, of which the exponent counts) as bf16.
 __device__ __forceinline__ bf16x8 wgrad_decode(int lo, int hi, float scale) {
     typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
@@ -112,10 +148,10 @@ template <int BLOCK_M, int BLOCK_N, int STAGES, bool SPLIT>
 __global__ void __launch_bounds__(256, 2)
 fp8_wgrad_kernel(WgradProblem p, WgradWorkspace w, int parts) {
     constexpr int NW = 4, WTM = BLOCK_M / 2, WTN = BLOCK_N / 2, TM = WTM / 16, TN = WTN / 16;
-    using StA = TileStager<BLOCK_M, NW>;
-    using StB = TileStager<BLOCK_N, NW>;
+    using StA = WgradStager<BLOCK_M, NW>;
+    using StB = WgradStager<BLOCK_N, NW>;
     constexpr int NUM_COPIES = StA::PASSES + StB::PASSES + 1, A_BYTES = BLOCK_M * kRowBytes, STAGE_BYTES = (BLOCK_M + BLOCK_N) * kRowBytes;
-    static_assert(StA::PADDED_ROWS == BLOCK_M && StB::PADDED_ROWS == BLOCK_N && (STAGES - 1) * NUM_COPIES <= 63);
+    static_assert((STAGES - 1) * NUM_COPIES <= 63);
     // Scales are copied with their k-tile, a dword of four k-tiles' a row, a row a lane: loaded into registers every fourth k-tile they made the wave wait for all
     // copies under way (64 tiles of 64 x 64, 64 k-tiles: 54.7 us, 36.5 so; 512 of 128 x 128, 64 k-tiles: 87.5 / 82.2).
     constexpr int SCALE_ROWS = NW * kWaveSize;
@@ -157,10 +193,12 @@ fp8_wgrad_kernel(WgradProblem p, WgradWorkspace w, int parts) {
         const uint32_t off_s = uint32_t(min(wave * kWaveSize + lane - (of_a ? 0 : BLOCK_M), rows_s - 1)) * ld_s;
         StA stage_a;
         StB stage_b;
-        stage_a.init(0, p.k, wave, lane);
-        stage_b.init(0, p.k, wave, lane);
+        stage_a.init(p.k, wave, lane);
+        stage_b.init(p.k, wave, lane);
+        stage_a.aim(rows_a, p.k, wave);
+        stage_b.aim(rows_b, p.k, wave);
         const int count = hi - lo;
-        // (a copy of nothing, out of range, may still write its zeros when it has been counted as done: none is issued, the ring is used again below)
+        // (behind the range's last k-tile there is none: the ring is used again below)
         auto copy = [&](int kt, int st) {
             if (kt >= count) return;
             uint8_t* const stage = ring + st * STAGE_BYTES;
@@ -323,9 +361,8 @@ __global__ void __launch_bounds__(256, 1)
 fp8_wgrad_tall_kernel(WgradProblem p) {
     constexpr int BLOCK_M = 256, NW = 4, TM = 8, TN = BLOCK_N / 32, WTM = 128, WTN = BLOCK_N / 2;
     static_assert(BLOCK_N % 128 == 0 && TN >= 4 && TN <= 8);
-    using StA = TileStager<BLOCK_M, NW>;
-    using StB = TileStager<BLOCK_N, NW>;
-    static_assert(StA::PADDED_ROWS == BLOCK_M && StB::PADDED_ROWS == BLOCK_N);
+    using StA = WgradStager<BLOCK_M, NW>;
+    using StB = WgradStager<BLOCK_N, NW>;
     constexpr int A_BYTES = BLOCK_M * kRowBytes, STAGE_BYTES = (BLOCK_M + BLOCK_N) * kRowBytes, PASSES = StA::PASSES + StB::PASSES;
     static_assert(PASSES <= 3 * TN);            // a row of the step behind the barrier has two copies at most, of the one after it one
     // the sums leave through pieces of 16 rows by PIECE columns, two a wave
@@ -372,8 +409,8 @@ fp8_wgrad_tall_kernel(WgradProblem p) {
 
     StA stage_a;
     StB stage_b;
-    stage_a.init(0, p.k, wave, lane);
-    stage_b.init(0, p.k, wave, lane);
+    stage_a.init(p.k, wave, lane);
+    stage_b.init(p.k, wave, lane);
     const int koff[2] = {frag_offset<16>(lane, 2 * g), frag_offset<16>(lane, 2 * g + 1)};
     const int a_lane = wm * WTM * kRowBytes, b_lane = A_BYTES + wn * WTN * kRowBytes;
 
@@ -385,15 +422,26 @@ fp8_wgrad_tall_kernel(WgradProblem p) {
     __amdgpu_buffer_rsrc_t rsrc_a, rsrc_b;
     auto aim_copies = [&] {
         const WgradTile& t = copy_tile;
-        const int rows_a = t.count ? min(BLOCK_M, p.m - t.m0) : 0, rows_b = t.count ? min(BLOCK_N, p.n - t.n0) : 0;
-        rsrc_a = make_rsrc(p.a + size_t(t.m0) * p.k + size_t(t.lo) * 128, rows_a ? uint32_t(rows_a) * p.k - uint32_t(t.lo) * 128 : 0);
-        rsrc_b = make_rsrc(p.b + size_t(t.n0) * p.k + size_t(t.lo) * 128, rows_b ? uint32_t(rows_b) * p.k - uint32_t(t.lo) * 128 : 0);
+        const int rows_a = min(BLOCK_M, p.m - t.m0), rows_b = min(BLOCK_N, p.n - t.n0);
+        rsrc_a = make_rsrc(p.a + size_t(t.m0) * p.k + size_t(t.lo) * 128, uint32_t(rows_a) * p.k - uint32_t(t.lo) * 128);
+        rsrc_b = make_rsrc(p.b + size_t(t.n0) * p.k + size_t(t.lo) * 128, uint32_t(rows_b) * p.k - uint32_t(t.lo) * 128);
+        stage_a.aim(rows_a, p.k, wave);
+        stage_b.aim(rows_b, p.k, wave);
     };
+    // Behind the walk's last k-tile that one is copied again, two times, into stages whose codes are not used any more: the count of copies under way stays
+    // what the waits below take it for, and none is out of range.
+    bool walking = true;
     auto advance_copies = [&] {
+        if (!walking) return;
         if (++copy_kt < copy_tile.count) return;
-        copy_kt = 0;
-        if (copy_tile.count) copy_tile = seek(copy_tile.slot + gridDim.x);
-        aim_copies();           // behind the last tile: descriptors of nothing
+        const WgradTile next = seek(copy_tile.slot + gridDim.x);
+        walking = next.count != 0;
+        if (!walking) {
+            --copy_kt;
+            return;
+        }
+        copy_tile = next, copy_kt = 0;
+        aim_copies();
     };
     auto copy = [&](int d, int stage) __attribute__((always_inline)) {
         if (d < StA::PASSES) stage_a.issue_pass(rsrc_a, stages + stage, copy_kt * kRowBytes, wave, d);
@@ -621,6 +669,7 @@ fp8_wgrad_tall_kernel(WgradProblem p) {
         if (nxt.count == 0) break;
         cur = nxt;
     }
+    __builtin_amdgcn_s_waitcnt(waitcnt_imm(STORES < 63 ? STORES : 63, 0));         // the copies behind the last k-tile have landed: the LDS may be another's from here on
 }
 
 // Which kernel a problem runs on, and in how many parts its K ranges. Every kernel was timed on 246 shapes (32 to 8192 rows and columns, 1 to 199 k-tiles, 1
