@@ -184,6 +184,43 @@ def test_route_of_nothing(tokens):
     assert bool((dx == 0).all()) and dx.shape == logits.shape
 
 
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize('experts,top_k', [(40, 5), (256, 8), (1000, 3)])
+def test_sigmoid_rows_far_below_zero(experts, top_k, dtype):
+    """What is a quotient of scores is defined however small they are: weights, shares and their gradient, large gradients of the weights included."""
+    g = _gen(experts)
+    centre = torch.tensor([-20.0, -60, -80, -86, -88, -95, -103, -200, -1000, -1e6, 3.0, -0.5], device='cuda')
+    logits = (centre[:, None] + torch.randn(12, experts, generator=g, device='cuda').clamp(-6, 6)).to(dtype)
+    logits[10, 1:] = -95.0                          # but one
+    logits[10, :1] = 2.0
+    w, i, c, loss = yan.moe_route(logits, top_k, 'sigmoid', True)
+    leaf = logits.double().requires_grad_()
+    log_s = torch.nn.functional.logsigmoid(leaf)
+    p, order = torch.softmax(log_s, 1), torch.argsort(logits.double(), dim=1, descending=True, stable=True)[:, :top_k]
+    want = torch.softmax(log_s.gather(1, order), 1)
+    assert torch.equal(i.long(), order) and int(c.sum()) == 12 * top_k
+    # a score 4 u, and |l - largest| <= 13 of it (row 10: those far below the one are less than 2^-126), a sum over the row, one over the picks, two quotients
+    score_off = (4 + 13 + 22 + 6 + 2) * U
+    normal = torch.full_like(want, 2.0 ** -126)
+    _close(w, want, (score_off * want + normal).detach(), 'weights')
+    loss_want = experts / (top_k * 144) * (c.double() * p.sum(0)).sum()
+    _close(loss, loss_want, (score_off + 112 * U) * loss_want.detach(), 'loss')
+    dw, dl = 1e6 * torch.randn(12, top_k, generator=g, device='cuda'), torch.tensor(50.0, device='cuda')
+    got = yan.moe_route_backward(logits, i, c, dw, dl, 'sigmoid', True)
+    ((want * dw.double()).sum() + dl.double() * loss_want).backward()
+    pull = 50.0 * experts * c.double() / (top_k * 144)
+    size = torch.zeros_like(p).scatter_(1, order, want * (dw.double().abs() + (want * dw.double().abs()).sum(1, keepdim=True)))
+    size = (size + p * (pull + (p * pull).sum(1, keepdim=True))).detach()
+    bound = (5 * score_off + 30 * U) * size + 1e7 * 2.0 ** -126
+    if dtype == torch.bfloat16:
+        bound = bound + 2.0 ** -8 * (leaf.grad.abs() + bound)
+    _close(got, leaf.grad, bound, 'gradient')
+    # without renormalising a weight is the score, which is 0 below the smallest normal number
+    w, i, _, _ = yan.moe_route(logits, top_k, 'sigmoid', False)
+    want = torch.sigmoid(logits.double()).gather(1, order)
+    _close(w, want, score_off * want + 2.0 ** -126, 'scores')
+
+
 # Dispatch
 
 def _places(indices, experts):

@@ -4,7 +4,8 @@
 //   w_i = s_i, or s_i / (sum of s over the picks);  c_e = picks of expert e;  n = tokens that are not masked
 //   p = s (softmax), s / (sum of s over the row) (sigmoid);  loss = E / (k n^2) sum_e c_e sum_t p[t, e]
 //   backward: with g_e = dloss E c_e / (k n^2), c_e taken as a constant, and h_i = dw_i, or (dw_i - sum_j w_j dw_j) / (sum of s over the
-//   picks), zero elsewhere:   softmax: dl = s (h + g - sum_e s_e (h_e + g_e));   sigmoid: dl = s (1 - s) (h + (g - sum_e p_e g_e) / sum_e s_e)
+//   picks), zero elsewhere:   softmax: dl = s (h + g - sum_e s_e (h_e + g_e));   sigmoid: dl = (1 - s) (s h + p (g - sum_e p_e g_e)),
+//   where s h of a renormalised pick is w_i (dw_i - sum_j w_j dw_j)
 //
 // A group of LANES lanes holds a row, VALUES neighbouring logits a lane, so that lower lanes have lower experts. Picks are made on the logits
 // (both scores grow with them) as unsigned keys of the same order: every lane sorts its own, then a round is the maximum over the lanes' first keys, and the
@@ -85,26 +86,40 @@ __device__ __forceinline__ float inverse_of(float x) {
 }
 constexpr float kMostLogit = std::numeric_limits<float>::max();
 __device__ __forceinline__ float finite_top(float top) { return top < -kMostLogit ? 0.f : (top > kMostLogit ? kMostLogit : top); }
-// sigmoid(l), or exp(l - top); a logit of +infinity counts as the largest finite number
+// What a row's scores are multiples of. Softmax: exp(top), top the largest logit. Sigmoid: exp(top), top the largest logit where that is below zero, else 1. So the
+// largest is not below a half, the sums that scores are divided by are normal numbers, and quotients are as exact in a row of logits all far below zero
+// as in any other (from -88 on the scores themselves are less than the smallest normal number, which counts as 0). `unit`, sigmoid: exp(top).
+struct ScoreBase {
+    float top, unit;
+};
 template <bool SIGMOID>
-__device__ __forceinline__ float score_of(float l, float top) {
+__device__ __forceinline__ ScoreBase score_base(float largest) {
     if constexpr (SIGMOID) {
-        // of the magnitude, so that no exponential overflows: 1 / (1 + e^-|l|), or that times e^-|l|
-        const float t = exp_of(-fabsf(l)), r = inverse_of(1.f + t);
+        const float top = fminf(finite_top(largest), 0.f);
+        return {top, exp_of(top)};
+    }
+    return {finite_top(largest), 1.f};
+}
+// A score in multiples of its row's base: sigmoid(l) / unit, or exp(l - top); a logit of +infinity counts as the largest finite number
+template <bool SIGMOID>
+__device__ __forceinline__ float score_of(float l, ScoreBase base) {
+    if constexpr (SIGMOID) {
+        // of the magnitude, so that no exponential overflows: 1 / (1 + e^-|l|), or that times e^-|l|, which is t * unit
+        const float t = exp_of(fminf(l - base.top, -l)), r = inverse_of(fmaf(t, base.unit, 1.f));
         return l < 0.f ? t * r : r;
     } else {
-        return exp_of((l > kMostLogit ? kMostLogit : l) - top);
+        return exp_of((l > kMostLogit ? kMostLogit : l) - base.top);
     }
 }
 
-// A row's scores: v are the logits (-infinity past the row's end), `top` the largest as finite_top gives it; returns their sum (softmax: before they
-// were divided by it). A row of -infinity alone has scores of zero.
+// A row's scores: v are the logits (-infinity past the row's end). Returns their sum, both in multiples of the base (softmax: the sum, by which they have been divided).
+// A row of -infinity alone has scores of zero.
 template <bool SIGMOID, int LANES, int VALUES>
-__device__ __forceinline__ float row_scores(float (&s)[VALUES], const float (&v)[VALUES], float top) {
+__device__ __forceinline__ float row_scores(float (&s)[VALUES], const float (&v)[VALUES], ScoreBase base) {
     float sum = 0.f;
 #pragma unroll
     for (int j = 0; j < VALUES; ++j) {
-        s[j] = score_of<SIGMOID>(v[j], top);
+        s[j] = score_of<SIGMOID>(v[j], base);
         sum += s[j];
     }
     sum = sum_lanes<LANES>(sum);
@@ -206,11 +221,12 @@ moe_route_kernel(const T* __restrict__ logits, const uint8_t* __restrict__ mask,
         const uint32_t my_key = mine_at.y;
         if (live && in_group < top_k) atomicAdd(&lds_counts[my_pick], 1);
         asm volatile("" ::: "memory");
-        top = finite_top(top);
-        const float sum = row_scores<SIGMOID, LANES>(s, v, top), inverse = inverse_of(sum);
+        const ScoreBase base = score_base<SIGMOID>(top);
+        const float sum = row_scores<SIGMOID, LANES>(s, v, base), inverse = inverse_of(sum);
         // lane i has pick i: its score again, from the logit that its key stands for
-        float mine = in_group < top_k ? score_of<SIGMOID>(value_of_key(my_key), top) * (SIGMOID ? 1.f : inverse) : 0.f;
+        float mine = in_group < top_k ? score_of<SIGMOID>(value_of_key(my_key), base) * (SIGMOID ? 1.f : inverse) : 0.f;
         if (renormalize) mine *= inverse_of(sum_lanes<LANES>(mine));
+        else if (SIGMOID) mine *= base.unit;
         if (sum != sum) mine = sum;
         if (t < tokens && in_group < top_k) {
             weights[size_t(t) * top_k + in_group] = live ? mine : 0.f;
@@ -377,12 +393,15 @@ moe_route_backward_kernel(const T* __restrict__ logits, const int* __restrict__ 
         float top = v[0];
 #pragma unroll
         for (int j = 1; j < VALUES; ++j) top = fmaxf(top, v[j]);
-        top = finite_top(max_lanes<LANES>(top));
-        const float sum = row_scores<SIGMOID, LANES>(s, v, top), inverse = inverse_of(sum);
+        const ScoreBase base = score_base<SIGMOID>(max_lanes<LANES>(top));
+        const float sum = row_scores<SIGMOID, LANES>(s, v, base), inverse = inverse_of(sum);
+        // sigmoid: s h, in which the base cancels out where weights are renormalised; softmax: h
         if (renormalize) {
-            const float mine = pick < 0 ? 0.f : score_of<SIGMOID>(logit, top) * (SIGMOID ? 1.f : inverse);
-            const float part = inverse_of(sum_lanes<LANES>(mine));
-            dw = (dw - sum_lanes<LANES>(mine * part * dw)) * part;
+            const float mine = pick < 0 ? 0.f : score_of<SIGMOID>(logit, base) * (SIGMOID ? 1.f : inverse);
+            const float part = inverse_of(sum_lanes<LANES>(mine)), weight = mine * part;
+            dw = (dw - sum_lanes<LANES>(weight * dw)) * (SIGMOID ? weight : part);
+        } else if (SIGMOID) {
+            dw *= pick < 0 ? 0.f : score_of<SIGMOID>(logit, base) * base.unit;
         }
         asm volatile("" ::: "memory");              // a wave's LDS operations are done in order: the zeros, the picks, then the reads
         if (pick >= 0) h_row[pick] = dw;
@@ -391,13 +410,13 @@ moe_route_backward_kernel(const T* __restrict__ logits, const int* __restrict__ 
 #pragma unroll
         for (int j = 0; j < VALUES; ++j) {
             d[j] = h_row[first + j] + (SIGMOID ? 0.f : g[j]);
-            dot += s[j] * (SIGMOID ? g[j] : d[j]);
+            dot += SIGMOID ? s[j] * inverse * g[j] : s[j] * d[j];
         }
         asm volatile("" ::: "memory");
         dot = sum_lanes<LANES>(dot);
 #pragma unroll
         for (int j = 0; j < VALUES; ++j) {
-            if constexpr (SIGMOID) d[j] = s[j] * (1.f - s[j]) * (d[j] + (g[j] - dot * inverse) * inverse);
+            if constexpr (SIGMOID) d[j] = (1.f - s[j] * base.unit) * (d[j] + s[j] * inverse * (g[j] - dot));
             else d[j] = s[j] * (d[j] - dot);
             if (!live) d[j] = 0.f;
         }

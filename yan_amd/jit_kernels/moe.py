@@ -129,7 +129,7 @@ def moe_route(logits: torch.Tensor, top_k: int, scoring: str = 'softmax', renorm
 
     logits: bf16 or fp32 `[tokens, experts]`, contiguous; up to 1024 experts, top_k up to 16
     scoring: scores s are 'softmax' or 'sigmoid' of the logits
-    renormalize: weights are s over the sum of s of the token's picks; else s itself
+    renormalize: weights are s over the sum of s of the token's picks; else s itself (0 for sigmoid scores below 2^-126)
     mask: bool `[tokens]`; tokens where it is false are padding: indices -1, weights 0, in neither counts nor loss
     Returns weights fp32 `[tokens, top_k]`, indices int32 `[tokens, top_k]` (largest logit first, ties to the lowest expert), counts int32
     `[experts]` and loss, fp32 with no dimensions: `experts * sum_e f_e P_e`, f_e the share of the picks that are e and P_e the mean over the tokens
