@@ -221,6 +221,34 @@ def test_sigmoid_rows_far_below_zero(experts, top_k, dtype):
     _close(w, want, score_off * want + 2.0 ** -126, 'scores')
 
 
+@pytest.mark.parametrize('renormalize', [True, False])
+def test_sigmoid_gradient_of_confident_logits(renormalize):
+    """The slope of a score near one is as exact, relatively, as anywhere else: 1 - s is not a difference of rounded numbers."""
+    g = _gen(17)
+    tokens, experts, top_k = 64, 32, 4
+    logits = 60 * torch.rand(tokens, experts, generator=g, device='cuda') - 30
+    logits[:8] = 20 + 10 * torch.rand(8, experts, generator=g, device='cuda')
+    w, i, c, loss = yan.moe_route(logits, top_k, 'sigmoid', renormalize)
+    dw = torch.randn(tokens, top_k, generator=g, device='cuda')
+    for dl in (None, torch.tensor(3.0, device='cuda')):
+        got = yan.moe_route_backward(logits, i, c, dw, dl, 'sigmoid', renormalize)
+        l = logits.double()
+        s, slope = torch.sigmoid(l), torch.sigmoid(-l)
+        p = s / s.sum(1, keepdim=True)
+        weight = s.gather(1, i.long())
+        if renormalize:
+            weight = weight / weight.sum(1, keepdim=True)
+            inner, spread = dw.double() - (weight * dw.double()).sum(1, keepdim=True), dw.double().abs() + (weight * dw.double().abs()).sum(1, keepdim=True)
+        else:
+            inner, spread = dw.double(), dw.double().abs()
+        pull = (0.0 if dl is None else 3.0) * experts * c.double() / (top_k * tokens * tokens)
+        back = p * (pull - (p * pull).sum(1, keepdim=True))
+        want = slope * (torch.zeros_like(s).scatter_(1, i.long(), weight * inner) + back)
+        size = slope * (torch.zeros_like(s).scatter_(1, i.long(), weight * spread) + p * (pull + (p * pull).sum(1, keepdim=True)))
+        # as for the gradient above, an exponential's argument of up to 30
+        _close(got, want, (5 * (4 + 30 + 22 + 6 + 2) * U + 30 * U) * size + 2.0 ** -126, f'gradient with loss {dl is not None}')
+
+
 # Dispatch
 
 def _places(indices, experts):

@@ -79,11 +79,12 @@ __device__ __forceinline__ float exp_of(float x) {
     const float y = __builtin_amdgcn_exp2f(high);
     return x < -87.f ? 0.f : fmaf(y, low * LN_2, y);
 }
-// 1 / x for normal numbers, one step of Newton behind the hardware's estimate; 0 for 0
-__device__ __forceinline__ float inverse_of(float x) {
+// 1 / x for normal numbers, one step of Newton behind the hardware's estimate; and that with 0 for 0
+__device__ __forceinline__ float inverse_of_normal(float x) {
     const float r = __builtin_amdgcn_rcpf(x);
-    return x == 0.f ? 0.f : fmaf(fmaf(-x, r, 1.f), r, r);
+    return fmaf(fmaf(-x, r, 1.f), r, r);
 }
+__device__ __forceinline__ float inverse_of(float x) { return x == 0.f ? 0.f : inverse_of_normal(x); }
 constexpr float kMostLogit = std::numeric_limits<float>::max();
 __device__ __forceinline__ float finite_top(float top) { return top < -kMostLogit ? 0.f : (top > kMostLogit ? kMostLogit : top); }
 // What a row's scores are multiples of. Softmax: exp(top), top the largest logit. Sigmoid: exp(top), top the largest logit where that is below zero, else 1. So the
@@ -100,12 +101,14 @@ __device__ __forceinline__ ScoreBase score_base(float largest) {
     }
     return {finite_top(largest), 1.f};
 }
-// A score in multiples of its row's base: sigmoid(l) / unit, or exp(l - top); a logit of +infinity counts as the largest finite number
+// A score in multiples of its row's base: sigmoid(l) / unit, or exp(l - top); a logit of +infinity counts as the largest finite number. Sigmoid: `rest` gets 1 - s,
+// which near s = 1 is no difference of rounded numbers.
 template <bool SIGMOID>
-__device__ __forceinline__ float score_of(float l, ScoreBase base) {
+__device__ __forceinline__ float score_of(float l, ScoreBase base, float* rest = nullptr) {
     if constexpr (SIGMOID) {
         // of the magnitude, so that no exponential overflows: 1 / (1 + e^-|l|), or that times e^-|l|, which is t * unit
-        const float t = exp_of(fminf(l - base.top, -l)), r = inverse_of(fmaf(t, base.unit, 1.f));
+        const float t = exp_of(fminf(l - base.top, -l)), r = inverse_of_normal(fmaf(t, base.unit, 1.f));
+        if (rest) *rest = l < 0.f ? r : t * r;
         return l < 0.f ? t * r : r;
     } else {
         return exp_of((l > kMostLogit ? kMostLogit : l) - base.top);
@@ -113,13 +116,13 @@ __device__ __forceinline__ float score_of(float l, ScoreBase base) {
 }
 
 // A row's scores: v are the logits (-infinity past the row's end). Returns their sum, both in multiples of the base (softmax: the sum, by which they have been divided).
-// A row of -infinity alone has scores of zero.
+// A row of -infinity alone has scores of zero. `rest`: [VALUES], as score_of has it.
 template <bool SIGMOID, int LANES, int VALUES>
-__device__ __forceinline__ float row_scores(float (&s)[VALUES], const float (&v)[VALUES], ScoreBase base) {
+__device__ __forceinline__ float row_scores(float (&s)[VALUES], const float (&v)[VALUES], ScoreBase base, float* rest = nullptr) {
     float sum = 0.f;
 #pragma unroll
     for (int j = 0; j < VALUES; ++j) {
-        s[j] = score_of<SIGMOID>(v[j], base);
+        s[j] = score_of<SIGMOID>(v[j], base, rest ? rest + j : nullptr);
         sum += s[j];
     }
     sum = sum_lanes<LANES>(sum);
@@ -394,7 +397,8 @@ moe_route_backward_kernel(const T* __restrict__ logits, const int* __restrict__ 
 #pragma unroll
         for (int j = 1; j < VALUES; ++j) top = fmaxf(top, v[j]);
         const ScoreBase base = score_base<SIGMOID>(max_lanes<LANES>(top));
-        const float sum = row_scores<SIGMOID, LANES>(s, v, base), inverse = inverse_of(sum);
+        float rest[VALUES];
+        const float sum = row_scores<SIGMOID, LANES>(s, v, base, rest), inverse = inverse_of(sum);
         // sigmoid: s h, in which the base cancels out where weights are renormalised; softmax: h
         if (renormalize) {
             const float mine = pick < 0 ? 0.f : score_of<SIGMOID>(logit, base) * (SIGMOID ? 1.f : inverse);
@@ -410,13 +414,14 @@ moe_route_backward_kernel(const T* __restrict__ logits, const int* __restrict__ 
 #pragma unroll
         for (int j = 0; j < VALUES; ++j) {
             d[j] = h_row[first + j] + (SIGMOID ? 0.f : g[j]);
-            dot += SIGMOID ? s[j] * inverse * g[j] : s[j] * d[j];
+            dot += s[j] * (SIGMOID ? g[j] : d[j]);
         }
         asm volatile("" ::: "memory");
         dot = sum_lanes<LANES>(dot);
+        const float pull = dot * inverse;           // sigmoid: the sum of p g
 #pragma unroll
         for (int j = 0; j < VALUES; ++j) {
-            if constexpr (SIGMOID) d[j] = (1.f - s[j] * base.unit) * (d[j] + s[j] * inverse * (g[j] - dot));
+            if constexpr (SIGMOID) d[j] = rest[j] * (d[j] + s[j] * ((g[j] - pull) * inverse));
             else d[j] = s[j] * (d[j] - dot);
             if (!live) d[j] = 0.f;
         }
@@ -462,7 +467,7 @@ inline hipError_t launch_moe_route_backward(const T* logits, const int* indices,
     if (tokens == 0) return hipSuccess;
     if (!logits || !indices || !counts || !grad_logits) return hipErrorInvalidValue;
     // as many workgroups as are resident, so that each reads the counts once (fp32, 16384 tokens, 1024 / 2048 / 4096 workgroups: 256 experts 12.1, 11.8, 12.4 us,
-    // 512 experts 18.6, 20.8, 25.9)
+    // 512 experts 18.6, 20.8, 25.9; with exact slopes sigmoid takes 12.4 and 19.4, softmax 11.3 and 17.2)
     constexpr int MOST = VALUES > 4 ? 1024 : 2048;
     const int blocks = std::min(ceil_div(tokens, 256 / LANES), MOST);
     hipLaunchKernelGGL((moe_route_backward_kernel<T, SIGMOID, LANES, VALUES>), dim3(blocks), dim3(256), 0, stream, logits, indices,
