@@ -249,6 +249,28 @@ def test_sigmoid_gradient_of_confident_logits(renormalize):
         _close(got, want, (5 * (4 + 30 + 22 + 6 + 2) * U + 30 * U) * size + 2.0 ** -126, f'gradient with loss {dl is not None}')
 
 
+def test_route_of_more_picks_than_a_number_of_31_bits_counts():
+    """The limits are 2^30 tokens and 16 picks, whose product no 32 bits hold: loss and gradient of 402653184 equal tokens with 8 picks."""
+    tokens, experts, top_k = 3 << 27, 16, 8
+    row = torch.linspace(1, -1, experts, device='cuda').bfloat16()
+    logits = row.expand(tokens, experts).contiguous()
+    w, i, c, loss = yan.moe_route(logits, top_k)
+    assert c.tolist() == [tokens] * top_k + [0] * (experts - top_k) and i[-1].tolist() == list(range(top_k))
+    p = torch.softmax(row.double(), 0)
+    _close(w[-1], p[:top_k] / p[:top_k].sum(), 50 * U * torch.ones(top_k, device='cuda'))
+    # a lane adds up the shares of every 16384th token, then come the sums over a workgroup and over 256 of them
+    want = experts / top_k * p[:top_k].sum()
+    _close(loss, want, (tokens / 16384 + 100 + 50) * U * want, 'loss')
+    del w
+    got = yan.moe_route_backward(logits, i, c, None, torch.full((1, ), float(tokens), device='cuda'))
+    pull = torch.zeros_like(p)
+    pull[:top_k] = experts / top_k
+    want = p * (pull - (p * pull).sum())
+    bound = 200 * U * p * (pull + (p * pull).sum())
+    for at in (0, tokens // 2, tokens - 1):
+        _close(got[at], want, bound + 2.0 ** -8 * (want.abs() + bound), 'gradient')
+
+
 # Dispatch
 
 def _places(indices, experts):

@@ -134,27 +134,37 @@ __device__ __forceinline__ float row_scores(float (&s)[VALUES], const float (&v)
     return sum;
 }
 
+// The picks of all experts, up to 2^34: sums of the counts' lower 16 bits and of what is above them, neither of which passes 2^26.
+struct Picks {
+    int low, high;
+    __device__ __forceinline__ void add(int count) { low += count & 0xffff, high += count >> 16; }
+    template <int LANES>
+    __device__ __forceinline__ Picks over_lanes() const { return {sum_lanes<LANES>(low), sum_lanes<LANES>(high)}; }
+    __device__ __forceinline__ float number() const { return float((long long)high * 65536 + low); }
+};
+
 // What the workgroups of a launch leave for the second kernel: [blocks][E] sums of p, [blocks][E] counts, and per group of 16 experts the
-// sums of c p and of c; `arrived` counts those groups.
+// sums of c p and of c (in two parts); `arrived` counts those groups.
 struct RouteWorkspace {
     float* share;
     int* counts;
     float* pull;
-    int* picks;
+    int *picks_low, *picks_high;
     unsigned* arrived;
     __host__ __device__ RouteWorkspace(void* at, int blocks, int e) {
         share = static_cast<float*>(at);
         counts = reinterpret_cast<int*>(share + size_t(blocks) * e);
         pull = reinterpret_cast<float*>(counts + size_t(blocks) * e);
-        picks = reinterpret_cast<int*>(pull + (e + 15) / 16);
-        arrived = reinterpret_cast<unsigned*>(picks + (e + 15) / 16);
+        picks_low = reinterpret_cast<int*>(pull + (e + 15) / 16);
+        picks_high = picks_low + (e + 15) / 16;
+        arrived = reinterpret_cast<unsigned*>(picks_high + (e + 15) / 16);
     }
-    __host__ static size_t bytes(int blocks, int e) { return (size_t(blocks) * e * 2 + 2 * ((e + 15) / 16) + 1) * 4; }
+    __host__ static size_t bytes(int blocks, int e) { return (size_t(blocks) * e * 2 + 3 * ((e + 15) / 16) + 1) * 4; }
 };
 
-__device__ __forceinline__ float balance_loss(float pull, int picks, int top_k, int e) {
-    const float n = float(picks) / float(top_k);
-    return picks == 0 ? 0.f : pull * float(e) / (float(top_k) * n * n);
+__device__ __forceinline__ float balance_loss(float pull, Picks picks, int top_k, int e) {
+    const float n = picks.number() / float(top_k);
+    return n == 0.f ? 0.f : pull * float(e) / (float(top_k) * n * n);
 }
 
 template <typename T, bool SIGMOID, int LANES, int VALUES, int THREADS>
@@ -166,7 +176,7 @@ moe_route_kernel(const T* __restrict__ logits, const uint8_t* __restrict__ mask,
     __shared__ int lds_counts[LANES * VALUES];
     __shared__ uint2 lds_pick[GROUPS][kMaxTopK];
     __shared__ float lds_pull[WAVES];
-    __shared__ int lds_picks[WAVES];
+    __shared__ Picks lds_picks[WAVES];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, in_group = lane % LANES, first = in_group * VALUES, group_base = lane - in_group;
     float share[VALUES];
 #pragma unroll
@@ -252,7 +262,7 @@ moe_route_kernel(const T* __restrict__ logits, const uint8_t* __restrict__ mask,
     // see each other's lines.
     unsigned long long* const meet = reinterpret_cast<unsigned long long*>(static_cast<uint8_t*>(workspace) + kSplitKCounterBytes);
     float pull = 0.f;
-    int picks = 0;
+    Picks picks{0, 0};
     for (int x = threadIdx.x; x < e; x += THREADS) {
         float sum = 0.f;
 #pragma unroll
@@ -261,7 +271,7 @@ moe_route_kernel(const T* __restrict__ logits, const uint8_t* __restrict__ mask,
         if (alone) {
             counts[x] = number;
             pull += float(number) * sum;
-            picks += number;
+            picks.add(number);
         } else if (join) {
             __hip_atomic_store(meet + size_t(blockIdx.x) * e + x, uint64_t(uint32_t(number)) << 32 | __builtin_bit_cast(uint32_t, sum), __ATOMIC_RELAXED,
                                __HIP_MEMORY_SCOPE_AGENT);
@@ -297,14 +307,16 @@ moe_route_kernel(const T* __restrict__ logits, const uint8_t* __restrict__ mask,
             }
             counts[x] = number;
             pull += float(number) * sum;
-            picks += number;
+            picks.add(number);
         }
     }
-    pull = sum_lanes<64>(pull), picks = sum_lanes<64>(picks);
+    pull = sum_lanes<64>(pull), picks = picks.over_lanes<64>();
     if (lane == 0) lds_pull[wave] = pull, lds_picks[wave] = picks;
     __syncthreads();
     if (wave == 0) {
-        pull = sum_lanes<16>(lane < WAVES ? lds_pull[lane] : 0.f), picks = sum_lanes<16>(lane < WAVES ? lds_picks[lane] : 0);
+        pull = sum_lanes<16>(lane < WAVES ? lds_pull[lane] : 0.f);
+        picks = lane < WAVES ? lds_picks[lane] : Picks{0, 0};
+        picks = picks.over_lanes<16>();
         if (lane == 0) *loss = balance_loss(pull, picks, top_k, e);
     }
 }
@@ -331,12 +343,15 @@ moe_route_finish_kernel(int* __restrict__ counts, float* __restrict__ loss, void
     share = sum_groups<16>(share), number = sum_groups<16>(number);
     if (threadIdx.x < 16 && x < e) counts[x] = number;
     float pull = sum_lanes<16>(float(number) * share);
-    int picks = sum_lanes<16>(number);
+    Picks picks{0, 0};
+    picks.add(number);
+    picks = picks.over_lanes<16>();
     // Written and read at device scope: the workgroups are on different XCDs, whose L2s do not see each other's lines.
     unsigned before = 0;
     if (threadIdx.x == 0) {
         __hip_atomic_store(from.pull + blockIdx.x, pull, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        __hip_atomic_store(from.picks + blockIdx.x, picks, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        __hip_atomic_store(from.picks_low + blockIdx.x, picks.low, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        __hip_atomic_store(from.picks_high + blockIdx.x, picks.high, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         __builtin_amdgcn_s_waitcnt(waitcnt_imm(0, 0));
         asm volatile("" ::: "memory");
         before = __hip_atomic_fetch_add(from.arrived, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
@@ -344,12 +359,13 @@ moe_route_finish_kernel(int* __restrict__ counts, float* __restrict__ loss, void
     before = __builtin_amdgcn_readfirstlane(before);
     asm volatile("" ::: "memory");
     if (before != gridDim.x - 1) return;
-    pull = 0.f, picks = 0;                  // at most kMaxExperts / 16 = 64 groups
+    pull = 0.f, picks = Picks{0, 0};        // at most kMaxExperts / 16 = 64 groups
     if (threadIdx.x < gridDim.x) {
         pull = __hip_atomic_load(from.pull + threadIdx.x, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        picks = __hip_atomic_load(from.picks + threadIdx.x, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        picks.low = __hip_atomic_load(from.picks_low + threadIdx.x, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        picks.high = __hip_atomic_load(from.picks_high + threadIdx.x, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     }
-    pull = sum_lanes<64>(pull), picks = sum_lanes<64>(picks);
+    pull = sum_lanes<64>(pull), picks = picks.over_lanes<64>();
     if (threadIdx.x == 0) *loss = balance_loss(pull, picks, top_k, e);
 }
 
@@ -366,11 +382,11 @@ moe_route_backward_kernel(const T* __restrict__ logits, const int* __restrict__ 
     // g: the balance loss's pull on the share of each of this lane's experts
     float g[VALUES];
     {
-        int picks = 0, c[VALUES];
+        Picks picks{0, 0};
+        int c[VALUES];
 #pragma unroll
-        for (int j = 0; j < VALUES; ++j) c[j] = first + j < e ? counts[first + j] : 0, picks += c[j];
-        picks = sum_lanes<LANES>(picks);
-        const float n = float(picks) / float(top_k), scale = grad_loss && picks ? *grad_loss * float(e) / (float(top_k) * n * n) : 0.f;
+        for (int j = 0; j < VALUES; ++j) c[j] = first + j < e ? counts[first + j] : 0, picks.add(c[j]);
+        const float n = picks.template over_lanes<LANES>().number() / float(top_k), scale = grad_loss && n > 0.f ? *grad_loss * float(e) / (float(top_k) * n * n) : 0.f;
 #pragma unroll
         for (int j = 0; j < VALUES; ++j) g[j] = scale * float(c[j]);
     }

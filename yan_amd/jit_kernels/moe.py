@@ -156,7 +156,7 @@ def moe_route(logits: torch.Tensor, top_k: int, scoring: str = 'softmax', renorm
     # the workgroups' counts and shares: joined within the kernel, in the split-K workspace of the stream, or left in scratch for a second one
     joined, token = split_k_workspace(device, stream) if route_joins(blocks, experts) else (None, None)
     # RouteWorkspace::bytes of moe/route.hpp
-    scratch = None if joined is not None or blocks == 1 else torch.empty(4 * (2 * blocks * experts + 2 * ceil_div(experts, 16) + 1), dtype=torch.uint8, device=device)
+    scratch = None if joined is not None or blocks == 1 else torch.empty(4 * (2 * blocks * experts + 3 * ceil_div(experts, 16) + 1), dtype=torch.uint8, device=device)
     workspace = joined if joined is not None else scratch if scratch is not None else weights.view(torch.uint8)
     mask_bytes = workspace if mask is None else mask.view(torch.uint8)
     done = _run(route_kernel_plan(logits.dtype, scoring, experts, False, threads), _route_includes,
