@@ -167,6 +167,22 @@ def test_more_tokens_than_a_launch_counts_are_refused():
             _refused(moe._check_combine, y, rows, None, out)
 
 
+def test_more_pairs_than_row_numbers_hold_are_refused():
+    """Rows are numbers of 32 bits, with every expert's rounded up, and so are the places of a chunk's pairs behind the last token."""
+    for tokens, top_k, experts in ((143165576, 15, 16), (143165576, 15, 1), ((1 << 27) - 1, 16, 4), ((1 << 31) - 1, 1, 64)):
+        x, indices = torch.empty(tokens, 128, dtype=torch.bfloat16, device='meta'), torch.empty(tokens, top_k, dtype=torch.int32, device='meta')
+        codes, scales = torch.empty(256, 128, dtype=F8, device='meta'), torch.empty(256, 1, device='meta')
+        _refused(moe._check_dispatch, x, indices, codes, scales, experts)
+    most = moe.MAX_PAIRS
+    assert most + 127 * moe.MAX_EXPERTS < 1 << 31 and most + moe.TOKENS_PER_BLOCK * moe.MAX_TOP_K < 1 << 31
+    for pairs, taken in ((most, True), (most + 1, False)):
+        x, indices = torch.empty(pairs, 128, dtype=torch.bfloat16, device='meta'), torch.empty(pairs, 1, dtype=torch.int32, device='meta')
+        if taken:
+            moe._check_dispatch(x, indices, codes, scales, moe.MAX_EXPERTS)
+        else:
+            _refused(moe._check_dispatch, x, indices, codes, scales, moe.MAX_EXPERTS)
+
+
 def _stores_of_16_bytes(tmp_path, code):
     import subprocess
     from yan_amd.jit.compiler import get_hipcc_compiler, get_jit_include_dir, get_offload_arch

@@ -20,6 +20,8 @@ namespace yan {
 constexpr int kExpertAlignment = 128;
 constexpr int kFewPairs = 4096;             // up to here every workgroup counts all pairs itself
 constexpr int kTokensPerBlock = 16;         // above: tokens of a chunk
+constexpr long long kMaxPairs = (1ll << 31) - (1 << 18);        // so that rows, every expert's rounded up to 128, and a chunk's pairs behind the last token are numbers of 32 bits
+static_assert(kMaxPairs + (kExpertAlignment - 1) * kMaxExperts < 1ll << 31 && kMaxPairs + kTokensPerBlock * kMaxTopK < 1ll << 31);
 constexpr long long kDispatchCacheBytes = 192ll << 20;
 
 struct DispatchShape {
@@ -286,7 +288,7 @@ inline hipError_t launch_moe_dispatch(const T* x, const int* indices, void* code
                                       int top_k, int experts, int m_max, int rows, hipStream_t stream) {
     if (tokens < 0 || k < 128 || k % 128 != 0 || top_k < 1 || top_k > kMaxTopK || experts < 1 || experts > kMaxExperts || m_max < 0 || rows < 0) return hipErrorInvalidValue;
     if (m_max ? rows != experts * m_max : rows % kExpertAlignment != 0) return hipErrorInvalidValue;
-    if ((long long)tokens * top_k >= 1ll << 31 || (long long)experts * m_max >= 1ll << 31) return hipErrorInvalidValue;
+    if ((long long)tokens * top_k > kMaxPairs || (long long)experts * m_max >= 1ll << 31) return hipErrorInvalidValue;
     if (!m_indices || (!m_max && !offsets)) return hipErrorInvalidValue;
     if (tokens && (!x || !indices || !rows_of)) return hipErrorInvalidValue;
     if (rows && (!codes || !scales || (!m_max && !source))) return hipErrorInvalidValue;

@@ -23,12 +23,13 @@ from .split_k import split_k_launch_failed, split_k_workspace
 from .tuner import FrozenKeys, jit_tuner
 from .utils import assert_on_current_device, ceil_div, current_raw_stream, get_m_alignment_for_contiguous_layout
 
-# kMaxTopK, kMaxTokens and kMaxExperts of moe/route.hpp, kFewPairs and kTokensPerBlock of moe/dispatch.hpp
+# kMaxTopK, kMaxTokens and kMaxExperts of moe/route.hpp, kFewPairs, kTokensPerBlock and kMaxPairs of moe/dispatch.hpp
 MAX_TOP_K = 16
 MAX_TOKENS = 1 << 30
 MAX_EXPERTS = 1024
 FEW_PAIRS = 4096
 TOKENS_PER_BLOCK = 16
+MAX_PAIRS = (1 << 31) - (1 << 18)
 
 _ELEMENTS = {torch.bfloat16: '__bf16', torch.float32: 'float'}
 _SCORINGS = {'softmax': 0, 'sigmoid': 1}
@@ -235,7 +236,7 @@ def get_contiguous_layout_rows(num_tokens: int, top_k: int, num_experts: int) ->
 def _check_dispatch(x, indices, codes, scales, num_experts):
     assert x.dim() == 2 and x.dtype in _ELEMENTS and x.is_contiguous() and x.size(1) % 128 == 0 and x.size(1) > 0
     assert indices.dim() == 2 and indices.size(0) == x.size(0) and indices.dtype == torch.int32 and indices.is_contiguous()
-    assert 1 <= indices.size(1) <= MAX_TOP_K and 1 <= num_experts <= MAX_EXPERTS and indices.numel() < 1 << 31
+    assert 1 <= indices.size(1) <= MAX_TOP_K and 1 <= num_experts <= MAX_EXPERTS and indices.numel() <= MAX_PAIRS
     assert codes.dtype == torch.float8_e4m3fn and codes.is_contiguous() and codes.size(-1) == x.size(1)
     assert scales.dtype == torch.float32 and scales.shape == (*codes.shape[:-1], x.size(1) // 128)
     assert codes.numel() // x.size(1) < 1 << 31 and all(0 <= s < 1 << 31 for s in scales.stride())
