@@ -416,6 +416,18 @@ def test_combine_and_its_gradient(tokens, n, m, top_k, weighted):
         assert grad_w is None
 
 
+def test_combine_of_no_columns():
+    rows = torch.tensor([[0, 1], [2, -1], [3, 5]], dtype=torch.int32, device='cuda')
+    source = torch.tensor([0, 0, 1, 2, -1, 2], dtype=torch.int32, device='cuda')
+    y, out, w = torch.empty(6, 0, dtype=torch.bfloat16, device='cuda'), torch.empty(3, 0, dtype=torch.bfloat16, device='cuda'), torch.ones(3, 2, device='cuda')
+    for _ in range(2):          # the second natively
+        yan.moe_combine(y, rows, w, out)
+        grad_y, grad_w = yan.moe_combine_backward(out, y, rows, w, source)
+        assert grad_y.shape == y.shape and grad_y.dtype == y.dtype and grad_w.shape == w.shape and bool((grad_w == 0).all())
+        grad_y, grad_w = yan.moe_combine_backward(out, y, rows, None, source)
+        assert grad_y.shape == y.shape and grad_w is None
+
+
 # Quantiser
 
 def _turned(x, source):

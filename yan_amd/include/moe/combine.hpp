@@ -161,8 +161,9 @@ template <int TOP_K>
 inline hipError_t launch_moe_combine_backward(const __bf16* grad_out, const __bf16* y, const int* rows_of, const float* weights, const int* source,
                                               __bf16* grad_y, float* grad_weights, int tokens, int columns, int rows, hipStream_t stream) {
     if (tokens < 0 || tokens > kMaxTokens || columns < 0 || columns % 8 != 0 || rows < 0) return hipErrorInvalidValue;
-    if (tokens && (!grad_out || !rows_of)) return hipErrorInvalidValue;
-    if (rows && (!source || !grad_y || !y)) return hipErrorInvalidValue;
+    // (without columns there is nothing behind y and the gradients, and the weights' gradient is zero)
+    if (tokens && (!rows_of || (columns && !grad_out))) return hipErrorInvalidValue;
+    if (rows && (!source || (columns && (!grad_y || !y)))) return hipErrorInvalidValue;
     const int pieces = columns / 8;
     const bool wide = pieces > kWaveSize;
     const int token_blocks = wide ? tokens : ceil_div(tokens, 4), clear_blocks = ceil_div(rows, kRowsPerClearBlock);
