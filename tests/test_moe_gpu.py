@@ -731,6 +731,41 @@ def test_training_step_of_a_layer():
     _close(grad_x, want.sum(1), 2.0 ** -8 * want.sum(1).abs() + 8 * U * want.abs().sum(1), 'gradient of the tokens')
 
 
+@pytest.mark.parametrize('m_sum', [0, 128])
+def test_training_step_of_no_tokens(m_sum):
+    """An empty batch goes through the layer, forward and backward; its layout has no rows, or more than it needs."""
+    hidden, inner, experts, top_k = 256, 384, 6, 3
+    x, logits, w8, ws, dout = _layer(0, hidden, inner, experts, top_k, 13)
+    assert yan.get_contiguous_layout_rows(0, top_k, experts) == 0
+    for _ in range(2):          # the second natively
+        weights, indices, counts, loss = yan.moe_route(logits, top_k)
+        codes, scales = torch.zeros(m_sum, hidden, dtype=torch.uint8, device='cuda').view(F8), torch.zeros(hidden // 128, m_sum, device='cuda').t()
+        rows, m_indices, source, offsets = yan.moe_dispatch_to_fp8_contiguous(x, indices, experts, (codes, scales))
+        assert rows.shape == (0, top_k) and offsets.tolist() == [0] * (experts + 1) and m_indices.tolist() == source.tolist() == [-1] * m_sum
+        y, out = torch.zeros(m_sum, inner, dtype=torch.bfloat16, device='cuda'), torch.empty(0, inner, dtype=torch.bfloat16, device='cuda')
+        yan.moe_combine(y, rows, weights, out)
+        grad_y, grad_weights = yan.moe_combine_backward(dout, y, rows, weights, source)
+        assert grad_y.shape == y.shape and bool((grad_y == 0).all()) and grad_weights.shape == (0, top_k)
+        grad_w = torch.full((experts, inner, hidden), 3.0, device='cuda')
+        sides = yan.per_channel_cast_to_fp8(grad_y), yan.per_channel_cast_to_fp8(x, source)
+        yan.k_grouped_gemm_fp8_fp8_fp32_nt_contiguous(*sides, grad_w, offsets, accumulate=True)
+        assert bool((grad_w == 3.0).all())
+        yan.k_grouped_gemm_fp8_fp8_fp32_nt_contiguous(*sides, grad_w, offsets)
+        assert bool((grad_w == 0).all())
+        assert yan.moe_route_backward(logits, indices, counts, grad_weights, loss).shape == (0, experts)
+
+
+def test_tokens_that_find_no_row_at_all():
+    """A layout without rows: every pair has none."""
+    g = _gen(9)
+    x, indices = torch.randn(40, 128, generator=g, device='cuda').bfloat16(), torch.randint(0, 3, (40, 2), generator=g, device='cuda').int()
+    for tokens in (40, 40 * 64):          # few pairs and many
+        many, chosen = x.repeat(tokens // 40, 1), indices.repeat(tokens // 40, 1)
+        codes, scales = torch.zeros(0, 128, dtype=torch.uint8, device='cuda').view(F8), torch.zeros(0, 1, device='cuda')
+        rows, m_indices, source, offsets = yan.moe_dispatch_to_fp8_contiguous(many, chosen, 3, (codes, scales))
+        assert bool((rows == -1).all()) and m_indices.numel() == source.numel() == 0 and offsets.tolist() == [0] * 4
+
+
 def test_decode_step_of_a_layer():
     tokens, hidden, inner, experts, top_k, m_max, expected_m = testing.MOE_DECODE_LAYER
     x, logits, w8, ws, _ = _layer(tokens, hidden, inner, experts, top_k, 12)

@@ -289,9 +289,9 @@ inline hipError_t launch_moe_dispatch(const T* x, const int* indices, void* code
     if (tokens < 0 || k < 128 || k % 128 != 0 || top_k < 1 || top_k > kMaxTopK || experts < 1 || experts > kMaxExperts || m_max < 0 || rows < 0) return hipErrorInvalidValue;
     if (m_max ? rows != experts * m_max : rows % kExpertAlignment != 0) return hipErrorInvalidValue;
     if ((long long)tokens * top_k > kMaxPairs || (long long)experts * m_max >= 1ll << 31) return hipErrorInvalidValue;
-    if (!m_indices || (!m_max && !offsets)) return hipErrorInvalidValue;
+    if (m_max ? !m_indices : !offsets) return hipErrorInvalidValue;
     if (tokens && (!x || !indices || !rows_of)) return hipErrorInvalidValue;
-    if (rows && (!codes || !scales || (!m_max && !source))) return hipErrorInvalidValue;
+    if (rows && (!codes || !scales || (!m_max && (!source || !m_indices)))) return hipErrorInvalidValue;
     const DispatchShape s{tokens, k / 128, top_k, experts, m_max, rows, stride_g, stride_m, stride_k};
     auto* to = static_cast<uint8_t*>(codes);
     const int pairs = tokens * top_k;
