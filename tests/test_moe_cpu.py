@@ -290,6 +290,15 @@ def test_notes_of_a_call_say_which_argument_is_which_also_where_two_are_the_same
         assert got == {'x': 0, 'source': None if picked is None else 1, 'q': None, 'scales': None}
 
 
+def test_weight_gradient_kernels_are_whole():
+    """Every kernel that a library of theirs launches is in it: the library loads with all of its symbols."""
+    import os
+    from yan_amd.jit import build
+    name, keys, arg_defs, template = wgrad.wgrad_kernel_plan()
+    runtime = build(name, arg_defs, generate(wgrad.includes, arg_defs, cpp_format(template, dict(keys))))
+    ctypes.CDLL(os.path.join(runtime.path, 'kernel.so'), mode=os.RTLD_NOW)
+
+
 def test_no_copy_of_a_weight_gradient_is_out_of_range_for_every_lane(tmp_path):
     """The LDS that the copies go to is used again: each one has a row to wait for, whatever the operand's number of rows."""
     import subprocess
@@ -302,7 +311,7 @@ int check() {
     using Stager = yan::WgradStager<ROWS, 4>;
     for (int rows = 1; rows <= ROWS; ++rows)
         for (int group = 0; group < Stager::PASSES * 4; ++group) {
-            const int wave = group % 4, from = Stager::first_group(wave, rows) + 4 * Stager::source_pass(group / 4, Stager::passes_behind(wave, rows));
+            const int from = Stager::source_group(group, rows);
             if (from < 0 || from * 8 >= rows || (group * 8 < rows && from != group)) return 1;
         }
     return Stager::PASSES * 32 != ROWS;

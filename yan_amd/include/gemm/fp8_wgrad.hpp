@@ -7,7 +7,8 @@
 // The codes are multiplied as bf16, which holds code * 2^e exactly: gfx950 converts two codes and applies a power of two in one instruction, so
 // the scales cost nothing and the sums stay in the matrix core's accumulators from the first k-tile to the last. The FP8 MFMAs are twice as
 // fast and add up less exactly than fp32 sums do: small products next to large ones lose bits inside of the instruction, whatever its shape
-// and also from a zero accumulator, 1.3e-5 of the result's norm for normal operands and 6e-5 where values spread more widely (bf16: 1e-7).
+// and also from a zero accumulator, 1.5e-5 of the result's norm for normal operands and 4e-5 to 5e-5 where values spread more widely, at K = 128 as at 16384 (bf16:
+// 1e-8 to 7e-8 and 2e-7 to 9e-7).
 // A gradient that is summed up in fp32 over micro-batches is to keep what fp32 keeps.
 //
 // Tiles are staged as in the other GEMMs (tile_io.hpp): 128-byte rows, swizzled, HBM -> LDS directly, in a ring. A row's scale bytes lie
@@ -59,27 +60,26 @@ template <int ROWS, int NUM_WAVES>
 struct WgradStager {
     static_assert(ROWS % (8 * NUM_WAVES) == 0 && NUM_WAVES % 2 == 0);
     static constexpr int PASSES = ROWS / 8 / NUM_WAVES;
-    uint32_t voff;                  // of this lane's chunk in a group
-    uint32_t first_at, pass_pitch;  // where the wave's first group starts, and from one pass's group to the next one's (uniform)
-    int last_pass;                  // that has rows
+    uint32_t chunk_at;              // of this lane's chunk in a group
+    // Of its chunks in the tile. (A scalar offset a pass is a choice, a product and two sums behind every copy, and a lone wave has no room for them in the shadow
+    // of its MFMAs: 99 k-tiles of 2048 x 4096 on 256 x 128 tiles 179 us, 162 so. The bound is a plain number since with PASSES, or anything else that depends on
+    // the template's arguments, the compiler leaves out the host side of a kernel that is launched.)
+    uint32_t voff[8];
+    static_assert(PASSES <= 8);
 
-    // Of an operand with `rows` >= 1 rows in the tile: the first group that `wave` copies, and how many passes more have rows.
-    __host__ __device__ __forceinline__ static int first_group(int wave, int rows) { return wave < (rows - 1) >> 3 ? wave : (rows - 1) >> 3; }
-    __host__ __device__ __forceinline__ static int passes_behind(int wave, int rows) { return (((rows - 1) >> 3) - first_group(wave, rows)) / NUM_WAVES; }
-    __host__ __device__ __forceinline__ static int source_pass(int pass, int last_pass) { return pass < last_pass ? pass : last_pass; }
+    // Which group of an operand with `rows` >= 1 rows in the tile is copied for `group`.
+    __host__ __device__ __forceinline__ static int source_group(int group, int rows) { return group < (rows - 1) >> 3 ? group : (rows - 1) >> 3; }
 
     __device__ __forceinline__ void init(uint32_t ld_bytes, int wave, int lane) {
         const int sub = lane >> 3, slot = lane & 7;
-        voff = uint32_t(sub) * ld_bytes + (slot ^ sub ^ (wave & 1)) * kChunk;         // (slot ^ swizzle_of_row of the row that the place in LDS is for)
-        pass_pitch = uint32_t(NUM_WAVES * 8) * ld_bytes;
+        chunk_at = uint32_t(sub) * ld_bytes + (slot ^ sub ^ (wave & 1)) * kChunk;         // (slot ^ swizzle_of_row of the row that the place in LDS is for)
     }
     __device__ __forceinline__ void aim(int rows, uint32_t ld_bytes, int wave) {
-        first_at = uint32_t(first_group(wave, rows) * 8) * ld_bytes;
-        last_pass = passes_behind(wave, rows);
+#pragma unroll
+        for (int j = 0; j < PASSES; ++j) voff[j] = chunk_at + uint32_t(source_group(j * NUM_WAVES + wave, rows) * 8) * ld_bytes;
     }
     __device__ __forceinline__ void issue_pass(__amdgpu_buffer_rsrc_t rsrc, uint8_t* lds_tile, int k_byte0, int wave, int j) const {
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, YAN_LDS_PTR(lds_tile + (j * NUM_WAVES + wave) * 8 * kRowBytes), kChunk, voff,
-                                                 k_byte0 + first_at + uint32_t(source_pass(j, last_pass)) * pass_pitch, 0, 0);
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, YAN_LDS_PTR(lds_tile + (j * NUM_WAVES + wave) * 8 * kRowBytes), kChunk, voff[j], k_byte0, 0, 0);
     }
     __device__ __forceinline__ void issue(__amdgpu_buffer_rsrc_t rsrc, uint8_t* lds_tile, int k_byte0, int wave) const {
 #pragma unroll

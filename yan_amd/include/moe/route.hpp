@@ -71,8 +71,8 @@ __host__ __device__ inline bool rows_in_pieces(const void* base, int e) {
 }
 
 // exp(x) for x <= 88, within 2 units in the last place; 0 below -87 (the smallest normal numbers), NaN for NaN. The product with log2(e) is carried to twice
-// the bits, its lower part applied to the result. The library's function, with its care for every x, and the division it goes with were 200 of
-// the 450 vector instructions of a row.
+// the bits, its lower part applied to the result: eight instructions, where the library's function cares for every x. A row of 256 logits and 8 picks takes 409 vector
+// instructions forward and 266 backward with softmax, 453 and 317 with sigmoid (SQ_INSTS_VALU; 512 logits, sigmoid: 1356 and 413).
 __device__ __forceinline__ float exp_of(float x) {
     constexpr float LOG2_E = 1.44269504f, LOG2_E_LOW = 1.92596299e-8f, LN_2 = 0.693147181f;
     const float high = x * LOG2_E, low = fmaf(x, LOG2_E, -high) + x * LOG2_E_LOW;
