@@ -72,7 +72,7 @@ __host__ __device__ inline bool rows_in_pieces(const void* base, int e) {
 
 // exp(x) for x <= 88, within 2 units in the last place; 0 below -87 (the smallest normal numbers), NaN for NaN. The product with log2(e) is carried to twice
 // the bits, its lower part applied to the result: eight instructions, where the library's function cares for every x. A row of 256 logits and 8 picks takes 409 vector
-// instructions forward and 266 backward with softmax, 453 and 317 with sigmoid (SQ_INSTS_VALU; 512 logits, sigmoid: 1356 and 413).
+// instructions forward and 266 backward with softmax, 453 and 277 with sigmoid (SQ_INSTS_VALU; 512 logits, sigmoid: 1356 and 365).
 __device__ __forceinline__ float exp_of(float x) {
     constexpr float LOG2_E = 1.44269504f, LOG2_E_LOW = 1.92596299e-8f, LN_2 = 0.693147181f;
     const float high = x * LOG2_E, low = fmaf(x, LOG2_E, -high) + x * LOG2_E_LOW;
@@ -101,6 +101,15 @@ __device__ __forceinline__ ScoreBase score_base(float largest) {
     }
     return {finite_top(largest), 1.f};
 }
+// Whether every group of the wave has a lane whose `largest` is zero or more
+template <int LANES>
+__device__ __forceinline__ bool every_group_reaches_zero(float largest) {
+    const unsigned long long have = __ballot(largest >= 0.f);
+    if constexpr (LANES == 64) return have != 0;
+    const uint32_t low = uint32_t(have), high = uint32_t(have >> 32);
+    if constexpr (LANES == 32) return low && high;
+    return (low & 0xffff) && low >> 16 && (high & 0xffff) && high >> 16;
+}
 // A score in multiples of its row's base: sigmoid(l) / unit, or exp(l - top); a logit of +infinity counts as the largest finite number. Sigmoid: `rest` gets 1 - s,
 // which near s = 1 is no difference of rounded numbers.
 template <bool SIGMOID>
@@ -120,11 +129,17 @@ __device__ __forceinline__ float score_of(float l, ScoreBase base, float* rest =
 template <bool SIGMOID, int LANES, int VALUES>
 __device__ __forceinline__ float row_scores(float (&s)[VALUES], const float (&v)[VALUES], ScoreBase base, float* rest = nullptr) {
     float sum = 0.f;
+    const auto scores = [&](ScoreBase of) __attribute__((always_inline)) {
 #pragma unroll
-    for (int j = 0; j < VALUES; ++j) {
-        s[j] = score_of<SIGMOID>(v[j], base, rest ? rest + j : nullptr);
-        sum += s[j];
-    }
+        for (int j = 0; j < VALUES; ++j) {
+            s[j] = score_of<SIGMOID>(v[j], of, rest ? rest + j : nullptr);
+            sum += s[j];
+        }
+    };
+    // Where all of a wave's rows have a logit of zero or more, as nearly all have, the base is a constant (sigmoid, 16384 rows, backward: 256 logits 12.4 -> 12.2 us, 512
+    // 19.4 -> 18.9, 4096 of 1024 18.2 -> 17.3; forward no difference).
+    if (SIGMOID && rest && !__any(base.top < 0.f)) scores({0.f, 1.f});
+    else scores(base);
     sum = sum_lanes<LANES>(sum);
     if constexpr (!SIGMOID) {
         const float inverse = inverse_of(sum);
@@ -412,7 +427,9 @@ moe_route_backward_kernel(const T* __restrict__ logits, const int* __restrict__ 
         float top = v[0];
 #pragma unroll
         for (int j = 1; j < VALUES; ++j) top = fmaxf(top, v[j]);
-        const ScoreBase base = score_base<SIGMOID>(max_lanes<LANES>(top));
+        // the largest of all lanes is asked for only where it is a base (256 logits 12.2 -> 11.6 us, 512 18.9 -> 18.0)
+        ScoreBase base{0.f, 1.f};
+        if (!SIGMOID || !every_group_reaches_zero<LANES>(top)) base = score_base<SIGMOID>(max_lanes<LANES>(top));
         float rest[VALUES];
         const float sum = row_scores<SIGMOID, LANES>(s, v, base, rest), inverse = inverse_of(sum);
         // sigmoid: s h, in which the base cancels out where weights are renormalised; softmax: h
@@ -483,7 +500,7 @@ inline hipError_t launch_moe_route_backward(const T* logits, const int* indices,
     if (tokens == 0) return hipSuccess;
     if (!logits || !indices || !counts || !grad_logits) return hipErrorInvalidValue;
     // as many workgroups as are resident, so that each reads the counts once (fp32, 16384 tokens, 1024 / 2048 / 4096 workgroups: 256 experts 12.1, 11.8, 12.4 us,
-    // 512 experts 18.6, 20.8, 25.9; with exact slopes sigmoid takes 12.4 and 19.4, softmax 11.3 and 17.2)
+    // 512 experts 18.6, 20.8, 25.9; since then 256 take 11.3 with softmax, 11.6 with sigmoid, 512 17.2 and 18.0)
     constexpr int MOST = VALUES > 4 ? 1024 : 2048;
     const int blocks = std::min(ceil_div(tokens, 256 / LANES), MOST);
     hipLaunchKernelGGL((moe_route_backward_kernel<T, SIGMOID, LANES, VALUES>), dim3(blocks), dim3(256), 0, stream, logits, indices,
