@@ -576,6 +576,22 @@ def test_weight_gradients_of_one_k_tile_with_few_rows_in_the_last_tile(kernel, m
         _check_product(grouped[q], _decode(a)[:, 128 * q:128 * q + 128].contiguous(), _decode(b)[:, 128 * q:128 * q + 128].contiguous(), held[q].double())
 
 
+@pytest.mark.parametrize('low,high', [(10, 246), (246, 10), (10, 10), (19, 235)])
+def test_weight_gradients_with_scales_at_the_ends_of_their_range(low, high):
+    """Every code times a scale of 2^-117 to 2^119 is a normal bf16 number, so products of both ends are those of the definition."""
+    g = _gen(low)
+    for kernel in KERNELS[:4]:
+        a, b = _operand(g, 72, 512), _operand(g, 68, 512)
+        a[1].fill_(low)
+        b[1].fill_(high)
+        out = torch.zeros(72, 68, device='cuda')
+        wgrad._wgrad(a, b, out, None, False, kernel)
+        want = _decode(a) @ _decode(b).t().contiguous()
+        size = _decode(a).abs() @ _decode(b).abs().t().contiguous()
+        # (of two small scales the products are less than the smallest normal number of fp32)
+        _close(out, want, (512 / 32 + 48) * 2 * U * size + 2.0 ** -126, 'product')
+
+
 def test_weight_gradient_edges():
     """K of zero, NaN codes, offsets that do not ascend or leave K (whatever they say, nothing outside is read), a cap on compute units."""
     g = _gen(1)

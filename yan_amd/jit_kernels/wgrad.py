@@ -88,7 +88,8 @@ def gemm_fp8_fp8_fp32_nt(lhs: Tuple[torch.Tensor, torch.Tensor], rhs: Tuple[torc
     `out = lhs @ rhs.T`, or `out += lhs @ rhs.T`, of the decoded operands.
 
     lhs: (e4m3fn `[m, k]`, uint8 `[m, k/128]`), rhs: (e4m3fn `[n, k]`, uint8 `[n, k/128]`): codes contiguous; scales are exponents + 127 (E8M0), their
-         rows contiguous and a multiple of 4 bytes apart, as `per_channel_cast_to_fp8` returns both
+         rows contiguous and a multiple of 4 bytes apart, as `per_channel_cast_to_fp8` returns both. Bytes of 10 to 246 are exact for every code: a code
+         times its scale is multiplied as bf16, and beyond them it may leave bf16's normal numbers (the cast's stay inside for values up to 3.2e38).
     out: fp32 `[m, n]` contiguous, written in place
     Requires k % 128 == 0 and n % 4 == 0; m is arbitrary.
     """
