@@ -730,6 +730,10 @@ def jit_kernels_in_use(num_cus: int = 256):
         for backward in (False, True):
             name, keys, arg_defs, code_template = moe.combine_kernel_plan(top_k, backward)
             add(name, arg_defs, moe._combine_includes, code_template, keys)
+    for name, keys, arg_defs, includes, code_template in norm_plans():
+        add(name, arg_defs, includes, code_template, keys)
+    name, keys, arg_defs, code_template = moe.layout_kernel_plan()
+    add(name, arg_defs, moe._layout_includes, code_template, keys)
     for kernel, parts in WGRAD_KERNELS:
         name, keys, arg_defs, code_template = wgrad.wgrad_kernel_plan(kernel, parts)
         add(name, arg_defs, wgrad.includes, code_template, keys)
@@ -767,3 +771,27 @@ def prebuild_jit_kernels(num_cus: int = 256, verbose: bool = False, jobs: int = 
     with ThreadPoolExecutor(max_workers=jobs) as pool:
         list(pool.map(one, kernels))
     return len(kernels)
+
+
+# rows, k of the norm and its gradient, and what a call has: x's type, the residual's (None: none), the weight's, codes, 16 bits
+NORM_SHAPES = [(1, 8), (1, 128), (5, 128), (17, 72), (33, 264), (100, 512), (64, 7168), (1023, 2112), (2, 16384), (3, 8200), (1025, 128), (1030, 2048), (1100, 4096), (1027, 16384)]
+NORM_CALLS = [('bf16', 'bf16', 'bf16', True, False), ('bf16', None, 'bf16', True, True), ('fp32', 'bf16', 'fp32', False, True), ('bf16', 'fp32', 'fp32', True, True),
+              ('fp32', None, 'bf16', False, True), ('fp32', 'fp32', 'bf16', True, False)]
+# gradient's type, h's, the weight's, with a residual's gradient, with the weight's
+NORM_BACKWARD_CALLS = [('bf16', 'bf16', 'bf16', True, True), ('fp32', 'bf16', 'fp32', False, True), ('bf16', 'fp32', 'bf16', False, False), ('fp32', 'fp32', 'fp32', True, True)]
+NORM_TYPES = {'bf16': torch.bfloat16, 'fp32': torch.float32}
+
+
+def norm_plans():
+    """(name, keys, arg_defs, includes, template) of the kernels that those run."""
+    from yan_amd.jit_kernels import norm
+    plans = []
+    for rows, k in NORM_SHAPES:
+        for x, h, w, codes, normed in NORM_CALLS:
+            if not codes or k % 128 == 0:
+                name, keys, arg_defs, code = norm.norm_kernel_plan(NORM_TYPES[x], NORM_TYPES[h or x], NORM_TYPES[w], *norm.norm_lanes(rows, k), h is not None, codes, normed)
+                plans.append((name, keys, arg_defs, norm.includes, code))
+        for g, h, w, residual, weight in NORM_BACKWARD_CALLS:
+            name, keys, arg_defs, code = norm.norm_backward_kernel_plan(NORM_TYPES[g], NORM_TYPES[h], NORM_TYPES[w], *norm.norm_backward_lanes(k), residual, weight)
+            plans.append((name, keys, arg_defs, norm.includes, code))
+    return plans

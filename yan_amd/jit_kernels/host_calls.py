@@ -30,6 +30,7 @@ if getattr(_host_calls, 'built_for', None) != f'torch {torch.__version__} {torch
 # which entry a remembered call belongs to
 FP8, CAST_FP8, BF16, FP16, FLOAT, CONTIGUOUS, MASKED, PER_TOKEN, PER_BLOCK = range(1, 10)
 ROUTE, ROUTE_BACKWARD, DISPATCH, COMBINE, COMBINE_BACKWARD, PER_CHANNEL, WGRAD = range(10, 17)
+NORM, NORM_BACKWARD, LAYOUT, RAGGED_NT, RAGGED_NN, RAGGED_TN = range(17, 23)
 _TENSOR, _CONSTANT, _STREAM, _WORKSPACE, _OUTPUT = range(5)
 _THE_STREAM, _THE_WORKSPACE = (_STREAM, 0), (_WORKSPACE, 0)
 
@@ -107,6 +108,8 @@ def remember_new(call: tuple, name: str, runtime: Runtime, args: tuple, outputs:
             spec.append((_CONSTANT, arg))
         elif kind is _STREAM:
             spec.append(_THE_STREAM)
+        elif kind is None:          # the call's own, which go where floats go
+            continue
         elif workspace is not None and arg is workspace:
             spec.append(_THE_WORKSPACE)
         elif tensors < len(given) and views.get(id(arg), arg) is given[tensors]:

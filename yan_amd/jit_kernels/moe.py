@@ -18,7 +18,7 @@ from typing import Optional, Tuple
 
 import torch
 
-from .host_calls import COMBINE, COMBINE_BACKWARD, DISPATCH, ROUTE, ROUTE_BACKWARD, remember_new, repeat_call, repeat_new
+from .host_calls import COMBINE, COMBINE_BACKWARD, DISPATCH, LAYOUT, ROUTE, ROUTE_BACKWARD, remember_new, repeat_call, repeat_new
 from .split_k import split_k_launch_failed, split_k_workspace
 from .tuner import FrozenKeys, jit_tuner
 from .utils import assert_on_current_device, ceil_div, current_raw_stream, get_m_alignment_for_contiguous_layout
@@ -30,6 +30,9 @@ MAX_EXPERTS = 1024
 FEW_PAIRS = 4096
 TOKENS_PER_BLOCK = 16
 MAX_PAIRS = (1 << 31) - (1 << 18)
+# kLayoutChunk and kLayoutFewChunks of moe/layout.hpp
+LAYOUT_CHUNK = 1024
+LAYOUT_FEW_CHUNKS = 8
 
 _ELEMENTS = {torch.bfloat16: '__bf16', torch.float32: 'float'}
 _SCORINGS = {'softmax': 0, 'sigmoid': 1}
@@ -313,6 +316,56 @@ def moe_dispatch_to_fp8_masked(x: torch.Tensor, indices: torch.Tensor, out: Tupl
     rows = torch.empty_like(indices)
     masked_m = torch.empty((num_experts, ), dtype=torch.int32, device=x.device)
     return _dispatch(call, x, indices, codes, scales, num_experts, m_max, (rows, masked_m))
+
+
+# The same rows without padding and without copies of the tokens, for the 16-bit products
+
+_layout_includes = ('"moe/layout.hpp"', )
+
+layout_template = """
+using namespace yan;
+__return_code = static_cast<int>(launch_moe_layout(indices, rows, source, offsets, workspace, workspace_bytes, pairs, top_k, experts, stream));
+"""
+layout_arg_defs = (('indices', torch.int), ('rows', torch.int), ('source', torch.int), ('offsets', torch.int), ('workspace', torch.uint8), ('workspace_bytes', int),
+                   ('pairs', int), ('top_k', int), ('experts', int), ('stream', torch.cuda.Stream))
+
+
+@functools.lru_cache(maxsize=None)
+def layout_kernel_plan():
+    """(name, keys, arg_defs, template) of the ragged layout's kernels; needs no GPU."""
+    return 'moe_ragged_layout', FrozenKeys({}), layout_arg_defs, layout_template
+
+
+def moe_ragged_layout(indices: torch.Tensor, num_experts: int) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """
+    The rows of every expert right behind those of the one before it: the layout of `m_grouped_gemm_bf16_bf16_bf16_nt_ragged`, which gathers its rows itself.
+
+    indices: int32 `[tokens, top_k]`, the experts of every token; others than 0 .. num_experts - 1 (-1 of a masked token) have no row
+    Returns rows int32 `[tokens, top_k]` (the row of every pair, -1: none), source int32 `[tokens * top_k]` (the token of every row, -1 behind the last one) and
+    offsets int32 `[num_experts + 1]` (where every expert's rows start, and where the last one's end). An expert's rows are in the order of (token, pick).
+    """
+    call = (LAYOUT, indices, num_experts)
+    made = repeat_new(*call)
+    if made is not None:
+        return made
+    assert indices.dim() == 2 and indices.dtype == torch.int32 and indices.is_contiguous()
+    assert 1 <= indices.size(1) <= MAX_TOP_K and 1 <= num_experts <= MAX_EXPERTS and indices.numel() <= MAX_PAIRS
+    assert_on_current_device(indices)
+    device, pairs = indices.device, indices.numel()
+    rows = torch.empty_like(indices)
+    source = torch.empty((pairs, ), dtype=torch.int32, device=device)
+    offsets = torch.empty((num_experts + 1, ), dtype=torch.int32, device=device)
+    # moe_layout_workspace_bytes of moe/layout.hpp
+    chunks = ceil_div(pairs, LAYOUT_CHUNK)
+    workspace_bytes = 0 if chunks <= LAYOUT_FEW_CHUNKS else (chunks + 1) * num_experts * 4
+    assert workspace_bytes < 1 << 31
+    scratch = torch.empty(workspace_bytes, dtype=torch.uint8, device=device) if workspace_bytes else None
+    made = (rows, source, offsets)
+    done = _run(layout_kernel_plan(), _layout_includes,
+                (indices, rows, source, offsets, offsets.view(torch.uint8) if scratch is None else scratch, workspace_bytes, pairs, indices.size(1), num_experts,
+                 current_raw_stream()))
+    remember_new(call, *done, made, () if scratch is None else (scratch, ))
+    return made
 
 
 # And back
