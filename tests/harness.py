@@ -730,7 +730,7 @@ def jit_kernels_in_use(num_cus: int = 256):
         for backward in (False, True):
             name, keys, arg_defs, code_template = moe.combine_kernel_plan(top_k, backward)
             add(name, arg_defs, moe._combine_includes, code_template, keys)
-    for name, keys, arg_defs, includes, code_template in norm_plans():
+    for name, keys, arg_defs, includes, code_template in norm_plans() + grouped16_plans():
         add(name, arg_defs, includes, code_template, keys)
     name, keys, arg_defs, code_template = moe.layout_kernel_plan()
     add(name, arg_defs, moe._layout_includes, code_template, keys)
@@ -794,4 +794,20 @@ def norm_plans():
         for g, h, w, residual, weight in NORM_BACKWARD_CALLS:
             name, keys, arg_defs, code = norm.norm_backward_kernel_plan(NORM_TYPES[g], NORM_TYPES[h], NORM_TYPES[w], *norm.norm_backward_lanes(k), residual, weight)
             plans.append((name, keys, arg_defs, norm.includes, code))
+    return plans
+
+
+# the ragged products' kernels, the rule's choice first
+GROUPED16_KERNELS = ['kGroupedAny', 'kGrouped128', 'kGrouped64', 'kGrouped32']
+
+
+def grouped16_plans():
+    """(name, keys, arg_defs, includes, template) of the ragged products' kernels: each by name in one type, the rule's choice in both."""
+    from yan_amd.jit_kernels import ragged
+    plans = []
+    for mode, gather in (('NT', False), ('NT', True), ('NN', False), ('TN', False), ('TN', True)):
+        for kernel in GROUPED16_KERNELS:
+            for dtype in (torch.bfloat16, torch.half) if kernel == 'kGroupedAny' else (torch.bfloat16, ):
+                name, keys, arg_defs, code = ragged.grouped16_kernel_plan(dtype, mode, gather, kernel)
+                plans.append((name, keys, arg_defs, ragged.includes, code))
     return plans

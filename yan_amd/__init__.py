@@ -8,6 +8,8 @@ from .jit_kernels import (gemm, gemm_float_nt, gemm_bf16_tn, gemm_fp16_tn, gemm_
                           gemm_fp8_fp8_fp32_nt, k_grouped_gemm_fp8_fp8_fp32_nt_contiguous,
                           moe_route, moe_route_backward, moe_dispatch_to_fp8_contiguous, moe_dispatch_to_fp8_masked, moe_combine, moe_combine_backward,
                           get_contiguous_layout_rows, moe_ragged_layout,
+                          m_grouped_gemm_bf16_bf16_bf16_nt_ragged, m_grouped_gemm_fp16_fp16_fp16_nt_ragged, m_grouped_gemm_bf16_bf16_bf16_nn_ragged,
+                          m_grouped_gemm_fp16_fp16_fp16_nn_ragged, k_grouped_gemm_bf16_bf16_fp32_tn_ragged, k_grouped_gemm_fp16_fp16_fp32_tn_ragged,
                           rms_norm, rms_norm_to_fp8, rms_norm_backward,
                           set_num_sms, get_num_sms, ceil_div, get_m_alignment_for_contiguous_layout)
 from .utils import bench_kineto, calc_diff, count_bytes
