@@ -798,7 +798,7 @@ def norm_plans():
 
 
 # the ragged products' kernels, the rule's choice first
-GROUPED16_KERNELS = ['kGroupedAny', 'kGrouped128', 'kGrouped64', 'kGrouped32']
+GROUPED16_KERNELS = ['kGroupedAny', 'kGroupedTall', 'kGrouped128', 'kGrouped64', 'kGrouped32']
 
 
 def grouped16_plans():

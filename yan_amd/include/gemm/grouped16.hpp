@@ -21,6 +21,7 @@
 
 #include <algorithm>
 #include <type_traits>
+#include <utility>
 
 #include "utils.hpp"
 #include "mfma_utils.hpp"
@@ -176,15 +177,36 @@ struct TurnedCopies {
     }
 };
 
-// Eight consecutive k of one column out of a turned k-tile.
+// Eight consecutive k of one column out of a turned k-tile. (Of a read of LDS of which nothing is known the compiler thinks that it may be of what any copy under way brings, and
+// waits for all of them in front of it; a restricted pointer is something known. What has landed when is the kernels' own business.)
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 template <typename Frag, int DIM>
-__device__ __forceinline__ Frag read_turned(const uint8_t* at) {
+__device__ __forceinline__ Frag read_turned(const uint8_t* __restrict__ at) {
     typedef __attribute__((address_space(3))) s16x4* LdsPtr;
-    const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<LdsPtr>(YAN_LDS_PTR(at)));
-    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<LdsPtr>(YAN_LDS_PTR(at + 4 * Turned<DIM>::ROW_BYTES)));
+    const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsPtr)(at));
+    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsPtr)(at + 4 * Turned<DIM>::ROW_BYTES));
     typedef short s16x8 __attribute__((ext_vector_type(8)));
     return __builtin_bit_cast(Frag, s16x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]});
+}
+
+// One of the two reads of that.
+template <typename Frag>
+__device__ __forceinline__ void read_turned_part(Frag& f, const uint8_t* __restrict__ at, int part) {
+    typedef __attribute__((address_space(3))) s16x4* LdsPtr;
+    typedef short s16x8 __attribute__((ext_vector_type(8)));
+    const s16x4 v = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsPtr)(at));
+    s16x8 all = __builtin_bit_cast(s16x8, f);
+    if (part == 0) all[0] = v[0], all[1] = v[1], all[2] = v[2], all[3] = v[3];
+    else all[4] = v[0], all[5] = v[1], all[6] = v[2], all[7] = v[3];
+    f = __builtin_bit_cast(Frag, all);
+}
+
+typedef int i32x16_unaligned __attribute__((ext_vector_type(16), aligned(4)));
+
+// f(0), f(1), ... f(N - 1), each with its number as a constant.
+template <int N, typename F>
+__device__ __forceinline__ void static_for(F&& f) {
+    [&]<int... I>(std::integer_sequence<int, I...>) __attribute__((always_inline)) { (f(std::integral_constant<int, I>{}), ...); }(std::make_integer_sequence<int, N>{});
 }
 
 // Tiles of 128 x 128 and less: 4 waves, a ring of STAGES k-tiles, one tile a workgroup, or a walk under a cap. Two workgroups or more a compute unit hide each other's waits.
@@ -425,7 +447,507 @@ grouped16_kernel(GroupedProblem p, int slots) {
     }
 }
 
-enum Grouped16Kernel { kGroupedAny, kGrouped128, kGrouped64, kGrouped32 };
+// The groups' rows cut into runs of BLOCK_M, as count_row_tiles and find_row_tile have them, with the first 64 groups in registers: a walk that looks a tile up among its
+// copies does not wait for memory.
+template <int BLOCK_M>
+struct RowRuns {
+    int lo, hi, upto;               // of group `lane`: its rows, and the runs up to its last
+    __device__ __forceinline__ void init(const GroupedProblem& p, int lane) {
+        lo = hi = 0;
+        if (lane < p.groups) grouped_range(p, lane, lo, hi);
+        upto = ceil_div(hi - lo, BLOCK_M);
+#pragma unroll
+        for (int d = 1; d < kWaveSize; d *= 2) {
+            const int below = __shfl_up(upto, d, kWaveSize);
+            if (lane >= d) upto += below;
+        }
+    }
+    __device__ __forceinline__ RowTile find(const GroupedProblem& p, int tile, int lane) const {
+        const unsigned long long behind = __ballot(upto > tile);
+        if (!behind) return find_row_tile<BLOCK_M>(p, tile, lane);
+        const int at = __builtin_ctzll(behind);
+        const int start = __builtin_amdgcn_readlane(lo, at), end = __builtin_amdgcn_readlane(hi, at), last = __builtin_amdgcn_readlane(upto, at);
+        const int row0 = start + (tile - (last - ceil_div(end - start, BLOCK_M))) * BLOCK_M;
+        return {at, row0, min(BLOCK_M, end - row0)};
+    }
+};
+
+// Tiles of 256 x 256 on 4 waves, one a SIMD, each with 128 x 128 outputs in 16x16x32 MFMAs, its sums in the accumulation registers: the design of dense_gemm_body_4w
+// (bf16_gemm.hpp). LDS is a ring of five units of 32 KB, a unit being one operand's k-tile; the fragments of half a k-tile are read while the half before it is
+// multiplied; copies run two k-tiles ahead of the MFMAs, along K and on into the next tile of a persistent walk, whose first k-tiles are under way when this one's sums leave.
+// What is different:
+//   * row atoms alternate between the two waves that share a tile's rows, so that a tile at a group's end has them split evenly; one with up to 128 rows (FLAT) runs half of
+//     the MFMAs and copies half of the rows. Groups end in the middle of a tile, on average; with 512 rows a group whole tiles would be a quarter more work.
+//   * lane offsets of the copies are worked out anew for every tile, and for a k-tile that is not whole: rows that stand in for those that do not exist, gathered rows;
+//   * descriptors of turned operands move on with the k-tile, so that ranges may be of any length;
+//   * any number of k-tiles, one for instance: the copies' place in the walk is its own.
+struct GroupedTile {
+    int slot, group, m0, rows, n0, cols, k0, depth;         // depth 0: none
+    __device__ __forceinline__ int count() const { return ceil_div(depth, kDepth); }
+    // In the lanes of one register, for tiles that wait for their turn.
+    __device__ __forceinline__ int packed(int lane) const {
+        return lane & 4 ? (lane & 2 ? (lane & 1 ? depth : k0) : (lane & 1 ? cols : n0)) : (lane & 2 ? (lane & 1 ? rows : m0) : (lane & 1 ? group : slot));
+    }
+    __device__ __forceinline__ static GroupedTile unpacked(int v) {
+        const auto lane = [&](int i) { return __builtin_amdgcn_readlane(v, i); };
+        return {lane(0), lane(1), lane(2), lane(3), lane(4), lane(5), lane(6), lane(7)};
+    }
+};
+
+template <typename Elem, Grouped MODE, bool GATHER>
+__global__ void __launch_bounds__(256, 1)
+grouped16_tall_kernel(GroupedProblem p) {
+    constexpr bool TURN_A = MODE == Grouped::TN, TURN_B = MODE != Grouped::NT, SOURCES = GATHER && MODE == Grouped::TN, GATHER_A = GATHER && MODE == Grouped::NT;
+    constexpr int BLOCK = 256, TN = 8, TM = 8, UNITS = 5, UNIT_BYTES = BLOCK * kRowBytes, PASSES = 8;
+    static_assert(!(GATHER && MODE == Grouped::NN));
+    using Frag = typename Mfma16<Elem>::Frag;
+    constexpr int ROW_BYTES = Turned<BLOCK>::ROW_BYTES;
+    __shared__ __attribute__((aligned(1024))) uint8_t ring[UNITS * UNIT_BYTES];
+
+    const int lane = get_lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWaveSize);
+    const int wn = wave % 2, wm = wave / 2, g = lane / 16, col = lane % 16;
+    RowRuns<BLOCK> runs;
+    int with_rows = 0, row_tiles, tiles_m = 1;
+    if constexpr (MODE == Grouped::TN) {
+        tiles_m = ceil_div(p.m, BLOCK);
+        row_tiles = tiles_m * p.groups;
+    } else {
+        runs.init(p, lane);
+        row_tiles = count_row_tiles<BLOCK>(p, lane, &with_rows);
+    }
+    const int band = MODE == Grouped::TN ? tiles_m : with_rows ? row_tiles / with_rows : 1;
+    auto tile_at = [&](int slot) __attribute__((always_inline)) {
+        // (worked out anew for every tile: a dozen scalar registers less over the k-loop, which has none to spare)
+        int rows_anew = row_tiles;
+        asm volatile("" : "+s"(rows_anew));
+        XcdTileScheduler<> sched(rows_anew * BLOCK, p.n, BLOCK, BLOCK);
+        sched.fit_bands_to_groups(band);
+        // groups of TN differ in their depth: patches of 32 tiles are dealt out to the XCDs
+        const TileCoord c = MODE == Grouped::TN ? sched.dealt_band_tile_of(slot) : sched.tile_of(slot);
+        GroupedTile t{slot, -1, 0, 0, 0, 0, 0, 0};
+        if (!c.valid) return t;
+        t.n0 = c.n_idx * BLOCK, t.cols = min(BLOCK, p.n - t.n0);
+        if constexpr (MODE == Grouped::TN) {
+            t.group = c.m_idx / tiles_m, t.m0 = (c.m_idx - t.group * tiles_m) * BLOCK, t.rows = min(BLOCK, p.m - t.m0);
+            int hi;
+            grouped_range(p, t.group, t.k0, hi);
+            t.depth = hi - t.k0;
+        } else {
+            const RowTile r = runs.find(p, c.m_idx, lane);
+            t.group = r.group, t.m0 = r.row0, t.rows = r.rows, t.depth = p.k;
+        }
+        return t;
+    };
+    const int slots = XcdTileScheduler<>(row_tiles * BLOCK, p.n, BLOCK, BLOCK).grid_size();
+    // the next tile of this workgroup's walk, from `slot` on
+    auto seek = [&](int slot) __attribute__((always_inline)) {
+        for (; slot < slots; slot += gridDim.x) {
+            const GroupedTile t = tile_at(slot);
+            if (t.depth > 0) return t;
+        }
+        return GroupedTile{slots, -1, 0, 0, 0, 0, 0, 0};
+    };
+    // the tiles of groups without rows
+    if (MODE == Grouped::TN && !p.accumulate)
+        for (int slot = blockIdx.x; slot < slots; slot += gridDim.x) {
+            const GroupedTile t = tile_at(slot);
+            if (t.group < 0 || t.depth > 0) continue;
+            for (int r = wave; r < t.rows; r += 4) {
+                float* const line = static_cast<float*>(p.out) + (size_t(t.group) * p.m + t.m0 + r) * p.n + t.n0;
+                for (int c = 4 * lane; c < t.cols; c += 4 * kWaveSize) *reinterpret_cast<f32x4*>(line + c) = f32x4{0.f, 0.f, 0.f, 0.f};
+            }
+        }
+    GroupedTile cur = seek(blockIdx.x);
+    if (cur.depth == 0) return;
+
+    // Four consecutive passes of a wave's copies share one LDS base (M0) and differ in the instruction's immediate offset, which the hardware adds on the LDS side and on
+    // the global side alike: the lane offsets take it back out, and the descriptors start kCopyBias bytes early so that no lane offset goes below zero.
+    constexpr uint32_t kCopyBias = 3 * 1024;
+    const uint32_t ld_a = uint32_t(MODE == Grouped::TN ? p.m : p.k) * 2, ld_b = uint32_t(MODE == Grouped::NT ? p.k : p.n) * 2;
+    auto describe = [&](const uint8_t* base, long long bytes) __attribute__((always_inline)) { return make_rsrc(base - kCopyBias, reach(bytes + kCopyBias)); };
+    // A plain operand's pass r of wave w has rows 128 (r / 4) + 32 w + 8 (r % 4) .. + 7, a turned one's k 16 w + 2 r and the one behind. `l`: the lane, out of which all of
+    // this is worked out anew where it is needed, since the registers are.
+    auto plain_row = [&](int l, int r) __attribute__((always_inline)) { return 128 * (r / 4) + 32 * wave + 8 * (r % 4) + (l >> 3); };
+    auto plain_chunk = [&](int l, int r) __attribute__((always_inline)) { return (l & 7) ^ (l >> 3) ^ (r & 1); };
+    auto turned_row = [&](int l, int r) __attribute__((always_inline)) { return 16 * wave + 2 * r + l / 32; };
+    auto turned_chunk = [&](int l, int r, int columns) __attribute__((always_inline)) { return min((l & 31) ^ (Turned<BLOCK>::spread(turned_row(l, r)) << 1), columns / 8 - 1); };
+    auto unit_base = [&](int r, bool turned) __attribute__((always_inline)) { return turned ? wave * 8192 + (r / 4) * 4096 : (r / 4) * 16384 + wave * 4096; };
+    auto lane_anew = [&] __attribute__((always_inline)) {
+        int l = lane;
+        asm volatile("" : "+v"(l));
+        return l;
+    };
+    auto product = [](uint32_t row, uint32_t ld, uint32_t more) __attribute__((always_inline)) {
+        uint32_t v = row * ld + more;
+        asm volatile("" : "+v"(v));         // (else it keeps the upper half of a 64-bit product's register pair)
+        return v;
+    };
+
+    // Where the copies are: k-tile copy_kt of `ahead`, their operands' descriptors and lane offsets.
+    GroupedTile ahead = cur;
+    int copy_kt = 0;
+    __amdgpu_buffer_rsrc_t rsrc_a, rsrc_b;
+    uint32_t voff_a[8], voff_b[8];
+    const uint8_t *from_a, *from_b;         // of turned operands: where the k-tile starts
+    uint32_t bad = 0;                       // a bit a pass: the gathered row that this lane copies is none
+    i32x16_unaligned sources;               // SOURCES: of this wave's rows of the k-tile
+    auto here_of = [&](const GroupedTile& t, int kt) __attribute__((always_inline)) { return min(kDepth, t.depth - kt * kDepth); };
+    // the lane offsets for k-tiles of which `here` of k exist
+    auto aim_lanes = [&](int here) __attribute__((always_inline)) {
+        const GroupedTile& t = ahead;
+        const int l = lane_anew();
+        if constexpr (GATHER_A) bad = 0;
+#pragma unroll
+        for (int r = 0; r < PASSES; ++r) {
+            const uint32_t bias = kCopyBias - (r % 4) * 1024;
+            const uint32_t in_row = uint32_t(plain_chunk(l, r) < here / 8 ? plain_chunk(l, r) : 0) * kChunk + bias;
+            if constexpr (TURN_A) {
+                voff_a[r] = product(min(turned_row(l, r), here - 1), ld_a, turned_chunk(l, r, t.rows) * kChunk + bias);
+            } else {
+                int row = min(plain_row(l, r), t.rows - 1);
+                if constexpr (GATHER_A) {
+                    const int s = p.source[t.m0 + row];
+                    const bool there = uint32_t(s) < uint32_t(p.source_rows);
+                    row = there ? s : 0;
+                    bad |= there ? 0u : 1u << r;
+                }
+                voff_a[r] = product(row, ld_a, in_row);
+            }
+            if constexpr (SOURCES) voff_b[r] = turned_chunk(l, r, t.cols) * kChunk + bias;         // its row is added when it is known
+            else if constexpr (TURN_B) voff_b[r] = product(min(turned_row(l, r), here - 1), ld_b, turned_chunk(l, r, t.cols) * kChunk + bias);
+            else voff_b[r] = product(min(plain_row(l, r), t.cols - 1), ld_b, in_row);
+        }
+    };
+    auto describe_turned = [&] __attribute__((always_inline)) {
+        const GroupedTile& t = ahead;
+        const int row = t.k0 + copy_kt * kDepth;
+        if constexpr (TURN_A) rsrc_a = describe(from_a, (long long)(p.rows - row) * ld_a - t.m0 * 2);
+        if constexpr (TURN_B && !SOURCES) rsrc_b = describe(from_b, (long long)((MODE == Grouped::TN ? p.rows : p.k) - row) * ld_b - t.n0 * 2);
+    };
+    auto aim_copies = [&] __attribute__((always_inline)) {
+        const GroupedTile& t = ahead;
+        if constexpr (TURN_A) from_a = p.lhs + size_t(t.k0) * ld_a + t.m0 * 2;
+        else if constexpr (GATHER_A) rsrc_a = describe(p.lhs, (long long)p.source_rows * ld_a);
+        else rsrc_a = describe(p.lhs + size_t(t.m0) * ld_a, (long long)t.rows * ld_a);
+        const uint8_t* const rhs = MODE == Grouped::TN ? p.rhs : p.rhs + size_t(t.group) * p.n * p.k * 2;
+        if constexpr (SOURCES) rsrc_b = describe(p.rhs + t.n0 * 2, (long long)p.source_rows * ld_b - t.n0 * 2);
+        else if constexpr (TURN_B) from_b = rhs + size_t(t.k0) * ld_b + t.n0 * 2;
+        else rsrc_b = describe(rhs + size_t(t.n0) * ld_b, (long long)t.cols * ld_b);
+        describe_turned();
+        aim_lanes(here_of(t, 0));
+    };
+    // Behind the walk's last k-tile that one is copied again, two times, into units that nobody reads any more: the count of copies under way stays what the waits below take it for.
+    bool walking = true;
+    // the tiles behind the current one, as far as the copies have come: up to three, of one k-tile each; and how many k of the next one's first k-tile exist
+    int next1 = 0, next2 = 0, next3 = 0, lead = 0, next_here = kDepth;
+    // Most k-tiles are followed by a whole one of the same tile: what that takes is a few scalar instructions, which ride under the last MFMAs of a k-tile.
+    auto within = [&] __attribute__((always_inline)) { return (copy_kt + 2) * kDepth <= ahead.depth; };
+    auto advance_within = [&] __attribute__((always_inline)) {
+        ++copy_kt;
+        if constexpr (TURN_A) from_a += size_t(kDepth) * ld_a;
+        if constexpr (TURN_B && !SOURCES) from_b += size_t(kDepth) * ld_b;
+        describe_turned();
+    };
+    auto advance_beyond = [&] __attribute__((always_inline)) {
+        if (!walking) return;
+        if (copy_kt + 1 < ahead.count()) {          // a last k-tile that is not whole
+            advance_within();
+            aim_lanes(here_of(ahead, copy_kt));
+            return;
+        }
+        const GroupedTile next = seek(ahead.slot + gridDim.x);
+        walking = next.depth != 0;
+        if (!walking) return;
+        ahead = next, copy_kt = 0;
+        const int waiting = next.packed(lane);
+        next1 = lead == 0 ? waiting : next1, next2 = lead == 1 ? waiting : next2, next3 = lead == 2 ? waiting : next3;
+        next_here = lead == 0 ? here_of(next, 0) : next_here;
+        ++lead;
+        aim_copies();
+    };
+    // the sources of this wave's 16 rows of the copies' k-tile
+    auto load_sources = [&] __attribute__((always_inline)) {
+        if constexpr (SOURCES) {
+            typedef const __attribute__((address_space(4))) int* Scalars;
+            const Scalars from = (Scalars)(uintptr_t)(p.source + ahead.k0);
+            const int first = copy_kt * kDepth + 16 * wave;
+            if (first + 16 <= ahead.depth) {
+                sources = *(const __attribute__((address_space(4))) i32x16_unaligned*)(from + first);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) sources[i] = from[min(first + i, ahead.depth - 1)];
+            }
+            bad = 0;
+        }
+    };
+    auto copy = [&](__amdgpu_buffer_rsrc_t rsrc, uint32_t voff, uint32_t at, int r, int base) __attribute__((always_inline)) {
+        auto* to = YAN_LDS_PTR(ring + base);
+        switch (r & 3) {        // the immediate offset is part of the instruction
+            case 0: __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, to, kChunk, voff, at, 0 * 1024, 0); break;
+            case 1: __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, to, kChunk, voff, at, 1 * 1024, 0); break;
+            case 2: __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, to, kChunk, voff, at, 2 * 1024, 0); break;
+            default: __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, to, kChunk, voff, at, 3 * 1024, 0); break;
+        }
+    };
+    auto copy_a = [&](int r, int unit) __attribute__((always_inline)) {
+        copy(rsrc_a, voff_a[r], TURN_A ? 0u : uint32_t(copy_kt) * kRowBytes, r, unit + unit_base(r, TURN_A));
+    };
+    auto copy_b = [&](int r, int unit) __attribute__((always_inline)) {
+        uint32_t voff = voff_b[r];
+        if constexpr (SOURCES) {
+            const int s0 = sources[2 * r], s1 = sources[2 * r + 1];
+            const bool there0 = uint32_t(s0) < uint32_t(p.source_rows), there1 = uint32_t(s1) < uint32_t(p.source_rows);
+            const uint32_t at0 = there0 ? uint32_t(s0) * ld_b : 0u, at1 = there1 ? uint32_t(s1) * ld_b : 0u;
+            voff += lane < 32 ? at0 : at1;
+            bad |= (lane < 32 ? there0 : there1) ? 0u : 1u << r;
+        }
+        copy(rsrc_b, voff, TURN_B ? 0u : uint32_t(copy_kt) * kRowBytes, r, unit + unit_base(r, TURN_B));
+    };
+    // Zeros in place of what the k-tile in units (a, b) has been given for what does not exist, by the wave that copied it.
+    auto clear = [&](int here, uint32_t bad_here, int a, int b) __attribute__((always_inline)) {
+        if (here == kDepth && !(GATHER && __ballot(bad_here != 0))) return;
+        const i32x4 zeros = i32x4{0, 0, 0, 0};
+        const int l = lane_anew();
+#pragma unroll
+        for (int r = 0; r < PASSES; ++r) {
+            const int place = (r & 3) * 1024 + l * kChunk;
+            const bool plain_tail = plain_chunk(l, r) >= here / 8, turned_tail = turned_row(l, r) >= here, none = GATHER && ((bad_here >> r) & 1);
+            if ((TURN_A ? turned_tail : plain_tail) || (GATHER_A && none)) *reinterpret_cast<i32x4*>(ring + a + unit_base(r, TURN_A) + place) = zeros;
+            if ((TURN_B ? turned_tail : plain_tail) || (SOURCES && none)) *reinterpret_cast<i32x4*>(ring + b + unit_base(r, TURN_B) + place) = zeros;
+        }
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_s_waitcnt(waitcnt_imm(kNoWaitVm, 0));
+    };
+
+    f32x4 acc[TN][TM];
+    Frag nf[2][TN], mf[2][TM];
+    auto mma = [&](auto first_c, auto kh_c, int i, int j) __attribute__((always_inline)) {
+        constexpr int KH = decltype(kh_c)::value;
+        f32x4& sum = acc[i][j];
+        const Frag &n = nf[KH][i], &m = mf[KH][j];
+        if constexpr (decltype(first_c)::value) {
+            if constexpr (__is_same(Elem, __bf16)) asm volatile("v_mfma_f32_16x16x32_bf16 %0, %1, %2, 0" : "=a"(sum) : "v"(n), "v"(m));
+            else asm volatile("v_mfma_f32_16x16x32_f16 %0, %1, %2, 0" : "=a"(sum) : "v"(n), "v"(m));
+        } else {
+            if constexpr (__is_same(Elem, __bf16)) asm volatile("v_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+a"(sum) : "v"(n), "v"(m));
+            else asm volatile("v_mfma_f32_16x16x32_f16 %0, %1, %2, %0" : "+a"(sum) : "v"(n), "v"(m));
+        }
+    };
+    const int plain[2] = {frag_offset<16>(lane, 2 * g), frag_offset<16>(lane, 2 * g + 1)}, turned = Turned<BLOCK>::lane_offset(lane);
+    // fragment j of the rows, i of the columns, of half RK of the k-tile in unit `unit`; a turned one in two reads, of which this is number `part`
+    auto read_m = [&](auto kh_c, auto rk_c, int unit, int j, int part) __attribute__((always_inline)) {
+        constexpr int KH = decltype(kh_c)::value, RK = decltype(rk_c)::value;
+        if constexpr (TURN_A) read_turned_part<Frag>(mf[KH][j], ring + unit + RK * 8 * ROW_BYTES + part * 4 * ROW_BYTES + (turned ^ ((2 * j + wm) * 32)), part);
+        else mf[KH][j] = *reinterpret_cast<const Frag*>(ring + unit + (32 * j + 16 * wm) * kRowBytes + plain[RK]);
+    };
+    auto read_n = [&](auto kh_c, auto rk_c, int unit, int i, int part) __attribute__((always_inline)) {
+        constexpr int KH = decltype(kh_c)::value, RK = decltype(rk_c)::value;
+        if constexpr (TURN_B) read_turned_part<Frag>(nf[KH][i], ring + unit + RK * 8 * ROW_BYTES + part * 4 * ROW_BYTES + (turned ^ ((8 * wn + i) * 32)), part);
+        else nf[KH][i] = *reinterpret_cast<const Frag*>(ring + unit + (128 * wn + 16 * i) * kRowBytes + plain[RK]);
+    };
+    constexpr int PARTS_A = TURN_A ? 2 : 1, PARTS_B = TURN_B ? 2 : 1;
+    using Half0 = std::integral_constant<int, 0>;
+    using Half1 = std::integral_constant<int, 1>;
+    // read number x of a half's fragments, those of the rows first; `whole`: of all eight row atoms, or of four
+    auto read = [&](auto kh_c, auto rk_c, auto tm_c, int a, int b, int x) __attribute__((always_inline)) {
+        constexpr int RM = decltype(tm_c)::value * PARTS_A;
+        if (x < RM) read_m(kh_c, rk_c, a, x / PARTS_A, x % PARTS_A);
+        else if (x - RM < TN * PARTS_B) read_n(kh_c, rk_c, b, (x - RM) / PARTS_B, (x - RM) % PARTS_B);
+    };
+    // Half a k-tile: TN rows of TMR MFMAs on fragment buffer KH. Beside all rows but the last one go COPIES copies and the reads of the next half (units a, b; half RK) into the
+    // other buffer, beside the last one what `last_row(j)` does, j = 0 .. TMR - 1. The next half may be another tile's, with all of its row atoms: those are always read.
+    auto half_step = [&](auto kh_c, auto rk_c, auto first_c, auto tm_c, auto copies_c, int a, int b, auto&& copy_one, auto&& last_row) __attribute__((always_inline)) {
+        constexpr int KH = decltype(kh_c)::value, TMR = decltype(tm_c)::value, COPIES = decltype(copies_c)::value;
+        using Other = std::integral_constant<int, KH ^ 1>;
+        using ReadM = std::integral_constant<int, TM>;
+        constexpr int ALL = TM * PARTS_A + TN * PARTS_B, SIDE = ALL + COPIES, SLOTS = (TN - 1) * TMR;
+        static_for<TN * TMR>([&](auto slot_c) __attribute__((always_inline)) {
+            constexpr int SLOT = decltype(slot_c)::value;
+            mma(first_c, kh_c, SLOT / TMR, SLOT % TMR);
+            if constexpr (SLOT >= SLOTS) {
+                last_row(SLOT - SLOTS);
+            } else {
+                // copies and reads evenly among each other and over the MFMAs
+                constexpr int FROM = SLOT * SIDE / SLOTS, UPTO = (SLOT + 1) * SIDE / SLOTS;
+                static_for<UPTO - FROM>([&](auto s_c) __attribute__((always_inline)) {
+                    constexpr int S = FROM + decltype(s_c)::value, COPIED = S * COPIES / SIDE;
+                    if constexpr ((S + 1) * COPIES / SIDE > COPIED) copy_one(COPIED);
+                    else read(Other{}, rk_c, ReadM{}, a, b, S - COPIED);
+                });
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        });
+    };
+    auto meet = [] __attribute__((always_inline)) {
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+    };
+
+    // the first two k-tiles of the walk into units 0 .. 3
+    aim_copies();
+    uint32_t bad1 = 0, bad2 = 0;            // of the next k-tile, and of the one behind
+    for (int s = 0; s < 2; ++s) {
+        load_sources();
+#pragma unroll
+        for (int r = 0; r < PASSES; ++r) copy_a(r, 2 * s * UNIT_BYTES);
+#pragma unroll
+        for (int r = 0; r < PASSES; ++r) copy_b(r, (2 * s + 1) * UNIT_BYTES);
+        bad1 = bad2, bad2 = bad;
+        if (within()) advance_within();
+        else advance_beyond();
+    }
+    __builtin_amdgcn_s_waitcnt(waitcnt_imm(0, 0));
+    asm volatile("" ::: "memory");
+    clear(here_of(cur, 0), bad1, 0, UNIT_BYTES);
+    meet();
+#pragma unroll
+    for (int x = 0; x < TM * PARTS_A + TN * PARTS_B; ++x) read(Half0{}, Half0{}, std::integral_constant<int, TM>{}, 0, UNIT_BYTES, x);
+    __builtin_amdgcn_sched_barrier(0);
+
+    const bool stream_out = MODE == Grouped::TN ? size_t(p.groups) * p.m * p.n * 4 > (size_t(32) << 20) : size_t(p.m) * p.n * 2 > (size_t(32) << 20);
+    // stores of a tile by a wave, whatever of it exists, and how many of them are behind the current tile's first copies
+    constexpr int STORES_ALL = MODE == Grouped::TN ? 64 : 32;
+    int stores_before = 0;
+    auto wait_for_all_but = [](auto count_c) __attribute__((always_inline)) {
+        constexpr int MOST = decltype(count_c)::value < kNoWaitVm ? decltype(count_c)::value : kNoWaitVm;
+        __builtin_amdgcn_s_waitcnt(waitcnt_imm(MOST, 0));
+    };
+    // byte offsets of the units that hold A and B of the current k-tile, of the next one, and of the fifth unit
+    int oa = 0, ob = UNIT_BYTES, oa1 = 2 * UNIT_BYTES, ob1 = 3 * UNIT_BYTES, o5 = 4 * UNIT_BYTES;
+    while (true) {
+        const int count = cur.count();
+        using AllCopies = std::integral_constant<int, PASSES>;
+        auto nothing = [](int) __attribute__((always_inline)) {};
+        auto k_tile = [&](auto first_c, auto tm_c, int kt) __attribute__((always_inline)) {
+            load_sources();
+            // (a tile of up to 128 rows has no second half of rows to copy, but for columns in a turned operand's rows, which come with the others')
+            const bool flat_copies = !TURN_A && ahead.rows <= 128;
+            half_step(Half0{}, Half1{}, first_c, tm_c, AllCopies{}, oa, ob,
+                      [&](int r) __attribute__((always_inline)) { if (r < PASSES / 2 || !flat_copies) copy_a(r, o5); }, nothing);
+            // The next k-tile has landed. Behind its copies a wave has issued those above and, in a tile's first k-tile, the stores of the tile before; neither need be done.
+            constexpr int SEEN = decltype(first_c)::value ? 1 : 0;
+            const int stores = SEEN ? stores_before : 0;
+            if (stores == STORES_ALL) wait_for_all_but(std::integral_constant<int, STORES_ALL + PASSES / 2>{});
+            else if (stores == STORES_ALL / 2) wait_for_all_but(std::integral_constant<int, STORES_ALL / 2 + PASSES / 2>{});
+            else if (flat_copies) wait_for_all_but(std::integral_constant<int, PASSES / 2>{});
+            else wait_for_all_but(std::integral_constant<int, PASSES>{});
+            asm volatile("" ::: "memory");
+            if (GATHER || kt + 2 >= count) clear(kt + 1 == count ? next_here : here_of(cur, kt + 1), bad2, oa1, ob1);
+            meet();                             // every wave is done reading this k-tile
+            const int into = oa;
+            bool inside;
+            half_step(Half1{}, Half0{}, std::false_type{}, tm_c, AllCopies{}, oa1, ob1, [&](int r) __attribute__((always_inline)) { copy_b(r, into); },
+                      [&](int j) __attribute__((always_inline)) {
+                          if (j == 0) inside = within();
+                          if (j == 1) bad2 = bad;
+                          if (j == 1) { const int ta = oa1; oa1 = o5; o5 = ob; ob = ob1; ob1 = oa; oa = ta; }
+                          if (j == 2 && inside) advance_within();
+                      });
+            if (!inside) advance_beyond();
+        };
+        auto walk_k = [&](auto tm_c) __attribute__((always_inline)) {
+            k_tile(std::true_type{}, tm_c, 0);
+            for (int kt = 1; kt < count; ++kt) k_tile(std::false_type{}, tm_c, kt);
+        };
+        // The 4 registers of atom (i, j) are columns 128 wn + 16 i + 4 g + {0..3} of row 32 j + 16 wm + col. Each wave turns its slab round through the fifth unit, 16 rows by 64
+        // columns at a time and two such pieces in turn: the sums of piece u go in, piece u - 1 comes out, piece u - 2 is stored.
+        auto epilogue = [&](auto policy_c, auto tm_c, auto accumulate_c) __attribute__((always_inline)) {
+            constexpr bool ACCUMULATE = decltype(accumulate_c)::value, WIDE = MODE == Grouped::TN;          // fp32 outputs
+            constexpr int SIZE = WIDE ? 4 : 2, PIECE = 64, PITCH = WIDE ? PIECE * 4 : PIECE * 2 + 16, PIECE_BYTES = 16 * PITCH, PIECES = 2 * decltype(tm_c)::value;
+            constexpr int LANES_PER_ROW = PIECE * SIZE / 16, ROWS_PER_STORE = kWaveSize / LANES_PER_ROW, STORES = 16 / ROWS_PER_STORE, AHEAD = 1;
+            static_assert(PIECES * STORES == STORES_ALL * decltype(tm_c)::value / TM);
+            static_assert(4 * 2 * PIECE_BYTES <= UNIT_BYTES);
+            uint8_t* const buffers = ring + o5 + wave * (2 * PIECE_BYTES);
+            const uint32_t row_bytes = uint32_t(p.n) * SIZE;
+            const size_t first = WIDE ? (size_t(cur.group) * p.m + cur.m0) * p.n + cur.n0 : size_t(cur.m0) * p.n + cur.n0;
+            const __amdgpu_buffer_rsrc_t rsrc_out = make_rsrc(static_cast<uint8_t*>(p.out) + first * SIZE, uint32_t(cur.rows) * row_bytes - uint32_t(cur.n0) * SIZE);
+            const int row_in = lane / LANES_PER_ROW, c = lane % LANES_PER_ROW;
+            // chunk c of a row of fp32 in slot c ^ row; rows of 16 bits 16 bytes further apart than they are long
+            const auto place = [&](int row, int chunk) __attribute__((always_inline)) { return row * PITCH + (WIDE ? (chunk ^ (row & (LANES_PER_ROW - 1))) : chunk) * 16; };
+            uint32_t off[2];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int column = 128 * wn + PIECE * h + c * (16 / SIZE);
+                off[h] = column < cur.cols ? uint32_t(16 * wm + row_in) * row_bytes + uint32_t(column) * SIZE : kOutOfRange;
+            }
+            i32x4 back[2][STORES], held[ACCUMULATE ? AHEAD + 1 : 1][STORES];
+            auto load = [&](int u) __attribute__((always_inline)) {
+#pragma unroll
+                for (int s = 0; s < STORES; ++s)
+                    held[u % (AHEAD + 1)][s] = __builtin_amdgcn_raw_buffer_load_b128(rsrc_out, off[u % 2], (u / 2 * 32 + ROWS_PER_STORE * s) * row_bytes, 0);
+            };
+            if constexpr (ACCUMULATE) {
+#pragma unroll
+                for (int u = 0; u < AHEAD; ++u) load(u);
+            }
+#pragma unroll
+            for (int u = 0; u < PIECES + 2; ++u) {
+                if (u < PIECES) {
+                    const int j = u / 2, h = u % 2;
+#pragma unroll
+                    for (int a = 0; a < PIECE / 16; ++a) {
+                        // the sums come out of the accumulation registers here and nowhere earlier
+                        const f32x4& sum = acc[h * (PIECE / 16) + a][j];
+                        f32x4 v;
+                        asm volatile("v_accvgpr_read_b32 %0, %1" : "=v"(v[0]) : "a"(sum[0]));
+                        asm volatile("v_accvgpr_read_b32 %0, %1" : "=v"(v[1]) : "a"(sum[1]));
+                        asm volatile("v_accvgpr_read_b32 %0, %1" : "=v"(v[2]) : "a"(sum[2]));
+                        asm volatile("v_accvgpr_read_b32 %0, %1" : "=v"(v[3]) : "a"(sum[3]));
+                        uint8_t* const to = buffers + (u & 1) * PIECE_BYTES;
+                        if constexpr (WIDE) *reinterpret_cast<f32x4*>(to + place(col, 4 * a + g)) = v;
+                        else *reinterpret_cast<decltype(pack4(v, Elem{}))*>(to + place(col, 0) + (16 * a + 4 * g) * 2) = pack4(v, Elem{});
+                    }
+                }
+                __builtin_amdgcn_sched_barrier(0);
+                if (u >= 1 && u - 1 < PIECES) {
+#pragma unroll
+                    for (int s = 0; s < STORES; ++s) back[(u - 1) & 1][s] = *reinterpret_cast<const i32x4*>(buffers + ((u - 1) & 1) * PIECE_BYTES + place(ROWS_PER_STORE * s + row_in, c));
+                }
+                if (u >= 2) {
+                    const int w = u - 2;
+                    if constexpr (ACCUMULATE) {
+                        if (w + AHEAD < PIECES) load(w + AHEAD);
+                    }
+#pragma unroll
+                    for (int s = 0; s < STORES; ++s) {
+                        i32x4 v = back[w & 1][s];
+                        if constexpr (ACCUMULATE) v = __builtin_bit_cast(i32x4, __builtin_bit_cast(f32x4, v) + __builtin_bit_cast(f32x4, held[w % (AHEAD + 1)][s]));
+                        // (all of the offset in the lane's register, see wgrad_store in fp8_wgrad.hpp)
+                        buffer_store_16(v, rsrc_out, off[w % 2] + uint32_t(w / 2 * 32 + ROWS_PER_STORE * s) * row_bytes, decltype(policy_c)::value);
+                    }
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        };
+        auto leave = [&](auto tm_c, auto accumulate_c) __attribute__((always_inline)) {
+            if (stream_out) epilogue(std::true_type{}, tm_c, accumulate_c);
+            else epilogue(std::false_type{}, tm_c, accumulate_c);
+        };
+        auto tile = [&](auto tm_c) __attribute__((always_inline)) {
+            walk_k(tm_c);
+            asm volatile("s_nop 15\n\ts_nop 15" ::: "memory");      // the last MFMAs retire before the sums are read
+            if (MODE == Grouped::TN && p.accumulate) leave(tm_c, std::bool_constant<MODE == Grouped::TN>{});
+            else leave(tm_c, std::false_type{});
+        };
+        // (both branches to the end of the tile: sums that a flat tile does not have would else be kept for it)
+        const bool flat = cur.rows <= 128;
+        if (flat) tile(std::integral_constant<int, TM / 2>{});
+        else tile(std::integral_constant<int, TM>{});
+        if (lead == 0) break;
+        stores_before = flat ? STORES_ALL / 2 : STORES_ALL;
+        cur = GroupedTile::unpacked(next1);
+        next1 = next2, next2 = next3;
+        --lead;
+        next_here = lead ? here_of(GroupedTile::unpacked(next1), 0) : kDepth;
+        // every wave is out of the fifth unit before the next copies go into it
+        __builtin_amdgcn_s_waitcnt(waitcnt_imm(kNoWaitVm, 0));
+        meet();
+    }
+    __builtin_amdgcn_s_waitcnt(waitcnt_imm(0, 0));          // the copies behind the last k-tile have landed: the LDS may be another's from here on
+}
+
+enum Grouped16Kernel { kGroupedAny, kGroupedTall, kGrouped128, kGrouped64, kGrouped32 };
 
 // Rows that offsets speak of, and columns of a matrix: less than so many, so that tiles and ranges stay within 32-bit offsets.
 constexpr int kGroupedMostRows = 1 << 29, kGroupedMostColumns = 1 << 21;
@@ -455,10 +977,19 @@ inline hipError_t launch_grouped16(const void* lhs, const void* rhs, void* out, 
     };
     Grouped16Kernel which = KERNEL;
     if (which == kGroupedAny) {
-        const long long each = MODE == Grouped::TN ? m : rows / groups;
-        which = MODE != Grouped::TN && each <= 24 ? kGrouped32 : slots_of(128, 128) >= device_cu_count() ? kGrouped128 : kGrouped64;
+        const long long each = rows / groups;
+        if (each >= 128 && (MODE == Grouped::TN || k != 0) && slots_of(256, 256) >= 64) which = kGroupedTall;
+        else if (MODE != Grouped::TN && each <= 24) which = kGrouped32;
+        else which = slots_of(128, 128) >= device_cu_count() ? kGrouped128 : kGrouped64;
     }
     switch (which) {
+        case kGroupedTall: {
+            if ((MODE != Grouped::TN && k == 0) || (MODE == Grouped::TN && (long long)groups * ceil_div(m, 256) * 256 >= 1ll << 31)) return hipErrorInvalidValue;
+            const int cus = capped ? capped_grid(device_cu_count(), num_sms, device_cu_count()) : device_cu_count() / kNumXCD * kNumXCD;
+            const long long slots = MODE == Grouped::TN ? ceil_div<long long>((long long)groups * ceil_div(m, 256) * ceil_div(n, 256), kNumXCD) * kNumXCD : slots_of(256, 256);
+            hipLaunchKernelGGL((grouped16_tall_kernel<Elem, MODE, GATHER>), dim3(uint32_t(std::min<long long>(cus, slots))), dim3(256), 0, stream, p);
+            return hipGetLastError();
+        }
         case kGrouped32: return launch(grouped16_kernel<Elem, MODE, 32, 128, 4, GATHER>, 32, 128);
         case kGrouped64: return launch(grouped16_kernel<Elem, MODE, 64, 64, 4, GATHER>, 64, 64);
         default: return launch(grouped16_kernel<Elem, MODE, 128, 128, 2, GATHER>, 128, 128);
