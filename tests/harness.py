@@ -811,3 +811,5 @@ def grouped16_plans():
                 name, keys, arg_defs, code = ragged.grouped16_kernel_plan(dtype, mode, gather, kernel)
                 plans.append((name, keys, arg_defs, ragged.includes, code))
     return plans
+# tokens, hidden, inner, experts, top_k of the layer in 16 bits
+RAGGED_LAYER = (701, 512, 384, 6, 3)

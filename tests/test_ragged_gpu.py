@@ -180,3 +180,298 @@ def test_weight_gradients_of_whole_numbers(size, gather, kernel, dtype):
             _call('TN', dtype, kernel, lhs, rhs, out, offsets, source, accumulate)
             assert torch.equal(out.double(), want)
             assert bool((around[:1024] == 7).all()) and bool((around[1024 + left.numel():] == 7).all())
+
+
+@pytest.fixture
+def capped():
+    """Sets the compute-unit cap for a test and takes it back."""
+    before = yan.get_num_sms()
+    yield yan.set_num_sms
+    yan.set_num_sms(before)
+
+
+@pytest.mark.parametrize('kernel', testing.GROUPED16_KERNELS[1:])
+@pytest.mark.parametrize('cap', [1, 3, 8, 24])
+def test_walks_of_many_tiles(cap, kernel, capped):
+    """Few workgroups walk over all tiles: of one k-tile each, of several, of depths that are no multiple, of groups without rows in between."""
+    capped(cap)
+    g = _gen(cap)
+    for rows, n, k in (([300, 0, 1, 129, 0, 513, 64], 520, 8), ([257, 100, 0, 128], 264, 72), ([140, 600, 3], 776, 264), ([20] * 30, 264, 64)):
+        offsets = _offsets(rows)
+        m = int(offsets[-1])
+        lhs, weights, source = _whole(g, m, k, dtype=torch.bfloat16), _whole(g, len(rows), n, k, dtype=torch.bfloat16), torch.randperm(m, generator=g, device='cuda').int()
+        for mode in ('NT', 'NN', 'gathered'):
+            taken = lhs[source.long()] if mode == 'gathered' else lhs
+            want = torch.cat([taken[at].double() @ weights[i].double().t().contiguous() for i, at in enumerate(_groups(offsets))]).bfloat16()
+            out = torch.full((m, n), 7.0, dtype=torch.bfloat16, device='cuda')
+            _call('NN' if mode == 'NN' else 'NT', 'bf16', kernel, lhs, weights.transpose(1, 2).contiguous() if mode == 'NN' else weights, out, offsets,
+                  source if mode == 'gathered' else None)
+            assert torch.equal(out, want), (mode, rows)
+    for rows, m, n in (([5, 0, 64, 1, 63, 0, 0, 64, 2], 264, 520), ([65, 128, 0, 200, 1], 520, 264), ([1000, 30], 264, 136)):
+        offsets = _offsets(rows)
+        total = int(offsets[-1])
+        lhs, rhs, source = _whole(g, total, m, dtype=torch.bfloat16), _whole(g, total, n, dtype=torch.bfloat16), torch.randperm(total, generator=g, device='cuda').int()
+        for gather in (False, True):
+            taken = rhs[source.long()] if gather else rhs
+            products = torch.stack([lhs[at].double().t().contiguous() @ taken[at].double() for at in _groups(offsets)])
+            for accumulate in (False, True):
+                out = torch.full((len(rows), m, n), 7.0, device='cuda')
+                _call('TN', 'bf16', kernel, lhs, rhs, out, offsets, source if gather else None, accumulate)
+                assert torch.equal(out.double(), products + (7 if accumulate else 0)), (gather, accumulate, rows)
+
+
+def test_many_groups():
+    """More groups than a wave has lanes, most of them empty, runs of empty ones at both ends."""
+    g = _gen(9)
+    for groups in (64, 65, 129, 1000, 1024):
+        counts = torch.where(torch.rand(groups, generator=g, device='cuda') < 0.2, torch.randint(1, 40, (groups, ), generator=g, device='cuda'), 0)
+        counts[:5], counts[-70 % groups:] = 0, 0
+        counts[groups // 2] = 700
+        offsets = _offsets(counts.tolist())
+        m = int(offsets[-1])
+        lhs, weights = _whole(g, m, 72, dtype=torch.bfloat16), _whole(g, groups, 136, 72, dtype=torch.bfloat16)
+        want = torch.cat([lhs[at].double() @ weights[i].double().t().contiguous() for i, at in enumerate(_groups(offsets))]).bfloat16()
+        grads = torch.stack([want[at].double().t().contiguous() @ lhs[at].double() for at in _groups(offsets)])
+        for kernel in testing.GROUPED16_KERNELS:
+            out = torch.empty(m, 136, dtype=torch.bfloat16, device='cuda')
+            _call('NT', 'bf16', kernel, lhs, weights, out, offsets)
+            assert torch.equal(out, want), (groups, kernel)
+            if kernel != 'kGrouped32':
+                grad = torch.empty(groups, 136, 72, device='cuda')
+                _call('TN', 'bf16', kernel, want, lhs, grad, offsets)
+                _close(grad, grads, 40 * U * 700 * want.double().abs().max() * 3, 'gradients')
+
+
+# An fp32 sum of n products of 16-bit numbers is off by at most n steps, a step of 2 u at most of the sum of the products' magnitudes (whether the matrix cores round or cut off).
+REAL_SIZES = [([700, 0, 300, 24, 1], 520, 2048), ([64] * 8, 1032, 520), ([2000], 256, 7168), ([3, 1, 0, 2], 4096, 7168), ([129, 255, 257, 511], 776, 1544)]
+
+
+@pytest.mark.parametrize('kernel,dtype', KERNELS)
+@pytest.mark.parametrize('size', range(len(REAL_SIZES)))
+def test_products_of_normal_numbers(size, kernel, dtype):
+    rows, n, k = REAL_SIZES[size]
+    g = _gen(size + 50)
+    offsets, half = _offsets(rows), 2.0 ** (-8 if dtype == 'bf16' else -11)
+    m = int(offsets[-1])
+    lhs = torch.randn(m, k, generator=g, device='cuda').to(TYPES[dtype])
+    weights = (torch.randn(len(rows), n, k, generator=g, device='cuda') / k ** 0.5).to(TYPES[dtype])
+    grad = torch.randn(m, n, generator=g, device='cuda').to(TYPES[dtype])
+    out, back, for_weights = torch.empty_like(grad), torch.empty_like(lhs), torch.empty(len(rows), n, k, device='cuda')
+    _call('NT', dtype, kernel, lhs, weights, out, offsets)
+    _call('NN', dtype, kernel, grad, weights, back, offsets)
+    if kernel != 'kGrouped32':
+        _call('TN', dtype, kernel, grad, lhs, for_weights, offsets)
+    for i, at in enumerate(_groups(offsets)):
+        a, w, d = lhs[at].double(), weights[i].double(), grad[at].double()
+        for got, x, y, depth, step in ((out[at], a, w.t().contiguous(), k, half), (back[at], d, w, n, half), (for_weights[i], d.t().contiguous(), a, a.size(0), 0.0)):
+            if not got.numel() or (step == 0.0 and kernel == 'kGrouped32'):
+                continue
+            want, size_of = x @ y, x.abs() @ y.abs()
+            _close(got, want, 2 * depth * U * size_of * (1 + step) + step * want.abs() + (2.0 ** -25 if dtype == 'fp16' else 0), 'product')
+
+
+def test_offsets_past_32_bits():
+    """Outputs and operands of more than 4 GiB: the last rows are where they belong, and so are those of a group that starts far into its operand."""
+    g = _gen(12)
+    m, n = (1 << 20) + 131, 2056
+    offsets = torch.tensor([0, 1, m - 300, m], dtype=torch.int32, device='cuda')
+    lhs, weights = _whole(g, m, 8, dtype=torch.bfloat16), _whole(g, 3, n, 8, dtype=torch.bfloat16)
+    for kernel in ('kGroupedTall', 'kGrouped128'):
+        out = torch.zeros(m, n, dtype=torch.bfloat16, device='cuda')
+        _call('NT', 'bf16', kernel, lhs, weights, out, offsets)
+        for i, at in ((0, slice(0, 1)), (1, slice(1, 300)), (1, slice(m - 700, m - 300)), (2, slice(m - 300, m))):
+            assert torch.equal(out[at], (lhs[at].double() @ weights[i].double().t().contiguous()).bfloat16())
+        del out
+    # both operands of the weights' gradient, and the rows' one, read from beyond 4 GiB on
+    wide = torch.zeros(m, n, dtype=torch.bfloat16, device='cuda')
+    tail = _whole(g, 700, n, dtype=torch.bfloat16)
+    wide[m - 700:] = tail
+    offsets = torch.tensor([m - 700, m - 640, m], dtype=torch.int32, device='cuda')
+    for kernel in ('kGroupedTall', 'kGrouped128', 'kGrouped64'):
+        grad = torch.empty(2, n, 8, device='cuda')
+        _call('TN', 'bf16', kernel, wide, lhs, grad, offsets)
+        for i, (first, last) in enumerate(((0, 60), (60, 700))):
+            assert torch.equal(grad[i].double(), tail[first:last].double().t().contiguous() @ lhs[m - 700 + first:m - 700 + last].double())
+    back = torch.empty(m, 8, dtype=torch.bfloat16, device='cuda')
+    _call('NN', 'bf16', 'kGroupedTall', wide, weights[:2].contiguous(), back, offsets)
+    assert torch.equal(back[m - 640:], (tail[60:].double() @ weights[1].double()).bfloat16())
+
+
+def test_offsets_that_make_no_sense_stay_within_the_operands():
+    """Whatever the offsets hold, rows and groups are within theirs: nothing outside is written, and ascending groups among them are right."""
+    g = _gen(13)
+    m, n, k = 500, 264, 72
+    lhs, weights = _inside(_whole(g, m, k, dtype=torch.bfloat16)), _inside(_whole(g, 4, n, k, dtype=torch.bfloat16))
+    grad = _inside(_whole(g, m, n, dtype=torch.bfloat16))
+    for values in ([-5, 100, 1 << 30, 1 << 30, 2147483647], [400, 300, 200, 100, 0], [-2147483648, -1, 0, 0, 0], [500, 500, 500, 500, 500], [0, 500, 0, 500, 0], [0, 700, 100, 900, 501]):
+        offsets = torch.tensor(values, dtype=torch.int64, device='cuda').to(torch.int32)
+        for kernel in testing.GROUPED16_KERNELS:
+            around = torch.full((m * n + 4096, ), 7.0, dtype=torch.bfloat16, device='cuda')
+            _call('NT', 'bf16', kernel, lhs, weights, around[2048:2048 + m * n].view(m, n), offsets)
+            assert bool((around[:2048] == 7).all()) and bool((around[2048 + m * n:] == 7).all())
+            around = torch.full((4 * n * k + 2048, ), 7.0, device='cuda')
+            _call('TN', 'bf16', kernel, grad, lhs, around[1024:1024 + 4 * n * k].view(4, n, k), offsets)
+            assert bool((around[:1024] == 7).all()) and bool((around[1024 + 4 * n * k:] == 7).all())
+
+
+def _layer_inputs(g, tokens, hidden, inner, experts, top_k, padded):
+    x = torch.randn(tokens, hidden, generator=g, device='cuda').bfloat16()
+    logits = torch.randn(tokens, experts, generator=g, device='cuda')
+    w1 = (torch.randn(experts, inner, hidden, generator=g, device='cuda') / hidden ** 0.5).bfloat16()
+    w2 = (torch.randn(experts, hidden, inner, generator=g, device='cuda') / inner ** 0.5).bfloat16()
+    mask = torch.rand(tokens, generator=g, device='cuda') > 0.2 if padded else None
+    return x, logits, w1, w2, mask
+
+
+@pytest.mark.parametrize('padded', [False, True])
+def test_training_step_of_a_layer_in_16_bits(padded):
+    """A norm, the router, two expert products with an activation between them and the way back, as they are used together; gradients against 64 bits."""
+    g = _gen(21)
+    tokens, hidden, inner, experts, top_k = testing.RAGGED_LAYER
+    x, logits, w1, w2, mask = _layer_inputs(g, tokens, hidden, inner, experts, top_k, padded)
+    gain, grad_out = (1 + 0.2 * torch.randn(hidden, generator=g, device='cuda')).bfloat16(), torch.randn(tokens, hidden, generator=g, device='cuda').bfloat16()
+    normed = torch.empty_like(x)
+    inverse = yan.rms_norm(x, gain, normed)
+    weights, indices, counts, _ = yan.moe_route(logits, top_k, mask=mask)
+    rows, source, offsets = yan.moe_ragged_layout(indices, experts)
+    m = source.numel()
+    y1, y2 = torch.zeros(m, inner, dtype=torch.bfloat16, device='cuda'), torch.zeros(m, hidden, dtype=torch.bfloat16, device='cuda')
+    yan.m_grouped_gemm_bf16_bf16_bf16_nt_ragged(normed, w1, y1, offsets, source)
+    h = torch.relu(y1)
+    yan.m_grouped_gemm_bf16_bf16_bf16_nt_ragged(h, w2, y2, offsets)
+    out = torch.empty_like(x)
+    yan.moe_combine(y2, rows, weights, out)
+    # and back
+    grad_y2, grad_weights = yan.moe_combine_backward(grad_out, y2, rows, weights, source)
+    grad_h, grad_rows, grad_normed = torch.zeros_like(h), torch.zeros(m, hidden, dtype=torch.bfloat16, device='cuda'), torch.empty_like(x)
+    yan.m_grouped_gemm_bf16_bf16_bf16_nn_ragged(grad_y2, w2, grad_h, offsets)
+    grad_w2, grad_w1 = torch.zeros(experts, hidden, inner, device='cuda'), torch.zeros(experts, inner, hidden, device='cuda')
+    yan.k_grouped_gemm_bf16_bf16_fp32_tn_ragged(grad_y2, h, grad_w2, offsets, accumulate=True)
+    grad_y1 = grad_h * (y1 > 0)
+    yan.m_grouped_gemm_bf16_bf16_bf16_nn_ragged(grad_y1, w1, grad_rows, offsets)
+    yan.k_grouped_gemm_bf16_bf16_fp32_tn_ragged(grad_y1, normed, grad_w1, offsets, accumulate=True, source=source)
+    yan.moe_combine(grad_rows, rows, None, grad_normed)
+    grad_gain = torch.empty(hidden, device='cuda')
+    grad_x = yan.rms_norm_backward(grad_normed, x, gain, inverse, grad_gain)
+
+    # the same in 64 bits, by autograd
+    leaves = [t.double().requires_grad_() for t in (x, w1, w2, gain)]
+    dx, dw1, dw2, dgain = leaves
+    v = dx / torch.sqrt(dx.square().mean(1, keepdim=True) + 1e-6) * dgain
+    live = torch.ones(tokens, device='cuda') if mask is None else mask.double()
+    picked = torch.softmax(logits.double(), 1).gather(1, indices.clamp(min=0).long())
+    share = picked / picked.sum(1, keepdim=True) * live[:, None]
+    total = torch.zeros_like(v)
+    for e in range(experts):
+        through = torch.relu(v @ dw1[e].t()) @ dw2[e].t()
+        total = total + through * (share * (indices == e)).sum(1, keepdim=True)
+    (total * grad_out.double()).sum().backward()
+    # every product and every sum over them is rounded to 8 bits on the way: 5 such roundings to out, 9 to the farthest gradient, each half a step of 2^-8 of its value at most. Of
+    # sums of many terms with signs of their own what that comes to relative to the norm is less than twice the largest of them, in quadrature below a tenth of that
+    for name, got, want, roundings in (('out', out, total, 5), ('grad_w2', grad_w2, dw2.grad, 7), ('grad_w1', grad_w1, dw1.grad, 8), ('grad_x', grad_x, dx.grad, 9), ('grad_gain', grad_gain, dgain.grad, 9)):
+        off = (got.double() - want.detach()).norm() / want.detach().norm()
+        assert float(off) <= roundings * 2.0 ** -8, f'{name}: {float(off):.4f}'
+
+
+def test_padded_groups_of_the_contiguous_layout():
+    """The 128-row groups of the FP8 layout are groups as well: padding has no source, and comes out as zeros."""
+    g = _gen(22)
+    tokens, experts, top_k, k, n = 150, 5, 2, 256, 136
+    x = _whole(g, tokens, k, dtype=torch.bfloat16)
+    indices = torch.stack([torch.randperm(experts, generator=g, device='cuda')[:top_k] for _ in range(tokens)]).int()
+    m = yan.get_contiguous_layout_rows(tokens, top_k, experts)
+    codes, scales = torch.zeros(m, k, dtype=torch.uint8, device='cuda').view(torch.float8_e4m3fn), torch.zeros(m, k // 128, device='cuda')
+    rows, _, source, offsets = yan.moe_dispatch_to_fp8_contiguous(x, indices, experts, (codes, scales))
+    weights = _whole(g, experts, n, k, dtype=torch.bfloat16)
+    out = torch.full((m, n), 7.0, dtype=torch.bfloat16, device='cuda')
+    yan.m_grouped_gemm_bf16_bf16_bf16_nt_ragged(x, weights, out, offsets, source)
+    grad = torch.empty(experts, n, k, device='cuda')
+    dy = _whole(g, m, n, dtype=torch.bfloat16)
+    yan.k_grouped_gemm_bf16_bf16_fp32_tn_ragged(dy, x, grad, offsets, False, source)
+    taken = torch.where((source >= 0)[:, None], x[source.clamp(min=0).long()], 0).double()
+    for i, at in enumerate(_groups(offsets)):
+        assert torch.equal(out[at], (taken[at] @ weights[i].double().t().contiguous()).bfloat16())
+        assert torch.equal(grad[i].double(), dy[at].double().t().contiguous() @ taken[at])
+    assert bool((out[int(offsets[-1]):] == 7).all())
+
+
+def test_edges_of_ragged_products():
+    """No rows, no depth, no columns, one of each; outputs that are not asked for stay."""
+    empty = torch.zeros(3, dtype=torch.int32, device='cuda')
+    w = torch.ones(2, 16, 8, dtype=torch.bfloat16, device='cuda')
+    out = torch.zeros(0, 16, dtype=torch.bfloat16, device='cuda')
+    yan.m_grouped_gemm_bf16_bf16_bf16_nt_ragged(torch.zeros(0, 8, dtype=torch.bfloat16, device='cuda'), w, out, empty)
+    yan.m_grouped_gemm_bf16_bf16_bf16_nt_ragged(torch.zeros(0, 8, dtype=torch.bfloat16, device='cuda'), w, out, empty, empty[:0])
+    out = torch.full((4, 16), 7.0, dtype=torch.bfloat16, device='cuda')
+    yan.m_grouped_gemm_bf16_bf16_bf16_nt_ragged(torch.ones(4, 8, dtype=torch.bfloat16, device='cuda'), w, out, empty)
+    assert bool((out == 7).all())
+    offsets = torch.tensor([1, 1, 3], dtype=torch.int32, device='cuda')
+    yan.m_grouped_gemm_bf16_bf16_bf16_nt_ragged(torch.zeros(4, 0, dtype=torch.bfloat16, device='cuda'), w[:, :, :0], out, offsets)
+    assert bool((out[1:3] == 0).all()) and bool((out[[0, 3]] == 7).all())
+    grad = torch.full((2, 16, 8), 7.0, device='cuda')
+    nothing = torch.zeros(0, 16, dtype=torch.bfloat16, device='cuda')
+    yan.k_grouped_gemm_bf16_bf16_fp32_tn_ragged(nothing, nothing[:, :8], grad, empty, True)
+    assert bool((grad == 7).all())
+    yan.k_grouped_gemm_bf16_bf16_fp32_tn_ragged(nothing, nothing[:, :8], grad, empty)
+    assert bool((grad == 0).all())
+
+
+def test_infinities_and_nan_stay_in_their_rows():
+    """A row that is not finite makes itself not finite and no other one, whichever tile they share; rows without a group are not read into any sum."""
+    g = _gen(23)
+    for kernel in testing.GROUPED16_KERNELS:
+        offsets = torch.tensor([2, 40, 170], dtype=torch.int32, device='cuda')
+        lhs = _whole(g, 200, 72, dtype=torch.bfloat16)
+        lhs[0], lhs[180] = float('nan'), float('inf')
+        weights = _whole(g, 2, 136, 72, dtype=torch.bfloat16)
+        clean = torch.empty(200, 136, dtype=torch.bfloat16, device='cuda')
+        _call('NT', 'bf16', kernel, lhs, weights, clean, offsets)
+        assert bool(clean[2:170].isfinite().all())
+        dirty, out = lhs.clone(), torch.empty_like(clean)
+        dirty[39], dirty[100] = float('inf'), float('nan')
+        _call('NT', 'bf16', kernel, dirty, weights, out, offsets)
+        rest = torch.ones(200, dtype=torch.bool, device='cuda')
+        rest[:2], rest[170:], rest[39], rest[100] = False, False, False, False
+        assert torch.equal(out[rest], clean[rest]) and bool((~out[39].isfinite()).all()) and bool(out[100].isnan().all())
+
+
+def test_ragged_products_in_a_graph_and_on_other_streams():
+    g = _gen(24)
+    tokens, hidden, inner, experts, top_k = testing.RAGGED_LAYER
+    x, logits, w1, _, _ = _layer_inputs(g, tokens, hidden, inner, experts, top_k, False)
+    grad = torch.zeros(experts, inner, hidden, device='cuda')
+
+    def step(out, back):
+        _, indices, _, _ = yan.moe_route(logits, top_k)
+        rows, source, offsets = yan.moe_ragged_layout(indices, experts)
+        yan.m_grouped_gemm_bf16_bf16_bf16_nt_ragged(x, w1, out, offsets, source)
+        yan.m_grouped_gemm_bf16_bf16_bf16_nn_ragged(out, w1, back, offsets)
+        yan.k_grouped_gemm_bf16_bf16_fp32_tn_ragged(out, x, grad, offsets, True, source)
+        return rows, source, offsets
+
+    m = tokens * top_k
+    buffers = [(torch.empty(m, inner, dtype=torch.bfloat16, device='cuda'), torch.empty(m, hidden, dtype=torch.bfloat16, device='cuda')) for _ in range(3)]
+    made = step(*buffers[0])
+    want = [t.clone() for t in (*made, *buffers[0], grad)]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    grad.zero_()
+    with torch.cuda.stream(side):
+        got = step(*buffers[1])
+    torch.cuda.synchronize()
+    for a, b in zip((*got, *buffers[1]), want):
+        assert torch.equal(a, b)
+    grad.zero_()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step(*buffers[2])
+    for turn in range(3):
+        for t in (*got, *buffers[2]):
+            t.zero_()
+        grad.zero_()
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip((*got, *buffers[2], grad), want):
+            assert torch.equal(a, b), turn
+        x.mul_(1)               # eager work between the replays

@@ -55,6 +55,12 @@ __device__ __forceinline__ void grouped_range(const GroupedProblem& p, int g, in
     hi = min(max(p.offsets[g + 1], lo), p.rows);
 }
 
+// Runs of `block_m` rows that ascending offsets cut `rows` rows into at most.
+__host__ __device__ inline int most_row_tiles(int rows, int groups, int block_m) {
+    const long long runs = ((long long)rows + (long long)(block_m - 1) * groups) / block_m;
+    return runs < rows ? int(runs) : rows;
+}
+
 // A run of up to BLOCK_M rows of one group, and how many such runs the groups have: a wave looks at 64 groups at a time.
 struct RowTile {
     int group, row0, rows;
@@ -74,7 +80,8 @@ __device__ __forceinline__ int count_row_tiles(const GroupedProblem& p, int lane
         with_rows += __shfl_xor(with_rows, d, kWaveSize);
     }
     *groups_with_rows = __builtin_amdgcn_readfirstlane(with_rows);
-    return __builtin_amdgcn_readfirstlane(tiles);
+    // (offsets that do not ascend could say more, of which there is no end)
+    return min(__builtin_amdgcn_readfirstlane(tiles), most_row_tiles(p.rows, p.groups, BLOCK_M));
 }
 template <int BLOCK_M>
 __device__ __forceinline__ RowTile find_row_tile(const GroupedProblem& p, int tile, int lane) {
@@ -101,8 +108,12 @@ __device__ __forceinline__ RowTile find_row_tile(const GroupedProblem& p, int ti
     return {0, 0, 0};
 }
 
-// Bytes from `from` on that a descriptor of at most 2 GiB may reach.
-__device__ __forceinline__ uint32_t reach(long long bytes) { return bytes < (long long)kOutOfRange ? uint32_t(bytes) : kOutOfRange; }
+// Bytes, not less than none, that a descriptor of at most 2 GiB may reach. (In halves: the scalar unit does not compare numbers of 64 bits, and a descriptor that is not in
+// scalar registers is taken there lane by lane, in front of every copy.)
+__device__ __forceinline__ uint32_t reach(long long bytes) {
+    const uint32_t upper = uint32_t((unsigned long long)bytes >> 32), lower = uint32_t(bytes);
+    return upper != 0 || lower > kOutOfRange ? kOutOfRange : lower;
+}
 
 // Copies of a plain operand's k-tiles, DIM rows of 128 bytes: instruction j of wave w has rows 8 (4 j + w) .. + 7.
 template <int DIM>
@@ -230,7 +241,7 @@ grouped16_kernel(GroupedProblem p, int slots) {
     const int wn = wave % WAVES_N, wm = wave / WAVES_N, g = lane / 16, col = lane % 16;
     int with_rows = 0;
     const int row_tiles = MODE == Grouped::TN ? 0 : count_row_tiles<BLOCK_M>(p, lane, &with_rows);
-    XcdTileScheduler<> sched(MODE == Grouped::TN ? p.m : row_tiles * BLOCK_M, p.n, BLOCK_M, BLOCK_N);
+    XcdTileScheduler<> sched(MODE == Grouped::TN ? p.m : row_tiles, p.n, MODE == Grouped::TN ? BLOCK_M : 1, BLOCK_N);
     if (MODE != Grouped::TN) sched.fit_bands_to_groups(with_rows ? row_tiles / with_rows : 1);
     const int per_group = sched.grid_size();
     if (MODE != Grouped::TN) slots = per_group;
@@ -520,7 +531,7 @@ grouped16_tall_kernel(GroupedProblem p) {
         // (worked out anew for every tile: a dozen scalar registers less over the k-loop, which has none to spare)
         int rows_anew = row_tiles;
         asm volatile("" : "+s"(rows_anew));
-        XcdTileScheduler<> sched(rows_anew * BLOCK, p.n, BLOCK, BLOCK);
+        XcdTileScheduler<> sched(rows_anew, p.n, 1, BLOCK);
         sched.fit_bands_to_groups(band);
         // groups of TN differ in their depth: patches of 32 tiles are dealt out to the XCDs
         const TileCoord c = MODE == Grouped::TN ? sched.dealt_band_tile_of(slot) : sched.tile_of(slot);
@@ -538,7 +549,7 @@ grouped16_tall_kernel(GroupedProblem p) {
         }
         return t;
     };
-    const int slots = XcdTileScheduler<>(row_tiles * BLOCK, p.n, BLOCK, BLOCK).grid_size();
+    const int slots = XcdTileScheduler<>(row_tiles, p.n, 1, BLOCK).grid_size();
     // the next tile of this workgroup's walk, from `slot` on
     auto seek = [&](int slot) __attribute__((always_inline)) {
         for (; slot < slots; slot += gridDim.x) {
@@ -965,9 +976,7 @@ inline hipError_t launch_grouped16(const void* lhs, const void* rhs, void* out, 
     const bool capped = num_sms > 0 && num_sms < device_cu_count();
     const auto slots_of = [&](int block_m, int block_n) -> long long {
         if (MODE == Grouped::TN) return (long long)XcdTileScheduler<>(m, n, block_m, block_n).grid_size() * groups;
-        // as many runs as the groups' rows can have
-        const long long runs = std::min<long long>(m, ((long long)m + (long long)(block_m - 1) * groups) / block_m);
-        return ceil_div<long long>(runs * ceil_div(n, block_n), kNumXCD) * kNumXCD;
+        return ceil_div<long long>((long long)most_row_tiles(m, groups, block_m) * ceil_div(n, block_n), kNumXCD) * kNumXCD;
     };
     const auto launch = [&](auto kernel, int block_m, int block_n) {
         const long long slots = slots_of(block_m, block_n);
@@ -984,9 +993,10 @@ inline hipError_t launch_grouped16(const void* lhs, const void* rhs, void* out, 
     }
     switch (which) {
         case kGroupedTall: {
-            if ((MODE != Grouped::TN && k == 0) || (MODE == Grouped::TN && (long long)groups * ceil_div(m, 256) * 256 >= 1ll << 31)) return hipErrorInvalidValue;
+            if (MODE != Grouped::TN && k == 0) return hipErrorInvalidValue;
             const int cus = capped ? capped_grid(device_cu_count(), num_sms, device_cu_count()) : device_cu_count() / kNumXCD * kNumXCD;
             const long long slots = MODE == Grouped::TN ? ceil_div<long long>((long long)groups * ceil_div(m, 256) * ceil_div(n, 256), kNumXCD) * kNumXCD : slots_of(256, 256);
+            if (slots >= 1ll << 30) return hipErrorInvalidValue;
             hipLaunchKernelGGL((grouped16_tall_kernel<Elem, MODE, GATHER>), dim3(uint32_t(std::min<long long>(cus, slots))), dim3(256), 0, stream, p);
             return hipGetLastError();
         }

@@ -116,12 +116,12 @@ def _run(plan, args):
 def _norm(call, x, weight, eps, residual, col_major_scales, normed, with_codes):
     _check(x, weight, residual, normed)
     assert normed is None or normed.dtype == torch.bfloat16
+    assert not with_codes or x.size(1) % 128 == 0, 'a scale covers 128 elements'
     assert_on_current_device(x, weight, residual, normed)
     rows, k = x.shape
     inverse_rms = torch.empty((rows, ), dtype=torch.float32, device=x.device)
     codes = scales = None
     if with_codes:
-        assert k % 128 == 0, 'a scale covers 128 elements'
         codes = torch.empty((rows, k), dtype=torch.float8_e4m3fn, device=x.device)
         scales = torch.empty((k // 128, rows), dtype=torch.float32, device=x.device).t() if col_major_scales else torch.empty((rows, k // 128), dtype=torch.float32, device=x.device)
     made = (codes, scales, inverse_rms) if with_codes else (inverse_rms, )
