@@ -489,7 +489,7 @@ struct RowRuns {
 // What is different:
 //   * row atoms alternate between the two waves that share a tile's rows, so that a tile at a group's end has them split evenly; one with up to 128 rows (FLAT) runs half of
 //     the MFMAs and copies half of the rows. Groups end in the middle of a tile, on average; with 512 rows a group whole tiles would be a quarter more work.
-//   * lane offsets of the copies are worked out anew for every tile, and for a k-tile that is not whole: rows that stand in for those that do not exist, gathered rows;
+//   * lane offsets of the copies are worked out anew for tiles that are not whole (rows that stand in for those that do not exist) and for gathered rows;
 //   * descriptors of turned operands move on with the k-tile, so that ranges may be of any length;
 //   * any number of k-tiles, one for instance: the copies' place in the walk is its own.
 struct GroupedTile {
@@ -533,8 +533,9 @@ grouped16_tall_kernel(GroupedProblem p) {
         asm volatile("" : "+s"(rows_anew));
         XcdTileScheduler<> sched(rows_anew, p.n, 1, BLOCK);
         sched.fit_bands_to_groups(band);
-        // groups of TN differ in their depth: patches of 32 tiles are dealt out to the XCDs
-        const TileCoord c = MODE == Grouped::TN ? sched.dealt_band_tile_of(slot) : sched.tile_of(slot);
+        // Patches of 32 tiles are dealt out to the XCDs: tiles at a group's end take less time than others, groups of TN differ in their depth, and a range of tiles for each XCD would
+        // leave some with more work than others (32768 rows of 64 experts x 2048 x 7168 916 -> 886 us, 6144 of 16 x 7168 x 4096 back 401 -> 381).
+        const TileCoord c = sched.dealt_band_tile_of(slot);
         GroupedTile t{slot, -1, 0, 0, 0, 0, 0, 0};
         if (!c.valid) return t;
         t.n0 = c.n_idx * BLOCK, t.cols = min(BLOCK, p.n - t.n0);
@@ -600,18 +601,25 @@ grouped16_tall_kernel(GroupedProblem p) {
     __amdgpu_buffer_rsrc_t rsrc_a, rsrc_b;
     uint32_t voff_a[8], voff_b[8];
     const uint8_t *from_a, *from_b;         // of turned operands: where the k-tile starts
-    uint32_t bad = 0;                       // a bit a pass: the gathered row that this lane copies is none
+    // A bit a pass: the gathered row that this lane copies is none. Eight of the copies' k-tile, behind them eight each of the one before and of that before it.
+    uint32_t none_of = 0;
+    auto age_none = [&] __attribute__((always_inline)) { if (GATHER) none_of = (none_of & 0xff) | none_of << 8; };
     i32x16_unaligned sources;               // SOURCES: of this wave's rows of the k-tile
     auto here_of = [&](const GroupedTile& t, int kt) __attribute__((always_inline)) { return min(kDepth, t.depth - kt * kDepth); };
-    // the lane offsets for k-tiles of which `here` of k exist
+    // The lane offsets, of turned operands for k-tiles of which `here` of k are copied. They are the same for all tiles that are whole, and so is what they were last worked out for.
+    // What is copied of k behind the contraction's end is made zeros later; it only has to exist, and so it does, as the next row's or as rows of another group, but at the end of a
+    // turned operand: there the last k-tile (`tail_aims`) has its last row instead. Of a plain operand's last row that is out of the descriptor's range, for some lanes of a copy.
+    bool aimed_whole = false, tail_aims = false;
     auto aim_lanes = [&](int here) __attribute__((always_inline)) {
         const GroupedTile& t = ahead;
+        const bool whole = !GATHER_A && here == kDepth && t.rows == BLOCK && t.cols == BLOCK;
+        if (whole && aimed_whole) return;
+        aimed_whole = whole;
         const int l = lane_anew();
-        if constexpr (GATHER_A) bad = 0;
+        if constexpr (GATHER_A) none_of &= ~0xffu;
 #pragma unroll
         for (int r = 0; r < PASSES; ++r) {
-            const uint32_t bias = kCopyBias - (r % 4) * 1024;
-            const uint32_t in_row = uint32_t(plain_chunk(l, r) < here / 8 ? plain_chunk(l, r) : 0) * kChunk + bias;
+            const uint32_t bias = kCopyBias - (r % 4) * 1024, in_row = plain_chunk(l, r) * kChunk + bias;
             if constexpr (TURN_A) {
                 voff_a[r] = product(min(turned_row(l, r), here - 1), ld_a, turned_chunk(l, r, t.rows) * kChunk + bias);
             } else {
@@ -620,7 +628,7 @@ grouped16_tall_kernel(GroupedProblem p) {
                     const int s = p.source[t.m0 + row];
                     const bool there = uint32_t(s) < uint32_t(p.source_rows);
                     row = there ? s : 0;
-                    bad |= there ? 0u : 1u << r;
+                    none_of |= there ? 0u : 1u << r;
                 }
                 voff_a[r] = product(row, ld_a, in_row);
             }
@@ -633,7 +641,8 @@ grouped16_tall_kernel(GroupedProblem p) {
         const GroupedTile& t = ahead;
         const int row = t.k0 + copy_kt * kDepth;
         if constexpr (TURN_A) rsrc_a = describe(from_a, (long long)(p.rows - row) * ld_a - t.m0 * 2);
-        if constexpr (TURN_B && !SOURCES) rsrc_b = describe(from_b, (long long)((MODE == Grouped::TN ? p.rows : p.k) - row) * ld_b - t.n0 * 2);
+        if constexpr (MODE == Grouped::TN && !SOURCES) rsrc_b = describe(from_b, (long long)(p.rows - row) * ld_b - t.n0 * 2);
+        if constexpr (MODE == Grouped::NN) rsrc_b = describe(from_b, ((long long)(p.groups - t.group) * p.k - row) * ld_b - t.n0 * 2);
     };
     auto aim_copies = [&] __attribute__((always_inline)) {
         const GroupedTile& t = ahead;
@@ -645,14 +654,15 @@ grouped16_tall_kernel(GroupedProblem p) {
         else if constexpr (TURN_B) from_b = rhs + size_t(t.k0) * ld_b + t.n0 * 2;
         else rsrc_b = describe(rhs + size_t(t.n0) * ld_b, (long long)t.cols * ld_b);
         describe_turned();
-        aim_lanes(here_of(t, 0));
+        tail_aims = t.depth % kDepth != 0 && (MODE == Grouped::TN ? t.k0 + t.count() * kDepth > p.rows : MODE == Grouped::NN && t.group == p.groups - 1);
+        aim_lanes(tail_aims ? here_of(t, 0) : kDepth);
     };
     // Behind the walk's last k-tile that one is copied again, two times, into units that nobody reads any more: the count of copies under way stays what the waits below take it for.
     bool walking = true;
     // the tiles behind the current one, as far as the copies have come: up to three, of one k-tile each; and how many k of the next one's first k-tile exist
     int next1 = 0, next2 = 0, next3 = 0, lead = 0, next_here = kDepth;
     // Most k-tiles are followed by a whole one of the same tile: what that takes is a few scalar instructions, which ride under the last MFMAs of a k-tile.
-    auto within = [&] __attribute__((always_inline)) { return (copy_kt + 2) * kDepth <= ahead.depth; };
+    auto within = [&] __attribute__((always_inline)) { return tail_aims ? (copy_kt + 2) * kDepth <= ahead.depth : (copy_kt + 1) * kDepth < ahead.depth; };
     auto advance_within = [&] __attribute__((always_inline)) {
         ++copy_kt;
         if constexpr (TURN_A) from_a += size_t(kDepth) * ld_a;
@@ -661,7 +671,7 @@ grouped16_tall_kernel(GroupedProblem p) {
     };
     auto advance_beyond = [&] __attribute__((always_inline)) {
         if (!walking) return;
-        if (copy_kt + 1 < ahead.count()) {          // a last k-tile that is not whole
+        if (copy_kt + 1 < ahead.count()) {          // a last k-tile that is aimed at anew
             advance_within();
             aim_lanes(here_of(ahead, copy_kt));
             return;
@@ -688,7 +698,7 @@ grouped16_tall_kernel(GroupedProblem p) {
 #pragma unroll
                 for (int i = 0; i < 16; ++i) sources[i] = from[min(first + i, ahead.depth - 1)];
             }
-            bad = 0;
+            none_of &= ~0xffu;
         }
     };
     auto copy = [&](__amdgpu_buffer_rsrc_t rsrc, uint32_t voff, uint32_t at, int r, int base) __attribute__((always_inline)) {
@@ -710,19 +720,22 @@ grouped16_tall_kernel(GroupedProblem p) {
             const bool there0 = uint32_t(s0) < uint32_t(p.source_rows), there1 = uint32_t(s1) < uint32_t(p.source_rows);
             const uint32_t at0 = there0 ? uint32_t(s0) * ld_b : 0u, at1 = there1 ? uint32_t(s1) * ld_b : 0u;
             voff += lane < 32 ? at0 : at1;
-            bad |= (lane < 32 ? there0 : there1) ? 0u : 1u << r;
+            none_of |= (lane < 32 ? there0 : there1) ? 0u : 1u << r;
         }
         copy(rsrc_b, voff, TURN_B ? 0u : uint32_t(copy_kt) * kRowBytes, r, unit + unit_base(r, TURN_B));
     };
-    // Zeros in place of what the k-tile in units (a, b) has been given for what does not exist, by the wave that copied it.
-    auto clear = [&](int here, uint32_t bad_here, int a, int b) __attribute__((always_inline)) {
-        if (here == kDepth && !(GATHER && __ballot(bad_here != 0))) return;
+    // Zeros in place of what the k-tile in units (a, b) has been given for what does not exist, by the wave that copied it, `age` k-tiles before the last one that it did.
+    auto clear = [&](int here, int age, int a, int b) __attribute__((always_inline)) {
+        // (of turned operands a wave has copied 16 k)
+        const bool none_of_mine = TURN_A && TURN_B ? 16 * wave + 16 <= here : here == kDepth;
+        const uint32_t none_here = none_of >> (8 * age) & 0xff;
+        if (none_of_mine && !(GATHER && __ballot(none_here != 0))) return;
         const i32x4 zeros = i32x4{0, 0, 0, 0};
         const int l = lane_anew();
 #pragma unroll
         for (int r = 0; r < PASSES; ++r) {
             const int place = (r & 3) * 1024 + l * kChunk;
-            const bool plain_tail = plain_chunk(l, r) >= here / 8, turned_tail = turned_row(l, r) >= here, none = GATHER && ((bad_here >> r) & 1);
+            const bool plain_tail = plain_chunk(l, r) >= here / 8, turned_tail = turned_row(l, r) >= here, none = GATHER && ((none_here >> r) & 1);
             if ((TURN_A ? turned_tail : plain_tail) || (GATHER_A && none)) *reinterpret_cast<i32x4*>(ring + a + unit_base(r, TURN_A) + place) = zeros;
             if ((TURN_B ? turned_tail : plain_tail) || (SOURCES && none)) *reinterpret_cast<i32x4*>(ring + b + unit_base(r, TURN_B) + place) = zeros;
         }
@@ -797,20 +810,19 @@ grouped16_tall_kernel(GroupedProblem p) {
 
     // the first two k-tiles of the walk into units 0 .. 3
     aim_copies();
-    uint32_t bad1 = 0, bad2 = 0;            // of the next k-tile, and of the one behind
     for (int s = 0; s < 2; ++s) {
         load_sources();
 #pragma unroll
         for (int r = 0; r < PASSES; ++r) copy_a(r, 2 * s * UNIT_BYTES);
 #pragma unroll
         for (int r = 0; r < PASSES; ++r) copy_b(r, (2 * s + 1) * UNIT_BYTES);
-        bad1 = bad2, bad2 = bad;
+        age_none();
         if (within()) advance_within();
         else advance_beyond();
     }
     __builtin_amdgcn_s_waitcnt(waitcnt_imm(0, 0));
     asm volatile("" ::: "memory");
-    clear(here_of(cur, 0), bad1, 0, UNIT_BYTES);
+    clear(here_of(cur, 0), 2, 0, UNIT_BYTES);
     meet();
 #pragma unroll
     for (int x = 0; x < TM * PARTS_A + TN * PARTS_B; ++x) read(Half0{}, Half0{}, std::integral_constant<int, TM>{}, 0, UNIT_BYTES, x);
@@ -833,27 +845,32 @@ grouped16_tall_kernel(GroupedProblem p) {
         auto k_tile = [&](auto first_c, auto tm_c, int kt) __attribute__((always_inline)) {
             load_sources();
             // (a tile of up to 128 rows has no second half of rows to copy, but for columns in a turned operand's rows, which come with the others')
-            const bool flat_copies = !TURN_A && ahead.rows <= 128;
+            int passes = __builtin_amdgcn_readfirstlane(TURN_A || ahead.rows > 128 ? PASSES : PASSES / 2);
+            asm volatile("" : "+s"(passes));            // (a number, of which every copy is one compare)
             half_step(Half0{}, Half1{}, first_c, tm_c, AllCopies{}, oa, ob,
-                      [&](int r) __attribute__((always_inline)) { if (r < PASSES / 2 || !flat_copies) copy_a(r, o5); }, nothing);
+                      [&](int r) __attribute__((always_inline)) { if (TURN_A || r < PASSES / 2 || passes == PASSES) copy_a(r, o5); }, nothing);
             // The next k-tile has landed. Behind its copies a wave has issued those above and, in a tile's first k-tile, the stores of the tile before; neither need be done.
-            constexpr int SEEN = decltype(first_c)::value ? 1 : 0;
-            const int stores = SEEN ? stores_before : 0;
-            if (stores == STORES_ALL) wait_for_all_but(std::integral_constant<int, STORES_ALL + PASSES / 2>{});
-            else if (stores == STORES_ALL / 2) wait_for_all_but(std::integral_constant<int, STORES_ALL / 2 + PASSES / 2>{});
-            else if (flat_copies) wait_for_all_but(std::integral_constant<int, PASSES / 2>{});
-            else wait_for_all_but(std::integral_constant<int, PASSES>{});
+            if constexpr (decltype(first_c)::value) {
+                if (stores_before == STORES_ALL) wait_for_all_but(std::integral_constant<int, STORES_ALL + PASSES / 2>{});
+                else if (stores_before == STORES_ALL * 3 / 4) wait_for_all_but(std::integral_constant<int, STORES_ALL * 3 / 4 + PASSES / 2>{});
+                else if (stores_before == STORES_ALL / 2) wait_for_all_but(std::integral_constant<int, STORES_ALL / 2 + PASSES / 2>{});
+                else if (stores_before == STORES_ALL / 4) wait_for_all_but(std::integral_constant<int, STORES_ALL / 4 + PASSES / 2>{});
+                else wait_for_all_but(std::integral_constant<int, PASSES / 2>{});
+            } else {
+                wait_for_all_but(std::integral_constant<int, PASSES>{});
+                if (!TURN_A && passes != PASSES) wait_for_all_but(std::integral_constant<int, PASSES / 2>{});
+            }
             asm volatile("" ::: "memory");
-            if (GATHER || kt + 2 >= count) clear(kt + 1 == count ? next_here : here_of(cur, kt + 1), bad2, oa1, ob1);
+            if (GATHER || kt + 2 >= count) clear(kt + 1 == count ? next_here : here_of(cur, kt + 1), 1, oa1, ob1);
             meet();                             // every wave is done reading this k-tile
             const int into = oa;
             bool inside;
             half_step(Half1{}, Half0{}, std::false_type{}, tm_c, AllCopies{}, oa1, ob1, [&](int r) __attribute__((always_inline)) { copy_b(r, into); },
                       [&](int j) __attribute__((always_inline)) {
                           if (j == 0) inside = within();
-                          if (j == 1) bad2 = bad;
+                          if (j == 1) age_none();
                           if (j == 1) { const int ta = oa1; oa1 = o5; o5 = ob; ob = ob1; ob1 = oa; oa = ta; }
-                          if (j == 2 && inside) advance_within();
+                          if (j == (decltype(tm_c)::value > 2 ? 2 : 1) && inside) advance_within();
                       });
             if (!inside) advance_beyond();
         };
@@ -942,11 +959,12 @@ grouped16_tall_kernel(GroupedProblem p) {
             else leave(tm_c, std::false_type{});
         };
         // (both branches to the end of the tile: sums that a flat tile does not have would else be kept for it)
-        const bool flat = cur.rows <= 128;
-        if (flat) tile(std::integral_constant<int, TM / 2>{});
+        if (MODE != Grouped::TN && cur.rows <= 64) tile(std::integral_constant<int, TM / 4>{});
+        else if (cur.rows <= 128) tile(std::integral_constant<int, TM / 2>{});
+        else if (MODE != Grouped::TN && cur.rows <= 192) tile(std::integral_constant<int, TM * 3 / 4>{});
         else tile(std::integral_constant<int, TM>{});
         if (lead == 0) break;
-        stores_before = flat ? STORES_ALL / 2 : STORES_ALL;
+        stores_before = MODE == Grouped::TN ? ceil_div(cur.rows, 128) * (STORES_ALL / 2) : ceil_div(cur.rows, 64) * (STORES_ALL / 4);
         cur = GroupedTile::unpacked(next1);
         next1 = next2, next2 = next3;
         --lead;
