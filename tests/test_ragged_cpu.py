@@ -56,6 +56,14 @@ def test_norm_refuses():
     _refused(back, x.half(), x, w, r)
 
 
+def test_norm_refuses_its_residual_for_its_output():
+    x, residual, w = torch.zeros(4, 256, dtype=BF16), torch.zeros(4, 256, dtype=BF16), torch.ones(256)
+    with pytest.raises(AssertionError, match='a place of their own'):
+        yan.rms_norm(x, w, residual, 1e-6, residual)
+    with pytest.raises(AssertionError, match='a place of their own'):
+        yan.rms_norm_to_fp8(x, w, 1e-6, residual, False, residual)
+
+
 def test_layout_refuses():
     i = torch.zeros(4, 2, dtype=torch.int32)
     _refused(yan.moe_ragged_layout, i.long(), 4)

@@ -207,6 +207,8 @@ def test_walks_of_many_tiles(cap, kernel, capped):
             _call('NN' if mode == 'NN' else 'NT', 'bf16', kernel, lhs, weights.transpose(1, 2).contiguous() if mode == 'NN' else weights, out, offsets,
                   source if mode == 'gathered' else None)
             assert torch.equal(out, want), (mode, rows)
+    if kernel == 'kGrouped32':
+        return
     for rows, m, n in (([5, 0, 64, 1, 63, 0, 0, 64, 2], 264, 520), ([65, 128, 0, 200, 1], 520, 264), ([1000, 30], 264, 136)):
         offsets = _offsets(rows)
         total = int(offsets[-1])
@@ -309,6 +311,8 @@ def test_offsets_that_make_no_sense_stay_within_the_operands():
             around = torch.full((m * n + 4096, ), 7.0, dtype=torch.bfloat16, device='cuda')
             _call('NT', 'bf16', kernel, lhs, weights, around[2048:2048 + m * n].view(m, n), offsets)
             assert bool((around[:2048] == 7).all()) and bool((around[2048 + m * n:] == 7).all())
+            if kernel == 'kGrouped32':
+                continue
             around = torch.full((4 * n * k + 2048, ), 7.0, device='cuda')
             _call('TN', 'bf16', kernel, grad, lhs, around[1024:1024 + 4 * n * k].view(4, n, k), offsets)
             assert bool((around[:1024] == 7).all()) and bool((around[1024 + 4 * n * k:] == 7).all())
@@ -475,3 +479,60 @@ def test_ragged_products_in_a_graph_and_on_other_streams():
         for a, b in zip((*got, *buffers[2], grad), want):
             assert torch.equal(a, b), turn
         x.mul_(1)               # eager work between the replays
+
+
+@pytest.mark.parametrize('kernel', testing.GROUPED16_KERNELS)
+def test_rows_without_a_source_are_nothing_to_what_is_not_finite(kernel):
+    """Weights that are not finite leave the outputs of such rows zeros, and gradients that nobody has written into their rows leave the weights' gradients as they were."""
+    g = _gen(31)
+    rows = [70, 0, 130, 257, 1, 64]
+    offsets, total = _offsets(rows), sum(rows)
+    source = torch.randint(0, 50, (total, ), generator=g, device='cuda', dtype=torch.int32)
+    none = torch.rand(total, generator=g, device='cuda') < 0.3
+    none[70:73] = True
+    source[none] = -1
+    source[none.nonzero()[::2]] = 50            # one row behind the last one
+    tokens = _whole(g, 50, 136, dtype=torch.bfloat16)
+    weights = _whole(g, 6, 264, 136, dtype=torch.bfloat16)
+    weights[2, 5], weights[3, 17], weights[5] = float('inf'), float('nan'), float('nan')
+    out = torch.full((total, 264), 9.0, dtype=torch.bfloat16, device='cuda')
+    _call('NT', 'bf16', kernel, tokens, weights, out, offsets, source)
+    assert bool((out[none] == 0).all())
+    for i, at in enumerate(_groups(offsets)):
+        live = ~none[at]
+        want = (tokens[source[at][live].long()].float() @ weights[i].float().t().contiguous()).bfloat16()
+        assert torch.equal(out[at][live].nan_to_num(7, 7, 7), want.nan_to_num(7, 7, 7))
+    if kernel == 'kGrouped32':
+        return
+    grads = _whole(g, total, 72, dtype=torch.bfloat16)
+    want = torch.zeros(6, 72, 136, device='cuda')
+    for i, at in enumerate(_groups(offsets)):
+        live = ~none[at]
+        want[i] = grads[at][live].float().t().contiguous() @ tokens[source[at][live].long()].float()
+    grads[none] = float('nan')
+    grads[none.nonzero()[::3]] = float('inf')
+    for accumulate in (False, True):
+        got = torch.full((6, 72, 136), 2.0, device='cuda')
+        _call('TN', 'bf16', kernel, grads, tokens, got, offsets, source, accumulate)
+        assert torch.equal(got, want + 2 if accumulate else want)
+
+
+def test_more_tiles_than_a_launch_has_workgroups():
+    """The widest weights there may be, of 1024 groups with a row or two: more tiles than a launch may have threads for."""
+    g = _gen(32)
+    n, groups = (1 << 21) - 8, 1024
+    rows = [1] * groups
+    rows[7], rows[1000] = 40, 38
+    offsets, total = _offsets(rows), sum(rows)
+    weights = torch.zeros(groups, n, 8, dtype=torch.bfloat16, device='cuda')
+    lhs = _whole(g, total, 8, dtype=torch.bfloat16)
+    out = torch.full((total, n), 9.0, dtype=torch.bfloat16, device='cuda')
+    known = (0, 7, 511, 1000, 1023)
+    for i in known:
+        weights[i] = _whole(g, n, 8, dtype=torch.bfloat16)
+    yan.m_grouped_gemm_bf16_bf16_bf16_nt_ragged(lhs, weights, out, offsets)
+    for i, at in enumerate(_groups(offsets)):
+        if i in known:
+            assert torch.equal(out[at], (lhs[at].float() @ weights[i].float().t().contiguous()).bfloat16())
+        else:
+            assert not bool(out[at].any())

@@ -4,7 +4,7 @@
 //   NT   out[r, j]    = sum_t lhs[s(r), t] rhs[g, j, t]      rows r of group g, s(r) = source[r] or r itself
 //   NN   out[r, j]    = sum_t lhs[r, t]    rhs[g, t, j]
 //   TN   out[g, i, j] (+)= sum_r lhs[r, i] rhs[s(r), j]      over the rows r of group g, fp32
-// fp32 sums from the first k-tile to the last; a row whose source is none is a row of zeros.
+// fp32 sums from the first k-tile to the last. A row whose source is none is a row of zeros of NT's out, and no row of TN's sum, whatever the other operand holds.
 //
 // Two kinds of operand. A plain one has the contraction along its rows: its k-tiles are staged and read as in the other GEMMs (tile_io.hpp). A turned one has the
 // contraction across its rows (the weights of NN, both sides of TN): its k-tile is 64 rows of as many columns as the tile has, and a fragment, eight consecutive k of one
@@ -339,14 +339,12 @@ grouped16_kernel(GroupedProblem p, int slots) {
             bool any = here < kDepth;
             if constexpr (SOURCES) any |= __ballot(((none >> (8 * age)) & 255) != 0) != 0;
             if (!any) return;
-            if constexpr (TURN_A) copies_a.clear(stage, wave, lane, [&](int, int r) { return r >= here; });
+            // (a row without a source counts for nothing, whatever the other operand has there: both have the same rows in the same lanes)
+            static_assert(!SOURCES || BLOCK_M == BLOCK_N);
+            const auto bad = [&](int j, int r) { return r >= here || (SOURCES && ((none >> (8 * age + j)) & 1)); };
+            if constexpr (TURN_A) copies_a.clear(stage, wave, lane, bad);
             else copies_a.clear(stage, here / 8, wave, lane);
-            if constexpr (TURN_B)
-                copies_b.clear(stage + A_BYTES, wave, lane, [&](int j, int r) {
-                    bool bad = r >= here;
-                    if constexpr (SOURCES) bad |= (none >> (8 * age + j)) & 1;
-                    return bad;
-                });
+            if constexpr (TURN_B) copies_b.clear(stage + A_BYTES, wave, lane, bad);
             else copies_b.clear(stage + A_BYTES, here / 8, wave, lane);
             asm volatile("" ::: "memory");
             __builtin_amdgcn_s_waitcnt(waitcnt_imm(kNoWaitVm, 0));
@@ -418,7 +416,7 @@ grouped16_kernel(GroupedProblem p, int slots) {
             i32x4 held[STORES];
             if (p.accumulate) {
 #pragma unroll
-                for (int u = 0; u < STORES; ++u) held[u] = __builtin_amdgcn_raw_buffer_load_b128(rsrc_out, to, u * ROWS_PER_STORE * row_bytes, 0);
+                for (int u = 0; u < STORES; ++u) held[u] = __builtin_amdgcn_raw_buffer_load_b128(rsrc_out, to + u * ROWS_PER_STORE * row_bytes, 0, 0);
             }
 #pragma unroll
             for (int j = 0; j < TM; ++j)
@@ -601,9 +599,9 @@ grouped16_tall_kernel(GroupedProblem p) {
     __amdgpu_buffer_rsrc_t rsrc_a, rsrc_b;
     uint32_t voff_a[8], voff_b[8];
     const uint8_t *from_a, *from_b;         // of turned operands: where the k-tile starts
-    // A bit a pass: the gathered row that this lane copies is none. Eight of the copies' k-tile, behind them eight each of the one before and of that before it.
+    // SOURCES, a bit a pass: the gathered row that this lane copies is none. Eight of the copies' k-tile, behind them eight each of the one before and of that before it.
     uint32_t none_of = 0;
-    auto age_none = [&] __attribute__((always_inline)) { if (GATHER) none_of = (none_of & 0xff) | none_of << 8; };
+    auto age_none = [&] __attribute__((always_inline)) { if (SOURCES) none_of = (none_of & 0xff) | none_of << 8; };
     i32x16_unaligned sources;               // SOURCES: of this wave's rows of the k-tile
     auto here_of = [&](const GroupedTile& t, int kt) __attribute__((always_inline)) { return min(kDepth, t.depth - kt * kDepth); };
     // The lane offsets, of turned operands for k-tiles of which `here` of k are copied. They are the same for all tiles that are whole, and so is what they were last worked out for.
@@ -616,7 +614,6 @@ grouped16_tall_kernel(GroupedProblem p) {
         if (whole && aimed_whole) return;
         aimed_whole = whole;
         const int l = lane_anew();
-        if constexpr (GATHER_A) none_of &= ~0xffu;
 #pragma unroll
         for (int r = 0; r < PASSES; ++r) {
             const uint32_t bias = kCopyBias - (r % 4) * 1024, in_row = plain_chunk(l, r) * kChunk + bias;
@@ -626,9 +623,7 @@ grouped16_tall_kernel(GroupedProblem p) {
                 int row = min(plain_row(l, r), t.rows - 1);
                 if constexpr (GATHER_A) {
                     const int s = p.source[t.m0 + row];
-                    const bool there = uint32_t(s) < uint32_t(p.source_rows);
-                    row = there ? s : 0;
-                    none_of |= there ? 0u : 1u << r;
+                    row = uint32_t(s) < uint32_t(p.source_rows) ? s : 0;
                 }
                 voff_a[r] = product(row, ld_a, in_row);
             }
@@ -662,7 +657,7 @@ grouped16_tall_kernel(GroupedProblem p) {
     // the tiles behind the current one, as far as the copies have come: up to three, of one k-tile each; and how many k of the next one's first k-tile exist
     int next1 = 0, next2 = 0, next3 = 0, lead = 0, next_here = kDepth;
     // Most k-tiles are followed by a whole one of the same tile: what that takes is a few scalar instructions, which ride under the last MFMAs of a k-tile.
-    auto within = [&] __attribute__((always_inline)) { return tail_aims ? (copy_kt + 2) * kDepth <= ahead.depth : (copy_kt + 1) * kDepth < ahead.depth; };
+    auto within = [&] __attribute__((always_inline)) { return (copy_kt + 1) * kDepth + (tail_aims ? kDepth : 1) <= ahead.depth; };
     auto advance_within = [&] __attribute__((always_inline)) {
         ++copy_kt;
         if constexpr (TURN_A) from_a += size_t(kDepth) * ld_a;
@@ -729,15 +724,16 @@ grouped16_tall_kernel(GroupedProblem p) {
         // (of turned operands a wave has copied 16 k)
         const bool none_of_mine = TURN_A && TURN_B ? 16 * wave + 16 <= here : here == kDepth;
         const uint32_t none_here = none_of >> (8 * age) & 0xff;
-        if (none_of_mine && !(GATHER && __ballot(none_here != 0))) return;
+        if (none_of_mine && !(SOURCES && __ballot(none_here != 0))) return;
         const i32x4 zeros = i32x4{0, 0, 0, 0};
         const int l = lane_anew();
 #pragma unroll
         for (int r = 0; r < PASSES; ++r) {
             const int place = (r & 3) * 1024 + l * kChunk;
-            const bool plain_tail = plain_chunk(l, r) >= here / 8, turned_tail = turned_row(l, r) >= here, none = GATHER && ((none_here >> r) & 1);
-            if ((TURN_A ? turned_tail : plain_tail) || (GATHER_A && none)) *reinterpret_cast<i32x4*>(ring + a + unit_base(r, TURN_A) + place) = zeros;
-            if ((TURN_B ? turned_tail : plain_tail) || (SOURCES && none)) *reinterpret_cast<i32x4*>(ring + b + unit_base(r, TURN_B) + place) = zeros;
+            // (of a row without a source both operands, which have the same rows in the same lanes: it counts for nothing, whatever the other has there)
+            const bool plain_tail = plain_chunk(l, r) >= here / 8, turned_tail = turned_row(l, r) >= here || (SOURCES && ((none_here >> r) & 1));
+            if (TURN_A ? turned_tail : plain_tail) *reinterpret_cast<i32x4*>(ring + a + unit_base(r, TURN_A) + place) = zeros;
+            if (TURN_B ? turned_tail : plain_tail) *reinterpret_cast<i32x4*>(ring + b + unit_base(r, TURN_B) + place) = zeros;
         }
         asm volatile("" ::: "memory");
         __builtin_amdgcn_s_waitcnt(waitcnt_imm(kNoWaitVm, 0));
@@ -861,7 +857,7 @@ grouped16_tall_kernel(GroupedProblem p) {
                 if (!TURN_A && passes != PASSES) wait_for_all_but(std::integral_constant<int, PASSES / 2>{});
             }
             asm volatile("" ::: "memory");
-            if (GATHER || kt + 2 >= count) clear(kt + 1 == count ? next_here : here_of(cur, kt + 1), 1, oa1, ob1);
+            if (SOURCES || kt + 2 >= count) clear(kt + 1 == count ? next_here : here_of(cur, kt + 1), 1, oa1, ob1);
             meet();                             // every wave is done reading this k-tile
             const int into = oa;
             bool inside;
@@ -880,6 +876,7 @@ grouped16_tall_kernel(GroupedProblem p) {
         };
         // The 4 registers of atom (i, j) are columns 128 wn + 16 i + 4 g + {0..3} of row 32 j + 16 wm + col. Each wave turns its slab round through the fifth unit, 16 rows by 64
         // columns at a time and two such pieces in turn: the sums of piece u go in, piece u - 1 comes out, piece u - 2 is stored.
+        uint32_t gone = 0;                      // GATHER_A, a bit an atom of rows: this lane's row in it has no source, and its outputs are zeros whatever the weights hold
         auto epilogue = [&](auto policy_c, auto tm_c, auto accumulate_c) __attribute__((always_inline)) {
             constexpr bool ACCUMULATE = decltype(accumulate_c)::value, WIDE = MODE == Grouped::TN;          // fp32 outputs
             constexpr int SIZE = WIDE ? 4 : 2, PIECE = 64, PITCH = WIDE ? PIECE * 4 : PIECE * 2 + 16, PIECE_BYTES = 16 * PITCH, PIECES = 2 * decltype(tm_c)::value;
@@ -899,11 +896,15 @@ grouped16_tall_kernel(GroupedProblem p) {
                 const int column = 128 * wn + PIECE * h + c * (16 / SIZE);
                 off[h] = column < cur.cols ? uint32_t(16 * wm + row_in) * row_bytes + uint32_t(column) * SIZE : kOutOfRange;
             }
+            [[maybe_unused]] const bool any_gone = __ballot(gone != 0) != 0;
             i32x4 back[2][STORES], held[ACCUMULATE ? AHEAD + 1 : 1][STORES];
             auto load = [&](int u) __attribute__((always_inline)) {
 #pragma unroll
-                for (int s = 0; s < STORES; ++s)
-                    held[u % (AHEAD + 1)][s] = __builtin_amdgcn_raw_buffer_load_b128(rsrc_out, off[u % 2], (u / 2 * 32 + ROWS_PER_STORE * s) * row_bytes, 0);
+                for (int s = 0; s < STORES; ++s) {
+                    uint32_t down = uint32_t(u / 2 * 32 + ROWS_PER_STORE * s) * row_bytes;
+                    asm volatile("" : "+s"(down));          // (added here, not ahead of the walk into a register for each)
+                    held[u % (AHEAD + 1)][s] = __builtin_amdgcn_raw_buffer_load_b128(rsrc_out, off[u % 2] + down, 0, 0);
+                }
             };
             if constexpr (ACCUMULATE) {
 #pragma unroll
@@ -922,6 +923,9 @@ grouped16_tall_kernel(GroupedProblem p) {
                         asm volatile("v_accvgpr_read_b32 %0, %1" : "=v"(v[1]) : "a"(sum[1]));
                         asm volatile("v_accvgpr_read_b32 %0, %1" : "=v"(v[2]) : "a"(sum[2]));
                         asm volatile("v_accvgpr_read_b32 %0, %1" : "=v"(v[3]) : "a"(sum[3]));
+                        if constexpr (GATHER_A) {
+                            if (any_gone) v = (gone >> j) & 1 ? f32x4{0.f, 0.f, 0.f, 0.f} : v;
+                        }
                         uint8_t* const to = buffers + (u & 1) * PIECE_BYTES;
                         if constexpr (WIDE) *reinterpret_cast<f32x4*>(to + place(col, 4 * a + g)) = v;
                         else *reinterpret_cast<decltype(pack4(v, Elem{}))*>(to + place(col, 0) + (16 * a + 4 * g) * 2) = pack4(v, Elem{});
@@ -942,7 +946,9 @@ grouped16_tall_kernel(GroupedProblem p) {
                         i32x4 v = back[w & 1][s];
                         if constexpr (ACCUMULATE) v = __builtin_bit_cast(i32x4, __builtin_bit_cast(f32x4, v) + __builtin_bit_cast(f32x4, held[w % (AHEAD + 1)][s]));
                         // (all of the offset in the lane's register, see wgrad_store in fp8_wgrad.hpp)
-                        buffer_store_16(v, rsrc_out, off[w % 2] + uint32_t(w / 2 * 32 + ROWS_PER_STORE * s) * row_bytes, decltype(policy_c)::value);
+                        uint32_t down = uint32_t(w / 2 * 32 + ROWS_PER_STORE * s) * row_bytes;
+                        if constexpr (WIDE) asm volatile("" : "+s"(down));
+                        buffer_store_16(v, rsrc_out, off[w % 2] + down, decltype(policy_c)::value);
                     }
                 }
                 __builtin_amdgcn_sched_barrier(0);
@@ -954,6 +960,13 @@ grouped16_tall_kernel(GroupedProblem p) {
         };
         auto tile = [&](auto tm_c) __attribute__((always_inline)) {
             walk_k(tm_c);
+            if constexpr (GATHER_A) {
+#pragma unroll
+                for (int j = 0; j < decltype(tm_c)::value; ++j) {
+                    const int s = p.source[cur.m0 + min(32 * j + 16 * wm + col, cur.rows - 1)];
+                    gone |= uint32_t(s) < uint32_t(p.source_rows) ? 0u : 1u << j;
+                }
+            }
             asm volatile("s_nop 15\n\ts_nop 15" ::: "memory");      // the last MFMAs retire before the sums are read
             if (MODE == Grouped::TN && p.accumulate) leave(tm_c, std::bool_constant<MODE == Grouped::TN>{});
             else leave(tm_c, std::false_type{});
@@ -998,8 +1011,9 @@ inline hipError_t launch_grouped16(const void* lhs, const void* rhs, void* out, 
     };
     const auto launch = [&](auto kernel, int block_m, int block_n) {
         const long long slots = slots_of(block_m, block_n);
-        if (slots >= 1ll << 24) return hipErrorInvalidValue;          // a launch has less than 2^32 threads
-        hipLaunchKernelGGL(kernel, dim3(uint32_t(capped ? capped_grid(int(slots), num_sms, device_cu_count()) : slots)), dim3(256), 0, stream, p, int(slots));
+        if (slots >= 1ll << 30) return hipErrorInvalidValue;
+        const int most = int(std::min(slots, 1ll << 20));             // a launch has less than 2^32 threads: beyond this a workgroup has several tiles
+        hipLaunchKernelGGL(kernel, dim3(uint32_t(capped ? capped_grid(most, num_sms, device_cu_count()) : most)), dim3(256), 0, stream, p, int(slots));
         return hipGetLastError();
     };
     Grouped16Kernel which = KERNEL;
@@ -1018,7 +1032,9 @@ inline hipError_t launch_grouped16(const void* lhs, const void* rhs, void* out, 
             hipLaunchKernelGGL((grouped16_tall_kernel<Elem, MODE, GATHER>), dim3(uint32_t(std::min<long long>(cus, slots))), dim3(256), 0, stream, p);
             return hipGetLastError();
         }
-        case kGrouped32: return launch(grouped16_kernel<Elem, MODE, 32, 128, 4, GATHER>, 32, 128);
+        case kGrouped32:
+            if constexpr (MODE != Grouped::TN) return launch(grouped16_kernel<Elem, MODE, 32, 128, 4, GATHER>, 32, 128);
+            else return hipErrorInvalidValue;
         case kGrouped64: return launch(grouped16_kernel<Elem, MODE, 64, 64, 4, GATHER>, 64, 64);
         default: return launch(grouped16_kernel<Elem, MODE, 128, 128, 2, GATHER>, 128, 128);
     }

@@ -144,11 +144,13 @@ def rms_norm_to_fp8(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, re
 
     x: bf16 or fp32 `[m, k]`, contiguous, k % 128 == 0, k up to 16384; weight: bf16 or fp32 `[k]`
     residual: bf16 or fp32 `[m, k]` (of x's type or not), or None: becomes `x + residual`, which is what is normed
-    normed: bf16 `[m, k]`, or None: gets the normed rows in 16 bits as well (for a router); may be x
+    normed: bf16 `[m, k]`, or None: gets the normed rows in 16 bits as well (for a router); may be x, not the residual
     Returns e4m3fn `[m, k]` and fp32 scales `[m, k/128]`, as `per_token_cast_to_fp8` makes them of the normed rows in fp32 (with `col_major_scales`
     token-contiguous), and fp32 `[m]`, the reciprocals of the root mean squares, for the gradient. Squares are summed in fp32.
     """
-    assert eps >= 0             # (no part of what a repeated call is found by)
+    # (no part of what a repeated call is found by)
+    assert eps >= 0
+    assert normed is None or normed is not residual, 'the normed rows have a place of their own'
     call = (NORM, x, weight, residual, normed, float(eps), 2 if col_major_scales else 1)
     made = repeat_new(*call)
     if made is not None:
@@ -158,15 +160,15 @@ def rms_norm_to_fp8(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, re
 
 def rms_norm(x: torch.Tensor, weight: torch.Tensor, out: torch.Tensor, eps: float = 1e-6, residual: Optional[torch.Tensor] = None) -> torch.Tensor:
     """
-    The normed rows in 16 bits: out bf16 `[m, k]`, written in place, k % 8 == 0; the rest as for `rms_norm_to_fp8`. Returns the reciprocals of the root mean
+    The normed rows in 16 bits: out bf16 `[m, k]`, written in place (may be x, not the residual), k % 8 == 0; the rest as for `rms_norm_to_fp8`. Returns the reciprocals of the root mean
     squares, fp32 `[m]`.
     """
     assert eps >= 0
+    assert out is not None and out is not residual, 'the normed rows have a place of their own'
     call = (NORM, x, weight, residual, out, float(eps), 0)
     made = repeat_new(*call)
     if made is not None:
         return made[0]
-    assert out is not None
     return _norm(call, x, weight, eps, residual, False, out, False)[0]
 
 

@@ -126,7 +126,7 @@ def m_grouped_gemm_bf16_bf16_bf16_nt_ragged(lhs: torch.Tensor, rhs: torch.Tensor
     lhs: bf16 `[m, k]`, rhs: bf16 `[num_groups, n, k]`, out: bf16 `[m, n]`, written in place; all contiguous
     offsets: int32 `[num_groups + 1]`, ascending: group g has the rows offsets[g] .. offsets[g + 1] - 1, any number of them; rows of `out` that no group has are left as
              they were
-    source: int32 `[m]`, or None: row r is `lhs[source[r]]`, lhs then having any number of rows, less than 2 GiB of them; zeros where source[r] is none of them
+    source: int32 `[m]`, or None: row r is `lhs[source[r]]`, lhs then having any number of rows, less than 2 GiB of them; `out[r]` is zeros where source[r] is none of them
     Requires n % 8 == 0 and k % 8 == 0; up to 1024 groups.
     """
     _m_grouped(RAGGED_NT, torch.bfloat16, lhs, rhs, out, offsets, source)
@@ -159,7 +159,8 @@ def k_grouped_gemm_bf16_bf16_fp32_tn_ragged(lhs: torch.Tensor, rhs: torch.Tensor
 
     lhs: bf16 `[rows, m]`, the gradients of the outputs; rhs: bf16 `[rows, n]`, the inputs; out: fp32 `[num_groups, m, n]`, written in place; all contiguous
     offsets: as for `m_grouped_gemm_bf16_bf16_bf16_nt_ragged`, of the rows; a group without rows is zero, or unchanged with `accumulate`
-    source: int32 `[rows]`, or None: the input of row r is `rhs[source[r]]`, rhs then having any number of rows, less than 2 GiB of them; zeros where source[r] is none of them
+    source: int32 `[rows]`, or None: the input of row r is `rhs[source[r]]`, rhs then having any number of rows, less than 2 GiB of them; a row whose source[r] is none of them
+            counts for nothing, whatever lhs[r] holds
     Requires m % 8 == 0 and n % 8 == 0; up to 1024 groups.
     """
     _k_grouped(torch.bfloat16, lhs, rhs, out, offsets, accumulate, source)
