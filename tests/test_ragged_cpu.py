@@ -195,6 +195,32 @@ int main() {
     assert subprocess.run([str(exe)], input='\n'.join(cases), text=True).returncode == 0
 
 
+def test_every_kernel_is_some_calls(tmp_path):
+    """The kernel of a product follows from its sizes: each is chosen for some, one that a product does not have for none, and groups without rows or depth have one too."""
+    source, exe = tmp_path / 'plan.cpp', tmp_path / 'plan'
+    source.write_text("""
+#include "gemm/grouped16.hpp"
+#include <cstdio>
+int main() {
+    for (int groups : {1, 4, 16, 64, 1024})
+        for (int each : {0, 1, 16, 17, 79, 80, 160, 192, 500, 100000})
+            for (int n : {8, 512, 1024, 2048, 7168, (1 << 21) - 8})
+                for (int k : {0, 8, 512, 7168}) {
+                    const int rows = int(std::min(536870911ll, (long long)each * groups));
+                    std::printf("NT %d %d\\n", k == 0, int(yan::grouped16_plan<yan::Grouped::NT>(groups, rows, rows, n, k, 256)));
+                    if (k) std::printf("TN %d %d\\n", 0, int(yan::grouped16_plan<yan::Grouped::TN>(groups, rows, k, n, 0, 256)));
+                }
+}
+""")
+    subprocess.check_call([get_hipcc_compiler()[0], '-x', 'hip', '--cuda-host-only', '-std=c++20', '-O1', '-w', f'-I{get_jit_include_dir()}', str(source), '-o', str(exe)])
+    chosen = {}
+    for line in subprocess.run([str(exe)], capture_output=True, text=True, check=True).stdout.split('\n')[:-1]:
+        mode, shallow, kernel = line.split()
+        chosen.setdefault(f'{mode} {shallow}', set()).add(int(kernel))
+    # kGroupedTall, kGrouped128, kGrouped64, kGrouped32
+    assert chosen == {'NT 0': {1, 2, 3, 4}, 'NT 1': {2, 3, 4}, 'TN 0': {1, 2, 3}}
+
+
 class _Notes:
     """Stands in for the device and for the native module: launches report success, and what is noted of them is kept."""
 

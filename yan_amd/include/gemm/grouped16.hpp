@@ -991,6 +991,31 @@ grouped16_tall_kernel(GroupedProblem p) {
 
 enum Grouped16Kernel { kGroupedAny, kGroupedTall, kGrouped128, kGrouped64, kGrouped32 };
 
+// The kernel for a product: by the rows of a group on average, and by how many tiles of a kind there are at most for the chip's compute units. Fitted to every kernel's time
+// over 4 to 256 groups of 2 to 640 rows, (n, k) of 1024 x 512, 2048 x 2048, 4096 x 7168 and 7168 x 2048, bf16, on 256 compute units; over these the choice is 1.4 % (NT, NN)
+// and 0.5 % (TN) behind the best of the kernels in the mean, and 25 % at worst (16 groups of 24 rows, 7168 x 2048: 113, with 32 x 128 tiles 91). Microseconds, NT unless it says TN:
+//   256 x 256 tiles: one workgroup a compute unit, so the tiles have to number nearly as many. 16 groups of 81 rows, 4096 x 7168: 178 with them, 259 with 128 x 128. 64 groups of 88 rows,
+//       2048 x 2048: 130 | 141. Long groups earn them with fewer tiles: 4 of 496 rows, 4096 x 7168 (176 tiles): 127 | 181. Not so 4 of 522 rows, 1024 x 512 (48 tiles): 16.7 | 10.0.
+//       TN: 16 groups of 113 rows, 4096 x 7168 (7168 tiles): 368 | 394, 64 of 190, 1024 x 512 (512 tiles): 34 | 42, but 4 of 116, 7168 x 2048 (896 tiles): 64 | 52: few rows make a tile's
+//       stores most of its work, and two workgroups a compute unit overlap one's with the other's loads.
+//   32 x 128 tiles: up to 16 rows a group, few of which pass 32 then: 256 groups of 1 row, 1024 x 512: 47.6 with them, 62.4 with 64 x 64. 16 groups of 23 rows, 2048 x 2048: 30.1 | 23.0.
+//   64 x 64 tiles for as long as they come to about one round of two workgroups a compute unit: 4 groups of 26 rows, 4096 x 7168 (320 tiles): 37.5 with them, 74 with 128 x 128. 4 of 207
+//       rows, 2048 x 2048 (544): 16.6 | 25.4. 16 of 122 rows, 1024 x 512 (624): 12.2 | 10.1. 64 of 63 rows, 7168 x 2048 (14112): 488 | 356. TN, 4 groups, 1024 x 512 (512): 11.5 | 14.6.
+template <Grouped MODE>
+inline Grouped16Kernel grouped16_plan(int groups, int rows, int m, int n, int k, int cus) {
+    const int each = rows / groups;
+    const auto tiles = [&](int block_m, int block_n) {
+        return (MODE == Grouped::TN ? (long long)groups * ceil_div(m, block_m) : (long long)most_row_tiles(rows, groups, block_m)) * ceil_div(n, block_n);
+    };
+    if (MODE == Grouped::TN) {
+        if ((each >= 80 && tiles(256, 256) >= cus * 6ll) || (each >= 160 && tiles(256, 256) * 4 >= cus * 5ll)) return kGroupedTall;
+        return tiles(128, 128) * 4 >= cus * 3ll ? kGrouped128 : kGrouped64;
+    }
+    if (k != 0 && ((each >= 80 && tiles(256, 256) * 8 >= cus * 7ll) || (each >= 192 && tiles(256, 256) * 8 >= cus * 5ll))) return kGroupedTall;
+    if (each <= 16) return kGrouped32;
+    return tiles(64, 64) * 3 >= cus * 7ll ? kGrouped128 : kGrouped64;
+}
+
 // Rows that offsets speak of, and columns of a matrix: less than so many, so that tiles and ranges stay within 32-bit offsets.
 constexpr int kGroupedMostRows = 1 << 29, kGroupedMostColumns = 1 << 21;
 
@@ -1016,13 +1041,7 @@ inline hipError_t launch_grouped16(const void* lhs, const void* rhs, void* out, 
         hipLaunchKernelGGL(kernel, dim3(uint32_t(capped ? capped_grid(most, num_sms, device_cu_count()) : most)), dim3(256), 0, stream, p, int(slots));
         return hipGetLastError();
     };
-    Grouped16Kernel which = KERNEL;
-    if (which == kGroupedAny) {
-        const long long each = rows / groups;
-        if (each >= 128 && (MODE == Grouped::TN || k != 0) && slots_of(256, 256) >= 64) which = kGroupedTall;
-        else if (MODE != Grouped::TN && each <= 24) which = kGrouped32;
-        else which = slots_of(128, 128) >= device_cu_count() ? kGrouped128 : kGrouped64;
-    }
+    const Grouped16Kernel which = KERNEL != kGroupedAny ? KERNEL : grouped16_plan<MODE>(groups, rows, m, n, k, device_cu_count());
     switch (which) {
         case kGroupedTall: {
             if (MODE != Grouped::TN && k == 0) return hipErrorInvalidValue;
