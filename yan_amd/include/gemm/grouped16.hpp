@@ -220,7 +220,9 @@ __device__ __forceinline__ void static_for(F&& f) {
     [&]<int... I>(std::integer_sequence<int, I...>) __attribute__((always_inline)) { (f(std::integral_constant<int, I>{}), ...); }(std::make_integer_sequence<int, N>{});
 }
 
-// Tiles of 128 x 128 and less: 4 waves, a ring of STAGES k-tiles, one tile a workgroup, or a walk under a cap. Two workgroups or more a compute unit hide each other's waits.
+// Tiles of 128 x 128 and less: 4 waves, a ring of STAGES k-tiles, one tile a workgroup, or a walk under a cap. Two workgroups a compute unit hide each other's waits.
+// For few rows a group, where the weights' bytes bound the product (or those of their gradients): 32 experts of 8 rows, 4096 x 7168, bf16 (1.88 GB): 300 us, 6.3 TB/s. Gradients
+// added to 32 experts of 2048 x 1024 for 62 rows each (549 MB): 90 us, 6.1 TB/s.
 template <typename Elem, Grouped MODE, int BLOCK_M, int BLOCK_N, int STAGES, bool GATHER>
 __global__ void __launch_bounds__(256, 2)
 grouped16_kernel(GroupedProblem p, int slots) {
@@ -490,6 +492,9 @@ struct RowRuns {
 //   * lane offsets of the copies are worked out anew for tiles that are not whole (rows that stand in for those that do not exist) and for gathered rows;
 //   * descriptors of turned operands move on with the k-tile, so that ranges may be of any length;
 //   * any number of k-tiles, one for instance: the copies' place in the walk is its own.
+// Bound by the MFMAs for long groups: 16384 rows of one group x 4096 x 4096 1535 TFLOP/s (dense_gemm_body_4w 1554), NN 1430, TN 1519; of 16 equal groups 1390. Ragged ones lose what
+// their last tiles hold too little and the last round of tiles leaves idle: 32768 rows of 64 experts x 2048 x 7168, gathered: 870 us, 1105. TN writes fp32: of 16 experts x 4096 x 7168
+// (1.88 GB) 6144 rows take 540 us, 250 of MFMAs and the stores behind them.
 struct GroupedTile {
     int slot, group, m0, rows, n0, cols, k0, depth;         // depth 0: none
     __device__ __forceinline__ int count() const { return ceil_div(depth, kDepth); }
@@ -525,6 +530,11 @@ grouped16_tall_kernel(GroupedProblem p) {
         row_tiles = count_row_tiles<BLOCK>(p, lane, &with_rows);
     }
     const int band = MODE == Grouped::TN ? tiles_m : with_rows ? row_tiles / with_rows : 1;
+    // A last round of tiles for at most half of the workgroups is dealt out in halves of 128 rows, two slots a tile on one XCD (4 groups of 285 rows, 4096 x 7168, 96 tiles 126 -> 78 us;
+    // 16 of 364, 7168 x 4096 back, 868 tiles 368 -> 356).
+    const int slots = XcdTileScheduler<>(row_tiles, p.n, 1, BLOCK).grid_size(), last_round = slots % int(gridDim.x);
+    const bool halves = MODE != Grouped::TN && 2 * last_round <= int(gridDim.x) && last_round % kNumXCD == 0;
+    const int whole_slots = halves ? slots - last_round : slots, all_slots = halves ? slots + last_round : slots;
     auto tile_at = [&](int slot) __attribute__((always_inline)) {
         // (worked out anew for every tile: a dozen scalar registers less over the k-loop, which has none to spare)
         int rows_anew = row_tiles;
@@ -533,7 +543,8 @@ grouped16_tall_kernel(GroupedProblem p) {
         sched.fit_bands_to_groups(band);
         // Patches of 32 tiles are dealt out to the XCDs: tiles at a group's end take less time than others, groups of TN differ in their depth, and a range of tiles for each XCD would
         // leave some with more work than others (32768 rows of 64 experts x 2048 x 7168 916 -> 886 us, 6144 of 16 x 7168 x 4096 back 401 -> 381).
-        const TileCoord c = sched.dealt_band_tile_of(slot);
+        const int behind = slot - whole_slots, of_tile = MODE == Grouped::TN || behind < 0 ? slot : whole_slots + behind / (2 * kNumXCD) * kNumXCD + behind % kNumXCD;
+        const TileCoord c = sched.dealt_band_tile_of(of_tile);
         GroupedTile t{slot, -1, 0, 0, 0, 0, 0, 0};
         if (!c.valid) return t;
         t.n0 = c.n_idx * BLOCK, t.cols = min(BLOCK, p.n - t.n0);
@@ -544,18 +555,18 @@ grouped16_tall_kernel(GroupedProblem p) {
             t.depth = hi - t.k0;
         } else {
             const RowTile r = runs.find(p, c.m_idx, lane);
-            t.group = r.group, t.m0 = r.row0, t.rows = r.rows, t.depth = p.k;
+            const int from = behind >= 0 && behind / kNumXCD % 2 ? BLOCK / 2 : 0;
+            t.group = r.group, t.m0 = r.row0 + from, t.rows = min(behind < 0 ? BLOCK : BLOCK / 2, r.rows - from), t.depth = t.rows > 0 ? p.k : 0;
         }
         return t;
     };
-    const int slots = XcdTileScheduler<>(row_tiles, p.n, 1, BLOCK).grid_size();
     // the next tile of this workgroup's walk, from `slot` on
     auto seek = [&](int slot) __attribute__((always_inline)) {
-        for (; slot < slots; slot += gridDim.x) {
+        for (; slot < all_slots; slot += gridDim.x) {
             const GroupedTile t = tile_at(slot);
             if (t.depth > 0) return t;
         }
-        return GroupedTile{slots, -1, 0, 0, 0, 0, 0, 0};
+        return GroupedTile{all_slots, -1, 0, 0, 0, 0, 0, 0};
     };
     // the tiles of groups without rows
     if (MODE == Grouped::TN && !p.accumulate)
@@ -992,10 +1003,10 @@ grouped16_tall_kernel(GroupedProblem p) {
 enum Grouped16Kernel { kGroupedAny, kGroupedTall, kGrouped128, kGrouped64, kGrouped32 };
 
 // The kernel for a product: by the rows of a group on average, and by how many tiles of a kind there are at most for the chip's compute units. Fitted to every kernel's time
-// over 4 to 256 groups of 2 to 640 rows, (n, k) of 1024 x 512, 2048 x 2048, 4096 x 7168 and 7168 x 2048, bf16, on 256 compute units; over these the choice is 1.4 % (NT, NN)
-// and 0.5 % (TN) behind the best of the kernels in the mean, and 25 % at worst (16 groups of 24 rows, 7168 x 2048: 113, with 32 x 128 tiles 91). Microseconds, NT unless it says TN:
+// over 4 to 256 groups of 2 to 640 rows, (n, k) of 1024 x 512, 2048 x 2048, 4096 x 7168 and 7168 x 2048, bf16, on 256 compute units; over these the choice is 1.6 % (NT, NN)
+// and 0.5 % (TN) behind the best of the kernels in the mean, and 26 % at worst (16 groups of 24 rows, 7168 x 2048: 113, with 32 x 128 tiles 89). Microseconds, NT unless it says TN:
 //   256 x 256 tiles: one workgroup a compute unit, so the tiles have to number nearly as many. 16 groups of 81 rows, 4096 x 7168: 178 with them, 259 with 128 x 128. 64 groups of 88 rows,
-//       2048 x 2048: 130 | 141. Long groups earn them with fewer tiles: 4 of 496 rows, 4096 x 7168 (176 tiles): 127 | 181. Not so 4 of 522 rows, 1024 x 512 (48 tiles): 16.7 | 10.0.
+//       2048 x 2048: 130 | 141. Long groups earn them with fewer tiles: 4 of 496 rows, 4096 x 7168 (176 tiles): 128 | 180. Not so 4 of 522 rows, 1024 x 512 (48 tiles): 13.0 | 9.9.
 //       TN: 16 groups of 113 rows, 4096 x 7168 (7168 tiles): 368 | 394, 64 of 190, 1024 x 512 (512 tiles): 34 | 42, but 4 of 116, 7168 x 2048 (896 tiles): 64 | 52: few rows make a tile's
 //       stores most of its work, and two workgroups a compute unit overlap one's with the other's loads.
 //   32 x 128 tiles: up to 16 rows a group, few of which pass 32 then: 256 groups of 1 row, 1024 x 512: 47.6 with them, 62.4 with 64 x 64. 16 groups of 23 rows, 2048 x 2048: 30.1 | 23.0.
@@ -1048,7 +1059,7 @@ inline hipError_t launch_grouped16(const void* lhs, const void* rhs, void* out, 
             const int cus = capped ? capped_grid(device_cu_count(), num_sms, device_cu_count()) : device_cu_count() / kNumXCD * kNumXCD;
             const long long slots = MODE == Grouped::TN ? ceil_div<long long>((long long)groups * ceil_div(m, 256) * ceil_div(n, 256), kNumXCD) * kNumXCD : slots_of(256, 256);
             if (slots >= 1ll << 30) return hipErrorInvalidValue;
-            hipLaunchKernelGGL((grouped16_tall_kernel<Elem, MODE, GATHER>), dim3(uint32_t(std::min<long long>(cus, slots))), dim3(256), 0, stream, p);
+            hipLaunchKernelGGL((grouped16_tall_kernel<Elem, MODE, GATHER>), dim3(uint32_t(std::min<long long>(cus, MODE == Grouped::TN ? slots : 2 * slots))), dim3(256), 0, stream, p);
             return hipGetLastError();
         }
         case kGrouped32:

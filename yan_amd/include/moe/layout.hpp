@@ -6,7 +6,8 @@
 //
 // A thread a pair, 1024 pairs a workgroup. Lanes of a wave with one expert find each other by a ballot a bit of its number; the waves' counts meet in LDS. What
 // the pairs in front of the workgroup's add is counted by the workgroup itself for few pairs (one launch), read from a table of the chunks' histograms for more,
-// whose columns every workgroup adds up (two), or from that table scanned (three).
+// whose columns every workgroup adds up (two), or from that table scanned (three). The experts' starts are scanned by a thread an expert.
+// Few bytes: bound by launches, and by the latency of what is in them (256 experts, eight picks: 64 tokens 3.5 us, 1024 5.5, 16384 9.6, 65536 13.9).
 #pragma once
 
 #include "dispatch.hpp"
@@ -32,14 +33,15 @@ __global__ void __launch_bounds__(kLayoutChunk)
 moe_layout_kernel(const int* __restrict__ indices, const int* __restrict__ table, int* __restrict__ rows, int* __restrict__ source, int* __restrict__ offsets,
                   int pairs, int top_k, int experts, int chunks) {
     constexpr int WAVES = kLayoutChunk / kWaveSize;
-    __shared__ int counts[kMaxExperts], before[kMaxExperts], starts[kMaxExperts + 1];
+    static_assert(kMaxExperts <= kLayoutChunk);         // a thread an expert
+    __shared__ int counts[kMaxExperts], before[kMaxExperts], of_block[WAVES];
     __shared__ uint16_t of_wave[WAVES][kMaxExperts];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, chunk = blockIdx.x;
     const long long first = (long long)chunk * kLayoutChunk;
     const int p = int(min(first + tid, (long long)pairs)), e = p < pairs ? indices[p] : -1;
     const bool real = uint32_t(e) < uint32_t(experts);
-    for (int x = tid; x < experts; x += kLayoutChunk) counts[x] = before[x] = 0;
-    for (int x = tid; x < WAVES * kMaxExperts / 2; x += kLayoutChunk) reinterpret_cast<uint32_t*>(of_wave)[x] = 0;
+    if (tid < experts) counts[tid] = before[tid] = 0;
+    for (int x = lane; x < experts; x += kWaveSize) of_wave[wave][x] = 0;
     __syncthreads();
     if constexpr (COUNTS == LayoutCounts::Pairs) {
         for (int q = tid; q < pairs; q += kLayoutChunk) {
@@ -63,9 +65,9 @@ moe_layout_kernel(const int* __restrict__ indices, const int* __restrict__ table
             atomicAdd(&before[x], above);
         }
     } else {
-        for (int x = tid; x < experts; x += kLayoutChunk) {
-            counts[x] = table[size_t(chunks) * experts + x];
-            before[x] = table[size_t(chunk) * experts + x];
+        if (tid < experts) {
+            counts[tid] = table[size_t(chunks) * experts + tid];
+            before[tid] = table[size_t(chunk) * experts + tid];
         }
     }
     // the lanes of this wave with this lane's expert
@@ -74,36 +76,50 @@ moe_layout_kernel(const int* __restrict__ indices, const int* __restrict__ table
         const unsigned long long set = __ballot((e >> bit) & 1);
         same &= (e >> bit) & 1 ? set : ~set;
     }
-    int rank = __popcll(same & ((1ull << lane) - 1));
+    const int rank = __popcll(same & ((1ull << lane) - 1));
     if (real && rank == 0) of_wave[wave][e] = uint16_t(__popcll(same));
     __syncthreads();
-    if (wave == 0) {
-        int sum_before = 0;
-        for (int x0 = 0; x0 < experts; x0 += 64) {
-            const int x = x0 + lane, size = x < experts ? counts[x] : 0;
-            int sum = size;
+    // thread x: pairs of the experts before x, those of its wave's 64 first, and of x itself in the waves in front
+    const int size = tid < experts ? counts[tid] : 0;
+    int start = size;
 #pragma unroll
-            for (int d = 1; d < 64; d *= 2) {
-                const int below = __shfl_up(sum, d, 64);
-                if (lane >= d) sum += below;
-            }
-            if (x < experts) starts[x] = sum_before + sum - size;
-            sum_before += __shfl(sum, 63, 64);
+    for (int d = 1; d < 64; d *= 2) {
+        const int below = __shfl_up(start, d, 64);
+        if (lane >= d) start += below;
+    }
+    if (lane == 63) of_block[wave] = start;
+    start -= size;
+    if (tid < experts) {
+        int in_front = 0;
+#pragma unroll
+        for (int w = 0; w < WAVES; ++w) {
+            const int here = of_wave[w][tid];
+            of_wave[w][tid] = uint16_t(in_front);
+            in_front += here;
         }
-        if (lane == 0) starts[experts] = sum_before;
+    }
+    __syncthreads();
+    int total = 0;
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) {
+        const int here = of_block[w];
+        start += w < wave ? here : 0;
+        total += here;
+    }
+    if (tid < experts) before[tid] += start;
+    if (chunk == 0) {
+        if (tid < experts) offsets[tid] = start;
+        if (tid == 0) offsets[experts] = total;
     }
     __syncthreads();
     if (real) {
-        for (int w = 0; w < wave; ++w) rank += of_wave[w][e];
-        const int row = starts[e] + before[e] + rank;
+        const int row = before[e] + of_wave[wave][e] + rank;
         rows[p] = row;
         source[row] = p / top_k;
     } else if (p < pairs) {
         rows[p] = -1;
     }
-    if (p < pairs && p >= starts[experts]) source[p] = -1;
-    if (chunk == 0)
-        for (int x = tid; x <= experts; x += kLayoutChunk) offsets[x] = starts[x];
+    if (p < pairs && p >= total) source[p] = -1;
 }
 
 // indices [pairs / top_k, top_k], rows likewise, source [pairs], offsets [experts + 1].

