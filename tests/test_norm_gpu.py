@@ -217,3 +217,22 @@ def test_norm_in_a_graph_and_on_another_stream():
         for a, b in zip((*got, residual, grad_weight), want):
             assert torch.equal(a.view(torch.uint8) if a.dtype == torch.float8_e4m3fn else a, b.view(torch.uint8) if b.dtype == torch.float8_e4m3fn else b)
         x.mul_(1)               # eager work between the replays
+
+
+@pytest.mark.parametrize('rows,k', [(1, 128), (5, 1024), (37, 7168), (3, 16384)])
+def test_norm_of_one_tensor_in_two_places(rows, k):
+    """The rows are their own residual, and a gradient its own residual's: as of two tensors that hold the same."""
+    g = torch.Generator(device='cuda').manual_seed(rows * 31 + k)
+    x, w = torch.randn(rows, k, generator=g, device='cuda').bfloat16(), torch.rand(k, generator=g, device='cuda')
+    twin, residual = x.clone(), x.clone()
+    want = yan.rms_norm_to_fp8(x.clone(), w, 1e-6, residual)
+    got = yan.rms_norm_to_fp8(twin, w, 1e-6, twin)
+    assert torch.equal(twin, residual) and all(torch.equal(a.view(torch.uint8), b.view(torch.uint8)) for a, b in zip(got, want))
+    out, again = torch.empty_like(x), x.clone()
+    yan.rms_norm(again, w, out, 1e-6, again)
+    want_out, residual = torch.empty_like(x), x.clone()
+    yan.rms_norm(x, w, want_out, 1e-6, residual)
+    assert torch.equal(again, residual) and torch.equal(out, want_out)
+    grad, dw, want_dw = torch.randn(rows, k, generator=g, device='cuda').bfloat16(), torch.zeros(k, device='cuda'), torch.zeros(k, device='cuda')
+    want = yan.rms_norm_backward(grad, residual, w, got[2], want_dw, grad.clone())
+    assert torch.equal(yan.rms_norm_backward(grad, residual, w, got[2], dw, grad), want) and torch.equal(dw, want_dw)

@@ -83,8 +83,12 @@ __device__ __forceinline__ int count_row_tiles(const GroupedProblem& p, int lane
     // (offsets that do not ascend could say more, of which there is no end)
     return min(__builtin_amdgcn_readfirstlane(tiles), most_row_tiles(p.rows, p.groups, BLOCK_M));
 }
+// The group that run `tile` is of: its rows, and the runs of the groups before it.
+struct GroupRuns {
+    int group, lo, hi, before;
+};
 template <int BLOCK_M>
-__device__ __forceinline__ RowTile find_row_tile(const GroupedProblem& p, int tile, int lane) {
+__device__ __forceinline__ GroupRuns find_group(const GroupedProblem& p, int tile, int lane) {
     int before = 0;
     for (int g0 = 0; g0 < p.groups; g0 += kWaveSize) {
         int lo = 0, hi = 0;
@@ -99,13 +103,17 @@ __device__ __forceinline__ RowTile find_row_tile(const GroupedProblem& p, int ti
         const unsigned long long behind = __ballot(before + sum > tile);
         if (behind) {
             const int at = __builtin_ctzll(behind);
-            const int first = before + __builtin_amdgcn_readlane(sum - tiles, at), start = __builtin_amdgcn_readlane(lo, at), end = __builtin_amdgcn_readlane(hi, at);
-            const int row0 = start + (tile - first) * BLOCK_M;
-            return {g0 + at, row0, min(BLOCK_M, end - row0)};
+            return {g0 + at, __builtin_amdgcn_readlane(lo, at), __builtin_amdgcn_readlane(hi, at), before + __builtin_amdgcn_readlane(sum - tiles, at)};
         }
         before += __builtin_amdgcn_readlane(sum, kWaveSize - 1);
     }
-    return {0, 0, 0};
+    return {0, 0, 0, 0};
+}
+template <int BLOCK_M>
+__device__ __forceinline__ RowTile find_row_tile(const GroupedProblem& p, int tile, int lane) {
+    const GroupRuns g = find_group<BLOCK_M>(p, tile, lane);
+    const int row0 = g.lo + (tile - g.before) * BLOCK_M;
+    return {g.group, row0, min(BLOCK_M, g.hi - row0)};
 }
 
 // Bytes, not less than none, that a descriptor of at most 2 GiB may reach. (In halves: the scalar unit does not compare numbers of 64 bits, and a descriptor that is not in
@@ -458,7 +466,7 @@ grouped16_kernel(GroupedProblem p, int slots) {
     }
 }
 
-// The groups' rows cut into runs of BLOCK_M, as count_row_tiles and find_row_tile have them, with the first 64 groups in registers: a walk that looks a tile up among its
+// The groups' rows cut into runs of BLOCK_M, as count_row_tiles and find_group have them, with the first 64 groups in registers: a walk that looks a tile up among its
 // copies does not wait for memory.
 template <int BLOCK_M>
 struct RowRuns {
@@ -473,13 +481,12 @@ struct RowRuns {
             if (lane >= d) upto += below;
         }
     }
-    __device__ __forceinline__ RowTile find(const GroupedProblem& p, int tile, int lane) const {
+    __device__ __forceinline__ GroupRuns find(const GroupedProblem& p, int tile, int lane) const {
         const unsigned long long behind = __ballot(upto > tile);
-        if (!behind) return find_row_tile<BLOCK_M>(p, tile, lane);
+        if (!behind) return find_group<BLOCK_M>(p, tile, lane);
         const int at = __builtin_ctzll(behind);
-        const int start = __builtin_amdgcn_readlane(lo, at), end = __builtin_amdgcn_readlane(hi, at), last = __builtin_amdgcn_readlane(upto, at);
-        const int row0 = start + (tile - (last - ceil_div(end - start, BLOCK_M))) * BLOCK_M;
-        return {at, row0, min(BLOCK_M, end - row0)};
+        const int start = __builtin_amdgcn_readlane(lo, at), end = __builtin_amdgcn_readlane(hi, at);
+        return {at, start, end, __builtin_amdgcn_readlane(upto, at) - ceil_div(end - start, BLOCK_M)};
     }
 };
 
@@ -521,7 +528,7 @@ grouped16_tall_kernel(GroupedProblem p) {
     const int lane = get_lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWaveSize);
     const int wn = wave % 2, wm = wave / 2, g = lane / 16, col = lane % 16;
     RowRuns<BLOCK> runs;
-    int with_rows = 0, row_tiles, tiles_m = 1;
+    int with_rows, row_tiles, tiles_m = 1;
     if constexpr (MODE == Grouped::TN) {
         tiles_m = ceil_div(p.m, BLOCK);
         row_tiles = tiles_m * p.groups;
@@ -529,7 +536,6 @@ grouped16_tall_kernel(GroupedProblem p) {
         runs.init(p, lane);
         row_tiles = count_row_tiles<BLOCK>(p, lane, &with_rows);
     }
-    const int band = MODE == Grouped::TN ? tiles_m : with_rows ? row_tiles / with_rows : 1;
     // A last round of tiles for at most half of the workgroups is dealt out in halves of 128 rows, two slots a tile on one XCD (4 groups of 285 rows, 4096 x 7168, 96 tiles 126 -> 78 us;
     // 16 of 364, 7168 x 4096 back, 868 tiles 368 -> 356).
     const int slots = XcdTileScheduler<>(row_tiles, p.n, 1, BLOCK).grid_size(), last_round = slots % int(gridDim.x);
@@ -540,24 +546,32 @@ grouped16_tall_kernel(GroupedProblem p) {
         int rows_anew = row_tiles;
         asm volatile("" : "+s"(rows_anew));
         XcdTileScheduler<> sched(rows_anew, p.n, 1, BLOCK);
-        sched.fit_bands_to_groups(band);
+        if constexpr (MODE == Grouped::TN) sched.fit_bands_to_groups(tiles_m);
         // Patches of 32 tiles are dealt out to the XCDs: tiles at a group's end take less time than others, groups of TN differ in their depth, and a range of tiles for each XCD would
         // leave some with more work than others (32768 rows of 64 experts x 2048 x 7168 916 -> 886 us, 6144 of 16 x 7168 x 4096 back 401 -> 381).
         const int behind = slot - whole_slots, of_tile = MODE == Grouped::TN || behind < 0 ? slot : whole_slots + behind / (2 * kNumXCD) * kNumXCD + behind % kNumXCD;
-        const TileCoord c = sched.dealt_band_tile_of(of_tile);
         GroupedTile t{slot, -1, 0, 0, 0, 0, 0, 0};
-        if (!c.valid) return t;
-        t.n0 = c.n_idx * BLOCK, t.cols = min(BLOCK, p.n - t.n0);
         if constexpr (MODE == Grouped::TN) {
+            const TileCoord c = sched.dealt_band_tile_of(of_tile);
+            if (!c.valid) return t;
+            t.n0 = c.n_idx * BLOCK;
             t.group = c.m_idx / tiles_m, t.m0 = (c.m_idx - t.group * tiles_m) * BLOCK, t.rows = min(BLOCK, p.m - t.m0);
             int hi;
             grouped_range(p, t.group, t.k0, hi);
             t.depth = hi - t.k0;
         } else {
-            const RowTile r = runs.find(p, c.m_idx, lane);
-            const int from = behind >= 0 && behind / kNumXCD % 2 ? BLOCK / 2 : 0;
-            t.group = r.group, t.m0 = r.row0 + from, t.rows = min(behind < 0 ? BLOCK : BLOCK / 2, r.rows - from), t.depth = t.rows > 0 ? p.k : 0;
+            // A group's tiles follow each other, column by column of up to eight rows: its weights are read by one XCD or, column for column, by two. Bands of rows that
+            // do not end where groups do read most of them twice (16 experts x 7168 x 4096 back, 3967 rows 278 -> 265 us, 6144 rows 380 -> 374; forward, 64 experts x 2048 x 7168, the same).
+            constexpr int BAND = 8;
+            const int position = sched.dealt_position(of_tile), tiles_n = sched.tiles_n;
+            if (position < 0) return t;
+            const GroupRuns g = runs.find(p, position / tiles_n, lane);
+            const int in_group = position - g.before * tiles_n, band = in_group / (BAND * tiles_n), in_band = in_group - band * BAND * tiles_n;
+            const int height = min(BAND, ceil_div(g.hi - g.lo, BLOCK) - band * BAND), column = in_band / height;
+            const int from = g.lo + (band * BAND + in_band - column * height) * BLOCK + (behind >= 0 && behind / kNumXCD % 2 ? BLOCK / 2 : 0);
+            t.n0 = column * BLOCK, t.group = g.group, t.m0 = from, t.rows = min(behind < 0 ? BLOCK : BLOCK / 2, g.hi - from), t.depth = t.rows > 0 ? p.k : 0;
         }
+        t.cols = min(BLOCK, p.n - t.n0);
         return t;
     };
     // the next tile of this workgroup's walk, from `slot` on
