@@ -63,9 +63,12 @@ def norm_lanes(rows: int, k: int) -> Tuple[int, int]:
 
 
 def norm_backward_lanes(k: int) -> Tuple[int, int]:
-    """The same of its gradient's, where a lane has two rows and the weight's sums in its registers."""
+    """
+    The same of its gradient's, where a lane has two rows (up to 256 lanes) and the weight's sums in its registers. Wider rows one at a time on 1024 lanes (8192 x 16384
+    200 us; two of them on 512 lanes do not fit the registers: 317).
+    """
     runs = ceil_div(k, 8)
-    for lanes in (16, 64, 256, 512):
+    for lanes in (16, 64, 256, 1024):
         if runs <= lanes * (2 if lanes == 16 else 4):
             break
     each = ceil_div(runs, lanes)
@@ -75,7 +78,7 @@ def norm_backward_lanes(k: int) -> Tuple[int, int]:
 def norm_backward_workgroups(rows: int, k: int) -> int:
     """
     Workgroups of the gradient's kernel, each of which leaves its sums of the weight's gradient, to be added up behind it: one a compute unit where the rows that it has
-    in flight are enough to keep it busy (us with 256 and with 512: 8192 x 7168 92.7, 97.4; 1023 x 7168 16.4, 20.6; 8192 x 16384 313, 322; 32768 x 1024, four rows at a
+    in flight are enough to keep it busy (us with 256 and with 512: 8192 x 7168 92.7, 97.4; 1023 x 7168 16.4, 20.6; 8192 x 16384 200, 207; 32768 x 1024, four rows at a
     time, 45.7, 49.8), two where they are not (4096 x 2112 19.7, 16.4).
     """
     lanes, _ = norm_backward_lanes(k)
