@@ -123,7 +123,7 @@ def test_norm_kernels_hold_every_row():
             lanes, runs = norm.norm_lanes(rows, k)
             assert lanes * runs * 8 >= k and lanes in (16, 64, 256, 1024) and runs in (1, 2, 4, 8)
             lanes, runs = norm.norm_backward_lanes(k)
-            assert lanes * runs * 8 >= k and lanes in (16, 64, 256, 512) and runs in (1, 2, 4)
+            assert lanes * runs * 8 >= k and lanes in (16, 64, 256, 1024) and runs in (1, 2, 4) and lanes * runs <= 2048
             assert 1 <= norm.norm_backward_workgroups(rows, k) <= 512
 
 
@@ -160,6 +160,12 @@ def test_generated_code_of_the_ragged_products(tmp_path, mode, gather):
     for block in loops:
         between = block[block.index('v_mfma'):block.rindex('v_mfma')]
         assert 'scratch_' not in between and 'vmcnt(0)' not in between and 'v_readfirstlane' not in between
+
+
+@pytest.mark.parametrize('h,k', [(BF16, 8192), (BF16, 16384), (torch.float32, 16384)])
+def test_norm_gradient_stays_in_registers(tmp_path, h, k):
+    text = _asm(tmp_path, norm.includes, norm.norm_backward_kernel_plan(BF16, h, BF16, *norm.norm_backward_lanes(k), True, True))
+    assert 'rms_norm_backward_kernel' in text and 'scratch_' not in text and not re.search(r'private_segment_fixed_size: *[1-9]', text)
 
 
 @pytest.mark.parametrize('what', ['products', 'norm', 'layout'])
