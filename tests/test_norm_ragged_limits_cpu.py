@@ -1,0 +1,35 @@
+"""Edges of the norm, the ragged layout and the ragged products that a host can look at: ranges of descriptors, numbers near the ends of their types, refusals."""
+import subprocess
+
+from yan_amd.jit.compiler import get_hipcc_compiler, get_jit_include_dir
+
+
+def _host(tmp_path, body, lines=''):
+    """What a program of the kernels' headers, built for the host, says to `lines`."""
+    source, exe = tmp_path / 'host.cpp', tmp_path / 'host'
+    source.write_text(body)
+    subprocess.check_call([get_hipcc_compiler()[0], '-x', 'hip', '--cuda-host-only', '-std=c++20', '-O1', '-w', f'-I{get_jit_include_dir()}', str(source), '-o', str(exe)])
+    return subprocess.run([str(exe)], input=lines, capture_output=True, text=True, check=True).stdout.split('\n')[:-1]
+
+
+# rows, columns of gathered operands of less than 2 GiB by less than a row or by less than the descriptors' bias
+NEARLY_2_GIB = [(508400, 2112), (2097151, 512), (1048575, 1024), ((1 << 27) - 1, 8), (2064888, 520), (699050, 1536), (262143, 4096)]
+
+
+def test_large_tiles_reach_the_end_of_gathered_operands(tmp_path):
+    """The descriptors of the large tiles start early: what they reach ends where the operand does, for every size that is accepted."""
+    out = _host(tmp_path, """
+#include "gemm/grouped16.hpp"
+#include <cstdio>
+int main() {
+    long long bytes;
+    while (std::scanf("%lld", &bytes) == 1) std::printf("%u\\n", yan::biased_reach(bytes));
+    std::printf("%u\\n", yan::kCopyBias);
+}
+""", '\n'.join(str(2 * rows * columns) for rows, columns in NEARLY_2_GIB + [(1, 8), (1 << 20, 256)]))
+    bias = int(out[-1])
+    assert bias > 0
+    for (rows, columns), reached in zip(NEARLY_2_GIB + [(1, 8), (1 << 20, 256)], out):
+        assert 2 * rows * columns < 1 << 31 and int(reached) == 2 * rows * columns + bias
+        # the farthest byte that a copy asks for, behind a k-tile of the last row, is a number of 32 bits
+        assert 2 * rows * columns + bias + 128 < 1 << 32

@@ -1,0 +1,60 @@
+"""The norm, the ragged layout and the ragged products at the ends of their ranges, on the GPU."""
+import pytest
+import torch
+
+import yan_amd as yan
+from yan_amd.jit_kernels import ragged
+
+pytestmark = pytest.mark.gpu
+BF16 = torch.bfloat16
+
+
+def _gen(seed):
+    return torch.Generator(device='cuda').manual_seed(seed)
+
+
+def _whole(g, *shape, dtype=BF16, top=3):
+    """Whole numbers: products of a few thousand of them are summed without rounding, whatever the order."""
+    return torch.randint(-top, top + 1, shape, generator=g, device='cuda').to(dtype)
+
+
+def _nearly_2_gib(g, tokens, columns):
+    """Tokens of zeros but for the first two and the last eight, and 2048 picks of those."""
+    x = torch.zeros(tokens, columns, dtype=BF16, device='cuda')
+    x[:2], x[-8:] = _whole(g, 2, columns), _whole(g, 8, columns)
+    picks = torch.randint(-8, 2, (2048, ), generator=g, device='cuda')
+    return x, torch.where(picks < 0, picks + tokens, picks).int()
+
+
+@pytest.mark.parametrize('kernel', ['kGroupedAny', 'kGroupedTall', 'kGrouped128'])
+@pytest.mark.parametrize('tokens,k', [(508400, 2112), (2097151, 512), (1048575, 1024), ((1 << 27) - 1, 8)])
+def test_rows_gathered_from_the_end_of_2_gib(tokens, k, kernel):
+    g = _gen(k)
+    x, source = _nearly_2_gib(g, tokens, k)
+    n, offsets = 4608, torch.tensor([0, 1000, 2048], dtype=torch.int32, device='cuda')        # two long groups: large tiles by the rule as well
+    weights = _whole(g, 2, n, k)
+    out = torch.full((2048, n), 7.0, dtype=BF16, device='cuda')
+    if kernel == 'kGroupedAny':
+        yan.m_grouped_gemm_bf16_bf16_bf16_nt_ragged(x, weights, out, offsets, source)
+    else:
+        ragged._m_grouped(ragged.RAGGED_NT, BF16, x, weights, out, offsets, source, (kernel, ))
+    taken = x[source.long()].double()
+    for group, at in enumerate((slice(0, 1000), slice(1000, 2048))):
+        assert torch.equal(out[at], (taken[at] @ weights[group].double().t().contiguous()).bfloat16())
+
+
+@pytest.mark.parametrize('kernel', ['kGroupedAny', 'kGroupedTall', 'kGrouped128'])
+@pytest.mark.parametrize('tokens,n', [(2064888, 520), (2097151, 512), ((1 << 27) - 1, 8)])
+def test_weight_gradients_gathered_from_the_end_of_2_gib(tokens, n, kernel):
+    g = _gen(n + 1)
+    x, source = _nearly_2_gib(g, tokens, n)
+    m, offsets = 1 << 15, torch.tensor([0, 1000, 2048], dtype=torch.int32, device='cuda')     # (m: as many tiles as the rule wants for large ones)
+    grads = _whole(g, 2048, m)
+    out = torch.full((2, m, n), 7.0, device='cuda')
+    if kernel == 'kGroupedAny':
+        yan.k_grouped_gemm_bf16_bf16_fp32_tn_ragged(grads, x, out, offsets, False, source)
+    else:
+        ragged._k_grouped(BF16, grads, x, out, offsets, False, source, (kernel, ))
+    taken = x[source.long()].double()
+    for group, at in enumerate((slice(0, 1000), slice(1000, 2048))):
+        assert torch.equal(out[group].double(), grads[at].double().t().contiguous() @ taken[at])

@@ -118,10 +118,13 @@ __device__ __forceinline__ RowTile find_row_tile(const GroupedProblem& p, int ti
 
 // Bytes, not less than none, that a descriptor of at most 2 GiB may reach. (In halves: the scalar unit does not compare numbers of 64 bits, and a descriptor that is not in
 // scalar registers is taken there lane by lane, in front of every copy.)
-__device__ __forceinline__ uint32_t reach(long long bytes) {
+__host__ __device__ __forceinline__ uint32_t reach(long long bytes) {
     const uint32_t upper = uint32_t((unsigned long long)bytes >> 32), lower = uint32_t(bytes);
     return upper != 0 || lower > kOutOfRange ? kOutOfRange : lower;
 }
+// The same of a descriptor that starts kCopyBias bytes early, as the large tiles' do: the bias comes on top, so that `bytes` of up to 2 GiB are reached to the last one.
+constexpr uint32_t kCopyBias = 3 * 1024;
+__host__ __device__ __forceinline__ uint32_t biased_reach(long long bytes) { return reach(bytes) + kCopyBias; }
 
 // Copies of a plain operand's k-tiles, DIM rows of 128 bytes: instruction j of wave w has rows 8 (4 j + w) .. + 7.
 template <int DIM>
@@ -597,9 +600,8 @@ grouped16_tall_kernel(GroupedProblem p) {
 
     // Four consecutive passes of a wave's copies share one LDS base (M0) and differ in the instruction's immediate offset, which the hardware adds on the LDS side and on
     // the global side alike: the lane offsets take it back out, and the descriptors start kCopyBias bytes early so that no lane offset goes below zero.
-    constexpr uint32_t kCopyBias = 3 * 1024;
     const uint32_t ld_a = uint32_t(MODE == Grouped::TN ? p.m : p.k) * 2, ld_b = uint32_t(MODE == Grouped::NT ? p.k : p.n) * 2;
-    auto describe = [&](const uint8_t* base, long long bytes) __attribute__((always_inline)) { return make_rsrc(base - kCopyBias, reach(bytes + kCopyBias)); };
+    auto describe = [&](const uint8_t* base, long long bytes) __attribute__((always_inline)) { return make_rsrc(base - kCopyBias, biased_reach(bytes)); };
     // A plain operand's pass r of wave w has rows 128 (r / 4) + 32 w + 8 (r % 4) .. + 7, a turned one's k 16 w + 2 r and the one behind. `l`: the lane, out of which all of
     // this is worked out anew where it is needed, since the registers are.
     auto plain_row = [&](int l, int r) __attribute__((always_inline)) { return 128 * (r / 4) + 32 * wave + 8 * (r % 4) + (l >> 3); };
