@@ -33,3 +33,25 @@ int main() {
         assert 2 * rows * columns < 1 << 31 and int(reached) == 2 * rows * columns + bias
         # the farthest byte that a copy asks for, behind a k-tile of the last row, is a number of 32 bits
         assert 2 * rows * columns + bias + 128 < 1 << 32
+
+
+def test_copies_of_turned_weights_have_rows(tmp_path):
+    """Large tiles copy whole k-tiles of [k, n] weights unless the operand ends inside: two rows an instruction, one of which at least has to exist, for any depth and group."""
+    cases = [(groups, k) for groups in (1, 2, 3, 7, 8, 9, 64, 1024) for k in [*range(8, 200, 8), 1544, (1 << 21) - 8]]
+    out = _host(tmp_path, """
+#include "gemm/grouped16.hpp"
+#include <cstdio>
+int main() {
+    int left, k;
+    while (std::scanf("%d %d", &left, &k) == 2) std::printf("%d\\n", int(yan::weights_end_inside(left, k)));
+}
+""", '\n'.join(f'{groups - group} {k}' for groups, k in cases for group in range(groups)))
+    answers = iter(out)
+    for groups, k in cases:
+        whole = -(-k // 64) * 64
+        for group in range(groups):
+            inside = next(answers) == '1'
+            assert inside == (group * k + whole > groups * k), (groups, group, k)
+            # (otherwise the last k-tile's rows behind the contraction stand for its last row)
+            if not inside:
+                assert all(group * k + row < groups * k for row in range(whole - 64, whole)), (groups, group, k)

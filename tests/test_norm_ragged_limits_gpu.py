@@ -58,3 +58,22 @@ def test_weight_gradients_gathered_from_the_end_of_2_gib(tokens, n, kernel):
     taken = x[source.long()].double()
     for group, at in enumerate((slice(0, 1000), slice(1000, 2048))):
         assert torch.equal(out[group].double(), grads[at].double().t().contiguous() @ taken[at])
+
+
+@pytest.mark.parametrize('groups', [1, 2, 3, 9])
+def test_shallow_products_on_large_tiles(groups):
+    """Depths of a few rows, where a k-tile of one group's weights reaches over several groups behind it, and the last of them end inside; what lies behind the operands is NaN."""
+    g = _gen(groups)
+    rows = [(140, 0, 1, 300, 64)[i % 5] for i in range(groups)]
+    offsets = torch.tensor([0] + rows, device='cuda').cumsum(0).int()
+    m, n, ends = sum(rows), 264, [0, *offsets.tolist()[1:]]
+    for k in (8, 16, 24, 32, 40, 48, 56, 64, 72, 120):
+        flat = torch.full((groups * k * n + 64 * n, ), float('nan'), dtype=BF16, device='cuda')
+        weights = flat[:groups * k * n].view(groups, k, n)
+        weights.copy_(_whole(g, groups, k, n))
+        lhs = _whole(g, m, k)
+        want = torch.cat([lhs[ends[i]:ends[i + 1]].double() @ weights[i].double() for i in range(groups)]).bfloat16()
+        for kernel in ('kGroupedTall', 'kGrouped128'):
+            out = torch.full((m, n), 7.0, dtype=BF16, device='cuda')
+            ragged._m_grouped(ragged.RAGGED_NN, BF16, lhs, weights, out, offsets, None, (kernel, ))
+            assert torch.equal(out, want), (k, kernel)

@@ -126,6 +126,10 @@ __host__ __device__ __forceinline__ uint32_t reach(long long bytes) {
 constexpr uint32_t kCopyBias = 3 * 1024;
 __host__ __device__ __forceinline__ uint32_t biased_reach(long long bytes) { return reach(bytes) + kCopyBias; }
 
+// Whether whole k-tiles of a turned operand of `k` rows, with `left` such operands up to the last one, go beyond the end of that: of the last one itself where k is no whole number of
+// them, and of some before it where k is a few rows. (Eight operands have at least as many rows as the k-tiles of the first, k being a multiple of 8; more would pass 32 bits.)
+__host__ __device__ __forceinline__ bool weights_end_inside(int left, int k) { return (left < 8 ? left : 8) * k < ceil_div(k, kDepth) * kDepth; }
+
 // Copies of a plain operand's k-tiles, DIM rows of 128 bytes: instruction j of wave w has rows 8 (4 j + w) .. + 7.
 template <int DIM>
 struct PlainCopies {
@@ -633,7 +637,7 @@ grouped16_tall_kernel(GroupedProblem p) {
     auto here_of = [&](const GroupedTile& t, int kt) __attribute__((always_inline)) { return min(kDepth, t.depth - kt * kDepth); };
     // The lane offsets, of turned operands for k-tiles of which `here` of k are copied. They are the same for all tiles that are whole, and so is what they were last worked out for.
     // What is copied of k behind the contraction's end is made zeros later; it only has to exist, and so it does, as the next row's or as rows of another group, but at the end of a
-    // turned operand: there the last k-tile (`tail_aims`) has its last row instead. Of a plain operand's last row that is out of the descriptor's range, for some lanes of a copy.
+    // turned operand: there the last k-tile (`tail_aims`) has its own last row instead. Of a plain operand's last row that is out of the descriptor's range, for some lanes of a copy.
     bool aimed_whole = false, tail_aims = false;
     auto aim_lanes = [&](int here) __attribute__((always_inline)) {
         const GroupedTile& t = ahead;
@@ -676,7 +680,7 @@ grouped16_tall_kernel(GroupedProblem p) {
         else if constexpr (TURN_B) from_b = rhs + size_t(t.k0) * ld_b + t.n0 * 2;
         else rsrc_b = describe(rhs + size_t(t.n0) * ld_b, (long long)t.cols * ld_b);
         describe_turned();
-        tail_aims = t.depth % kDepth != 0 && (MODE == Grouped::TN ? t.k0 + t.count() * kDepth > p.rows : MODE == Grouped::NN && t.group == p.groups - 1);
+        tail_aims = t.depth % kDepth != 0 && (MODE == Grouped::TN ? t.k0 + t.count() * kDepth > p.rows : MODE == Grouped::NN && weights_end_inside(p.groups - t.group, p.k));
         aim_lanes(tail_aims ? here_of(t, 0) : kDepth);
     };
     // Behind the walk's last k-tile that one is copied again, two times, into units that nobody reads any more: the count of copies under way stays what the waits below take it for.
