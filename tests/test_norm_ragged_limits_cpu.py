@@ -55,3 +55,26 @@ int main() {
             # (otherwise the last k-tile's rows behind the contraction stand for its last row)
             if not inside:
                 assert all(group * k + row < groups * k for row in range(whole - 64, whole)), (groups, group, k)
+
+
+def test_rows_of_the_norm_up_to_31_bits(tmp_path):
+    """Every row is some group of lanes' and a group without one has the last, up to as many rows as there are numbers for."""
+    out = _host(tmp_path, """
+#include "norm/rms_norm.hpp"
+#include <cstdio>
+template <int ROWS> int check(int rows) {
+    const int blocks = yan::norm_blocks<ROWS>(rows);
+    if (blocks != int(((long long)rows + ROWS - 1) / ROWS)) return 1;
+    for (int b : {0, blocks / 2, blocks - 1})
+        for (int g = 0; g < ROWS; ++g) {
+            const long long row = (long long)b * ROWS + g;
+            if (yan::norm_row_exists<ROWS>(b, g, rows) != (row < rows) || yan::norm_row<ROWS>(b, g, rows) != int(row < rows ? row : rows - 1)) return 2;
+        }
+    return 0;
+}
+int main() {
+    int rows;
+    while (std::scanf("%d", &rows) == 1) std::printf("%d %d %d\\n", check<1>(rows), check<4>(rows), check<16>(rows));
+}
+""", '\n'.join(str(r) for r in [*range(1, 40), 1 << 28, (1 << 31) - 17, (1 << 31) - 16, (1 << 31) - 15, (1 << 31) - 4, (1 << 31) - 2, (1 << 31) - 1]))
+    assert len(out) == 46 and all(line == '0 0 0' for line in out)

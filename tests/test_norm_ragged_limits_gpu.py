@@ -77,3 +77,23 @@ def test_shallow_products_on_large_tiles(groups):
             out = torch.full((m, n), 7.0, dtype=BF16, device='cuda')
             ragged._m_grouped(ragged.RAGGED_NN, BF16, lhs, weights, out, offsets, None, (kernel, ))
             assert torch.equal(out, want), (k, kernel)
+
+
+def test_norm_gradient_of_as_many_rows_as_there_are_numbers_for():
+    """2^31 - 1 rows, one tensor for the gradient and the rows: dh = r (g - h r mean(g h r)) is 3/8 for ones and 0 for twos where r is 1/2, and the weight's sums follow."""
+    torch.cuda.empty_cache()
+    if torch.cuda.mem_get_info()[0] < 100 << 30:
+        pytest.skip('wants 78 GB of memory')
+    rows, twos = (1 << 31) - 1, 40
+    h = torch.ones(rows, 8, dtype=BF16, device='cuda')
+    h[-twos:] = 2
+    inverse, grad_weight = torch.full((rows, ), 0.5, device='cuda'), torch.empty(8, device='cuda')
+    got = yan.rms_norm_backward(h, h, torch.ones(8, device='cuda'), inverse, grad_weight)
+    assert bool((got[-twos:] == 0).all())
+    for first in range(0, rows - twos, 1 << 28):
+        assert bool((got[first:min(first + (1 << 28), rows - twos)] == 0.375).all())
+    # a part's sums of halves are exact; 8192 parts, 32 sums of every 32nd and those added up
+    total = 0.5 * (rows - twos) + 2 * twos
+    assert bool(((grad_weight.double() - total).abs() <= (256 + 32) * 2.0 ** -24 * total).all())
+    del h, inverse, got
+    torch.cuda.empty_cache()

@@ -89,6 +89,14 @@ __device__ __forceinline__ int norm_block_of(int bid, int blocks) {
     return bid % kNumXCD * per_xcd + bid / kNumXCD;
 }
 
+// Rows are taken ROWS at a time, by groups of lanes: how many times that is, whether row `group` of number `block` exists, and which it is, the last one where it does not. (No number here
+// passes the last row's, which may be the largest of 31 bits.)
+template <int ROWS> __host__ __device__ __forceinline__ int norm_blocks(int rows) { return rows / ROWS + (rows % ROWS != 0); }
+template <int ROWS> __host__ __device__ __forceinline__ bool norm_row_exists(int block, int group, int rows) { return group < rows - block * ROWS; }
+template <int ROWS> __host__ __device__ __forceinline__ int norm_row(int block, int group, int rows) {
+    return norm_row_exists<ROWS>(block, group, rows) ? block * ROWS + group : rows - 1;
+}
+
 // residual (RESIDUAL) is h's place too; codes and scales if CODES, normed if NORMED. `out` may be x.
 template <typename X, typename H, typename W, int LANES, int V, bool RESIDUAL, bool CODES, bool NORMED>
 __global__ void __launch_bounds__(LANES > 256 ? LANES : 256)
@@ -96,11 +104,11 @@ rms_norm_kernel(const X* x, H* residual, const W* __restrict__ weight, uint8_t* 
                 float* __restrict__ inverse_rms, NormShape s) {
     constexpr int THREADS = LANES > 256 ? LANES : 256, ROWS = THREADS / LANES;
     __shared__ float slots[LANES > 64 ? LANES / kWaveSize : 1];
-    const int lane = threadIdx.x % LANES, blocks = ceil_div(s.rows, ROWS), block = norm_block_of(blockIdx.x, blocks);
+    const int lane = threadIdx.x % LANES, blocks = norm_blocks<ROWS>(s.rows), block = norm_block_of(blockIdx.x, blocks);
     if (block >= blocks) return;
     // (rows behind the last one are read and reduced in its place, since all lanes of a wave have to take part, and not stored)
-    const int row = min(block * ROWS + int(threadIdx.x) / LANES, s.rows - 1);
-    const bool live = block * ROWS + int(threadIdx.x) / LANES < s.rows;
+    const int row = norm_row<ROWS>(block, threadIdx.x / LANES, s.rows);
+    const bool live = norm_row_exists<ROWS>(block, threadIdx.x / LANES, s.rows);
     const size_t at = size_t(row) * s.k;
     F32x8 h[V];
     Raw8<X> raw[V];
@@ -171,7 +179,7 @@ rms_norm_backward_kernel(const G* __restrict__ grad, const H* __restrict__ h, co
                          const G* __restrict__ grad_residual, G* __restrict__ grad_h, float* __restrict__ partial, int rows, int k) {
     constexpr int THREADS = LANES > 256 ? LANES : 256, ROWS = THREADS / LANES, WAVES = LANES > 64 ? LANES / kWaveSize : 1;
     __shared__ float slots[2][WAVES];
-    const int lane = threadIdx.x % LANES, group = threadIdx.x / LANES, blocks = ceil_div(rows, ROWS);
+    const int lane = threadIdx.x % LANES, group = threadIdx.x / LANES, blocks = norm_blocks<ROWS>(rows);
     Raw8<W> w[V];
     F32x8 sums[WEIGHT ? V : 1];
 #pragma unroll
@@ -187,7 +195,7 @@ rms_norm_backward_kernel(const G* __restrict__ grad, const H* __restrict__ h, co
         float inverse;
     };
     const auto load = [&](Row& r, int block) __attribute__((always_inline)) {
-        const int row = min(block * ROWS + group, rows - 1);
+        const int row = norm_row<ROWS>(block, group, rows);
         const size_t at = size_t(row) * k;
         r.inverse = inverse_rms[row];
 #pragma unroll
@@ -204,9 +212,8 @@ rms_norm_backward_kernel(const G* __restrict__ grad, const H* __restrict__ h, co
         }
     };
     const auto step = [&](Row& r, int block, int turn) __attribute__((always_inline)) {
-        const int row = block * ROWS + group;
-        const size_t at = size_t(min(row, rows - 1)) * k;
-        const bool live = row < rows;
+        const size_t at = size_t(norm_row<ROWS>(block, group, rows)) * k;
+        const bool live = norm_row_exists<ROWS>(block, group, rows);
         float dot = 0.f;
 #pragma unroll
         for (int v = 0; v < V; ++v) {
