@@ -1,6 +1,10 @@
 """Edges of the norm, the ragged layout and the ragged products that a host can look at: ranges of descriptors, numbers near the ends of their types, refusals."""
 import subprocess
 
+import pytest
+import torch
+
+import yan_amd as yan
 from yan_amd.jit.compiler import get_hipcc_compiler, get_jit_include_dir
 
 
@@ -78,3 +82,22 @@ int main() {
 }
 """, '\n'.join(str(r) for r in [*range(1, 40), 1 << 28, (1 << 31) - 17, (1 << 31) - 16, (1 << 31) - 15, (1 << 31) - 4, (1 << 31) - 2, (1 << 31) - 1]))
     assert len(out) == 46 and all(line == '0 0 0' for line in out)
+
+
+def test_norm_refuses_any_part_of_its_residual_for_its_output():
+    """Views of the residual, and tensors that only share some bytes with it, are no place for the normed rows: these would take the sums' place, which the next layer and the gradient read."""
+    memory, w = torch.zeros(12, 256, dtype=torch.bfloat16), torch.ones(256)
+    residual, x = memory[4:8], torch.zeros(4, 256, dtype=torch.bfloat16)
+    wide = torch.zeros(4, 256)                      # fp32: its first and its last half as 16 bits
+    inside = [(residual, out) for out in (residual.view(4, 256), residual[:], memory[4:8], memory[1:5], memory[7:11])]
+    inside += [(wide, wide.view(torch.bfloat16).view(8, 256)[at:at + 4]) for at in (0, 2, 4)]
+    for r, out in inside:
+        with pytest.raises(AssertionError, match='a place of their own'):
+            yan.rms_norm(x, w, out, 1e-6, r)
+        with pytest.raises(AssertionError, match='a place of their own'):
+            yan.rms_norm_to_fp8(x, w, 1e-6, r, False, out)
+    # neighbours are places of their own, and so are rows of none: refused for not being on a device at most
+    for r, out in ((residual, memory[:4]), (residual, memory[8:]), (memory[4:4], memory[4:4])):
+        with pytest.raises((AssertionError, RuntimeError)) as refusal:
+            yan.rms_norm(x[:r.size(0)], w, out, 1e-6, r)
+        assert 'a place of their own' not in str(refusal.value)

@@ -97,3 +97,18 @@ def test_norm_gradient_of_as_many_rows_as_there_are_numbers_for():
     assert bool(((grad_weight.double() - total).abs() <= (256 + 32) * 2.0 ** -24 * total).all())
     del h, inverse, got
     torch.cuda.empty_cache()
+
+
+def test_norm_refuses_views_of_its_residual_also_after_calls_that_it_took():
+    x, residual, out = (torch.ones(4, 256, dtype=BF16, device='cuda') for _ in range(3))
+    w = torch.ones(256, device='cuda')
+    for _ in range(2):
+        yan.rms_norm(x, w, out, 1e-6, residual)
+        yan.rms_norm_to_fp8(x, w, 1e-6, residual, False, out)
+    before = residual.clone()
+    for _ in range(2):
+        with pytest.raises(AssertionError, match='a place of their own'):
+            yan.rms_norm(x, w, residual.view(4, 256), 1e-6, residual)
+        with pytest.raises(AssertionError, match='a place of their own'):
+            yan.rms_norm_to_fp8(x, w, 1e-6, residual, False, residual[:])
+    assert torch.equal(residual, before)

@@ -113,6 +113,12 @@ def _check(x, weight, *others):
         assert t is None or (t.shape == x.shape and t.dtype in _ELEMENTS and t.is_contiguous())
 
 
+def _apart(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether two contiguous tensors share no byte, whatever they are views of (tensors without memory have address 0)."""
+    at, other = a.data_ptr(), b.data_ptr()
+    return at + a.nbytes <= other or other + b.nbytes <= at or not at
+
+
 def _run(plan, args):
     name, keys, arg_defs, code = plan
     runtime = jit_tuner.compile_and_tune(name=name, keys=keys, space=(), includes=includes, arg_defs=arg_defs, template=code, args=args)
@@ -152,13 +158,13 @@ def rms_norm_to_fp8(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, re
 
     x: bf16 or fp32 `[m, k]`, contiguous, k % 128 == 0, k up to 16384; weight: bf16 or fp32 `[k]`
     residual: bf16 or fp32 `[m, k]` (of x's type or not), or None: becomes `x + residual`, which is what is normed
-    normed: bf16 `[m, k]`, or None: gets the normed rows in 16 bits as well (for a router); may be x, not the residual
+    normed: bf16 `[m, k]`, or None: gets the normed rows in 16 bits as well (for a router); may be x itself, no part of the residual
     Returns e4m3fn `[m, k]` and fp32 scales `[m, k/128]`, as `per_token_cast_to_fp8` makes them of the normed rows in fp32 (with `col_major_scales`
     token-contiguous), and fp32 `[m]`, the reciprocals of the root mean squares, for the gradient. Squares are summed in fp32.
     """
     # (no part of what a repeated call is found by)
     assert eps >= 0
-    assert normed is None or normed is not residual, 'the normed rows have a place of their own'
+    assert normed is None or residual is None or (normed is not residual and _apart(normed, residual)), 'the normed rows have a place of their own'
     call = (NORM, x, weight, residual, normed, float(eps), 2 if col_major_scales else 1)
     made = repeat_new(*call)
     if made is not None:
@@ -168,11 +174,11 @@ def rms_norm_to_fp8(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, re
 
 def rms_norm(x: torch.Tensor, weight: torch.Tensor, out: torch.Tensor, eps: float = 1e-6, residual: Optional[torch.Tensor] = None) -> torch.Tensor:
     """
-    The normed rows in 16 bits: out bf16 `[m, k]`, written in place (may be x, not the residual), k % 8 == 0; the rest as for `rms_norm_to_fp8`. Returns the reciprocals of the root mean
+    The normed rows in 16 bits: out bf16 `[m, k]`, written in place (may be x itself, no part of the residual), k % 8 == 0; the rest as for `rms_norm_to_fp8`. Returns the reciprocals of the root mean
     squares, fp32 `[m]`.
     """
     assert eps >= 0
-    assert out is not None and out is not residual, 'the normed rows have a place of their own'
+    assert out is not None and (residual is None or (out is not residual and _apart(out, residual))), 'the normed rows have a place of their own'
     call = (NORM, x, weight, residual, out, float(eps), 0)
     made = repeat_new(*call)
     if made is not None:
