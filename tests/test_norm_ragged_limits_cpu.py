@@ -6,6 +6,7 @@ import torch
 
 import yan_amd as yan
 from yan_amd.jit.compiler import get_hipcc_compiler, get_jit_include_dir
+from yan_amd.jit_kernels import ragged
 
 
 def _host(tmp_path, body, lines=''):
@@ -101,3 +102,17 @@ def test_norm_refuses_any_part_of_its_residual_for_its_output():
         with pytest.raises((AssertionError, RuntimeError)) as refusal:
             yan.rms_norm(x[:r.size(0)], w, out, 1e-6, r)
         assert 'a place of their own' not in str(refusal.value)
+
+
+def test_types_of_the_ragged_entries_are_part_of_what_calls_are_found_by(monkeypatch):
+    """A call that was served once is found by what it was given: the bf16 and the fp16 entry with the same tensors are two calls."""
+    asked = []
+    monkeypatch.setattr(ragged, 'repeat_call', lambda *call: asked.append(call) or True)
+    lhs, weights, out, offsets = torch.zeros(6, 16, dtype=torch.bfloat16), torch.zeros(2, 16, 16, dtype=torch.bfloat16), torch.zeros(6, 16, dtype=torch.bfloat16), torch.zeros(3, dtype=torch.int32)
+    for one, other in ((yan.m_grouped_gemm_bf16_bf16_bf16_nt_ragged, yan.m_grouped_gemm_fp16_fp16_fp16_nt_ragged),
+                       (yan.m_grouped_gemm_bf16_bf16_bf16_nn_ragged, yan.m_grouped_gemm_fp16_fp16_fp16_nn_ragged),
+                       (yan.k_grouped_gemm_bf16_bf16_fp32_tn_ragged, yan.k_grouped_gemm_fp16_fp16_fp32_tn_ragged)):
+        one(lhs, weights, out, offsets)
+        other(lhs, weights, out, offsets)
+        first, second = ([part for part in call if not isinstance(part, torch.Tensor)] for call in asked[-2:])
+        assert first != second

@@ -112,3 +112,22 @@ def test_norm_refuses_views_of_its_residual_also_after_calls_that_it_took():
         with pytest.raises(AssertionError, match='a place of their own'):
             yan.rms_norm_to_fp8(x, w, 1e-6, residual, False, residual[:])
     assert torch.equal(residual, before)
+
+
+def test_entries_of_one_type_refuse_the_others_tensors_after_calls_of_the_other():
+    g = _gen(3)
+    offsets, source = torch.tensor([0, 5, 12], dtype=torch.int32, device='cuda'), torch.arange(12, dtype=torch.int32, device='cuda')
+    pairs = {BF16: (yan.m_grouped_gemm_bf16_bf16_bf16_nt_ragged, yan.m_grouped_gemm_bf16_bf16_bf16_nn_ragged, yan.k_grouped_gemm_bf16_bf16_fp32_tn_ragged),
+             torch.half: (yan.m_grouped_gemm_fp16_fp16_fp16_nt_ragged, yan.m_grouped_gemm_fp16_fp16_fp16_nn_ragged, yan.k_grouped_gemm_fp16_fp16_fp32_tn_ragged)}
+    for dtype, other in ((BF16, torch.half), (torch.half, BF16)):
+        lhs, weights, grad = _whole(g, 12, 64, dtype=dtype), _whole(g, 2, 64, 64, dtype=dtype), torch.zeros(2, 64, 64, device='cuda')
+        out = torch.zeros(12, 64, dtype=dtype, device='cuda')
+        calls = [lambda f: f[0](lhs, weights, out, offsets), lambda f: f[0](lhs, weights, out, offsets, source), lambda f: f[1](lhs, weights, out, offsets),
+                 lambda f: f[2](lhs, out, grad, offsets), lambda f: f[2](lhs, out, grad, offsets, True, source)]
+        for call in calls:
+            call(pairs[dtype])
+            call(pairs[dtype])
+            before = out.clone(), grad.clone()
+            with pytest.raises(AssertionError):
+                call(pairs[other])
+            assert torch.equal(out, before[0]) and torch.equal(grad, before[1])

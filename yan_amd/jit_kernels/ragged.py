@@ -75,7 +75,8 @@ def _launch(call, dtype, mode, lhs, rhs, out, offsets, source, groups, rows, m, 
 
 
 def _m_grouped(entry, dtype, lhs, rhs, out, offsets, source, kernel=()):
-    call = (entry, lhs, rhs, out, offsets, source)
+    # (the entry's type is part of what a repeated call is found by: one entry's tensors are not the other's)
+    call = (entry, lhs, rhs, out, offsets, source, 1 if dtype == torch.half else 0)
     if kernel == () and repeat_call(*call):
         return
     assert lhs.dim() == 2 and rhs.dim() == 3 and out.dim() == 2
@@ -95,7 +96,7 @@ def _m_grouped(entry, dtype, lhs, rhs, out, offsets, source, kernel=()):
 
 
 def _k_grouped(dtype, lhs, rhs, out, offsets, accumulate, source, kernel=()):
-    call = (RAGGED_TN, lhs, rhs, out, offsets, source, 1 if accumulate else 0)
+    call = (RAGGED_TN, lhs, rhs, out, offsets, source, 1 if accumulate else 0, 1 if dtype == torch.half else 0)
     if kernel == () and repeat_call(*call):
         return
     assert lhs.dim() == 2 and rhs.dim() == 2 and out.dim() == 3
