@@ -779,6 +779,8 @@ NORM_CALLS = [('bf16', 'bf16', 'bf16', True, False), ('bf16', None, 'bf16', True
               ('fp32', None, 'bf16', False, True), ('fp32', 'fp32', 'bf16', True, False)]
 # gradient's type, h's, the weight's, with a residual's gradient, with the weight's
 NORM_BACKWARD_CALLS = [('bf16', 'bf16', 'bf16', True, True), ('fp32', 'bf16', 'fp32', False, True), ('bf16', 'fp32', 'bf16', False, False), ('fp32', 'fp32', 'fp32', True, True)]
+# rows, k, with codes or 16 bits: of the norm, more rows than a launch has threads for (bf16, fp32 weights)
+NORM_LONG = [((1 << 28) + 37, 8, False), ((1 << 26) + 5, 264, False), ((1 << 24) + 3, 2176, True)]
 NORM_TYPES = {'bf16': torch.bfloat16, 'fp32': torch.float32}
 
 
@@ -794,6 +796,11 @@ def norm_plans():
         for g, h, w, residual, weight in NORM_BACKWARD_CALLS:
             name, keys, arg_defs, code = norm.norm_backward_kernel_plan(NORM_TYPES[g], NORM_TYPES[h], NORM_TYPES[w], *norm.norm_backward_lanes(k), residual, weight)
             plans.append((name, keys, arg_defs, norm.includes, code))
+    for rows, k, codes in NORM_LONG:
+        name, keys, arg_defs, code = norm.norm_kernel_plan(torch.bfloat16, torch.bfloat16, torch.float32, *norm.norm_lanes(rows, k), False, codes, not codes)
+        plans.append((name, keys, arg_defs, norm.includes, code))
+    name, keys, arg_defs, code = norm.norm_backward_kernel_plan(torch.bfloat16, torch.bfloat16, torch.float32, *norm.norm_backward_lanes(8), False, True)
+    plans.append((name, keys, arg_defs, norm.includes, code))
     return plans
 
 

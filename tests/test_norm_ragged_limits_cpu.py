@@ -116,3 +116,20 @@ def test_types_of_the_ragged_entries_are_part_of_what_calls_are_found_by(monkeyp
         other(lhs, weights, out, offsets)
         first, second = ([part for part in call if not isinstance(part, torch.Tensor)] for call in asked[-2:])
         assert first != second
+
+
+def test_norm_launches_hold_their_rows(tmp_path):
+    """A launch's workgroups, a whole number for every XCD, have less than 2^32 threads and the rows that it is given."""
+    out = _host(tmp_path, """
+#include "norm/rms_norm.hpp"
+#include <cstdio>
+int main() {
+    for (int lanes : {16, 64, 256, 1024}) {
+        const int threads = lanes > 256 ? lanes : 256, at_a_time = threads / lanes, rows = yan::norm_rows_per_launch(threads, at_a_time);
+        std::printf("%d %d %d\\n", threads, at_a_time, rows);
+    }
+}
+""")
+    assert len(out) == 4
+    for threads, at_a_time, rows in (map(int, line.split()) for line in out):
+        assert rows % (8 * at_a_time) == 0 and (1 << 32) - 16 * threads <= rows // at_a_time * threads < 1 << 32 and rows < 1 << 31

@@ -2,6 +2,7 @@
 import pytest
 import torch
 
+import harness as testing
 import yan_amd as yan
 from yan_amd.jit_kernels import ragged
 
@@ -131,3 +132,31 @@ def test_entries_of_one_type_refuse_the_others_tensors_after_calls_of_the_other(
             with pytest.raises(AssertionError):
                 call(pairs[other])
             assert torch.equal(out, before[0]) and torch.equal(grad, before[1])
+
+
+@pytest.mark.parametrize('rows,k,codes', testing.NORM_LONG)
+def test_norm_of_more_rows_than_a_launch_has_threads(rows, k, codes):
+    """Rows of ones and, in places, of twos whose root mean square is 1 and 2: the normed rows are the weight, and the reciprocals say which is which."""
+    torch.cuda.empty_cache()
+    if torch.cuda.mem_get_info()[0] < 150 << 30:
+        pytest.skip('wants up to 110 GB of memory')
+    x = torch.ones(rows, k, dtype=BF16, device='cuda')
+    places = torch.tensor([0, 17, rows // 2, (1 << 24) - 9, (1 << 24) - 1, (1 << 26) - 1, (1 << 28) - 129, (1 << 28) - 1, 1 << 28, 1 << 26, 1 << 24, rows - 2, rows - 1], device='cuda')
+    places = places[places < rows].unique()
+    x[places] = 2
+    weight = (1 + torch.arange(k, device='cuda') % 3).float()
+    if codes:
+        # (token-contiguous scales: the pieces of a column follow each other. Quotients rounded once: torch divides a tensor by a number as a product with its reciprocal, a rounding more)
+        got, scales, inverse = yan.rms_norm_to_fp8(x, weight, 0.0, col_major_scales=True)
+        assert bool((scales == torch.tensor(3 / 448, device='cuda')).all())
+        want = (weight * torch.tensor(448 / 3, device='cuda')).to(torch.float8_e4m3fn).view(torch.uint8)
+        same = lambda part: bool((got[part].view(torch.uint8) == want).all())
+    else:
+        got = torch.zeros(rows, k, dtype=BF16, device='cuda')
+        inverse = yan.rms_norm(x, weight, got, 0.0)
+        same = lambda part: bool((got[part] == weight.bfloat16()).all())
+    step = (1 << 31) // k
+    assert all(same(slice(first, first + step)) for first in range(0, rows, step))
+    assert bool((inverse[places] == 0.5).all()) and int((inverse == 0.5).sum()) == places.numel() and int((inverse == 1).sum()) == rows - places.numel()
+    del x, got, inverse
+    torch.cuda.empty_cache()

@@ -302,6 +302,9 @@ rms_norm_weight_sum_kernel(const float* __restrict__ partial, float* __restrict_
     }
 }
 
+// Rows of the norm that one launch takes: whole rounds of workgroups over the XCDs.
+constexpr int norm_rows_per_launch(int threads, int rows) { return int(((1ll << 32) / threads - 1) / kNumXCD * kNumXCD * rows); }
+
 // x [rows, k]; residual null where !RESIDUAL; scales [rows, k / 128] with the strides given.
 template <typename X, typename H, typename W, int LANES, int V, bool RESIDUAL, bool CODES, bool NORMED>
 inline hipError_t launch_rms_norm(const X* x, H* residual, const W* weight, void* codes, float* scales, long long stride_m, long long stride_k, void* normed,
@@ -311,11 +314,17 @@ inline hipError_t launch_rms_norm(const X* x, H* residual, const W* weight, void
     if (rows == 0) return hipSuccess;
     if (!x || !weight || !inverse_rms || (RESIDUAL && !residual) || (CODES && (!codes || !scales)) || (NORMED && !normed)) return hipErrorInvalidValue;
     constexpr int THREADS = LANES > 256 ? LANES : 256, ROWS = THREADS / LANES;
-    const long long blocks = ceil_div<long long>(ceil_div<long long>(rows, ROWS), kNumXCD) * kNumXCD;
-    if (blocks * THREADS >= 1ll << 32) return hipErrorInvalidValue;
-    hipLaunchKernelGGL((rms_norm_kernel<X, H, W, LANES, V, RESIDUAL, CODES, NORMED>), dim3(uint32_t(blocks)), dim3(THREADS), 0, stream, x, residual, weight,
-                       static_cast<uint8_t*>(codes), scales, static_cast<__bf16*>(normed), inverse_rms, NormShape{rows, k, eps, stride_m, stride_k});
-    return hipGetLastError();
+    // A launch has less than 2^32 threads; more rows than those have, from 2^24 of 256 lanes and 2^28 of 16 on, are several launches.
+    constexpr int MOST = norm_rows_per_launch(THREADS, ROWS);
+    for (long long first = 0; first < rows; first += MOST) {
+        const int here = int(std::min<long long>(MOST, rows - first));
+        const size_t at = size_t(first) * k;
+        hipLaunchKernelGGL((rms_norm_kernel<X, H, W, LANES, V, RESIDUAL, CODES, NORMED>), dim3(ceil_div(norm_blocks<ROWS>(here), kNumXCD) * kNumXCD), dim3(THREADS), 0, stream,
+                           x + at, RESIDUAL ? residual + at : nullptr, weight, CODES ? static_cast<uint8_t*>(codes) + at : nullptr, CODES ? scales + first * stride_m : nullptr,
+                           NORMED ? static_cast<__bf16*>(normed) + at : nullptr, inverse_rms + first, NormShape{here, k, eps, stride_m, stride_k});
+        if (const hipError_t rc = hipGetLastError(); rc != hipSuccess) return rc;
+    }
+    return hipSuccess;
 }
 
 // `partial`: fp32 [parts, k] of scratch, parts = workgroups * rows at a time, both as rms_norm_backward_workgroups in Python has them.
