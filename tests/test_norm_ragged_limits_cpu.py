@@ -6,7 +6,7 @@ import torch
 
 import yan_amd as yan
 from yan_amd.jit.compiler import get_hipcc_compiler, get_jit_include_dir
-from yan_amd.jit_kernels import ragged
+from yan_amd.jit_kernels import moe, ragged
 
 
 def _host(tmp_path, body, lines=''):
@@ -133,3 +133,28 @@ int main() {
     assert len(out) == 4
     for threads, at_a_time, rows in (map(int, line.split()) for line in out):
         assert rows % (8 * at_a_time) == 0 and (1 << 32) - 16 * threads <= rows // at_a_time * threads < 1 << 32 and rows < 1 << 31
+
+
+def test_layout_asks_for_the_workspace_that_its_launch_wants(tmp_path, monkeypatch):
+    """Of any batch that is documented, the tables of which pass 2 GiB at the end of the range."""
+    asked = []
+    monkeypatch.setattr(moe, 'assert_on_current_device', lambda *_: None)
+    monkeypatch.setattr(moe, 'current_raw_stream', lambda: 0)
+    monkeypatch.setattr(moe, 'remember_new', lambda *_: None)
+    monkeypatch.setattr(moe, '_run', lambda plan, includes, args: asked.append(args) or ('', None, args))
+    cases = [(0, 4, 2), (1024, 8, 256), (1025, 8, 256), (1 << 25, 16, 1024), ((1 << 25) + 3, 16, 1024), (moe.MAX_PAIRS // 16, 16, 1024), (moe.MAX_PAIRS, 1, 7)]
+    for tokens, top_k, experts in cases:
+        yan.moe_ragged_layout(torch.empty(tokens, top_k, dtype=torch.int32, device='meta'), experts)
+    out = _host(tmp_path, """
+#include "moe/layout.hpp"
+#include <cstdio>
+int main() {
+    long long pairs;
+    int experts;
+    while (std::scanf("%lld %d", &pairs, &experts) == 2) std::printf("%d\\n", yan::moe_layout_workspace_numbers(pairs, experts));
+}
+""", '\n'.join(f'{tokens * top_k} {experts}' for tokens, top_k, experts in cases))
+    assert max(map(int, out)) > 1 << 30
+    for args, numbers in zip(asked, map(int, out)):
+        workspace, said = args[4], args[5]
+        assert said == numbers and (numbers == 0 or (workspace.numel() == numbers and workspace.dtype == torch.int32))

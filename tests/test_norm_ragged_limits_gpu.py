@@ -160,3 +160,28 @@ def test_norm_of_more_rows_than_a_launch_has_threads(rows, k, codes):
     assert bool((inverse[places] == 0.5).all()) and int((inverse == 0.5).sum()) == places.numel() and int((inverse == 1).sum()) == rows - places.numel()
     del x, got, inverse
     torch.cuda.empty_cache()
+
+
+def test_layout_with_a_table_of_more_than_2_gib():
+    """2^29 pairs and a few of 1024 experts: pair p asks for expert p mod 1000, and every 1000th for none."""
+    torch.cuda.empty_cache()
+    tokens, top_k, experts, none = (1 << 25) + 3, 16, 1024, 7
+    pairs, step = tokens * top_k, 1 << 26
+    indices = torch.empty(pairs, dtype=torch.int32, device='cuda')
+    for first in range(0, pairs, step):
+        e = torch.arange(first, min(first + step, pairs), dtype=torch.int32, device='cuda') % 1000
+        indices[first:first + step] = torch.where(e == none, -1, e)
+    rows, source, offsets = yan.moe_ragged_layout(indices.view(tokens, top_k), experts)
+    counts = torch.tensor([(pairs - e + 999) // 1000 if e < 1000 and e != none else 0 for e in range(experts)], device='cuda')
+    starts = torch.cat([counts.new_zeros(1), counts.cumsum(0)])
+    assert torch.equal(offsets.long(), starts)
+    total, starts, flat = int(starts[-1]), starts.int(), rows.view(-1)
+    for first in range(0, pairs, step):
+        p = torch.arange(first, min(first + step, pairs), dtype=torch.int32, device='cuda')
+        e, part = p % 1000, flat[first:first + step]
+        assert torch.equal(part, torch.where(e == none, -1, starts[e.long()] + p // 1000))
+        real = e != none
+        assert torch.equal(source[part[real].long()], p[real] // top_k)
+    assert bool((source[total:] == -1).all())
+    del indices, rows, source, flat
+    torch.cuda.empty_cache()

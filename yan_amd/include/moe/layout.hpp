@@ -20,11 +20,12 @@ constexpr int kLayoutSummedChunks = 256;        // up to here it adds up the tab
 
 inline int moe_layout_chunks(long long pairs) { return int(ceil_div<long long>(pairs, kLayoutChunk)); }
 
-// Bytes of workspace a launch wants.
-inline size_t moe_layout_workspace_bytes(long long pairs, int experts) {
+// Numbers of 32 bits of workspace a launch wants: those of the largest layouts pass 2 GiB, but not 31 bits.
+inline int moe_layout_workspace_numbers(long long pairs, int experts) {
     const int chunks = moe_layout_chunks(pairs);
-    return chunks <= kLayoutFewChunks ? 0 : (size_t(chunks) + 1) * experts * 4;
+    return chunks <= kLayoutFewChunks ? 0 : (chunks + 1) * experts;
 }
+static_assert((kMaxPairs / kLayoutChunk + 2) * kMaxExperts < 1ll << 31);
 
 enum class LayoutCounts { Pairs, Table, ScannedTable };
 
@@ -123,18 +124,18 @@ moe_layout_kernel(const int* __restrict__ indices, const int* __restrict__ table
 }
 
 // indices [pairs / top_k, top_k], rows likewise, source [pairs], offsets [experts + 1].
-inline hipError_t launch_moe_layout(const int* indices, int* rows, int* source, int* offsets, void* workspace, long long workspace_bytes, int pairs, int top_k,
+inline hipError_t launch_moe_layout(const int* indices, int* rows, int* source, int* offsets, int* workspace, int workspace_numbers, int pairs, int top_k,
                                     int experts, hipStream_t stream) {
     if (pairs < 0 || pairs > kMaxPairs || top_k < 1 || top_k > kMaxTopK || pairs % top_k != 0 || experts < 1 || experts > kMaxExperts || !offsets) return hipErrorInvalidValue;
     if (pairs && (!indices || !rows || !source)) return hipErrorInvalidValue;
     const int chunks = moe_layout_chunks(pairs), grid = std::max(1, chunks);
-    int* const table = static_cast<int*>(workspace);
+    int* const table = workspace;
     const auto place = [&](auto kernel) {
         hipLaunchKernelGGL(kernel, dim3(grid), dim3(kLayoutChunk), 0, stream, indices, table, rows, source, offsets, pairs, top_k, experts, chunks);
         return hipGetLastError();
     };
     if (chunks <= kLayoutFewChunks) return place(moe_layout_kernel<LayoutCounts::Pairs>);
-    if (!workspace || size_t(workspace_bytes) < moe_layout_workspace_bytes(pairs, experts)) return hipErrorInvalidValue;
+    if (!workspace || workspace_numbers < moe_layout_workspace_numbers(pairs, experts)) return hipErrorInvalidValue;
     hipLaunchKernelGGL(moe_dispatch_count_kernel<0>, dim3(chunks), dim3(256), 0, stream, indices, table, pairs, kLayoutChunk, experts);
     if (const hipError_t rc = hipGetLastError(); rc != hipSuccess) return rc;
     if (chunks <= kLayoutSummedChunks) return place(moe_layout_kernel<LayoutCounts::Table>);

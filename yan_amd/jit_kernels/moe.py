@@ -324,9 +324,9 @@ _layout_includes = ('"moe/layout.hpp"', )
 
 layout_template = """
 using namespace yan;
-__return_code = static_cast<int>(launch_moe_layout(indices, rows, source, offsets, workspace, workspace_bytes, pairs, top_k, experts, stream));
+__return_code = static_cast<int>(launch_moe_layout(indices, rows, source, offsets, workspace, workspace_numbers, pairs, top_k, experts, stream));
 """
-layout_arg_defs = (('indices', torch.int), ('rows', torch.int), ('source', torch.int), ('offsets', torch.int), ('workspace', torch.uint8), ('workspace_bytes', int),
+layout_arg_defs = (('indices', torch.int), ('rows', torch.int), ('source', torch.int), ('offsets', torch.int), ('workspace', torch.int), ('workspace_numbers', int),
                    ('pairs', int), ('top_k', int), ('experts', int), ('stream', torch.cuda.Stream))
 
 
@@ -355,14 +355,13 @@ def moe_ragged_layout(indices: torch.Tensor, num_experts: int) -> Tuple[torch.Te
     rows = torch.empty_like(indices)
     source = torch.empty((pairs, ), dtype=torch.int32, device=device)
     offsets = torch.empty((num_experts + 1, ), dtype=torch.int32, device=device)
-    # moe_layout_workspace_bytes of moe/layout.hpp
+    # moe_layout_workspace_numbers of moe/layout.hpp
     chunks = ceil_div(pairs, LAYOUT_CHUNK)
-    workspace_bytes = 0 if chunks <= LAYOUT_FEW_CHUNKS else (chunks + 1) * num_experts * 4
-    assert workspace_bytes < 1 << 31
-    scratch = torch.empty(workspace_bytes, dtype=torch.uint8, device=device) if workspace_bytes else None
+    numbers = 0 if chunks <= LAYOUT_FEW_CHUNKS else (chunks + 1) * num_experts
+    scratch = torch.empty(numbers, dtype=torch.int32, device=device) if numbers else None
     made = (rows, source, offsets)
     done = _run(layout_kernel_plan(), _layout_includes,
-                (indices, rows, source, offsets, offsets.view(torch.uint8) if scratch is None else scratch, workspace_bytes, pairs, indices.size(1), num_experts,
+                (indices, rows, source, offsets, offsets.view(torch.int32) if scratch is None else scratch, numbers, pairs, indices.size(1), num_experts,
                  current_raw_stream()))
     remember_new(call, *done, made, () if scratch is None else (scratch, ))
     return made
