@@ -1,4 +1,5 @@
 """Edges of the norm, the ragged layout and the ragged products that a host can look at: ranges of descriptors, numbers near the ends of their types, refusals."""
+import random
 import subprocess
 
 import pytest
@@ -158,3 +159,49 @@ int main() {
     for args, numbers in zip(asked, map(int, out)):
         workspace, said = args[4], args[5]
         assert said == numbers and (numbers == 0 or (workspace.numel() == numbers and workspace.dtype == torch.int32))
+
+
+def test_the_walk_of_large_tiles_has_every_output_once(tmp_path):
+    """Slots to tiles of runs of rows and columns, halves of a last round among them: every row of every group meets every column once, whatever the groups, the columns and the
+    workgroups (which group a run is of, a wave's look-up on the device, is a loop here)."""
+    cases, rng = [], random.Random(5)
+    for _ in range(400):
+        groups = rng.choice([1, 2, 5, 16, 70])
+        counts = [rng.choice([0, 1, 127, 128, 129, 256, 257, rng.randint(0, 700), rng.randint(0, 3000) if groups < 16 else 300]) for _ in range(groups)]
+        cases.append((rng.choice([8, 256, 264, 1000, 2048, 4096]), rng.choice([1, 3, 8, 16, 24, 64, 128, 256]), counts))
+    out = _host(tmp_path, """
+#include "gemm/grouped16.hpp"
+#include <cstdio>
+#include <vector>
+int main() {
+    int n, workgroups, groups;
+    while (std::scanf("%d %d %d", &n, &workgroups, &groups) == 3) {
+        std::vector<int> lo(groups + 1), before(groups + 1);
+        for (int g = 0; g < groups; ++g) {
+            int rows;
+            if (std::scanf("%d", &rows) != 1) return 1;
+            lo[g + 1] = lo[g] + rows, before[g + 1] = before[g] + yan::ceil_div(rows, 256);
+        }
+        const yan::XcdTileScheduler<> sched(before[groups], n, 1, 256);
+        const yan::HalvedRound walk(sched.grid_size(), workgroups, true);
+        std::vector<int> seen(size_t(lo[groups]) * sched.tiles_n);
+        int halves = 0, bad = 0;
+        for (int slot = 0; slot < walk.all; ++slot) {
+            const int behind = slot - walk.whole, position = sched.dealt_position(behind < 0 ? slot : walk.tile_behind(behind));
+            if (position < 0) continue;
+            int g = 0;
+            while (before[g + 1] <= position / sched.tiles_n) ++g;
+            const yan::RunOfGroup at(position - before[g] * sched.tiles_n, before[g + 1] - before[g], sched.tiles_n);
+            const int from = lo[g] + at.run * 256 + (walk.is_lower(behind) ? 128 : 0), upto = std::min(from + (behind < 0 ? 256 : 128), lo[g + 1]);
+            halves += behind >= 0;
+            bad += at.column < 0 || at.column >= sched.tiles_n || at.run < 0 || at.run >= before[g + 1] - before[g];
+            for (int r = from; r < upto && !bad; ++r) ++seen[size_t(r) * sched.tiles_n + at.column];
+        }
+        for (const int times : seen) bad += times != 1;
+        std::printf("%d %d\\n", bad, halves);
+    }
+}
+""", '\n'.join(f'{n} {workgroups} {len(counts)} ' + ' '.join(map(str, counts)) for n, workgroups, counts in cases))
+    bad, halves = zip(*(map(int, line.split()) for line in out))
+    assert len(out) == len(cases) and not any(bad)
+    assert any(halves) and not all(halves)

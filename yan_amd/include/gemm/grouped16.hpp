@@ -522,6 +522,32 @@ struct GroupedTile {
     }
 };
 
+// The slots of the large tiles' walk. A last round of tiles for at most half of the workgroups is dealt out in halves of 128 rows, two slots a tile on one XCD (4 groups of 285 rows,
+// 4096 x 7168, 96 tiles 126 -> 78 us; 16 of 364, 7168 x 4096 back, 868 tiles 368 -> 356).
+struct HalvedRound {
+    int whole, all;                 // slots of whole tiles, and all of them
+    __host__ __device__ HalvedRound(int slots, int workgroups, bool may) {
+        const int last_round = slots % workgroups;
+        const bool halves = may && 2 * last_round <= workgroups && last_round % kNumXCD == 0;
+        whole = halves ? slots - last_round : slots, all = halves ? slots + last_round : slots;
+    }
+    // A slot that is `behind` the whole tiles' (not below 0) has a half of the tile of this slot, the lower one or the upper.
+    __host__ __device__ int tile_behind(int behind) const { return whole + behind / (2 * kNumXCD) * kNumXCD + behind % kNumXCD; }
+    __host__ __device__ static bool is_lower(int behind) { return behind >= 0 && behind / kNumXCD % 2; }
+};
+
+// A group's tiles follow each other, column by column of up to eight runs of rows: its weights are read by one XCD or, column for column, by two. Bands of rows that
+// do not end where groups do read most of them twice (16 experts x 7168 x 4096 back, 3967 rows 278 -> 265 us, 6144 rows 380 -> 374; forward, 64 experts x 2048 x 7168, the same).
+struct RunOfGroup {
+    int run, column;
+    __host__ __device__ RunOfGroup(int in_group, int runs, int tiles_n) {
+        constexpr int BAND = 8;
+        const int band = in_group / (BAND * tiles_n), in_band = in_group - band * BAND * tiles_n, left = runs - band * BAND, height = left < BAND ? left : BAND;
+        column = in_band / height;
+        run = band * BAND + in_band - column * height;
+    }
+};
+
 template <typename Elem, Grouped MODE, bool GATHER>
 __global__ void __launch_bounds__(256, 1)
 grouped16_tall_kernel(GroupedProblem p) {
@@ -543,11 +569,8 @@ grouped16_tall_kernel(GroupedProblem p) {
         runs.init(p, lane);
         row_tiles = count_row_tiles<BLOCK>(p, lane, &with_rows);
     }
-    // A last round of tiles for at most half of the workgroups is dealt out in halves of 128 rows, two slots a tile on one XCD (4 groups of 285 rows, 4096 x 7168, 96 tiles 126 -> 78 us;
-    // 16 of 364, 7168 x 4096 back, 868 tiles 368 -> 356).
-    const int slots = XcdTileScheduler<>(row_tiles, p.n, 1, BLOCK).grid_size(), last_round = slots % int(gridDim.x);
-    const bool halves = MODE != Grouped::TN && 2 * last_round <= int(gridDim.x) && last_round % kNumXCD == 0;
-    const int whole_slots = halves ? slots - last_round : slots, all_slots = halves ? slots + last_round : slots;
+    const int slots = XcdTileScheduler<>(row_tiles, p.n, 1, BLOCK).grid_size();
+    const HalvedRound walk(slots, gridDim.x, MODE != Grouped::TN);
     auto tile_at = [&](int slot) __attribute__((always_inline)) {
         // (worked out anew for every tile: a dozen scalar registers less over the k-loop, which has none to spare)
         int rows_anew = row_tiles;
@@ -556,7 +579,7 @@ grouped16_tall_kernel(GroupedProblem p) {
         if constexpr (MODE == Grouped::TN) sched.fit_bands_to_groups(tiles_m);
         // Patches of 32 tiles are dealt out to the XCDs: tiles at a group's end take less time than others, groups of TN differ in their depth, and a range of tiles for each XCD would
         // leave some with more work than others (32768 rows of 64 experts x 2048 x 7168 916 -> 886 us, 6144 of 16 x 7168 x 4096 back 401 -> 381).
-        const int behind = slot - whole_slots, of_tile = MODE == Grouped::TN || behind < 0 ? slot : whole_slots + behind / (2 * kNumXCD) * kNumXCD + behind % kNumXCD;
+        const int behind = slot - walk.whole, of_tile = MODE == Grouped::TN || behind < 0 ? slot : walk.tile_behind(behind);
         GroupedTile t{slot, -1, 0, 0, 0, 0, 0, 0};
         if constexpr (MODE == Grouped::TN) {
             const TileCoord c = sched.dealt_band_tile_of(of_tile);
@@ -567,27 +590,23 @@ grouped16_tall_kernel(GroupedProblem p) {
             grouped_range(p, t.group, t.k0, hi);
             t.depth = hi - t.k0;
         } else {
-            // A group's tiles follow each other, column by column of up to eight rows: its weights are read by one XCD or, column for column, by two. Bands of rows that
-            // do not end where groups do read most of them twice (16 experts x 7168 x 4096 back, 3967 rows 278 -> 265 us, 6144 rows 380 -> 374; forward, 64 experts x 2048 x 7168, the same).
-            constexpr int BAND = 8;
             const int position = sched.dealt_position(of_tile), tiles_n = sched.tiles_n;
             if (position < 0) return t;
             const GroupRuns g = runs.find(p, position / tiles_n, lane);
-            const int in_group = position - g.before * tiles_n, band = in_group / (BAND * tiles_n), in_band = in_group - band * BAND * tiles_n;
-            const int height = min(BAND, ceil_div(g.hi - g.lo, BLOCK) - band * BAND), column = in_band / height;
-            const int from = g.lo + (band * BAND + in_band - column * height) * BLOCK + (behind >= 0 && behind / kNumXCD % 2 ? BLOCK / 2 : 0);
-            t.n0 = column * BLOCK, t.group = g.group, t.m0 = from, t.rows = min(behind < 0 ? BLOCK : BLOCK / 2, g.hi - from), t.depth = t.rows > 0 ? p.k : 0;
+            const RunOfGroup at(position - g.before * tiles_n, ceil_div(g.hi - g.lo, BLOCK), tiles_n);
+            const int from = g.lo + at.run * BLOCK + (walk.is_lower(behind) ? BLOCK / 2 : 0);
+            t.n0 = at.column * BLOCK, t.group = g.group, t.m0 = from, t.rows = min(behind < 0 ? BLOCK : BLOCK / 2, g.hi - from), t.depth = t.rows > 0 ? p.k : 0;
         }
         t.cols = min(BLOCK, p.n - t.n0);
         return t;
     };
     // the next tile of this workgroup's walk, from `slot` on
     auto seek = [&](int slot) __attribute__((always_inline)) {
-        for (; slot < all_slots; slot += gridDim.x) {
+        for (; slot < walk.all; slot += gridDim.x) {
             const GroupedTile t = tile_at(slot);
             if (t.depth > 0) return t;
         }
-        return GroupedTile{all_slots, -1, 0, 0, 0, 0, 0, 0};
+        return GroupedTile{walk.all, -1, 0, 0, 0, 0, 0, 0};
     };
     // the tiles of groups without rows
     if (MODE == Grouped::TN && !p.accumulate)
