@@ -1,13 +1,17 @@
 """Edges of the norm, the ragged layout and the ragged products that a host can look at: ranges of descriptors, numbers near the ends of their types, refusals."""
+import itertools
 import random
+import re
 import subprocess
+from concurrent.futures import ThreadPoolExecutor
 
 import pytest
 import torch
 
 import yan_amd as yan
-from yan_amd.jit.compiler import get_hipcc_compiler, get_jit_include_dir
-from yan_amd.jit_kernels import moe, ragged
+from yan_amd.jit import cpp_format, generate
+from yan_amd.jit.compiler import get_compile_flags, get_hipcc_compiler, get_jit_include_dir
+from yan_amd.jit_kernels import moe, norm, ragged
 
 
 def _host(tmp_path, body, lines=''):
@@ -205,3 +209,22 @@ int main() {
     bad, halves = zip(*(map(int, line.split()) for line in out))
     assert len(out) == len(cases) and not any(bad)
     assert any(halves) and not all(halves)
+
+
+def test_norm_gradients_of_the_widest_rows_use_hardly_any_scratch(tmp_path):
+    """Of every combination of types with both gradients asked for: none, but 20 bytes of a lane where h and the weight are fp32."""
+    types = (torch.bfloat16, torch.float32)
+
+    def scratch(case):
+        _, keys, arg_defs, template = norm.norm_backward_kernel_plan(*case, *norm.norm_backward_lanes(norm.MAX_COLUMNS), True, True)
+        stem = '_'.join(str(t).split('.')[1] for t in case)
+        src, asm = tmp_path / f'{stem}.cu', tmp_path / f'{stem}.s'
+        src.write_text(generate(norm.includes, arg_defs, cpp_format(template, dict(keys))))
+        flags = [f for f in get_compile_flags() if f not in ('-shared', '-fPIC')]
+        subprocess.check_call([get_hipcc_compiler()[0], '-x', 'hip', '--cuda-device-only', '-S', *flags, f'-I{get_jit_include_dir()}', str(src), '-o', str(asm)])
+        return max(int(n) for n in re.findall(r'private_segment_fixed_size: *(\d+)', asm.read_text()))
+
+    cases = list(itertools.product(types, types, types))
+    with ThreadPoolExecutor(max_workers=4) as pool:
+        for (g, h, w), size in zip(cases, pool.map(scratch, cases)):
+            assert size <= (20 if h == w == torch.float32 else 0), (g, h, w)

@@ -10,9 +10,10 @@
 // contraction across its rows (the weights of NN, both sides of TN): its k-tile is 64 rows of as many columns as the tile has, and a fragment, eight consecutive k of one
 // column, comes out of LDS by ds_read_b64_tr_b16, which hands lane i of 16 column i of four rows by sixteen columns. No operand is transposed in memory.
 //
-// What does not exist is never read: rows behind a group's last one (NT, NN), columns behind a matrix' last one (a turned operand) and k behind the contraction's end
-// have the last one that exists copied in their place, so that every copy is within its operand and no copy is out of range for all its lanes. The former
-// are not stored. The latter are made zeros in LDS by the wave that copied them, in front of the barrier behind which they are read.
+// What does not exist is never read: rows behind a group's last one (NT, NN) and columns behind a matrix' last one have the last one that exists copied in their place, and are not
+// stored. So has k behind the contraction's end in the ring tiles; the large ones copy what comes next, the next row's k, another group's rows or, of a plain operand's last row, nothing for
+// the lanes that are out of the descriptor's range, and a turned operand's last row where that ends. Either way no copy reads outside of its operand, none is out of range for all
+// its lanes, and k behind the end is made zeros in LDS by the wave that copied it, in front of the barrier behind which it is read.
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -507,8 +508,9 @@ struct RowRuns {
 //   * descriptors of turned operands move on with the k-tile, so that ranges may be of any length;
 //   * any number of k-tiles, one for instance: the copies' place in the walk is its own.
 // Bound by the MFMAs for long groups: 16384 rows of one group x 4096 x 4096 1535 TFLOP/s (dense_gemm_body_4w 1554), NN 1430, TN 1519; of 16 equal groups 1390. Ragged ones lose what
-// their last tiles hold too little and the last round of tiles leaves idle: 32768 rows of 64 experts x 2048 x 7168, gathered: 870 us, 1105. TN writes fp32: of 16 experts x 4096 x 7168
-// (1.88 GB) 6144 rows take 540 us, 250 of MFMAs and the stores behind them.
+// their last tiles hold too little, 6 to 9 % of the MFMAs' rows, and more by a walk that gives every workgroup as many tiles whatever their heights: the busiest has 16 to 29 % more rows of
+// MFMAs than the mean in 32768 rows of 64 experts x 2048 x 7168, gathered: 867 to 889 us, 1080 to 1110. TN writes fp32: of 16 experts x 4096 x 7168
+// (1.88 GB) 6144 rows take 540 to 553 us, 250 of MFMAs and the stores behind them.
 struct GroupedTile {
     int slot, group, m0, rows, n0, cols, k0, depth;         // depth 0: none
     __device__ __forceinline__ int count() const { return ceil_div(depth, kDepth); }
@@ -1041,8 +1043,9 @@ grouped16_tall_kernel(GroupedProblem p) {
 
 enum Grouped16Kernel { kGroupedAny, kGroupedTall, kGrouped128, kGrouped64, kGrouped32 };
 
-// The kernel for a product: by the rows of a group on average, and by how many tiles of a kind there are at most for the chip's compute units. Fitted to every kernel's time
-// over 4 to 256 groups of 2 to 640 rows, (n, k) of 1024 x 512, 2048 x 2048, 4096 x 7168 and 7168 x 2048, bf16, on 256 compute units; over these the choice is 1.6 % (NT, NN)
+// The kernel for a product: by the rows of a group on average, and by how many tiles of a kind there are at most for the chip's compute units. How the rows are spread over the groups is
+// on the device, where the host cannot look: a few long groups among many short ones go by the mean of them all, and may get smaller tiles than they would alone. Fitted to every kernel's time
+// over 4 to 256 groups of 2 to 640 rows, (n, k) of 1024 x 512, 2048 x 2048, 4096 x 7168 and 7168 x 2048, bf16, on 256 compute units; over these the choice is 1.7 % (NT, NN)
 // and 0.5 % (TN) behind the best of the kernels in the mean, and 26 % at worst (16 groups of 24 rows, 7168 x 2048: 113, with 32 x 128 tiles 89). Microseconds, NT unless it says TN:
 //   256 x 256 tiles: one workgroup a compute unit, so the tiles have to number nearly as many. 16 groups of 81 rows, 4096 x 7168: 178 with them, 259 with 128 x 128. 64 groups of 88 rows,
 //       2048 x 2048: 130 | 141. Long groups earn them with fewer tiles: 4 of 496 rows, 4096 x 7168 (176 tiles): 128 | 180. Not so 4 of 522 rows, 1024 x 512 (48 tiles): 13.0 | 9.9.

@@ -7,8 +7,8 @@
 //
 // Bound by HBM. A row lies in the registers of LANES lanes from its load to its last store, V runs of 8 elements a lane, lane l of run v with elements
 // 8 (v LANES + l) .. + 7, so that 16 neighbouring lanes have the 128 elements of a scale and every load covers whole lines. One pass: separate kernels for
-// addition, norm and quantiser would move the row four times more. 8192 x 7168, bf16, a residual, codes and 16 bits (530 MB): 99.5 us, 5.3 TB/s, the rate of a large copy;
-// 64 x 7168: 3.9 us, a launch's latency and two trips to memory.
+// addition, norm and quantiser would move the row four times more. 8192 x 7168, bf16, a residual, codes and 16 bits (530 MB): 108 us, 4.9 TB/s, where a large copy has 5.1;
+// 64 x 7168: 3.8 us, a launch's latency and two trips to memory.
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -31,7 +31,7 @@ __device__ __forceinline__ Raw8<T> load_run(const T* p) {
     return r;
 }
 
-// Eight numbers rounded to T, to `p` on, and what they are then.
+// Eight numbers rounded to T.
 template <typename T>
 __device__ __forceinline__ Raw8<T> round_run(const F32x8& f) {
     Raw8<T> r;
@@ -46,6 +46,7 @@ __device__ __forceinline__ Raw8<T> round_run(const F32x8& f) {
     }
     return r;
 }
+// To `p` on.
 template <typename T>
 __device__ __forceinline__ void store_run(T* p, const Raw8<T>& r) {
 #pragma unroll
@@ -172,7 +173,7 @@ rms_norm_kernel(const X* x, H* residual, const W* __restrict__ weight, uint8_t* 
 
 // A workgroup takes rows blockIdx.x, + gridDim.x, ... (groups of THREADS / LANES of them), the next one's loads under way while it adds up; each lane keeps the
 // weight's sums of its columns and leaves them in row blockIdx.x * ROWS + its group of `partial` [parts, k] (WEIGHT). Adding to the gradient itself by atomics would
-// save the second launch and make results differ from run to run. 8192 x 7168 with a residual's gradient (470 MB): 93 us with the sums, 5.1 TB/s.
+// save the second launch and make results differ from run to run; a meeting of the workgroups, whose last adds up in order, would not, and has not been built. 8192 x 7168 with a residual's gradient (470 MB): 93 us with the sums, 5.1 TB/s.
 template <typename G, typename H, typename W, int LANES, int V, bool RESIDUAL, bool WEIGHT>
 __global__ void __launch_bounds__(LANES > 256 ? LANES : 256)
 rms_norm_backward_kernel(const G* __restrict__ grad, const H* __restrict__ h, const W* __restrict__ weight, const float* __restrict__ inverse_rms,
@@ -261,7 +262,8 @@ rms_norm_backward_kernel(const G* __restrict__ grad, const H* __restrict__ h, co
         }
     } else {
         // Wider rows, of 1024 lanes, have no registers for a second one. The loads of sixteen waves, and the stores of the row before, hide each other well enough: 8192 x 16384, bf16, with a
-        // residual's gradient (1.07 GB): 200 us, 5.4 TB/s.
+        // residual's gradient (1.07 GB): 200 us, 5.4 TB/s. Everything stays in registers but for 20 bytes of a lane where h and the weight are fp32 and both the residual's gradient and
+        // the weight's are asked for.
         Row a;
         for (int turn = 0; block < blocks; block += gridDim.x, turn ^= 1) {
             load(a, block);
@@ -327,7 +329,7 @@ inline hipError_t launch_rms_norm(const X* x, H* residual, const W* weight, void
     return hipSuccess;
 }
 
-// `partial`: fp32 [parts, k] of scratch, parts = workgroups * rows at a time, both as rms_norm_backward_workgroups in Python has them.
+// `partial`: fp32 [parts, k] of scratch, parts = workgroups * rows at a time, both as norm_backward_workgroups and norm_backward_lanes in Python have them.
 template <typename G, typename H, typename W, int LANES, int V, bool RESIDUAL, bool WEIGHT>
 inline hipError_t launch_rms_norm_backward(const G* grad, const H* h, const W* weight, const float* inverse_rms, const G* grad_residual, G* grad_h, float* partial,
                                            int workgroups, float* grad_weight, bool accumulate, int rows, int k, hipStream_t stream) {

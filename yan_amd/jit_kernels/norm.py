@@ -65,7 +65,7 @@ def norm_lanes(rows: int, k: int) -> Tuple[int, int]:
 def norm_backward_lanes(k: int) -> Tuple[int, int]:
     """
     The same of its gradient's, where a lane has two rows (up to 256 lanes) and the weight's sums in its registers. Wider rows one at a time on 1024 lanes (8192 x 16384
-    200 us; two of them on 512 lanes do not fit the registers: 317).
+    200 us; two of them on 512 lanes do not fit the registers: 317), which leaves 20 bytes of a lane in scratch where h and the weight are fp32 and both gradients are asked for.
     """
     runs = ceil_div(k, 8)
     for lanes in (16, 64, 256, 1024):
