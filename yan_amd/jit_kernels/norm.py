@@ -115,8 +115,10 @@ def _check(x, weight, *others):
 
 def _apart(a: torch.Tensor, b: torch.Tensor) -> bool:
     """Whether two contiguous tensors share no byte, whatever they are views of (tensors without memory have address 0)."""
-    at, other = a.data_ptr(), b.data_ptr()
-    return at + a.nbytes <= other or other + b.nbytes <= at or not at
+    ahead = b.data_ptr() - a.data_ptr()
+    if ahead:
+        return ahead >= a.nbytes if ahead > 0 else -ahead >= b.nbytes
+    return not a.data_ptr() or not a.nbytes or not b.nbytes
 
 
 def _run(plan, args):
