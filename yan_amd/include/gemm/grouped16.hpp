@@ -509,8 +509,8 @@ struct RowRuns {
 //   * any number of k-tiles, one for instance: the copies' place in the walk is its own.
 // Bound by the MFMAs for long groups: 16384 rows of one group x 4096 x 4096 1535 TFLOP/s (dense_gemm_body_4w 1554), NN 1430, TN 1519; of 16 equal groups 1390. Ragged ones lose what
 // their last tiles hold too little, 6 to 9 % of the MFMAs' rows, and more by a walk that gives every workgroup as many tiles whatever their heights: the busiest has 16 to 29 % more rows of
-// MFMAs than the mean in 32768 rows of 64 experts x 2048 x 7168, gathered: 867 to 889 us, 1080 to 1110. TN writes fp32: of 16 experts x 4096 x 7168
-// (1.88 GB) 6144 rows take 540 to 553 us, 250 of MFMAs and the stores behind them.
+// MFMAs than the mean in 32768 rows of 64 experts x 2048 x 7168, gathered: 867 to 970 us by how the router spreads them, 990 to 1110 TFLOP/s. TN writes fp32: of 16 experts x
+// 4096 x 7168 (1.88 GB) 6144 rows take 540 to 607 us, 250 of MFMAs and the stores behind them.
 struct GroupedTile {
     int slot, group, m0, rows, n0, cols, k0, depth;         // depth 0: none
     __device__ __forceinline__ int count() const { return ceil_div(depth, kDepth); }
